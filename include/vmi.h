@@ -486,6 +486,64 @@ int vmi_tree_commit(const int32_t* result, const vmi_tree_layer* layers, int n_l
                     int span, int pos0, const int32_t* pos_device, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The 8-bit KV cache (no counterpart in the reference, whose caches are mlx
+ * arrays in the model's type): a position's key or value of one kv head is 256
+ * codes c in [-127, 127] with one fp32 scale s and stands for s c, where
+ * a = max |x|, s = a / 127, c = round-to-nearest-even(127 x / a); a row of zeros
+ * has s = 0, a row with an infinity or NaN s = NaN (it reads back as NaN).  A
+ * row's codes depend on that row alone.  520 bytes per position and kv head
+ * where bf16 takes 1024.
+ *
+ * cache: vmi_kv8_bytes(n_kv_heads, max_len) bytes (0: sizes not taken), 16-byte
+ * aligned, max_len a multiple of 32.  Zero-filled it holds zero rows.  Per kv
+ * head max_len / 32 records of 16,640 bytes; in a record, position kt and dim d:
+ *   key code + 128 at   ((a*4 + (d>>6))*64 + ((d>>3)&3)*16 + nl)*16 + ((d>>5)&1)*8 + (d&7),
+ *                       nl = 4*(kt>>3) + (kt&3), a = (kt>>2)&1
+ *   value code + 128 at 8192 + ((d>>5)*64 + (kt>>3)*16 + (d&15))*16 + ((d>>4)&1)*8 + (kt&7)
+ *   key scale (fp32) at 16384 + 4 kt, value scale at 16512 + 4 kt
+ * (the operand order of the attention's matrix instructions).  head_dim is 256.
+ *
+ * vmi_kv8_write -- rows into the cache: keys and values bf16, row (g, i) at
+ * base + g * head + i * row elements (strides multiples of 4, 256 contiguous
+ * elements, 8-byte aligned), to positions pos0 .. pos0 + n - 1; other positions
+ * are left as they are.
+ * vmi_kv8_read -- positions pos0 .. pos0 + n - 1 as [n_kv_heads, n, 256] of
+ * dtype (VMI_F32, or VMI_BF16 rounded once); keys or values may be NULL.
+ * vmi_kv8_append -- a batch's heads: from the projections qkv f32 [T,
+ * (2 n_heads + 2 n_kv_heads) * 256] (q | gate per head, then keys, then values,
+ * as vmi_attention_layer's q_proj, k_proj and v_proj emit them) the queries and
+ * keys with their per-head RMSNorm (weights bf16 [256]) and rotary embedding on
+ * the first rope_dim dims at positions pos0 .., all in fp32: q_out bf16 [T,
+ * n_heads, 256] (NULL: not formed), keys and values into the cache.
+ * vmi_kv8_attention -- out bf16 [T, n_heads, 256] = softmax(q k / 16) v over the
+ * cache, query t seeing positions <= pos0 + t; with gate (f32, element strides
+ * gate_token and gate_head, 256 contiguous, rows 16-byte aligned) times
+ * sigmoid(gate).  q bf16 [T, n_heads, 256], T <= 8192.  Batches of T * n_heads /
+ * n_kv_heads <= 64 rows: a token's result does not depend on its batch or on
+ * max_len, bit for bit; larger ones equal it up to the order of fp32 sums.
+ * Positions behind a query's own never reach its result.  workspace: the
+ * query's bytes, 16-byte aligned, nothing kept between calls.
+ *
+ * pos_device (int32 on the device, or NULL) replaces pos0 when the kernels run;
+ * outside [0, max_len - T] it is clamped into it and VMI_STATUS_BAD_POS is OR-ed
+ * into *status (may be NULL).  One call at a time may write a range of
+ * positions; calls on different streams are the caller's to order.
+ * ------------------------------------------------------------------------ */
+size_t vmi_kv8_bytes(int n_kv_heads, int max_len);
+int vmi_kv8_write(const uint16_t* keys, int64_t key_head, int64_t key_row, const uint16_t* values, int64_t value_head,
+                  int64_t value_row, int n_kv_heads, int pos0, int n, uint8_t* cache, int max_len, void* stream);
+int vmi_kv8_read(const uint8_t* cache, int n_kv_heads, int max_len, int pos0, int n, void* keys, void* values,
+                 int dtype, void* stream);
+int vmi_kv8_append(const float* qkv, int T, int n_heads, int n_kv_heads, const uint16_t* q_norm,
+                   const uint16_t* k_norm, float eps, int rope_dim, float rope_theta, int pos0,
+                   const int32_t* pos_device, uint8_t* cache, int max_len, uint16_t* q_out, uint32_t* status,
+                   void* stream);
+size_t vmi_kv8_attention_workspace_bytes(int T, int n_heads, int n_kv_heads);
+int vmi_kv8_attention(const uint16_t* q, int T, int n_heads, int n_kv_heads, int pos0, const int32_t* pos_device,
+                      const uint8_t* cache, int max_len, const float* gate, int64_t gate_token, int64_t gate_head,
+                      uint16_t* out, uint32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * vmi_rmsnorm -- out = bf16(x * 1/sqrt(mean(x^2) + eps) * weight) per token
  * (mlx RMSNorm as the MTP module applies it: pre_fc_norm_embedding,
  * pre_fc_norm_hidden and norm, qwen3_next_mtp.py:27-31, 46-49, 54).  With ids

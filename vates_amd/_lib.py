@@ -123,6 +123,15 @@ _SIGNATURES = {
     "vmi_qgemm_workspace_bytes": (c_size_t, [c_int, c_int, QMat, c_int, c_int, c_int]),
     "vmi_qgemm": (c_int, [c_void_p, c_int, c_int, QMat, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t,
                           c_void_p]),
+    "vmi_kv8_bytes": (c_size_t, [c_int, c_int]),
+    "vmi_kv8_write": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
+                              c_int, c_void_p]),
+    "vmi_kv8_read": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "vmi_kv8_append": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_int, c_float, c_int,
+                               c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "vmi_kv8_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vmi_kv8_attention": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64,
+                                  c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "vmi_rmsnorm": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_float, c_void_p, c_int, c_void_p,
                             c_void_p]),
     "vmi_topk_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

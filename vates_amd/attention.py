@@ -9,6 +9,9 @@ and the number of committed positions, the analogue of mlx-lm's KVCache with
 its trim (mlx_streaming/mtp/kv_cache.py:222-251); its storage is blocks of 32
 positions in the attention kernel's operand order (``keys``/``values`` and
 ``write`` convert from and to [n_kv_heads, positions, 256]).
+``KVCache8`` holds them in 8 bits with a scale for each position and kv head,
+half the bytes; ``norm_rope_append`` forms a batch's heads and appends to it,
+``attend`` is the attention over it.
 Errors raise ``VmiError``; there is no fallback path.
 """
 from __future__ import annotations
@@ -18,8 +21,8 @@ from typing import Optional
 
 import torch
 
-from ._lib import QMat, VmiError, check, load
-from .moe import QuantizedProj, _require, _stream_handle, scratch, workspace
+from ._lib import VMI_BF16, VMI_F32, QMat, VmiError, check, load
+from .moe import QuantizedProj, _ptr, _require, _stream_handle, scratch, workspace
 
 
 class AttnDesc(ctypes.Structure):
@@ -149,6 +152,176 @@ class KVCache:
             blk = torch.empty_like(raw[:, b0:b1])
             blk[:, :, _block_perm(kind, raw.device)] = logical.reshape(raw.shape[0], b1 - b0, -1)
             raw[:, b0:b1] = blk
+
+
+class KVCache8(KVCache):
+    """Keys and values of one attention layer in 8 bits (vmi_kv8_*): each
+    position's key and value of a kv head is 256 codes and one fp32 scale, the
+    codes within half a step (1/254 of the row's largest magnitude) of what was
+    written.  A row is stored alike whatever is appended around it.  ``data``
+    holds the records (include/vmi.h), ``status`` (int32 [1] on the device) the
+    status bits that calls with a position on the device OR in."""
+
+    def __init__(self, n_kv_heads: int, max_len: int, device, head_dim: int = 256):
+        if head_dim != 256:
+            raise VmiError(f"head_dim={head_dim} (256 only)")
+        if max_len < 1 or n_kv_heads < 1:
+            raise VmiError(f"a cache of {n_kv_heads} kv heads and {max_len} positions")
+        self.max_len = -(-max_len // KV_BLOCK) * KV_BLOCK
+        self.n_kv = n_kv_heads
+        nbytes = load().vmi_kv8_bytes(n_kv_heads, self.max_len)
+        if not nbytes:
+            raise VmiError(f"a cache of {n_kv_heads} kv heads and {max_len} positions")
+        self.data = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.length = 0
+        self.tree_kv = None   # uint8: a draft tree's new rows
+        self._tree_flat = None
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def read(self, start: int = 0, stop: Optional[int] = None, *, dtype: torch.dtype = torch.bfloat16, stream=None):
+        """(keys, values) of positions start..stop-1 (default: all committed
+        ones) as [n_kv_heads, positions, 256], float32 or rounded to bfloat16."""
+        return self._read8(start, stop, dtype, True, True, stream)
+
+    def keys(self, start: int = 0, stop: Optional[int] = None, *, dtype: torch.dtype = torch.bfloat16,
+             stream=None) -> torch.Tensor:
+        return self._read8(start, stop, dtype, True, False, stream)[0]
+
+    def values(self, start: int = 0, stop: Optional[int] = None, *, dtype: torch.dtype = torch.bfloat16,
+               stream=None) -> torch.Tensor:
+        return self._read8(start, stop, dtype, False, True, stream)[1]
+
+    def _read8(self, start, stop, dtype, want_k, want_v, stream):
+        stop = self.length if stop is None else stop
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise VmiError(f"dtype {dtype} is not bfloat16 or float32")
+        if not 0 <= start <= stop <= self.max_len:
+            raise VmiError(f"positions {start}..{stop} outside the capacity {self.max_len}")
+        dev = _on_current(self.data)
+        with torch.cuda.stream(stream):
+            k, v = (torch.empty((self.n_kv, stop - start, 256), dtype=dtype, device=dev) if want else None
+                    for want in (want_k, want_v))
+        if stop > start:
+            check(load().vmi_kv8_read(self.data.data_ptr(), self.n_kv, self.max_len, start, stop - start, _ptr(k),
+                                      _ptr(v), VMI_F32 if dtype is torch.float32 else VMI_BF16, _stream_handle(stream)),
+                  "vmi_kv8_read")
+        return k, v
+
+    def write(self, start: int, keys: torch.Tensor, values: torch.Tensor, *, stream=None) -> None:
+        """Stores bfloat16 [n_kv_heads, n, 256] keys and values at positions
+        start..start+n-1.  Rows of 256 are contiguous; heads and positions may
+        be strided (a transposed view of token-major rows)."""
+        dev = _on_current(self.data)
+        n = keys.shape[1] if keys.dim() == 3 else 0
+        for name, t in (("keys", keys), ("values", values)):
+            if t.device != dev or t.dtype is not torch.bfloat16 or t.shape != (self.n_kv, n, 256) or t.stride(2) != 1:
+                raise VmiError(f"{name} must be bfloat16 [{self.n_kv}, {n}, 256] on {dev} with contiguous rows")
+        if start < 0 or start + n > self.max_len:
+            raise VmiError(f"positions {start}..{start + n} outside the capacity {self.max_len}")
+        if n:
+            check(load().vmi_kv8_write(keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(),
+                                       values.stride(0), values.stride(1), self.n_kv, start, n, self.data.data_ptr(),
+                                       self.max_len, _stream_handle(stream)), "vmi_kv8_write")
+
+
+def _on_current(t: torch.Tensor) -> torch.device:
+    """The tensor's device, which has to be the one that the calls go to."""
+    dev = t.device
+    if dev.type != "cuda" or dev.index != torch.cuda.current_device():
+        raise VmiError(f"tensors on {dev} are not on the current HIP device")
+    return dev
+
+
+def _position(cache: KVCache8, T: int, pos0: Optional[int], pos_device: Optional[torch.Tensor], dev) -> int:
+    if pos_device is not None:
+        if pos_device.device != dev or pos_device.dtype is not torch.int32 or pos_device.numel() != 1:
+            raise VmiError(f"pos_device must be int32 [1] on {dev}")
+        return 0
+    pos0 = cache.length if pos0 is None else pos0
+    if pos0 < 0 or pos0 + T > cache.max_len:
+        raise VmiError(f"positions {pos0}..{pos0 + T} outside the capacity {cache.max_len}")
+    return pos0
+
+
+def norm_rope_append(qkv: torch.Tensor, cache: KVCache8, q_norm: torch.Tensor, k_norm: torch.Tensor, *, n_heads: int,
+                     rope_dim: int = 64, rope_theta: float = 1e7, eps: float = 1e-6, pos0: Optional[int] = None,
+                     pos_device: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                     stream=None) -> torch.Tensor:
+    """The heads of T tokens from their projections (vmi_kv8_append): qkv f32
+    [T, (2 n_heads + 2 n_kv) * 256] holds q | gate per head, then the keys, then
+    the values.  Queries and keys get their per-head RMSNorm and rotary embedding
+    at positions pos0.. (default: cache.length); keys and values go into the cache,
+    whose length becomes pos0 + T; returns the queries, bfloat16 [T, n_heads, 256].
+    With pos_device (int32 [1] on the device) the position is read there when the
+    kernel runs, one outside the capacity is clamped and sets VMI_STATUS_BAD_POS in
+    cache.status, and cache.length is left to the caller."""
+    dev = _on_current(cache.data)
+    _require(qkv, "qkv", 4, dev)
+    if qkv.dtype is not torch.float32 or qkv.dim() != 2 or qkv.shape[1] != (2 * n_heads + 2 * cache.n_kv) * 256:
+        raise VmiError(f"qkv must be float32 [T, {(2 * n_heads + 2 * cache.n_kv) * 256}]")
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        _require(t, name, 2, dev)
+        if t.dtype is not torch.bfloat16 or t.numel() != 256:
+            raise VmiError(f"{name} must be bfloat16 [256]")
+    T = qkv.shape[0]
+    pos = _position(cache, T, pos0, pos_device, dev)
+    if out is None:
+        with torch.cuda.stream(stream):
+            out = torch.empty((T, n_heads, 256), dtype=torch.bfloat16, device=dev)
+    else:
+        _rows_bf16(out, "out", (T, n_heads, 256), dev)
+    if T:
+        check(load().vmi_kv8_append(qkv.data_ptr(), T, n_heads, cache.n_kv, q_norm.data_ptr(), k_norm.data_ptr(), eps,
+                                    rope_dim, rope_theta, pos, _ptr(pos_device), cache.data.data_ptr(), cache.max_len,
+                                    out.data_ptr(), cache.status.data_ptr(), _stream_handle(stream)), "vmi_kv8_append")
+    if pos_device is None:
+        cache.length = pos + T
+    return out
+
+
+def _rows_bf16(t: torch.Tensor, name: str, shape: tuple, dev) -> None:
+    _require(t, name, 2, dev)
+    if t.dtype is not torch.bfloat16 or t.shape != shape:
+        raise VmiError(f"{name} must be bfloat16 {list(shape)}")
+
+
+def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate: Optional[torch.Tensor] = None,
+           out: Optional[torch.Tensor] = None, pos_device: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """softmax(q k / 16) v over an 8-bit cache (vmi_kv8_attention): q bfloat16 [T,
+    n_heads, 256], the queries of positions pos0.. (default: the last T committed
+    ones), each seeing the positions up to its own; with gate (float32 [T, n_heads,
+    256], rows of 256 contiguous) times sigmoid(gate).  Returns bfloat16 [T,
+    n_heads, 256].  The result of a token of a batch of T * n_heads / n_kv <= 64
+    does not depend on the batch.  pos_device as for ``norm_rope_append``."""
+    dev = _on_current(cache.data)
+    if q.dim() != 3 or q.shape[1] % cache.n_kv or not q.shape[1]:
+        raise VmiError(f"q {tuple(q.shape)} does not fit a cache of {cache.n_kv} kv heads")
+    T, n_heads = q.shape[:2]
+    _rows_bf16(q, "q", (T, n_heads, 256), dev)
+    if pos0 is None and pos_device is None:
+        pos0 = cache.length - T
+    pos = _position(cache, T, pos0, pos_device, dev)
+    if gate is not None and (gate.device != dev or gate.dtype is not torch.float32 or gate.shape != q.shape or
+                             gate.stride(2) != 1):
+        raise VmiError(f"gate must be float32 {list(q.shape)} on {dev} with contiguous rows")
+    if out is None:
+        with torch.cuda.stream(stream):
+            out = torch.empty_like(q)
+    else:
+        _rows_bf16(out, "out", (T, n_heads, 256), dev)
+    if T:
+        lib = load()
+        nbytes = lib.vmi_kv8_attention_workspace_bytes(T, n_heads, cache.n_kv)
+        ws = scratch(nbytes, dev, stream)
+        check(lib.vmi_kv8_attention(q.data_ptr(), T, n_heads, cache.n_kv, pos, _ptr(pos_device), cache.data.data_ptr(),
+                                    cache.max_len, _ptr(gate), 0 if gate is None else gate.stride(0),
+                                    0 if gate is None else gate.stride(1), out.data_ptr(), cache.status.data_ptr(),
+                                    ws.data_ptr(), nbytes, _stream_handle(stream)), "vmi_kv8_attention")
+    return out
 
 
 class AttentionLayer:

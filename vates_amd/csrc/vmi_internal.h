@@ -72,4 +72,50 @@ hipError_t launch_rmsnorm(const uint16_t* x, const uint16_t* w, float eps, int T
 // Non-null, 16-byte aligned packed weights.
 bool qmat_ok(const vmi_qmat& m);
 
+// The 8-bit KV cache (vmi_kv8.hip).
+constexpr int kKv8Record = 16640;  // 32 positions of one kv head: key and value codes, then their scales
+constexpr int kKv8TreeRow = 528;   // a tree token's key codes, value codes and two scales, per path and kv head
+
+// q and k RMSNorm and rotary embedding of a batch's projections, k and v into
+// the cache (or a tree's rows into `tree`).  paths sequences of T tokens, all
+// from the same position.
+struct Kv8Heads {
+    const float* qkv;      // [paths * T, 2 n_heads + 2 n_kv, 256]: q | gate per head, then k, then v
+    int T, n_heads, n_kv;
+    int h0;                // first head formed: 0, or n_heads (keys and values only)
+    const uint16_t *q_norm, *k_norm;
+    float eps;
+    int rope_dim;
+    double rope_base;      // kv8_rope_base
+    int pos0;
+    const int32_t* pos_dev;
+    int max_len;
+    uint8_t* cache;
+    uint8_t* tree;         // or null: [paths][n_kv][T] rows instead of the cache
+    uint16_t* q;           // [paths * T, n_heads, 256]
+    uint32_t* status;      // or null (VMI_STATUS_BAD_POS)
+};
+double kv8_rope_base(float theta, int rope_dim);
+hipError_t launch_kv8_heads(const Kv8Heads& h, int paths, hipStream_t s);
+
+// Attention over the cache: paths sequences of span tokens at positions pos0 ..
+struct Kv8Attn {
+    const uint16_t* q;     // [paths * span, n_heads, 256]
+    const uint8_t* cache;
+    const uint8_t* tree;   // or null: the paths' own tokens
+    int n_heads, n_kv, span, paths, pos0, max_len;
+    const int32_t* pos_dev;
+    const float* gate;     // or null: f32, element strides gate_tok, gate_head
+    int64_t gate_tok, gate_head;
+    uint16_t* o;           // [paths * span, n_heads, 256]
+    uint32_t* status;      // or null
+    int rp;                // set by the launch: rows of a part, and the parts
+    float *part_o, *part_ml;
+};
+bool kv8_heads_ok(int n_heads, int n_kv);
+// Bytes of the parts (0: a form that is not built: several paths of more than
+// 64 rows, or more than 8192 tokens).
+size_t kv8_attention_parts_bytes(int paths, int span, int n_heads, int n_kv);
+hipError_t launch_kv8_attention(Kv8Attn a, void* parts, hipStream_t s);
+
 }  // namespace vmi
