@@ -461,8 +461,9 @@ int vmi_qgemm(const uint16_t* x, int T, int K, vmi_qmat w, int N, int bits, int 
  * ------------------------------------------------------------------------ */
 #define VMI_TREE_ATTENTION 1
 #define VMI_TREE_GDN 2
+#define VMI_TREE_ATTENTION_KV8 3       /* an 8-bit cache, see vmi_attention_tree_kv8 */
 typedef struct vmi_tree_layer {
-    int kind;                          /* VMI_TREE_ATTENTION or VMI_TREE_GDN */
+    int kind;                          /* one of the above */
     int n_kv_heads, max_len;           /* attention */
     int n_k_heads, n_v_heads, n_slots; /* Gated DeltaNet */
     uint16_t* k_cache;                 /* attention: the layer's caches and tree_kv */
@@ -542,6 +543,34 @@ size_t vmi_kv8_attention_workspace_bytes(int T, int n_heads, int n_kv_heads);
 int vmi_kv8_attention(const uint16_t* q, int T, int n_heads, int n_kv_heads, int pos0, const int32_t* pos_device,
                       const uint8_t* cache, int max_len, const float* gate, int64_t gate_token, int64_t gate_head,
                       uint16_t* out, uint32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The attention blocks over an 8-bit KV cache: vmi_attention_layer,
+ * vmi_attention_tree and vmi_attention_prompt with `cache` (above) in place of
+ * k_cache and v_cache, and the same shapes, results up to the rounding of the
+ * cached rows, and rules: T (span) <= 8, T * n_heads / n_kv_heads <= 64, paths *
+ * span <= 16 for the first two (a token's result does not depend on its batch,
+ * and a path's rows equal its tokens as a chain, bit for bit), up to 8192 tokens
+ * for prompts.  Queries and keys are rounded once, behind norm and rotation.
+ * tree: uint8 [paths][n_kv_heads][span] rows of VMI_KV8_TREE_ROW bytes (256 key
+ * codes + 128, 256 value codes + 128, the two scales, 8 bytes unused), 16-byte
+ * aligned.  A vmi_tree_layer of kind VMI_TREE_ATTENTION_KV8 holds the cache in
+ * k_cache and those rows in tree_kv.  status: a caller-owned word or NULL
+ * (VMI_STATUS_BAD_POS).  Workspaces keep nothing between calls;
+ * vmi_attention_kv8_workspace_bytes(1, T, ...) is the layer's, (paths, span, ...)
+ * the tree's; the queries return 0 for a form that is not built.
+ * ------------------------------------------------------------------------ */
+#define VMI_KV8_TREE_ROW 528
+size_t vmi_attention_kv8_workspace_bytes(int paths, int span, int hidden, int n_heads, int n_kv_heads);
+int vmi_attention_layer_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int T, int pos0,
+                            const int32_t* pos_device, uint8_t* cache, int max_len, uint16_t* out, uint32_t* status,
+                            void* workspace, size_t workspace_bytes, void* stream);
+int vmi_attention_tree_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int paths, int span, int pos0,
+                           const int32_t* pos_device, const uint8_t* cache, int max_len, uint8_t* tree, uint16_t* out,
+                           uint32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+size_t vmi_attention_prompt_kv8_workspace_bytes(const vmi_attn_layer_desc* desc, int T);
+int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int T, int pos0, uint8_t* cache,
+                             int max_len, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * vmi_rmsnorm -- out = bf16(x * 1/sqrt(mean(x^2) + eps) * weight) per token

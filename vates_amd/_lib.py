@@ -40,6 +40,8 @@ class QMat(ctypes.Structure):
 
 VMI_TREE_ATTENTION = 1
 VMI_TREE_GDN = 2
+VMI_TREE_ATTENTION_KV8 = 3
+VMI_KV8_TREE_ROW = 528
 
 
 class TreeLayer(ctypes.Structure):
@@ -132,6 +134,14 @@ _SIGNATURES = {
     "vmi_kv8_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "vmi_kv8_attention": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64,
                                   c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vmi_attention_kv8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "vmi_attention_layer_kv8": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                        c_void_p, c_size_t, c_void_p]),
+    "vmi_attention_tree_kv8": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vmi_attention_prompt_kv8_workspace_bytes": (c_size_t, [c_void_p, c_int]),
+    "vmi_attention_prompt_kv8": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                         c_size_t, c_void_p]),
     "vmi_rmsnorm": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_float, c_void_p, c_int, c_void_p,
                             c_void_p]),
     "vmi_topk_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

@@ -21,7 +21,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import VMI_BF16, VMI_F32, QMat, VmiError, check, load
+from ._lib import VMI_BF16, VMI_F32, VMI_KV8_TREE_ROW, QMat, VmiError, check, load
 from .moe import QuantizedProj, _ptr, _require, _stream_handle, scratch, workspace
 
 
@@ -110,6 +110,10 @@ class KVCache:
         self.tree_kv = None  # [paths, n_kv, 2, span, 256] bf16: a draft tree's new keys and values
         self._tree_flat = None
 
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
     def tree_buffer(self, paths: int, span: int) -> torch.Tensor:
         """The tree forward's keys and values [paths, n_kv, 2, span, 256]: one
         allocation for every tree of at most 16 tokens, so commit tables built
@@ -181,6 +185,17 @@ class KVCache8(KVCache):
     @property
     def device(self) -> torch.device:
         return self.data.device
+
+    def tree_buffer(self, paths: int, span: int) -> torch.Tensor:
+        """The tree forward's rows, uint8 [paths, n_kv, span, 528]: one
+        allocation for every tree of at most 16 tokens, as KVCache's."""
+        if paths * span > 16:
+            raise VmiError(f"a tree of {paths} x {span} tokens exceeds 16")
+        if self._tree_flat is None:
+            self._tree_flat = torch.zeros(16 * self.n_kv * VMI_KV8_TREE_ROW, dtype=torch.uint8, device=self.data.device)
+        self.tree_kv = self._tree_flat[:paths * self.n_kv * span * VMI_KV8_TREE_ROW].view(paths, self.n_kv, span,
+                                                                                          VMI_KV8_TREE_ROW)
+        return self.tree_kv
 
     def read(self, start: int = 0, stop: Optional[int] = None, *, dtype: torch.dtype = torch.bfloat16, stream=None):
         """(keys, values) of positions start..stop-1 (default: all committed
@@ -346,8 +361,43 @@ class AttentionLayer:
         d.q_norm, d.k_norm = q_norm.data_ptr(), k_norm.data_ptr()
         self.desc = d
 
-    def new_cache(self, max_len: int) -> KVCache:
-        return KVCache(self.n_kv, max_len, self.device)
+    def new_cache(self, max_len: int, bits: int = 16) -> KVCache:
+        """A cache for this layer: bf16, or with bits=8 a ``KVCache8``, which
+        every call of the layer takes in its place."""
+        if bits not in (8, 16):
+            raise VmiError(f"a cache of {bits} bits (8 or 16)")
+        return (KVCache8 if bits == 8 else KVCache)(self.n_kv, max_len, self.device)
+
+    def _cache8(self, x: torch.Tensor, cache: KVCache8, paths: int, span: int, pos0: Optional[int], out, stream,
+                pos_device) -> torch.Tensor:
+        """The block over an 8-bit cache: a batch (paths = 0) or a draft tree."""
+        dev = _on_current(cache.data)
+        if dev != self.device or cache.n_kv != self.n_kv:
+            raise VmiError(f"a cache of {cache.n_kv} kv heads on {dev} does not fit the layer")
+        T = max(paths, 1) * span
+        _rows_bf16(x, "x", (T, self.hidden), dev)
+        pos = _position(cache, span, pos0, pos_device, dev)
+        if out is None:
+            with torch.cuda.stream(stream):
+                out = torch.empty_like(x)
+        else:
+            _rows_bf16(out, "out", (T, self.hidden), dev)
+        lib = load()
+        nbytes = lib.vmi_attention_kv8_workspace_bytes(max(paths, 1), span, self.hidden, self.n_heads, self.n_kv)
+        if not nbytes:
+            raise VmiError(f"a batch of {max(paths, 1)} x {span} tokens is not built for this layer")
+        ws = scratch(nbytes, dev, stream)
+        rest = (out.data_ptr(), cache.status.data_ptr(), ws.data_ptr(), nbytes, _stream_handle(stream))
+        if paths:
+            check(lib.vmi_attention_tree_kv8(ctypes.byref(self.desc), x.data_ptr(), paths, span, pos, _ptr(pos_device),
+                                             cache.data.data_ptr(), cache.max_len, cache.tree_buffer(paths, span).data_ptr(),
+                                             *rest), "vmi_attention_tree_kv8")
+        else:
+            check(lib.vmi_attention_layer_kv8(ctypes.byref(self.desc), x.data_ptr(), span, pos, _ptr(pos_device),
+                                              cache.data.data_ptr(), cache.max_len, *rest), "vmi_attention_layer_kv8")
+            if pos_device is None:
+                cache.length = pos + span
+        return out
 
     def __call__(self, x: torch.Tensor, cache: KVCache, *, pos0: Optional[int] = None,
                  out: Optional[torch.Tensor] = None, stream=None,
@@ -357,6 +407,8 @@ class AttentionLayer:
         (int32 [1] on the device) the position is read there when the kernels
         run and cache.length is left to the caller."""
         T = x.shape[0]
+        if isinstance(cache, KVCache8):
+            return self._cache8(x, cache, 0, T, pos0, out, stream, pos_device)
         pos0 = cache.length if pos0 is None else pos0
         _require(x, "x", 2, self.device)
         if out is None:
@@ -373,8 +425,11 @@ class AttentionLayer:
             cache.length = pos0 + T
         return out
 
-    def prompt_workspace_bytes(self, T: int) -> int:
-        """Workspace of ``prompt`` on T tokens (0: a form it is not built for)."""
+    def prompt_workspace_bytes(self, T: int, cache: Optional[KVCache] = None) -> int:
+        """Workspace of ``prompt`` on T tokens (0: a form it is not built for)
+        into the cache (None: a bf16 one)."""
+        if isinstance(cache, KVCache8):
+            return load().vmi_attention_prompt_kv8_workspace_bytes(ctypes.byref(self.desc), T)
         return load().vmi_attention_prompt_workspace_bytes(ctypes.byref(self.desc), T)
 
     def prompt(self, x: torch.Tensor, cache: KVCache, *, pos0: int, keys_only: bool = False, stream=None,
@@ -389,7 +444,14 @@ class AttentionLayer:
         out = None if keys_only else torch.empty_like(x)
         sh = _stream_handle(stream)
         if ws is None:
-            ws = scratch(self.prompt_workspace_bytes(T), self.device, stream)
+            ws = scratch(self.prompt_workspace_bytes(T, cache), self.device, stream)
+        if isinstance(cache, KVCache8):
+            _on_current(cache.data)
+            check(load().vmi_attention_prompt_kv8(ctypes.byref(self.desc), x.data_ptr(), T, pos0, cache.data.data_ptr(),
+                                                  cache.max_len, _ptr(out), ws.data_ptr(), ws.numel(), sh),
+                  "vmi_attention_prompt_kv8")
+            cache.length = pos0 + T
+            return out
         check(load().vmi_attention_prompt(ctypes.byref(self.desc), x.data_ptr(), T, pos0, cache.k.data_ptr(),
                                           cache.v.data_ptr(), cache.max_len, None if keys_only else out.data_ptr(),
                                           ws.data_ptr(), ws.numel(), sh), "vmi_attention_prompt")
@@ -406,6 +468,8 @@ class AttentionLayer:
         if T % paths:
             raise VmiError(f"{T} rows do not split into {paths} paths")
         span = T // paths
+        if isinstance(cache, KVCache8):
+            return self._cache8(x, cache, paths, span, pos0, out, stream, pos_device)
         pos0 = cache.length if pos0 is None else pos0
         _require(x, "x", 2, self.device)
         if out is None:

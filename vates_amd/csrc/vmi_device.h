@@ -526,3 +526,17 @@ __device__ __forceinline__ int vmi_k_elem(int kt, int d) {
 __device__ __forceinline__ int vmi_v_elem(int kt, int d) {
     return ((((d >> 4) * 64 + (kt >> 3) * 16 + (d & 15)) << 3) + (kt & 7));
 }
+
+// 8-bit KV cache: per kv head, records of 32 positions (vmi.h, the 8-bit KV
+// cache, states the formulas).
+constexpr int kKv8Half = 8192;                    // bytes of a record's key codes, and of its value codes
+constexpr int kKv8Record = 2 * kKv8Half + 256;    // then 32 key and 32 value scales
+constexpr int kKv8TreeRow = 528;                  // a tree token's key codes, value codes and two scales
+__device__ __forceinline__ int kv8_k_off(int kt, int d) {
+    const int nl = 4 * (kt >> 3) + (kt & 3), a = (kt >> 2) & 1;
+    return ((a * 4 + (d >> 6)) * 64 + ((d >> 3) & 3) * 16 + nl) * 16 + ((d >> 5) & 1) * 8 + (d & 7);
+}
+__device__ __forceinline__ int kv8_v_off(int kt, int d) {
+    return kKv8Half + ((d >> 5) * 64 + (kt >> 3) * 16 + (d & 15)) * 16 + ((d >> 4) & 1) * 8 + (kt & 7);
+}
+__device__ __forceinline__ int kv8_scale_off(int kt, bool value) { return 2 * kKv8Half + (value ? 128 : 0) + kt * 4; }

@@ -465,6 +465,23 @@ __global__ __launch_bounds__(kGFThreads) void k_tree_commit(TreeCommitArgs a) {
         }
         return;
     }
+    if (Ly.kind == VMI_TREE_ATTENTION_KV8) {
+        if (hh >= Ly.n_kv_heads) return;
+        uint8_t* cache = reinterpret_cast<uint8_t*>(Ly.k_cache);
+        const uint8_t* tree = reinterpret_cast<const uint8_t*>(Ly.tree_kv);
+        for (int i = tid; i < acc * 256; i += kGFThreads) {
+            const int j = i >> 8, d = i & 255, pos = pos0 + j;
+            if (pos >= Ly.max_len) continue;
+            const uint8_t* side = tree + ((size_t)(win * Ly.n_kv_heads + hh) * a.span + j) * kKv8TreeRow;
+            uint8_t* rec = cache + ((size_t)hh * (Ly.max_len / VMI_KV_BLOCK) + pos / VMI_KV_BLOCK) * kKv8Record;
+            const int kt = pos % VMI_KV_BLOCK;
+            rec[kv8_k_off(kt, d)] = side[d];
+            rec[kv8_v_off(kt, d)] = side[256 + d];
+            if (d < 2)
+                *reinterpret_cast<float*>(rec + kv8_scale_off(kt, d)) = *reinterpret_cast<const float*>(side + 512 + 4 * d);
+        }
+        return;
+    }
     if (Ly.kind != VMI_TREE_GDN || hh >= Ly.n_v_heads) return;
     const int h = hh, n_k = Ly.n_k_heads, n_v = Ly.n_v_heads, hk = h / (n_v / n_k);
     const int conv_dim = 2 * n_k * kGHead + n_v * kGHead;

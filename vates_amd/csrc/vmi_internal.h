@@ -73,9 +73,7 @@ hipError_t launch_rmsnorm(const uint16_t* x, const uint16_t* w, float eps, int T
 bool qmat_ok(const vmi_qmat& m);
 
 // The 8-bit KV cache (vmi_kv8.hip).
-constexpr int kKv8Record = 16640;  // 32 positions of one kv head: key and value codes, then their scales
-constexpr int kKv8TreeRow = 528;   // a tree token's key codes, value codes and two scales, per path and kv head
-
+//
 // q and k RMSNorm and rotary embedding of a batch's projections, k and v into
 // the cache (or a tree's rows into `tree`).  paths sequences of T tokens, all
 // from the same position.

@@ -44,18 +44,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBlk = VMI_KV_BLOCK;           // positions per record
-constexpr int kHalfRec = kBlk * kHeadDim;    // bytes of a record's keys (or values)
-constexpr int kRec = vmi::kKv8Record;
-static_assert(kRec == 2 * kHalfRec + 2 * kBlk * 4, "record");
-
-__device__ __forceinline__ int kv8_k_off(int kt, int d) {
-    const int nl = 4 * (kt >> 3) + (kt & 3), a = (kt >> 2) & 1;
-    return ((a * 4 + (d >> 6)) * 64 + ((d >> 3) & 3) * 16 + nl) * 16 + ((d >> 5) & 1) * 8 + (d & 7);
-}
-__device__ __forceinline__ int kv8_v_off(int kt, int d) {
-    return kHalfRec + ((d >> 5) * 64 + (kt >> 3) * 16 + (d & 15)) * 16 + ((d >> 4) & 1) * 8 + (kt & 7);
-}
-__device__ __forceinline__ int kv8_scale_off(int kt, bool value) { return 2 * kHalfRec + (value ? kBlk * 4 : 0) + kt * 4; }
+constexpr int kHalfRec = kKv8Half;           // bytes of a record's keys (or values)
+constexpr int kRec = kKv8Record;
+static_assert(kRec == 2 * kHalfRec + 2 * kBlk * 4 && kHalfRec == kBlk * kHeadDim, "record");
 
 // One row, dims 4 l .. 4 l + 3 in lane l: the four codes + 128 in a word, the
 // row's scale in every lane.
@@ -304,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
         const uint32_t c = kv8_quantise(x[i], s);
         if (a.tree) {  // plain rows, one record per token
             if (!mine) continue;
-            uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * a.T + t) * vmi::kKv8TreeRow;
+            uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * a.T + t) * kKv8TreeRow;
             *reinterpret_cast<uint32_t*>(side + (is_v ? kHeadDim : 0) + 4 * lane) = c;
             if (lane == 0) *reinterpret_cast<float*>(side + 2 * kHeadDim + (is_v ? 4 : 0)) = s;
             continue;
@@ -575,7 +566,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_kv8_split(Kv8Attn a) {
         if (a.tree && kBlk * b + kBlk > pos0) {
             // a path's own tokens in place of what the cache holds there
             for (int t = max(kBlk * b - pos0, 0); t < min(T, kBlk * b + kBlk - pos0); ++t) {
-                const uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * T + t) * vmi::kKv8TreeRow;
+                const uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * T + t) * kKv8TreeRow;
                 const int kt = pos0 + t - kBlk * b;
                 const uint32_t kc = *reinterpret_cast<const uint32_t*>(side + 4 * lane);
                 const uint32_t vc = *reinterpret_cast<const uint32_t*>(side + kHeadDim + 4 * lane);
@@ -869,6 +860,134 @@ int launched(const char* what) {
 }
 
 }  // namespace
+
+namespace {
+
+constexpr int kMaxSpan = 8, kMaxBatch = 16;   // tokens of a path, of a call (as vmi_attention_layer)
+
+struct LayerWs {
+    size_t xn, qkv, q, o, parts, bytes;
+};
+
+LayerWs layer_ws(int paths, int span, int H, int n_heads, int n_kv) {
+    LayerWs L{};
+    const size_t T = (size_t)paths * span, rows = T * kHeadDim;
+    size_t off = 0;
+    auto take = [&](size_t b) {
+        const size_t o = off;
+        off += vmi::align256(b);
+        return o;
+    };
+    L.xn = take(T * H * 2);
+    L.qkv = take(rows * 2 * (n_heads + n_kv) * 4);
+    L.q = take(rows * n_heads * 2);
+    L.o = take(rows * n_heads * 2);
+    L.parts = take(vmi::kv8_attention_parts_bytes(paths, span, n_heads, n_kv));
+    L.bytes = off;
+    return L;
+}
+
+bool layer_shape_ok(int paths, int span, int hidden, int n_heads, int n_kv) {
+    return paths > 0 && span > 0 && span <= kMaxSpan && paths <= kMaxBatch && paths * span <= kMaxBatch && hidden > 0 &&
+           hidden % 512 == 0 && hidden <= 4096 && vmi::kv8_heads_ok(n_heads, n_kv) && n_kv <= 1024 &&
+           span * (n_heads / n_kv) <= kSplitRows &&
+           (size_t)std::min(paths * span, 8) * std::max(hidden, n_heads * kHeadDim) * 2 <= 65536;  // the GEMV's rows
+}
+
+// The attention block over `paths` sequences of `span` tokens that share the
+// cache below pos0 (one path: a batch, its rows into the cache; several: a draft
+// tree, its rows into `tree`).
+int layer_impl(const vmi_attn_layer_desc* desc, const uint16_t* x, int paths, int span, int pos0,
+               const int32_t* pos_device, uint8_t* cache, int max_len, uint8_t* tree, uint16_t* out, uint32_t* status,
+               void* workspace, size_t workspace_bytes, hipStream_t s) {
+    if (!desc) return vmi::fail(VMI_ERR_INVALID, "null desc");
+    const vmi_attn_layer_desc& D = *desc;
+    if (D.head_dim != kHeadDim) return vmi::fail(VMI_ERR_UNSUPPORTED, "head_dim=%d (256 only)", D.head_dim);
+    if ((D.bits != 4 && D.bits != 8) || D.group != 64) return vmi::fail(VMI_ERR_UNSUPPORTED, "bits=%d group=%d", D.bits, D.group);
+    if (!layer_shape_ok(paths, span, D.hidden, D.n_heads, D.n_kv_heads))
+        return vmi::fail(VMI_ERR_UNSUPPORTED, "paths=%d span=%d hidden=%d heads=%d/%d not built", paths, span, D.hidden,
+                         D.n_heads, D.n_kv_heads);
+    if (D.rope_dim < 0 || D.rope_dim > kHeadDim || D.rope_dim % 2 || !(D.rope_theta > 0.0f))
+        return vmi::fail(VMI_ERR_INVALID, "rope_dim=%d rope_theta=%g", D.rope_dim, (double)D.rope_theta);
+    const int rc = check_cache(cache, D.n_kv_heads, max_len, pos0, span, pos_device);
+    if (rc != VMI_OK) return rc;
+    if (!vmi::qmat_ok(D.q_proj) || !vmi::qmat_ok(D.k_proj) || !vmi::qmat_ok(D.v_proj) || !vmi::qmat_ok(D.o_proj))
+        return vmi::fail(VMI_ERR_INVALID, "projection weights must be non-null and 16-byte aligned");
+    if (!x || !out || !D.input_norm || !D.q_norm || !D.k_norm || !aligned(x, 16) || !aligned(out, 16) ||
+        !aligned(D.input_norm, 16))
+        return vmi::fail(VMI_ERR_INVALID, "x, out or norm weights null or not 16-byte aligned");
+    const int T = paths * span;
+    const LayerWs L = layer_ws(paths, span, D.hidden, D.n_heads, D.n_kv_heads);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < L.bytes)
+        return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes (got %zu)", L.bytes, workspace_bytes);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    float* qkv = reinterpret_cast<float*>(ws + L.qkv);
+    uint16_t* q = reinterpret_cast<uint16_t*>(ws + L.q);
+    uint16_t* o = reinterpret_cast<uint16_t*>(ws + L.o);
+    const int stride = (D.n_heads + D.n_kv_heads) * 2 * kHeadDim;
+
+    vmi::QgemvCall p{};
+    p.x = x; p.T = T; p.K = D.hidden; p.bits = D.bits;
+    p.m[0] = D.q_proj; p.m[1] = D.k_proj; p.m[2] = D.v_proj;
+    p.rows[0] = D.n_heads * 2 * kHeadDim; p.rows[1] = p.rows[2] = D.n_kv_heads * kHeadDim;
+    p.nrows = stride; p.out = qkv; p.out_stride = stride;
+    p.norm_w = D.input_norm; p.eps = D.norm_eps;
+    hipError_t e;
+    if (!vmi::qgemv_fuses_norm(p)) {
+        uint16_t* xn = reinterpret_cast<uint16_t*>(ws + L.xn);
+        e = vmi::launch_rmsnorm(x, D.input_norm, D.norm_eps, T, D.hidden, xn, s);
+        if (e != hipSuccess) return vmi::hip_fail(e, "input norm launch");
+        p.x = xn;
+        p.norm_w = nullptr;
+    }
+    e = vmi::launch_qgemv(p, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "qkv projection launch");
+    vmi::Kv8Heads h{};
+    h.qkv = qkv; h.T = span; h.n_heads = D.n_heads; h.n_kv = D.n_kv_heads;
+    h.q_norm = D.q_norm; h.k_norm = D.k_norm; h.eps = D.norm_eps; h.rope_dim = D.rope_dim;
+    h.rope_base = vmi::kv8_rope_base(D.rope_theta, D.rope_dim);
+    h.pos0 = pos0; h.pos_dev = pos_device; h.max_len = max_len; h.cache = cache; h.tree = tree; h.q = q; h.status = status;
+    e = vmi::launch_kv8_heads(h, paths, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "k_kv8_heads launch");
+    vmi::Kv8Attn a{};
+    a.q = q; a.cache = cache; a.tree = tree; a.n_heads = D.n_heads; a.n_kv = D.n_kv_heads; a.span = span; a.paths = paths;
+    a.pos0 = pos0; a.pos_dev = pos_device; a.max_len = max_len;
+    a.gate = qkv + kHeadDim; a.gate_tok = stride; a.gate_head = 2 * kHeadDim; a.o = o;
+    e = vmi::launch_kv8_attention(a, ws + L.parts, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "attention launch");
+    vmi::QgemvCall c{};
+    c.x = o; c.T = T; c.K = D.n_heads * kHeadDim; c.bits = D.bits;
+    c.m[0] = c.m[1] = c.m[2] = D.o_proj;
+    c.rows[0] = c.nrows = D.hidden;
+    c.out_stride = D.hidden; c.residual = x; c.out_bf16 = out;
+    e = vmi::launch_qgemv(c, s);
+    return e == hipSuccess ? VMI_OK : vmi::hip_fail(e, "o_proj launch");
+}
+
+}  // namespace
+
+extern "C" size_t vmi_attention_kv8_workspace_bytes(int paths, int span, int hidden, int n_heads, int n_kv_heads) {
+    return layer_shape_ok(paths, span, hidden, n_heads, n_kv_heads) ? layer_ws(paths, span, hidden, n_heads, n_kv_heads).bytes : 0;
+}
+
+extern "C" int vmi_attention_layer_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int T, int pos0,
+                                       const int32_t* pos_device, uint8_t* cache, int max_len, uint16_t* out,
+                                       uint32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
+    vmi::clear_error();
+    return layer_impl(desc, x, 1, T, pos0, pos_device, cache, max_len, nullptr, out, status, workspace, workspace_bytes,
+                      static_cast<hipStream_t>(stream));
+}
+
+extern "C" int vmi_attention_tree_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int paths, int span, int pos0,
+                                      const int32_t* pos_device, const uint8_t* cache, int max_len, uint8_t* tree,
+                                      uint16_t* out, uint32_t* status, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+    vmi::clear_error();
+    if (!tree || !aligned(tree, 16)) return vmi::fail(VMI_ERR_INVALID, "tree rows null or not 16-byte aligned");
+    // the cache is only read: every path's rows go to `tree`
+    return layer_impl(desc, x, paths, span, pos0, pos_device, const_cast<uint8_t*>(cache), max_len, tree, out, status,
+                      workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
 
 extern "C" size_t vmi_kv8_bytes(int n_kv_heads, int max_len) {
     if (n_kv_heads <= 0 || n_kv_heads > 1024 || max_len <= 0 || max_len % kBlk) return 0;

@@ -1222,6 +1222,91 @@ extern "C" int vmi_attention_prompt(const vmi_attn_layer_desc* desc, const uint1
     return e == hipSuccess ? VMI_OK : vmi::hip_fail(e, "o_proj launch");
 }
 
+namespace {
+
+struct Attn8Ws {
+    PrOperand xn, on;
+    float* qkv;
+    uint16_t *q, *o;
+    void* parts;
+    size_t bytes;
+};
+
+Attn8Ws attn8_ws(const vmi_attn_layer_desc& D, int T, void* base) {
+    Attn8Ws w;
+    Carve c(base);
+    w.xn = pr_operand(c, T, D.hidden);
+    w.on = pr_operand(c, T, D.n_heads * kHeadDim);
+    w.qkv = static_cast<float*>(c.take((size_t)T * (D.n_heads + D.n_kv_heads) * 2 * kHeadDim * 4));
+    w.q = static_cast<uint16_t*>(c.take((size_t)T * D.n_heads * kHeadDim * 2));
+    w.o = static_cast<uint16_t*>(c.take((size_t)T * D.n_heads * kHeadDim * 2));
+    w.parts = c.take(vmi::kv8_attention_parts_bytes(1, T, D.n_heads, D.n_kv_heads));
+    w.bytes = c.off;
+    return w;
+}
+
+bool attn8_form_ok(const vmi_attn_layer_desc& D, int T) { return attn_form_ok(D, T) && D.rope_theta > 0.0f; }
+
+}  // namespace
+
+extern "C" size_t vmi_attention_prompt_kv8_workspace_bytes(const vmi_attn_layer_desc* desc, int T) {
+    return desc && attn8_form_ok(*desc, T) ? attn8_ws(*desc, T, nullptr).bytes : 0;
+}
+
+extern "C" int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int T, int pos0,
+                                        uint8_t* cache, int max_len, uint16_t* out, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+    vmi::clear_error();
+    if (!desc) return vmi::fail(VMI_ERR_INVALID, "null desc");
+    const vmi_attn_layer_desc& D = *desc;
+    if (!attn8_form_ok(D, T)) return vmi::fail(VMI_ERR_UNSUPPORTED, "layer form or T=%d not built for prompts", T);
+    if (!x || !cache) return vmi::fail(VMI_ERR_INVALID, "null x/cache");
+    if (pos0 < 0 || max_len % VMI_KV_BLOCK || T > max_len || pos0 > max_len - T)
+        return vmi::fail(VMI_ERR_INVALID, "pos0=%d T=%d max_len=%d", pos0, T, max_len);
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache) |
+         reinterpret_cast<uintptr_t>(workspace)) & 15)
+        return vmi::fail(VMI_ERR_INVALID, "x, out, cache and workspace must be 16-byte aligned");
+    const Attn8Ws W = attn8_ws(D, T, workspace);
+    if (!workspace || workspace_bytes < W.bytes)
+        return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes (got %zu)", W.bytes, workspace_bytes);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int heads = D.n_heads, kv = D.n_kv_heads, stride = (heads + kv) * 2 * kHeadDim;
+    hipError_t e = pr_prep(x, D.input_norm, D.norm_eps, T, D.hidden, W.xn, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "input norm launch");
+    // without an output only the keys and values are formed (columns of the same rows)
+    const int qrows = out ? heads * 2 * kHeadDim : 0;
+    PrGemm p{};
+    p.x = W.xn; p.T = T; p.K = D.hidden;
+    p.m[0] = D.q_proj; p.m[1] = D.k_proj; p.m[2] = D.v_proj;
+    p.rows[0] = qrows; p.rows[1] = kv * kHeadDim; p.rows[2] = kv * kHeadDim; p.nrows = qrows + 2 * kv * kHeadDim;
+    p.out = W.qkv + (heads * 2 * kHeadDim - qrows); p.out_stride = stride;
+    e = pr_gemm(p, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "qkv projection launch");
+    vmi::Kv8Heads h{};
+    h.qkv = W.qkv; h.T = T; h.n_heads = heads; h.n_kv = kv; h.h0 = out ? 0 : heads;
+    h.q_norm = D.q_norm; h.k_norm = D.k_norm; h.eps = D.norm_eps; h.rope_dim = D.rope_dim;
+    h.rope_base = vmi::kv8_rope_base(D.rope_theta, D.rope_dim);
+    h.pos0 = pos0; h.max_len = max_len; h.cache = cache; h.q = W.q;
+    e = vmi::launch_kv8_heads(h, 1, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "k_kv8_heads launch");
+    if (!out) return VMI_OK;
+    vmi::Kv8Attn a{};
+    a.q = W.q; a.cache = cache; a.n_heads = heads; a.n_kv = kv; a.span = T; a.paths = 1;
+    a.pos0 = pos0; a.max_len = max_len;
+    a.gate = W.qkv + kHeadDim; a.gate_tok = stride; a.gate_head = 2 * kHeadDim; a.o = W.o;
+    e = vmi::launch_kv8_attention(a, W.parts, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "attention launch");
+    e = pr_prep(W.o, nullptr, 0.0f, T, heads * kHeadDim, W.on, s);
+    if (e != hipSuccess) return vmi::hip_fail(e, "o_proj operand launch");
+    PrGemm o{};
+    o.x = W.on; o.T = T; o.K = heads * kHeadDim;
+    o.m[0] = o.m[1] = o.m[2] = D.o_proj;
+    o.rows[0] = o.nrows = D.hidden;
+    o.out_stride = D.hidden; o.residual = x; o.out_bf16 = out;
+    e = pr_gemm(o, s);
+    return e == hipSuccess ? VMI_OK : vmi::hip_fail(e, "o_proj launch");
+}
+
 extern "C" size_t vmi_gdn_prompt_workspace_bytes(const vmi_gdn_layer_desc* desc, int T) {
     return desc && gdn_form_ok(*desc, T) ? gdn_ws(*desc, T, nullptr).bytes : 0;
 }

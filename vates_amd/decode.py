@@ -33,7 +33,7 @@ import torch
 
 from ._lib import VmiError, check, load
 from .accept import accept_greedy, accept_stochastic, raise_sampling_status, sample_top_p, spec_commit
-from .attention import AttentionLayer, KVCache
+from .attention import AttentionLayer, KVCache, KVCache8
 from .gdn import GatedDeltaNetLayer, GdnCache
 from .head import TiledHead, lm_head
 from .moe import MoELayer, scratch
@@ -95,10 +95,11 @@ class SpecModel:
         if mtp is not None and mtp.w.lm_head is head:
             mtp.head_tiles = self.head_tiles
 
-    def new_caches(self, max_len: int, max_batch: int = 8) -> list:
-        """Per layer: a KVCache (full attention), a GdnCache (linear attention,
-        verify batches up to max_batch tokens) or None."""
-        return [l.attn.new_cache(max_len) if l.attn is not None else
+    def new_caches(self, max_len: int, max_batch: int = 8, *, kv_bits: int = 16) -> list:
+        """Per layer: a KVCache (full attention; with kv_bits=8 a KVCache8, half
+        the bytes), a GdnCache (linear attention, verify batches up to max_batch
+        tokens) or None."""
+        return [l.attn.new_cache(max_len, kv_bits) if l.attn is not None else
                 l.gdn.new_cache(max_batch) if l.gdn is not None else None for l in self.layers]
 
     def forward(self, ids: torch.Tensor, caches: list, pos0: int, *, want_logits: bool = False,
@@ -158,14 +159,18 @@ class TreeCommit:
     The layer table lives in device memory."""
 
     def __init__(self, caches: list, paths: int, span: int):
-        from ._lib import VMI_TREE_ATTENTION, VMI_TREE_GDN, TreeLayer
+        from ._lib import VMI_TREE_ATTENTION, VMI_TREE_ATTENTION_KV8, VMI_TREE_GDN, TreeLayer
         rows = []
         heads = 1
         for c in caches:
             if c is None:
                 continue
             e = TreeLayer()
-            if isinstance(c, KVCache):
+            if isinstance(c, KVCache8):
+                e.kind, e.n_kv_heads, e.max_len = VMI_TREE_ATTENTION_KV8, c.n_kv, c.max_len
+                e.k_cache, e.tree_kv = c.data.data_ptr(), c.tree_buffer(paths, span).data_ptr()
+                heads = max(heads, c.n_kv)
+            elif isinstance(c, KVCache):
                 tkv = c.tree_buffer(paths, span)
                 e.kind, e.n_kv_heads, e.max_len = VMI_TREE_ATTENTION, c.n_kv, c.max_len
                 e.k_cache, e.v_cache, e.tree_kv = c.k.data_ptr(), c.v.data_ptr(), tkv.data_ptr()
@@ -180,7 +185,7 @@ class TreeCommit:
             rows.append(bytes(e))
         self.n, self.heads, self.paths, self.span = len(rows), heads, paths, span
         self.caches = caches
-        dev = next(c.k.device if isinstance(c, KVCache) else c.conv.device for c in caches if c is not None)
+        dev = next(c.device if isinstance(c, KVCache) else c.conv.device for c in caches if c is not None)
         self.table = torch.frombuffer(bytearray(b"".join(rows)), dtype=torch.uint8).to(dev)
 
     def __call__(self, rec: torch.Tensor, *, pos0: int = 0, pos_device: Optional[torch.Tensor] = None,
@@ -222,6 +227,17 @@ def _own(obj, name: str, cls) -> bool:
     return method is getattr(cls, name) and name not in getattr(obj, "__dict__", {})
 
 
+def _prompt_bytes(attn: AttentionLayer, T: int, cache) -> int:
+    """The attention layer's prompt workspace for this kind of cache."""
+    return attn.prompt_workspace_bytes(T, cache) if isinstance(cache, KVCache8) else attn.prompt_workspace_bytes(T)
+
+
+def _fill_bytes(drafter: MTPDrafter, T: int) -> int:
+    cache = getattr(drafter, "cache", None)
+    return (drafter.mtp.fill_workspace_bytes(T, cache) if isinstance(cache, KVCache8) else
+            drafter.mtp.fill_workspace_bytes(T))
+
+
 def _prompt_blocks(model: SpecModel, prompt: torch.Tensor, caches, drafter: Optional[MTPDrafter], chunk: int) -> list:
     """The (start, end) blocks in which ``prefill`` runs a prompt through the
     prompt kernels, or [] where it runs verify batches: short prompts, under
@@ -247,20 +263,23 @@ def _prompt_blocks(model: SpecModel, prompt: torch.Tensor, caches, drafter: Opti
     for layer, cache in zip(model.layers, caches):
         if layer.attn is not None:
             ok = (isinstance(cache, KVCache) and P <= cache.max_len and
-                  chunk * (layer.attn.n_heads // layer.attn.n_kv) <= 64 and layer.attn.prompt_workspace_bytes(step))
+                  chunk * (layer.attn.n_heads // layer.attn.n_kv) <= 64 and
+                  _prompt_bytes(layer.attn, step, cache))
         elif layer.gdn is not None:
             ok = (isinstance(cache, GdnCache) and cache.n_slots > chunk and layer.gdn.prompt_workspace_bytes(step))
         else:
             ok = True
         if not ok or not layer.moe.prompt_workspace_bytes(step):
             return []
-    if drafter is not None and not (P - 1 <= drafter.cache.max_len and drafter.mtp.fill_workspace_bytes(step) and
+    if drafter is not None and not (P - 1 <= drafter.cache.max_len and
+                                    _fill_bytes(drafter, step) and
                                     chunk * (drafter.mtp.w.attn.n_heads // drafter.mtp.w.attn.n_kv) <= 64):
         return []
     return [(s, min(P, s + step)) for s in range(0, P, step)]
 
 
-def _prompt_scratch(model: SpecModel, prompt: torch.Tensor, blocks: list, drafter: Optional[MTPDrafter]):
+def _prompt_scratch(model: SpecModel, prompt: torch.Tensor, blocks: list, drafter: Optional[MTPDrafter],
+                    caches: Optional[list] = None):
     """(blocks, workspace): one workspace for all of a prompt's layers and
     blocks, given back with the call.  Where the device has no room for it the
     blocks halve, down to none ([], None: the prompt runs as verify batches)."""
@@ -268,9 +287,10 @@ def _prompt_scratch(model: SpecModel, prompt: torch.Tensor, blocks: list, drafte
     while blocks:
         step = blocks[0][1]
         need = [l.moe.prompt_workspace_bytes(step) for l in model.layers]
-        need += [(l.attn or l.gdn).prompt_workspace_bytes(step) for l in model.layers if l.attn or l.gdn]
+        need += [_prompt_bytes(l.attn, step, c) if l.attn else l.gdn.prompt_workspace_bytes(step)
+                 for l, c in zip(model.layers, caches or [None] * len(model.layers)) if l.attn or l.gdn]
         if drafter is not None:
-            need.append(drafter.mtp.fill_workspace_bytes(step))
+            need.append(_fill_bytes(drafter, step))
         try:
             return blocks, scratch(max(need), prompt.device)
         except torch.OutOfMemoryError:
@@ -289,7 +309,7 @@ def prefill(model: SpecModel, prompt: torch.Tensor, caches, drafter: Optional[MT
     and by how near-ties of the routing fall."""
     P = prompt.numel()
     hs = []
-    blocks, ws = _prompt_scratch(model, prompt, _prompt_blocks(model, prompt, caches, drafter, chunk), drafter)
+    blocks, ws = _prompt_scratch(model, prompt, _prompt_blocks(model, prompt, caches, drafter, chunk), drafter, caches)
     if blocks:
         for s, e in blocks:
             x = rmsnorm(model.embed, None, ids=prompt[s:e])

@@ -104,9 +104,10 @@ class MTPLayer:
                                 logits=logits_out, argmax=argmax_out, top_prob=prob_out, stream=stream)
         return am, Hn, logits
 
-    def fill_workspace_bytes(self, T: int) -> int:
-        """Workspace of ``fill`` on T tokens (0: a form it is not built for)."""
-        parts = qgemm_workspace_bytes(self.w.fc, T, 2 * self.hidden), self.w.attn.prompt_workspace_bytes(T)
+    def fill_workspace_bytes(self, T: int, cache: Optional[KVCache] = None) -> int:
+        """Workspace of ``fill`` on T tokens (0: a form it is not built for)
+        into the cache (None: a bf16 one)."""
+        parts = qgemm_workspace_bytes(self.w.fc, T, 2 * self.hidden), self.w.attn.prompt_workspace_bytes(T, cache)
         return max(parts) if all(parts) else 0
 
     def fill(self, hidden: torch.Tensor, tokens: torch.Tensor, cache: KVCache, stream=None,
@@ -124,9 +125,10 @@ class MTPLayer:
 
 
 class MTPDrafter:
-    def __init__(self, mtp: MTPLayer, max_len: int):
+    def __init__(self, mtp: MTPLayer, max_len: int, *, kv_bits: int = 16):
+        """kv_bits=8: the MTP layer's cache is a KVCache8."""
         self.mtp = mtp
-        self.cache = mtp.w.attn.new_cache(max_len)
+        self.cache = mtp.w.attn.new_cache(max_len, kv_bits)
 
     def draft(self, H_last: torch.Tensor, x_tok: torch.Tensor, K: int) -> torch.Tensor:
         """K greedy drafts (int32 [K] on the device) from the main model's last
