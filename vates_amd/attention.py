@@ -217,9 +217,11 @@ class KVCache8(KVCache):
         if not 0 <= start <= stop <= self.max_len:
             raise VmiError(f"positions {start}..{stop} outside the capacity {self.max_len}")
         dev = _on_current(self.data)
-        with torch.cuda.stream(stream):
-            k, v = (torch.empty((self.n_kv, stop - start, 256), dtype=dtype, device=dev) if want else None
-                    for want in (want_k, want_v))
+        k = v = None
+        if want_k:
+            k = _new((self.n_kv, stop - start, 256), dtype, dev, stream)
+        if want_v:
+            v = _new((self.n_kv, stop - start, 256), dtype, dev, stream)
         if stop > start:
             check(load().vmi_kv8_read(self.data.data_ptr(), self.n_kv, self.max_len, start, stop - start, _ptr(k),
                                       _ptr(v), VMI_F32 if dtype is torch.float32 else VMI_BF16, _stream_handle(stream)),
@@ -241,6 +243,14 @@ class KVCache8(KVCache):
             check(load().vmi_kv8_write(keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(),
                                        values.stride(0), values.stride(1), self.n_kv, start, n, self.data.data_ptr(),
                                        self.max_len, _stream_handle(stream)), "vmi_kv8_write")
+
+
+def _new(shape, dtype: torch.dtype, dev, stream) -> torch.Tensor:
+    """An output of a call on `stream`: allocated in that stream's order."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=dev)
 
 
 def _on_current(t: torch.Tensor) -> torch.device:
@@ -285,8 +295,7 @@ def norm_rope_append(qkv: torch.Tensor, cache: KVCache8, q_norm: torch.Tensor, k
     T = qkv.shape[0]
     pos = _position(cache, T, pos0, pos_device, dev)
     if out is None:
-        with torch.cuda.stream(stream):
-            out = torch.empty((T, n_heads, 256), dtype=torch.bfloat16, device=dev)
+        out = _new((T, n_heads, 256), torch.bfloat16, dev, stream)
     else:
         _rows_bf16(out, "out", (T, n_heads, 256), dev)
     if T:
@@ -324,8 +333,7 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
                              gate.stride(2) != 1):
         raise VmiError(f"gate must be float32 {list(q.shape)} on {dev} with contiguous rows")
     if out is None:
-        with torch.cuda.stream(stream):
-            out = torch.empty_like(q)
+        out = _new(q.shape, torch.bfloat16, dev, stream)
     else:
         _rows_bf16(out, "out", (T, n_heads, 256), dev)
     if T:
@@ -378,8 +386,7 @@ class AttentionLayer:
         _rows_bf16(x, "x", (T, self.hidden), dev)
         pos = _position(cache, span, pos0, pos_device, dev)
         if out is None:
-            with torch.cuda.stream(stream):
-                out = torch.empty_like(x)
+            out = _new(x.shape, torch.bfloat16, dev, stream)
         else:
             _rows_bf16(out, "out", (T, self.hidden), dev)
         lib = load()

@@ -324,55 +324,76 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
 // --------------------------------------------------------------- attention
 using vmi::Kv8Attn;
 
-// Eight codes + 128 as fp16 1024 + (c + 128), exactly (0x6400 is 1024 with a
-// mantissa step of 1): one byte permute per pair.
+// Eight codes + 128 as fp16 subnormals (c + 128) 2^-24, exactly: one byte
+// permute per pair.  The matrix instructions take subnormals as they are.
 __device__ __forceinline__ vmi_u4 kv8_widen(uint32_t w0, uint32_t w1) {
     vmi_u4 r;
-    r[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
-    r[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u);
-    r[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u);
-    r[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u);
+    r[0] = __builtin_amdgcn_perm(0u, w0, 0x0c010c00u);
+    r[1] = __builtin_amdgcn_perm(0u, w0, 0x0c030c02u);
+    r[2] = __builtin_amdgcn_perm(0u, w1, 0x0c010c00u);
+    r[3] = __builtin_amdgcn_perm(0u, w1, 0x0c030c02u);
     return r;
 }
-// The codes themselves (1152 taken off again, exact).
+// The codes themselves, c 2^-24 (exact).
 __device__ __forceinline__ vmi_u4 kv8_signed(const vmi_u4& u) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const h2 off = {(_Float16)(-0x1p-17f), (_Float16)(-0x1p-17f)};
     vmi_u4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (uint32_t)u[i]) + off);
     return r;
 }
+__device__ __forceinline__ uint32_t kv8_pack_f16(float a, float b) {  // one conversion of both, to nearest even
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+}
 
-constexpr float kPScale = 16384.0f;   // probabilities times value scales, in fp16: at most this
+// Lane l and lane l ^ 32 (l ^ 16): both lanes' values, the lower lane's first.
+__device__ __forceinline__ float2 kv8_pair32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float2 kv8_pair16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float kv8_max32(float v) {
+    const float2 p = kv8_pair32(v);
+    return fmaxf(p.x, p.y);
+}
+__device__ __forceinline__ float kv8_max16(float v) {
+    const float2 p = kv8_pair16(v);
+    return fmaxf(p.x, p.y);
+}
+__device__ __forceinline__ float kv8_sum32(float v) {
+    const float2 p = kv8_pair32(v);
+    return p.x + p.y;
+}
+__device__ __forceinline__ float kv8_sum16(float v) {
+    const float2 p = kv8_pair16(v);
+    return p.x + p.y;
+}
+
+// A query row's power of two f, max |q| f in (2^13, 2^14]: elements down to
+// 2^-28 of the largest keep their eight bits in fp16.  Rows of magnitudes
+// outside 2^-100 .. 2^100 take the nearest factor.
+__device__ __forceinline__ float kv8_query_scale(float amax) {
+    return vmi_fp16_range_scale(fminf(fmaxf(amax, amax > 0.0f ? 0x1p-100f : 0.0f), 0x1p100f));
+}
+constexpr float kScoreUnit = 0.09016844005556021f * 0x1p24f;  // log2(e) / sqrt(256), codes in units of 2^-24
+
+constexpr float kPScale = 16384.0f;            // probabilities times value scales, in fp16: at most this
+constexpr float kSumUnit = 0x1p24f / kPScale;  // of their products' sums, codes in units of 2^-24
 constexpr float kMinRef = 1e-30f;
 
 // 16 MS query rows of a wave: lane (nl, q4) belongs to row 16 m + nl.
 template <int MS>
 struct Kv8Rows {
     vmi_u4 q[MS][8];   // fp16 query times a power of two, dims 32 kk + 8 q4 ..
-    float c0[MS];      // -1152 sum(q): what the codes' offset of 1152 adds to a score, taken off
-    float cx[MS];      // log2(e) / 16 over the power of two; NaN for a row that is not finite
+    float cx[MS];      // score unit over the power of two; NaN for a row that is not finite
     int last[MS];      // last visible position
-};
-
-// Running softmax of those rows.  o is in units of s / kPScale.
-template <int MS>
-struct Kv8Sums {
-    vmi_f4 o[MS][16];  // dims 16 dt + 4 q4 + r of row nl
-    float m[MS];       // maximum score, in powers of two
-    float l[MS];       // the lane's share of sum 2^(score - m)
-    float s[MS];       // largest value scale seen
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < MS; ++i) {
-            m[i] = -3.402823466e38f;
-            l[i] = 0.0f;
-            s[i] = kMinRef;
-#pragma unroll
-            for (int d = 0; d < 16; ++d) o[i][d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
-        }
-    }
 };
 
 // The wave's query rows, from row r0 of R (rows behind the last repeat it).
@@ -397,90 +418,175 @@ __device__ __forceinline__ void kv8_load_rows(const Kv8Attn& a, const uint16_t* 
             for (int i = 0; i < 4; ++i) am = max(am, max(o.q[m][kk][i] & 0x7fffu, (o.q[m][kk][i] >> 16) & 0x7fffu));
         am = max(am, (uint32_t)__shfl_xor((int)am, 16));
         am = max(am, (uint32_t)__shfl_xor((int)am, 32));
-        const float amax = __uint_as_float(am << 16);
-        // max |q| f in (2^13, 2^14]: the products of a finite row stay finite, and elements
-        // down to 2^-28 of the largest keep their eight bits
-        const bool fin = amax < INFINITY;
-        const float f = vmi_fp16_range_scale(amax);
-        float sum = 0.0f;
+        const float amax = __uint_as_float(am << 16), f = kv8_query_scale(amax);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t u = o.q[m][kk][i];
-                const _Float16 lo = (_Float16)(__uint_as_float(u << 16) * f), hi = (_Float16)(__uint_as_float(u & 0xffff0000u) * f);
-                sum += (float)lo;
-                sum += (float)hi;
-                o.q[m][kk][i] = vmi_h2_bits(lo, hi);
+                o.q[m][kk][i] = kv8_pack_f16(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f);
             }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        o.c0[m] = -1152.0f * sum;
-        o.cx[m] = fin ? 0.09016844005556021f / f : __builtin_nanf("");   // log2(e) / sqrt(256)
+        o.cx[m] = amax < 0x1p100f ? kScoreUnit / f : __builtin_nanf("");
     }
 }
 
-// One record's 32 keys, the first at position p0.  S^T = K Q^T: a lane holds
-// the scores of keys 8 q4 + e of its row, which are, as probabilities, already
-// the B operand of O^T = V^T P^T.  A key's scale enters its score, a value's its
-// probability; the product goes to fp16 (11 bits) relative to the row's largest
-// value scale so far, and whatever raises that or the running maximum rescales
-// the sums.  mask (wave-uniform): the record reaches past the visible positions
-// of some row; masked scores count as minus infinity and masked scales as zero,
-// so that nothing stored behind a row's last position reaches it.
-template <int MS>
-__device__ __forceinline__ void kv8_step(const uint8_t* rec, const Kv8Rows<MS>& Q, int p0, bool mask, Kv8Sums<MS>& S) {
-    const int lane = threadIdx.x & 63, q4 = lane >> 4;
-    const vmi_u4* K = reinterpret_cast<const vmi_u4*>(rec);
-    const vmi_u4* V = reinterpret_cast<const vmi_u4*>(rec + kHalfRec);
-    const vmi_f4* sc = reinterpret_cast<const vmi_f4*>(rec + 2 * kHalfRec + 32 * q4);
-    vmi_f4 s[MS][2];
+// A record in a wave's registers: lane (nl, q4) holds the keys 8 (nl>>2) + 4 a +
+// (nl&3) and the values of positions 8 q4 .., as they are stored.
+struct Kv8Rec {
+    vmi_u4 k[8], v[8];   // key operands 2 j, 2 j + 1 of tile a at 4 a + j; value operands 2 j, 2 j + 1 at j
+    vmi_f4 ks[2], vs[2]; // scales of positions 8 q4 ..
+};
+
+// Record b of a kv head, or nothing where there is none (zeros, and no memory
+// read): the loads take no branch, so that every wait counts only what it needs.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv8_rsrc(const uint8_t* head, int b, bool present) {
+    return vmi_rsrc(head + (size_t)b * kRec, present ? kRec : 0);
+}
+// ONCE: one workgroup alone reads the record (nontemporal); else another row tile's
+// reads it too.
+template <bool ONCE>
+__device__ __forceinline__ vmi_u4 kv8_bload(__amdgpu_buffer_rsrc_t rs, int at, int base) {
+    return ONCE ? vmi_bload_b128_nt(rs, (uint32_t)at, base) : vmi_bload_b128(rs, (uint32_t)at, base);
+}
+template <bool ONCE>
+__device__ __forceinline__ void kv8_load_keys(Kv8Rec& r, __amdgpu_buffer_rsrc_t rs) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int m = 0; m < MS; ++m) s[m][0] = s[m][1] = vmi_f4{Q.c0[m], Q.c0[m], Q.c0[m], Q.c0[m]};
+    for (int j = 0; j < 8; ++j) r.k[j] = kv8_bload<ONCE>(rs, 16 * lane, 1024 * j);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        r.ks[j] = __builtin_bit_cast(vmi_f4, kv8_bload<ONCE>(rs, 2 * kHalfRec + 32 * (lane >> 4) + 16 * j, 0));
+}
+template <bool ONCE>
+__device__ __forceinline__ void kv8_load_values(Kv8Rec& r, __amdgpu_buffer_rsrc_t rs) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        r.vs[j] = __builtin_bit_cast(vmi_f4, kv8_bload<ONCE>(rs, 2 * kHalfRec + 128 + 32 * (lane >> 4) + 16 * j, 0));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = kv8_bload<ONCE>(rs, 16 * lane, kHalfRec + 1024 * j);
+}
+
+// Position kt of the record from a tree token's row.
+__device__ __forceinline__ void kv8_insert(Kv8Rec& r, const uint8_t* row, int kt) {
+    const int lane = threadIdx.x & 63, nl = lane & 15, q4 = lane >> 4, e = kt & 7;
+    const bool mine = nl == 4 * (kt >> 3) + (kt & 3), at = q4 == kt >> 3;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        const uint2 lo = *reinterpret_cast<const uint2*>(row + 64 * j + 8 * q4);
+        const uint2 hi = *reinterpret_cast<const uint2*>(row + 64 * j + 32 + 8 * q4);
+        const vmi_u4 u = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const vmi_u4 u = K[(4 * a + j) * 64 + lane];
-            const vmi_u4 k0 = kv8_widen(u[0], u[1]), k1 = kv8_widen(u[2], u[3]);
+        for (int a = 0; a < 2; ++a)
+            if (mine && ((kt >> 2) & 1) == a) r.k[4 * a + j] = u;
+    }
+    const float2 sc = *reinterpret_cast<const float2*>(row + 2 * kHeadDim);
+    const uint32_t keep = ~(0xffu << (8 * (e & 3)));
 #pragma unroll
-            for (int m = 0; m < MS; ++m) s[m][a] = vmi_mfma_f16(k0, Q.q[m][2 * j], s[m][a]);
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t lo = (uint32_t)row[kHeadDim + 32 * j + nl] << (8 * (e & 3));
+        const uint32_t hi = (uint32_t)row[kHeadDim + 32 * j + 16 + nl] << (8 * (e & 3));
 #pragma unroll
-            for (int m = 0; m < MS; ++m) s[m][a] = vmi_mfma_f16(k1, Q.q[m][2 * j + 1], s[m][a]);
+        for (int i = 0; i < 2; ++i)
+            if (at && (e >> 2) == i) {
+                r.v[j][i] = (r.v[j][i] & keep) | lo;
+                r.v[j][2 + i] = (r.v[j][2 + i] & keep) | hi;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (at && i == e) {
+            r.ks[i >> 2][i & 3] = sc.x;
+            r.vs[i >> 2][i & 3] = sc.y;
+        }
+}
+
+// Running softmax of a wave's 16 MS rows.  o is in units of s kSumUnit.
+template <int MS>
+struct Kv8Sums {
+    vmi_f4 o[MS][16];  // dims 16 dt + 4 q4 + r of row 16 m + nl
+    float m[MS];       // maximum score, in powers of two
+    float l[MS];       // the lane's share of sum 2^(score - m)
+    float s[MS];       // largest value scale seen
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < MS; ++i) {
+            m[i] = -3.402823466e38f;
+            l[i] = 0.0f;
+            s[i] = kMinRef;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) o[i][d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    const vmi_f4 ks[2] = {sc[0], sc[1]}, vs[2] = {sc[8], sc[9]};
+};
+
+// One record's 32 keys, the first at position p0, against the rows q (fp16
+// operands in LDS).  S^T = K Q^T: a lane holds the scores of keys 8 q4 + e of its
+// row, which are, as probabilities, already the B operand of O^T = V^T P^T.  A
+// key's scale enters its score, a value's its probability; the product goes to fp16
+// (11 bits) relative to the row's largest value scale so far, and whatever raises
+// that or the running maximum rescales the sums.  mask (wave-uniform): the record
+// reaches past the visible positions of some row; masked scores count as minus
+// infinity and masked scales as zero, so that nothing stored behind a row's last
+// position reaches it.  The next record's keys are asked for once these are used,
+// its values at the end.
+template <int MS, bool ONCE>
+__device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const float (&cx)[MS], const int (&last)[MS], int p0,
+                                         bool mask, __amdgpu_buffer_rsrc_t next, Kv8Sums<MS>& S) {
+    const int lane = threadIdx.x & 63, q4 = lane >> 4;
+    vmi_f4 s[MS][2];
+#pragma unroll
+    for (int m = 0; m < MS; ++m) s[m][0] = s[m][1] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        vmi_u4 qr[MS][2];
+#pragma unroll
+        for (int m = 0; m < MS; ++m) {
+            qr[m][0] = q[(8 * m + 2 * j) * 64 + lane];
+            qr[m][1] = q[(8 * m + 2 * j + 1) * 64 + lane];
+        }
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const vmi_u4 u = rec.k[4 * a + j];
+            const vmi_u4 k0 = kv8_signed(kv8_widen(u[0], u[1])), k1 = kv8_signed(kv8_widen(u[2], u[3]));
+#pragma unroll
+            for (int m = 0; m < MS; ++m) s[m][a] = vmi_mfma_f16(k0, qr[m][0], s[m][a]);
+#pragma unroll
+            for (int m = 0; m < MS; ++m) s[m][a] = vmi_mfma_f16(k1, qr[m][1], s[m][a]);
+        }
+    }
+    float x[MS][8];
+#pragma unroll
+    for (int m = 0; m < MS; ++m)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[m][e] = s[m][e >> 2][e & 3] * (rec.ks[e >> 2][e & 3] * cx[m]);
+    kv8_load_keys<ONCE>(rec, next);
     vmi_u4 pb[MS];
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
-        float x[8], v[8];
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[e] = s[m][e >> 2][e & 3] * (ks[e >> 2][e & 3] * Q.cx[m]);
-            v[e] = vs[e >> 2][e & 3];
-        }
+        for (int e = 0; e < 8; ++e) v[e] = rec.vs[e >> 2][e & 3];
         if (mask) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const bool seen = p0 + 8 * q4 + e <= Q.last[m];
-                x[e] = seen ? x[e] : -INFINITY;
+                const bool seen = p0 + 8 * q4 + e <= last[m];
+                x[m][e] = seen ? x[m][e] : -INFINITY;
                 v[e] = seen ? v[e] : 0.0f;
             }
         }
         float nm = S.m[m], ns = S.s[m];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            nm = fmaxf(nm, x[e]);
+            nm = fmaxf(nm, x[m][e]);
             ns = fmaxf(ns, v[e]);
         }
-        nm = fmaxf(nm, __shfl_xor(nm, 16));
-        ns = fmaxf(ns, __shfl_xor(ns, 16));
-        nm = fmaxf(nm, __shfl_xor(nm, 32));
-        ns = fmaxf(ns, __shfl_xor(ns, 32));
+        nm = kv8_max32(kv8_max16(nm));
+        ns = kv8_max32(kv8_max16(ns));
         if (__any(nm > S.m[m] || ns > S.s[m])) {
             const float f = __builtin_amdgcn_exp2f(S.m[m] - nm);
             S.l[m] *= f;
-            const float fo = ns > S.s[m] ? f * (S.s[m] / ns) : f;
+            const float fo = ns > S.s[m] ? f * (S.s[m] * __builtin_amdgcn_rcpf(ns)) : f;
 #pragma unroll
             for (int d = 0; d < 16; ++d)
 #pragma unroll
@@ -488,265 +594,507 @@ __device__ __forceinline__ void kv8_step(const uint8_t* rec, const Kv8Rows<MS>& 
             S.m[m] = nm;
             S.s[m] = ns;
         }
-        const float inv = kPScale / ns;
-        float p[8];
+        const float inv = kPScale * __builtin_amdgcn_rcpf(ns);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(x[e] - nm);
-            S.l[m] += p[e];
-            p[e] *= v[e] * inv;
+            x[m][e] = __builtin_amdgcn_exp2f(x[m][e] - nm);
+            S.l[m] += x[m][e];
+            x[m][e] *= v[e] * inv;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pb[m][i] = vmi_h2_bits((_Float16)p[2 * i], (_Float16)p[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) pb[m][i] = kv8_pack_f16(x[m][2 * i], x[m][2 * i + 1]);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const vmi_u4 u = V[j * 64 + lane];
+        const vmi_u4 u = rec.v[j];
         const vmi_u4 v0 = kv8_signed(kv8_widen(u[0], u[1])), v1 = kv8_signed(kv8_widen(u[2], u[3]));
 #pragma unroll
         for (int m = 0; m < MS; ++m) S.o[m][2 * j] = vmi_mfma_f16(v0, pb[m], S.o[m][2 * j]);
 #pragma unroll
         for (int m = 0; m < MS; ++m) S.o[m][2 * j + 1] = vmi_mfma_f16(v1, pb[m], S.o[m][2 * j + 1]);
     }
+    kv8_load_values<ONCE>(rec, next);
 }
 
-// A record by DMA into a wave's LDS, 17 operations.
-constexpr int kRecOps = 17;
-__device__ __forceinline__ void kv8_fetch(const uint8_t* rec, uint8_t* lds) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) vmi_lds_dma16_opaque_nt(rec + 1024 * j + 16 * lane, lds + 1024 * j);
-    vmi_lds_dma4_opaque(rec + 2 * kHalfRec + 4 * lane, lds + 2 * kHalfRec);
-}
-
-// Waits for the wave's own LDS reads, before a slot that they read is refilled.
+// Waits for the wave's own LDS operations.
 __device__ __forceinline__ void kv8_lds_wait() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt 0
     asm volatile("" ::: "memory");
 }
 
-constexpr int kRing = 2;  // records of a wave's ring
+// Parts go out nontemporal: left in the XCDs' L2 they would be written back at the
+// kernel's end, before the merge can start (four tokens at 4000: 14.1 -> 11.9 us).
+__device__ __forceinline__ void kv8_store_part(__amdgpu_buffer_rsrc_t ro, int row, int d, const vmi_f4& y) {
+    vmi_bstore_b128_nt(__builtin_bit_cast(vmi_u4, y), ro, (uint32_t)(row * kHeadDim + d) * 4u, 0);
+}
 
-// grid (S, n_kv, paths): record b of a kv head belongs to wave (b / S) % 4 of
-// workgroup b % S, whatever the length, the batch and the capacity, so that a
-// row's sums do not depend on them, a short cache still spreads over the device,
-// and a long one keeps every CU reading.  A wave runs its records through its
-// own ring in LDS (no barrier until the end); the four waves then join in LDS
-// and the workgroup writes one part: maximum, sum and unnormalised output of
-// each row, in fp32.  Bound by the bytes of the cache from some ten thousand
-// positions on, below by the latency of a record and of the two launches.
-template <int MS>
-__global__ __launch_bounds__(kThreads, 1) void k_kv8_split(Kv8Attn a) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_ring[kWaves][kRing][kRec];
-    __shared__ float s_ml[kWaves][16 * MS][2];
+constexpr int kSplitWaves = 4, kSplitThreads = 64 * kSplitWaves;
+
+// grid (S, n_kv, paths * row tiles): record b of a kv head belongs to wave
+// (b / S) % 8 of workgroup b % S, whatever the length, the batch and the capacity,
+// so that a row's sums do not depend on them, a short cache still spreads over the
+// device, and a long one keeps every CU reading.  The workgroup forms the rows'
+// fp16 operands in LDS; a wave then works through its records in registers, two
+// waves a SIMD (one alone issues an instruction every six cycles), without a barrier
+// until the end, where the waves join in LDS and the workgroup writes one part:
+// maximum, sum and unnormalised output of each row, in fp32.  Bound by the bytes of
+// the cache from some ten thousand positions on, below by the latency of a record
+// and of the two launches.
+template <int MS, bool ONCE>
+__global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv8Attn a) {
+    __shared__ __attribute__((aligned(16))) float s_o[kSplitWaves * 16 * kHeadDim];   // one row group of each wave
+    __shared__ vmi_u4 s_q[MS * 8 * 64];
+    __shared__ float s_cx[16 * MS], s_ml[kSplitWaves][16 * MS][2];
     const int lane = threadIdx.x & 63, w = at_wave(), nl = lane & 15, q4 = lane >> 4;
-    const int wg = blockIdx.x, S = gridDim.x, g = blockIdx.y, path = blockIdx.z, T = a.span;
+    const int wg = blockIdx.x, S = gridDim.x, g = blockIdx.y, path = blockIdx.z % a.paths, T = a.span;
+    const int rz = 16 * MS * (blockIdx.z / a.paths);   // the workgroup's first row
     const int pos0 = kv8_pos0(a.pos0, a.pos_dev, T, a.max_len);
-    if (a.pos_dev && a.status && wg == 0 && g == 0 && path == 0 && threadIdx.x == 0 && *a.pos_dev != pos0)
+    if (a.pos_dev && a.status && wg == 0 && g == 0 && blockIdx.z == 0 && threadIdx.x == 0 && *a.pos_dev != pos0)
         atomicOr(a.status, VMI_STATUS_BAD_POS);
     const int nblk = (pos0 + T + kBlk - 1) / kBlk;
     if (wg >= nblk) return;   // whole workgroup
-    const int R = T * (a.n_heads / a.n_kv), step = kWaves * S, first = wg + S * w;
+    const int G = a.n_heads / a.n_kv, R = T * G, step = kSplitWaves * S, first = wg + S * w;
     const uint8_t* head = a.cache + (size_t)g * (a.max_len / kBlk) * kRec;
-    Kv8Rows<MS> Q;
-    kv8_load_rows<MS>(a, a.q + (size_t)path * T * a.n_heads * kHeadDim, g, 0, R, pos0, Q);
-    if (first < nblk) kv8_fetch(head + (size_t)first * kRec, s_ring[w][0]);
-    if (first + step < nblk) kv8_fetch(head + (size_t)(first + step) * kRec, s_ring[w][1]);
+    // rows 2 NQ w .. of the group, 32 lanes each, then the wave's first record
+    constexpr int NQ = 16 * MS / (2 * kSplitWaves);
+    vmi_u4 qv[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int row = min(rz + 2 * (NQ * w + i) + (lane >> 5), R - 1), t = row / G;
+        qv[i] = *reinterpret_cast<const vmi_u4*>(a.q + ((size_t)(path * T + t) * a.n_heads + g * G + row % G) * kHeadDim +
+                                                 8 * (lane & 31));
+    }
+    // a CU returns loads in the order they were issued: every wave's rows before any wave's record
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Kv8Rec rec;
+    {
+        const __amdgpu_buffer_rsrc_t rs = kv8_rsrc(head, first, first < nblk);
+        kv8_load_keys<ONCE>(rec, rs);
+        kv8_load_values<ONCE>(rec, rs);
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        uint32_t am = 0;   // largest magnitude, as bf16 bits
+#pragma unroll
+        for (int e = 0; e < 4; ++e) am = max(am, max(qv[i][e] & 0x7fffu, (qv[i][e] >> 16) & 0x7fffu));
+        am = max(am, vmi_dpp_u32<VMI_DPP_XOR1>(am));
+        am = max(am, vmi_dpp_u32<VMI_DPP_XOR2>(am));
+        am = max(am, vmi_dpp_u32<VMI_DPP_HALF_MIRROR>(am));
+        am = max(am, vmi_dpp_u32<VMI_DPP_MIRROR>(am));
+        {
+            const auto pr = __builtin_amdgcn_permlane16_swap(am, am, false, false);
+            am = max((uint32_t)pr[0], (uint32_t)pr[1]);
+        }
+        const float amax = __uint_as_float(am << 16), f = kv8_query_scale(amax);
+        vmi_u4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            h[e] = kv8_pack_f16(__uint_as_float(qv[i][e] << 16) * f, __uint_as_float(qv[i][e] & 0xffff0000u) * f);
+        const int r = 2 * (NQ * w + i) + (lane >> 5), d8 = lane & 31;   // row of the group, dims 8 d8 ..
+        s_q[(8 * (r >> 4) + (d8 >> 2)) * 64 + (d8 & 3) * 16 + (r & 15)] = h;
+        if (d8 == 0) s_cx[r] = amax < 0x1p100f ? kScoreUnit / f : __builtin_nanf("");
+    }
+    kv8_lds_wait();
+    __builtin_amdgcn_s_barrier();   // (not __syncthreads, which would wait for the records too)
+    asm volatile("" ::: "memory");
+    float cx[MS];
+    int last[MS];
+#pragma unroll
+    for (int m = 0; m < MS; ++m) {
+        cx[m] = s_cx[16 * m + nl];
+        last[m] = pos0 + min(rz + 16 * m + nl, R - 1) / G;
+    }
     Kv8Sums<MS> Y;
     Y.clear();
-    int slot = 0;
+#pragma unroll 1
     for (int b = first; b < nblk; b += step) {
-        if (b + step < nblk)
-            vmi_vm_wait_c<kRecOps>();   // the next record may be in flight
-        else
-            vmi_vm_wait_c<0>();
-        asm volatile("" ::: "memory");
-        uint8_t* rec = s_ring[w][slot];
+        asm volatile("" ::: "memory");   // the rows' operands stay in LDS: they would take the records' registers
         if (a.tree && kBlk * b + kBlk > pos0) {
             // a path's own tokens in place of what the cache holds there
-            for (int t = max(kBlk * b - pos0, 0); t < min(T, kBlk * b + kBlk - pos0); ++t) {
-                const uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * T + t) * kKv8TreeRow;
-                const int kt = pos0 + t - kBlk * b;
-                const uint32_t kc = *reinterpret_cast<const uint32_t*>(side + 4 * lane);
-                const uint32_t vc = *reinterpret_cast<const uint32_t*>(side + kHeadDim + 4 * lane);
-                *reinterpret_cast<uint32_t*>(rec + kv8_k_off(kt, 4 * lane)) = kc;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) rec[kv8_v_off(kt, 4 * lane + j)] = (uint8_t)(vc >> (8 * j));
-                if (lane < 2)
-                    *reinterpret_cast<float*>(rec + kv8_scale_off(kt, lane)) =
-                        *reinterpret_cast<const float*>(side + 2 * kHeadDim + 4 * lane);
-            }
-            kv8_lds_wait();
+            for (int t = max(kBlk * b - pos0, 0); t < min(T, kBlk * b + kBlk - pos0); ++t)
+                kv8_insert(rec, a.tree + ((size_t)(path * a.n_kv + g) * T + t) * kKv8TreeRow, pos0 + t - kBlk * b);
         }
-        kv8_step<MS>(rec, Q, kBlk * b, kBlk * b + kBlk - 1 > pos0, Y);
-        kv8_lds_wait();
-        if (b + kRing * step < nblk) kv8_fetch(head + (size_t)(b + kRing * step) * kRec, s_ring[w][slot]);
-        slot ^= 1;
+        kv8_step<MS, ONCE>(rec, s_q, cx, last, kBlk * b, kBlk * b + kBlk - 1 > pos0, kv8_rsrc(head, b + step, b + step < nblk), Y);
     }
-    // the four waves, in wave order
-    float* s_o = reinterpret_cast<float*>(&s_ring[0][0][0]);   // [waves][16][256], one row group at a time
-    static_assert(kWaves * 16 * kHeadDim * 4 <= (int)sizeof(s_ring), "row group");
+    const size_t part = ((size_t)(g * S + wg) * a.paths + path) * a.rp;
+    const __amdgpu_buffer_rsrc_t ro = vmi_rsrc(a.part_o + part * kHeadDim, (uint32_t)R * kHeadDim * 4);
+    float l[MS];
 #pragma unroll
-    for (int m = 0; m < MS; ++m) {
-        float l = Y.l[m];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+    for (int m = 0; m < MS; ++m) l[m] = kv8_sum32(kv8_sum16(Y.l[m]));
+    const int active = min(kSplitWaves, (nblk - wg + S - 1) / S);   // waves that had a record
+    if (active == 1) {   // the first one's sums are the part
+        if (w) return;
+#pragma unroll
+        for (int m = 0; m < MS; ++m) {
+            const int row = rz + 16 * m + nl;
+            if (row >= R) continue;
+            const float u = Y.s[m] * kSumUnit;
+#pragma unroll
+            for (int d = 0; d < 16; ++d)
+                kv8_store_part(ro, row, 16 * d + 4 * q4,
+                               vmi_f4{Y.o[m][d][0] * u, Y.o[m][d][1] * u, Y.o[m][d][2] * u, Y.o[m][d][3] * u});
+            if (q4 == 0) *reinterpret_cast<float2*>(a.part_ml + (part + row) * 2) = make_float2(Y.m[m], l[m]);
+        }
+        return;
+    }
+    // the waves in order: each brings its sums to the workgroup's maximum, a thread adds four dims of
+    // four rows
+#pragma unroll
+    for (int m = 0; m < MS; ++m)
         if (q4 == 0) {
             s_ml[w][16 * m + nl][0] = Y.m[m];
-            s_ml[w][16 * m + nl][1] = l;
+            s_ml[w][16 * m + nl][1] = l[m];
         }
-    }
-    const size_t part = ((size_t)(g * S + wg) * gridDim.z + path) * a.rp;
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
-        __syncthreads();   // every wave is done with its ring, or with the group before
-        const float u = Y.s[m] * (1.0f / kPScale);
+        if (m) __syncthreads();   // the group before is read
+        float M = s_ml[0][16 * m + nl][0];
 #pragma unroll
-        for (int d = 0; d < 16; ++d) {
-            const vmi_f4 y = {Y.o[m][d][0] * u, Y.o[m][d][1] * u, Y.o[m][d][2] * u, Y.o[m][d][3] * u};
-            *reinterpret_cast<vmi_f4*>(s_o + (w * 16 + nl) * kHeadDim + 4 * ((4 * d + q4) ^ nl)) = y;
+        for (int v = 1; v < kSplitWaves; ++v) M = fmaxf(M, s_ml[v][16 * m + nl][0]);
+        if (w < active) {
+            const float u = Y.s[m] * kSumUnit * __builtin_amdgcn_exp2f(Y.m[m] - M);
+#pragma unroll
+            for (int d = 0; d < 16; ++d)
+                *reinterpret_cast<vmi_f4*>(s_o + (w * 16 + nl) * kHeadDim + 4 * ((4 * d + q4) ^ nl)) =
+                    vmi_f4{Y.o[m][d][0] * u, Y.o[m][d][1] * u, Y.o[m][d][2] * u, Y.o[m][d][3] * u};
+        }
+        if (w == 0 && q4 == 0 && rz + 16 * m + nl < R) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kSplitWaves; ++v)
+                sum = fmaf(s_ml[v][16 * m + nl][1], __builtin_amdgcn_exp2f(s_ml[v][16 * m + nl][0] - M), sum);
+            *reinterpret_cast<float2*>(a.part_ml + (part + rz + 16 * m + nl) * 2) = make_float2(M, sum);
         }
         __syncthreads();
-        for (int r = w; r < 16; r += kWaves) {   // a wave per row, 4 dims a lane
-            const int row = 16 * m + r;
-            if (row >= R) break;
-            float M = s_ml[0][row][0];
+        vmi_f4 y[16 / kSplitWaves];
 #pragma unroll
-            for (int v = 1; v < kWaves; ++v) M = fmaxf(M, s_ml[v][row][0]);
-            float l = 0.0f;
-            vmi_f4 y = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 16 / kSplitWaves; ++i) {
+            const int r = w + kSplitWaves * i;
+            y[i] = *reinterpret_cast<const vmi_f4*>(s_o + r * kHeadDim + 4 * (lane ^ r));
+        }
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) {
-                const float f = __builtin_amdgcn_exp2f(s_ml[v][row][0] - M);
-                l = fmaf(s_ml[v][row][1], f, l);
+        for (int v = 1; v < kSplitWaves; ++v) {
+            if (v >= active) break;
+#pragma unroll
+            for (int i = 0; i < 16 / kSplitWaves; ++i) {
+                const int r = w + kSplitWaves * i;
                 const vmi_f4 z = *reinterpret_cast<const vmi_f4*>(s_o + (v * 16 + r) * kHeadDim + 4 * (lane ^ r));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = fmaf(z[e], f, y[e]);
+                for (int e = 0; e < 4; ++e) y[i][e] += z[e];
             }
-            *reinterpret_cast<vmi_f4*>(a.part_o + (part + row) * kHeadDim + 4 * lane) = y;
-            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + (part + row) * 2) = make_float2(M, l);
+        }
+#pragma unroll
+        for (int i = 0; i < 16 / kSplitWaves; ++i) {
+            const int row = rz + 16 * m + w + kSplitWaves * i;
+            if (row < R) kv8_store_part(ro, row, 4 * lane, y[i]);
         }
     }
 }
 
-__device__ __forceinline__ uint2 kv8_gated(const vmi_f4& y, float l, const float* gate) {
+// Four outputs y / l, times sigmoid(gate): reciprocals and exp2 of the hardware,
+// within 2^-21 of the exact ones.
+__device__ __forceinline__ uint2 kv8_gated(const vmi_f4& y, float inv_l, const float* gate) {
     float o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = y[e] / l;
+    for (int e = 0; e < 4; ++e) o[e] = y[e] * inv_l;
     if (gate) {
         const vmi_f4 z = *reinterpret_cast<const vmi_f4*>(gate);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] /= 1.0f + expf(-z[e]);
+        for (int e = 0; e < 4; ++e)
+            o[e] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[e] * -1.44269504088896341f));
     }
     return make_uint2(vmi_pack_bf16x2(o[0], o[1]), vmi_pack_bf16x2(o[2], o[3]));
 }
 
-// grid (rows of all heads), one wave per part in turn: the parts of a row in
-// index order per wave, the four waves in order.  Every row sees position 0, so
-// its sum is positive (or NaN, which it hands on).
-__global__ __launch_bounds__(kThreads) void k_kv8_merge(Kv8Attn a, int parts, bool by_record) {
-    __shared__ float s_m[kWaves], s_l[kWaves];
-    __shared__ vmi_f4 s_o[kWaves][64];
-    const int lane = threadIdx.x & 63, w = at_wave();
+// k_kv8_split's parts, many of few rows.  grid (rows of all heads, 4): a quarter of a row's dims per workgroup.  Part s is
+// added by slot s % 16 in increasing s, the sixteen slots in a fixed order.  Every
+// row sees position 0, so its sum is positive (or NaN, which it hands on).
+constexpr int kMaxParts = 256;
+__global__ __launch_bounds__(kThreads) void k_kv8_merge(Kv8Attn a, int parts) {
+    __shared__ float s_f[kMaxParts], s_red[2][kWaves];
+    __shared__ vmi_f4 s_num[kWaves][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = at_wave();
     const int t = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, G = a.n_heads / a.n_kv, g = h / G;
     const int path = t / a.span, row = (t - path * a.span) * G + h % G;
     const int nblk = (kv8_pos0(a.pos0, a.pos_dev, a.span, a.max_len) + a.span + kBlk - 1) / kBlk;
-    const int n = by_record ? min(parts, nblk) : parts;   // k_kv8_split: the workgroups that had a record
+    const int n = min(parts, nblk);   // the workgroups that had a record
     const size_t at = ((size_t)(g * parts) * a.paths + path) * a.rp + row, inc = (size_t)a.paths * a.rp;
-    float m = -3.402823466e38f, l = 0.0f;
-    vmi_f4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int s = w; s < n; s += kWaves) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at + s * inc) * 2);
-        const vmi_f4 z = *reinterpret_cast<const vmi_f4*>(a.part_o + (at + s * inc) * kHeadDim + 4 * lane);
-        const float nm = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - nm), fz = __builtin_amdgcn_exp2f(ml.x - nm);
-        m = nm;
-        l = fmaf(l, f, ml.y * fz);
+    const int slot = tid >> 4, d0 = 64 * blockIdx.y + 4 * (tid & 15);
+    const float* po = a.part_o + at * kHeadDim + d0;
+    // every part's maximum and sum, and the first eight of this slot's outputs
+    float2 ml = make_float2(-3.402823466e38f, 0.0f);
+    if (tid < n) ml = *reinterpret_cast<const float2*>(a.part_ml + (at + tid * inc) * 2);
+    constexpr int kAhead = 8;
+    vmi_f4 z[kAhead];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], f, z[e] * fz);
+    for (int i = 0; i < kAhead; ++i) {
+        const int s = slot + 16 * i;
+        z[i] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+        if (s < n) z[i] = *reinterpret_cast<const vmi_f4*>(po + s * inc * kHeadDim);
     }
-    s_o[w][lane] = y;
-    if (lane == 0) {
-        s_m[w] = m;
-        s_l[w] = l;
-    }
+    const float* gp = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + d0 : nullptr;
+    const float wm = vmi_wave_max(ml.x);
+    if (lane == 0) s_red[0][w] = wm;
     __syncthreads();
-    if (w) return;
-    float M = s_m[0];
+    const float M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    const float f = __builtin_amdgcn_exp2f(ml.x - M);
+    s_f[tid] = f;
+    const float wl = vmi_wave_sum_canon(ml.y * f);
+    if (lane == 0) s_red[1][w] = wl;
+    __syncthreads();
+    const float l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+    vmi_f4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) M = fmaxf(M, s_m[v]);
-    l = 0.0f;
-    y = vmi_f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-        const float f = __builtin_amdgcn_exp2f(s_m[v] - M);
-        l = fmaf(s_l[v], f, l);
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(z[i][e], s_f[slot + 16 * i], y[e]);
+    for (int s = slot + 16 * kAhead; s < n; s += 16) {
+        const vmi_f4 v = *reinterpret_cast<const vmi_f4*>(po + s * inc * kHeadDim);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = fmaf(s_o[v][lane][e], f, y[e]);
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(v[e], s_f[s], y[e]);
     }
-    const float* gate = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + 4 * lane : nullptr;
-    *reinterpret_cast<uint2*>(a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * lane) = kv8_gated(y, l, gate);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = kv8_sum32(kv8_sum16(y[e]));
+    if (lane < 16) s_num[w][lane] = y;
+    __syncthreads();
+    if (tid >= 16) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (s_num[0][tid][e] + s_num[1][tid][e]) + (s_num[2][tid][e] + s_num[3][tid][e]);
+    *reinterpret_cast<uint2*>(a.o + ((size_t)t * a.n_heads + h) * kHeadDim + d0) = kv8_gated(y, __fdiv_rn(1.0f, l), gp);
 }
 
-// grid (tiles of 64 M rows, n_kv, key parts): four waves of 16 M rows share
-// each record, two slots of LDS by DMA.  Part z of P takes an equal run of the
-// tile's records; with P > 1 the parts are written as k_kv8_split's are.
+// k_kv8_flash's parts, few of many rows: a wave per row, four dims a lane, the parts
+// in order.  A part may hold nothing of a row (its maximum is then the lowest).
+__global__ __launch_bounds__(kThreads) void k_kv8_merge_rows(Kv8Attn a, int parts) {
+    const int lane = threadIdx.x & 63, r = blockIdx.x * kWaves + at_wave();
+    const int t = r / a.n_heads, h = r % a.n_heads, G = a.n_heads / a.n_kv, g = h / G;
+    if (t >= a.span) return;
+    const size_t at = (size_t)g * parts * a.rp + t * G + h % G;
+    float M = -3.402823466e38f, l = 0.0f;
+    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[(at + (size_t)s * a.rp) * 2]);
+    vmi_f4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        const size_t p = at + (size_t)s * a.rp;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
+        const vmi_f4 z = *reinterpret_cast<const vmi_f4*>(a.part_o + p * kHeadDim + 4 * lane);
+        const float f = __builtin_amdgcn_exp2f(ml.x - M);
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(z[e], f, y[e]);
+    }
+    const float* gate = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + 4 * lane : nullptr;
+    *reinterpret_cast<uint2*>(a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * lane) = kv8_gated(y, __fdiv_rn(1.0f, l), gate);
+}
+
+constexpr int kFlashWaves = 8, kFlashThreads = 64 * kFlashWaves;
+
+// Codes of a value record as fp16 integers, exactly (0x6400 is 1024 with a
+// mantissa step of 1), times their positions' factors f.
+__device__ __forceinline__ vmi_u4 kv8_scaled(uint32_t w0, uint32_t w1, const vmi_u4& f) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const uint32_t c[4] = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u),
+                           __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)};
+    vmi_u4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(h2, c[i]) + off) * __builtin_bit_cast(h2, (uint32_t)f[i]));
+    return r;
+}
+
+// Value operands are in units of 2^(E - kValueBits), 2^E the power of two above the
+// record's largest value scale: integers times factors of up to 2^kValueBits.
+constexpr int kValueBits = 8, kMinExp = -100;
+// Probabilities go to fp16 times 2^kProbBits: a row's reference lags its largest
+// score by up to 2^kLazyMax and its largest value scale by up to 2^kLazyExp, so at
+// most 2^14; eleven bits down to 2^-20 of the reference.
+constexpr float kLazyMax = 6.0f;
+constexpr int kLazyExp = 2, kProbBits = 6;
+
+// grid (tiles of 128 M rows, n_kv, key parts): eight waves of 16 M rows share each
+// record.  It comes by DMA, two ahead; one ahead the waves turn it into fp16
+// operands in LDS together (a record's conversion in every wave would cost as
+// much VALU time as the softmax): keys as their codes, values times their scale over
+// the record's largest, in eleven bits.  A position whose value scale is not finite
+// gets zeros for its value and a NaN for its key's scale: the rows that see it end
+// as NaN by their scores, those before it keep theirs.  A wave's own step is matrix
+// instructions on operands as they are read, and the softmax.  One barrier a
+// record.  Part z of P takes an equal run of the tile's records; with P > 1 the
+// parts are written as k_kv8_split's are.
 template <int M>
-__global__ __launch_bounds__(kThreads, M == 4 ? 1 : 2) void k_kv8_flash(Kv8Attn a) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_rec[2][kRec];
+__global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[2][kRec];
+    __shared__ vmi_u4 s_f16[2][32 * 64];             // keys [a][kk], values [dt], 64 lanes each
+    __shared__ __attribute__((aligned(16))) float s_ks[2][kBlk];
+    __shared__ int s_exp[2];
+    constexpr int kTile = kFlashWaves * 16 * M;
     const int lane = threadIdx.x & 63, w = at_wave(), nl = lane & 15, q4 = lane >> 4;
     const int g = blockIdx.y, G = a.n_heads / a.n_kv, R = a.span * G, P = gridDim.z, z = blockIdx.z;
     const int pos0 = kv8_pos0(a.pos0, a.pos_dev, a.span, a.max_len);
     if (a.pos_dev && a.status && blockIdx.x == 0 && g == 0 && z == 0 && threadIdx.x == 0 && *a.pos_dev != pos0)
         atomicOr(a.status, VMI_STATUS_BAD_POS);
     const int tile = (int)gridDim.x - 1 - (int)blockIdx.x;   // late tiles see the most keys: first
-    const int r0 = tile * (64 * M) + 16 * M * w, last_row = min(tile * (64 * M) + 64 * M, R) - 1;
+    const int r0 = tile * kTile + 16 * M * w, last_row = min(tile * kTile + kTile, R) - 1;
     const int nb = (pos0 + last_row / G) / kBlk + 1;
     const int b0 = (int)((long)nb * z / P), b1 = (int)((long)nb * (z + 1) / P);
     const uint8_t* head = a.cache + (size_t)g * (a.max_len / kBlk) * kRec;
     auto issue = [&](int b, int u) {
         const uint8_t* rec = head + (size_t)b * kRec;
+        vmi_lds_dma16_opaque(rec + 1024 * w + 16 * lane, s_raw[u] + 1024 * w);
+        vmi_lds_dma16_opaque(rec + kHalfRec + 1024 * w + 16 * lane, s_raw[u] + kHalfRec + 1024 * w);
+        vmi_lds_dma4_opaque(rec + 2 * kHalfRec + 4 * lane, s_raw[u] + 2 * kHalfRec);   // every wave the same bytes
+    };
+    // the wave's share of a record: kilobyte w of its keys and of its values
+    auto convert = [&](int u) {
+        const uint8_t* raw = s_raw[u];
+        const vmi_u4 k = *reinterpret_cast<const vmi_u4*>(raw + 1024 * w + 16 * lane);
+        const vmi_u4 v = *reinterpret_cast<const vmi_u4*>(raw + kHalfRec + 1024 * w + 16 * lane);
+        const vmi_f4* vs = reinterpret_cast<const vmi_f4*>(raw + 2 * kHalfRec + 4 * kBlk + 32 * q4);
+        const vmi_f4 v0 = vs[0], v1 = vs[1];   // of positions 8 q4 ..
+        float top = fmaxf(fmaxf(fmaxf(v0[0], v0[1]), fmaxf(v0[2], v0[3])), fmaxf(fmaxf(v1[0], v1[1]), fmaxf(v1[2], v1[3])));
+        top = kv8_max32(kv8_max16(top));
+        const int e = max((int)(__float_as_uint(top) >> 23) - 126, kMinExp);
+        const float unit = ldexpf(1.0f, kValueBits - e);
+        vmi_u4 f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            vmi_lds_dma16_opaque(rec + 1024 * (4 * j + w) + 16 * lane, s_rec[u] + 1024 * (4 * j + w));
-        vmi_lds_dma4_opaque(rec + 2 * kHalfRec + 4 * lane, s_rec[u] + 2 * kHalfRec);   // every wave the same bytes
+        for (int i = 0; i < 4; ++i) {
+            const float x = i < 2 ? v0[2 * i] : v1[2 * i - 4], y = i < 2 ? v0[2 * i + 1] : v1[2 * i - 3];
+            f[i] = kv8_pack_f16(x == x ? x * unit : 0.0f, y == y ? y * unit : 0.0f);
+        }
+        s_f16[u][2 * w * 64 + lane] = kv8_signed(kv8_widen(k[0], k[1]));
+        s_f16[u][(2 * w + 1) * 64 + lane] = kv8_signed(kv8_widen(k[2], k[3]));
+        s_f16[u][(16 + 2 * w) * 64 + lane] = kv8_scaled(v[0], v[1], f);
+        s_f16[u][(16 + 2 * w + 1) * 64 + lane] = kv8_scaled(v[2], v[3], f);
+        if (w == 0 && lane < kBlk) {
+            const float ks = *reinterpret_cast<const float*>(raw + kv8_scale_off(lane, false));
+            const float x = *reinterpret_cast<const float*>(raw + kv8_scale_off(lane, true));
+            s_ks[u][lane] = x == x ? ks : x;
+            if (lane == 0) s_exp[u] = e;
+        }
     };
     Kv8Rows<M> Q;
     kv8_load_rows<M>(a, a.q, g, r0, R, pos0, Q);
     const int first = pos0 + min(r0, R - 1) / G;
-    Kv8Sums<M> Y;
-    Y.clear();
-    if (b0 < b1) issue(b0, 0);
+    vmi_f4 o[M][16];     // in units of 2^(ref - kValueBits - kProbBits)
+    float m[M], l[M];    // m: the reference score, before cx
+    int ref[M];          // and exponent of the value scales (wave-uniform)
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        m[i] = -3.402823466e38f;
+        l[i] = 0.0f;
+        ref[i] = kMinExp;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[i][d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (b0 < b1) {
+        issue(b0, 0);
+        if (b0 + 1 < b1) {
+            issue(b0 + 1, 1);
+            vmi_vm_wait_c<3>();
+        } else {
+            vmi_vm_wait_c<0>();
+        }
+        __syncthreads();
+        convert(0);
+    }
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
+        const int u = (b - b0) & 1;
         vmi_vm_wait_c<0>();
-        __syncthreads();
-        if (b + 1 < b1) issue(b + 1, (b + 1 - b0) & 1);
-        kv8_step<M>(s_rec[(b - b0) & 1], Q, kBlk * b, kBlk * b + kBlk - 1 > first, Y);
+        __syncthreads();   // record b is in operand order, b + 1 in LDS, and nobody reads what is written below
+        if (b + 1 < b1) convert(u ^ 1);
+        if (b + 2 < b1) issue(b + 2, u);
+        const vmi_u4* F = s_f16[u];
+        vmi_f4 s[M][2];
+#pragma unroll
+        for (int i = 0; i < M; ++i) s[i][0] = s[i][1] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const vmi_u4 k = F[(8 * t + kk) * 64 + lane];
+#pragma unroll
+                for (int i = 0; i < M; ++i) s[i][t] = vmi_mfma_f16(k, Q.q[i][kk], s[i][t]);
+            }
+        const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[u] + 8 * q4);   // of the lane's keys 8 q4 ..
+        const int e = __builtin_amdgcn_readfirstlane(s_exp[u]);
+        const bool masked = kBlk * b + kBlk - 1 > first;   // the record reaches past some row's last position
+        vmi_u4 pb[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            float x[8];
+            const vmi_f4 k0 = ks[0], k1 = ks[1];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                x[y] = s[i][0][y] * k0[y];
+                x[4 + y] = s[i][1][y] * k1[y];
+            }
+            if (masked) {
+                const int seen = Q.last[i] - (kBlk * b + 8 * q4);   // the lane's keys up to this one are visible
+#pragma unroll
+                for (int y = 0; y < 8; ++y) x[y] = y > seen ? -INFINITY : x[y];
+            }
+            float nm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            nm = fmaxf(m[i], kv8_max32(kv8_max16(nm)));
+            if (e > ref[i] + kLazyExp || __any((nm - m[i]) * Q.cx[i] > kLazyMax)) {
+                const int ne = max(e, ref[i]);
+                const float f = __builtin_amdgcn_exp2f((m[i] - nm) * Q.cx[i]);
+                l[i] *= f;
+                const float fo = ldexpf(f, ref[i] - ne);
+#pragma unroll
+                for (int d = 0; d < 16; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[i][d][r] *= fo;
+                m[i] = nm;
+                ref[i] = ne;
+            }
+            const int up = kProbBits + e - ref[i];
+            const float top = fmaxf(m[i] * Q.cx[i], -3.0e38f) - (float)up;
+            float sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                x[y] = __builtin_amdgcn_exp2f(fmaf(x[y], Q.cx[i], -top));
+                sum += x[y];
+            }
+            l[i] = fmaf(sum, ldexpf(1.0f, -up), l[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pb[i][j] = kv8_pack_f16(x[2 * j], x[2 * j + 1]);
+        }
+#pragma unroll
+        for (int d = 0; d < 16; ++d) {
+            const vmi_u4 v = F[(16 + d) * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < M; ++i) o[i][d] = vmi_mfma_f16(v, pb[i], o[i][d]);
+        }
     }
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-        float l = Y.l[m];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        const int row = r0 + 16 * m + nl;
+    for (int i = 0; i < M; ++i) {
+        const float sum = kv8_sum32(kv8_sum16(l[i]));
+        const int row = r0 + 16 * i + nl;
         if (row >= R) continue;
-        const float u = Y.s[m] * (1.0f / kPScale);
+        const float u = ldexpf(1.0f, ref[i] - kValueBits - kProbBits);
         const int t = row / G, h = g * G + row % G;
         if (P > 1) {
             const size_t at = (size_t)(g * P + z) * a.rp + row;
 #pragma unroll
             for (int d = 0; d < 16; ++d)
                 *reinterpret_cast<vmi_f4*>(a.part_o + at * kHeadDim + 16 * d + 4 * q4) =
-                    vmi_f4{Y.o[m][d][0] * u, Y.o[m][d][1] * u, Y.o[m][d][2] * u, Y.o[m][d][3] * u};
-            if (q4 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(Y.m[m], l);
+                    vmi_f4{o[i][d][0] * u, o[i][d][1] * u, o[i][d][2] * u, o[i][d][3] * u};
+            if (q4 == 0)
+                *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(fmaxf(m[i] * Q.cx[i], -3.0e38f), sum);
         } else {
+            const float inv_l = __fdiv_rn(1.0f, sum);
             const float* gate = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + 4 * q4 : nullptr;
-            uint16_t* o = a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * q4;
+            uint16_t* dst = a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * q4;
 #pragma unroll
             for (int d = 0; d < 16; ++d) {
-                const vmi_f4 y = {Y.o[m][d][0] * u, Y.o[m][d][1] * u, Y.o[m][d][2] * u, Y.o[m][d][3] * u};
-                *reinterpret_cast<uint2*>(o + 16 * d) = kv8_gated(y, l, gate ? gate + 16 * d : nullptr);
+                const vmi_f4 y = {o[i][d][0] * u, o[i][d][1] * u, o[i][d][2] * u, o[i][d][3] * u};
+                *reinterpret_cast<uint2*>(dst + 16 * d) = kv8_gated(y, inv_l, gate ? gate + 16 * d : nullptr);
             }
         }
     }
@@ -758,20 +1106,29 @@ constexpr int kMaxTok = 8192;
 
 // Workgroups per kv head that share its records in k_kv8_split: one per CU
 // over all kv heads.
-int split_groups(int n_kv) { return std::max(1, vmi::device_cus() / n_kv); }
+int split_groups(int n_kv) { return std::min(std::max(1, vmi::device_cus() / n_kv), kMaxParts); }
+
+// 16-row groups of a k_kv8_split workgroup.  Two for more than 16 rows over a cache
+// that gives a wave three records or more: the groups' workgroups read the cache once
+// each, which costs nothing while its records come from L2 (four tokens at 16,000
+// positions 15.6 us in one-group workgroups, 15.9 in two-group ones, at 32,764 18.9 and
+// 18.9; eight at 16,000 22.2 and 27.1) and the rate of HBM beyond (four at 64,000 28.8
+// and 23.4, at 262,000 89 and 56; eight at 64,000 49 and 43).  The results are the same.
+int split_row_groups(int rows, int records, int groups) {
+    return rows > 16 && records >= 3 * kSplitWaves * groups ? 2 : 1;
+}
 
 struct FlashPlan {
-    int m, tiles, parts;
+    int tiles, parts;
 };
 
-// Tiles of 64 M rows and the parts their keys are split into, from the rows
-// and kv heads alone.
+// Tiles of 128 rows and the parts their keys are split into, from the rows and
+// kv heads alone.
 FlashPlan flash_plan(int rows, int n_kv) {
     const int ncu = vmi::device_cus();
     FlashPlan p;
-    p.m = (rows + 127) / 128 * n_kv >= ncu ? 2 : 1;
-    p.tiles = (rows + 64 * p.m - 1) / (64 * p.m);
-    p.parts = std::max(1, std::min(2 * ncu / (p.tiles * n_kv), 64));
+    p.tiles = (rows + 127) / 128;
+    p.parts = std::max(1, std::min(ncu / (p.tiles * n_kv), 64));
     return p;
 }
 
@@ -815,28 +1172,36 @@ hipError_t vmi::launch_kv8_attention(Kv8Attn a, void* parts, hipStream_t s) {
         n = split_groups(a.n_kv);
         rows = (size_t)a.n_kv * n * a.paths * R;
         a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(parts) + align256(rows * kHeadDim * 4));
-        const dim3 grid(n, a.n_kv, a.paths), blk(kThreads);
-        switch ((R + 15) / 16) {
-            case 1: hipLaunchKernelGGL(k_kv8_split<1>, grid, blk, 0, s, a); break;
-            case 2: hipLaunchKernelGGL(k_kv8_split<2>, grid, blk, 0, s, a); break;
-            case 3: hipLaunchKernelGGL(k_kv8_split<3>, grid, blk, 0, s, a); break;
-            default: hipLaunchKernelGGL(k_kv8_split<4>, grid, blk, 0, s, a); break;
-        }
+        const dim3 blk(kSplitThreads);
+        // (with the position on the device, by the capacity)
+        const int ms = split_row_groups(R, (a.pos_dev ? a.max_len : a.pos0 + a.span) / kBlk, n);
+        const int tiles = (R + 16 * ms - 1) / (16 * ms);
+        const dim3 grid(n, a.n_kv, a.paths * tiles);
+        if (ms == 2)
+            if (tiles * a.paths == 1)
+                hipLaunchKernelGGL((k_kv8_split<2, true>), grid, blk, 0, s, a);
+            else
+                hipLaunchKernelGGL((k_kv8_split<2, false>), grid, blk, 0, s, a);
+        else if (tiles * a.paths == 1)
+            hipLaunchKernelGGL((k_kv8_split<1, true>), grid, blk, 0, s, a);
+        else
+            hipLaunchKernelGGL((k_kv8_split<1, false>), grid, blk, 0, s, a);
     } else {
         const FlashPlan p = flash_plan(R, a.n_kv);
         n = p.parts;
         rows = n > 1 ? (size_t)a.n_kv * n * R : 1;
         a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(parts) + align256(rows * kHeadDim * 4));
-        const dim3 grid(p.tiles, a.n_kv, p.parts), blk(kThreads);
-        if (p.m == 2)
-            hipLaunchKernelGGL(k_kv8_flash<2>, grid, blk, 0, s, a);
-        else
-            hipLaunchKernelGGL(k_kv8_flash<1>, grid, blk, 0, s, a);
+        const dim3 grid(p.tiles, a.n_kv, p.parts), blk(kFlashThreads);
+        hipLaunchKernelGGL(k_kv8_flash<1>, grid, blk, 0, s, a);
         if (n == 1) return hipGetLastError();
     }
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_kv8_merge, dim3(a.paths * a.span * a.n_heads), dim3(kThreads), 0, s, a, n, R <= kSplitRows);
+    const int rows_all = a.paths * a.span * a.n_heads;
+    if (R <= kSplitRows)
+        hipLaunchKernelGGL(k_kv8_merge, dim3(rows_all, 4), dim3(kThreads), 0, s, a, n);
+    else
+        hipLaunchKernelGGL(k_kv8_merge_rows, dim3((rows_all + kWaves - 1) / kWaves), dim3(kThreads), 0, s, a, n);
     return hipGetLastError();
 }
 

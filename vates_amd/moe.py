@@ -33,7 +33,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _stream_handle(stream) -> int:
     if stream is None:
-        stream = torch.cuda.current_stream()
+        # torch.cuda.current_stream().cuda_stream without making a Stream object (0.3 against 2.6 us)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream.cuda_stream
 
 
@@ -66,6 +67,8 @@ def scratch(nbytes: int, device: torch.device, stream=None) -> torch.Tensor:
     between them: uninitialised, from torch's allocator on the calls' stream, and
     given back when the caller drops it (torch hands it out again in that
     stream's order)."""
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
