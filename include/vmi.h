@@ -505,8 +505,8 @@ int vmi_tree_commit(const int32_t* result, const vmi_tree_layer* layers, int n_l
  * (the operand order of the attention's matrix instructions).  head_dim is 256.
  *
  * vmi_kv8_write -- rows into the cache: keys and values bf16, row (g, i) at
- * base + g * head + i * row elements (strides multiples of 4, 256 contiguous
- * elements, 8-byte aligned), to positions pos0 .. pos0 + n - 1; other positions
+ * base + g * head + i * row elements (strides multiples of 8, 256 contiguous
+ * elements, 16-byte aligned), to positions pos0 .. pos0 + n - 1; other positions
  * are left as they are.
  * vmi_kv8_read -- positions pos0 .. pos0 + n - 1 as [n_kv_heads, n, 256] of
  * dtype (VMI_F32, or VMI_BF16 rounded once); keys or values may be NULL.

@@ -216,12 +216,10 @@ class KVCache8(KVCache):
             raise VmiError(f"dtype {dtype} is not bfloat16 or float32")
         if not 0 <= start <= stop <= self.max_len:
             raise VmiError(f"positions {start}..{stop} outside the capacity {self.max_len}")
-        dev = _on_current(self.data)
-        k = v = None
-        if want_k:
-            k = _new((self.n_kv, stop - start, 256), dtype, dev, stream)
-        if want_v:
-            v = _new((self.n_kv, stop - start, 256), dtype, dev, stream)
+        _on_current(self.data)
+        rows = _like(self.data, (self.n_kv, stop - start, 256), dtype, stream)
+        k = rows if want_k else None
+        v = (rows if not want_k else _like(rows, None, dtype, stream)) if want_v else None
         if stop > start:
             check(load().vmi_kv8_read(self.data.data_ptr(), self.n_kv, self.max_len, start, stop - start, _ptr(k),
                                       _ptr(v), VMI_F32 if dtype is torch.float32 else VMI_BF16, _stream_handle(stream)),
@@ -245,12 +243,13 @@ class KVCache8(KVCache):
                                        self.max_len, _stream_handle(stream)), "vmi_kv8_write")
 
 
-def _new(shape, dtype: torch.dtype, dev, stream) -> torch.Tensor:
-    """An output of a call on `stream`: allocated in that stream's order."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=dev)
+def _like(t: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
+    """An output of a call on `stream`, on t's device (shape None: and of its
+    shape), allocated in that stream's order."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _like(t, shape, dtype, None)
+    return torch.empty_like(t) if shape is None else t.new_empty(shape, dtype=dtype)
 
 
 def _on_current(t: torch.Tensor) -> torch.device:
@@ -295,7 +294,7 @@ def norm_rope_append(qkv: torch.Tensor, cache: KVCache8, q_norm: torch.Tensor, k
     T = qkv.shape[0]
     pos = _position(cache, T, pos0, pos_device, dev)
     if out is None:
-        out = _new((T, n_heads, 256), torch.bfloat16, dev, stream)
+        out = _like(q_norm, (T, n_heads, 256), torch.bfloat16, stream)
     else:
         _rows_bf16(out, "out", (T, n_heads, 256), dev)
     if T:
@@ -333,13 +332,13 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
                              gate.stride(2) != 1):
         raise VmiError(f"gate must be float32 {list(q.shape)} on {dev} with contiguous rows")
     if out is None:
-        out = _new(q.shape, torch.bfloat16, dev, stream)
+        out = _like(q, None, torch.bfloat16, stream)
     else:
         _rows_bf16(out, "out", (T, n_heads, 256), dev)
     if T:
         lib = load()
         nbytes = lib.vmi_kv8_attention_workspace_bytes(T, n_heads, cache.n_kv)
-        ws = scratch(nbytes, dev, stream)
+        ws = _like(cache.data, (nbytes,), torch.uint8, stream)
         check(lib.vmi_kv8_attention(q.data_ptr(), T, n_heads, cache.n_kv, pos, _ptr(pos_device), cache.data.data_ptr(),
                                     cache.max_len, _ptr(gate), 0 if gate is None else gate.stride(0),
                                     0 if gate is None else gate.stride(1), out.data_ptr(), cache.status.data_ptr(),
@@ -386,14 +385,14 @@ class AttentionLayer:
         _rows_bf16(x, "x", (T, self.hidden), dev)
         pos = _position(cache, span, pos0, pos_device, dev)
         if out is None:
-            out = _new(x.shape, torch.bfloat16, dev, stream)
+            out = _like(x, None, torch.bfloat16, stream)
         else:
             _rows_bf16(out, "out", (T, self.hidden), dev)
         lib = load()
         nbytes = lib.vmi_attention_kv8_workspace_bytes(max(paths, 1), span, self.hidden, self.n_heads, self.n_kv)
         if not nbytes:
             raise VmiError(f"a batch of {max(paths, 1)} x {span} tokens is not built for this layer")
-        ws = scratch(nbytes, dev, stream)
+        ws = _like(cache.data, (nbytes,), torch.uint8, stream)
         rest = (out.data_ptr(), cache.status.data_ptr(), ws.data_ptr(), nbytes, _stream_handle(stream))
         if paths:
             check(lib.vmi_attention_tree_kv8(ctypes.byref(self.desc), x.data_ptr(), paths, span, pos, _ptr(pos_device),

@@ -5,15 +5,13 @@
 // A row (one position's key or value of one kv head, 256 dims) is held as
 // codes c in [-127, 127] and one fp32 scale s, and stands for s c:
 //   a = max |x|,  s = a / 127,  c = RNE(127 x / a)     (a = 0: s = 0, c = 0)
-// The quotient is taken as (x 127 k) / (a k) with one correctly rounded fp32
-// division (k = 2^-7 for a > 2^100, else 1: no overflow); for bf16 x the
-// numerator is exact and no quotient that is not a tie comes closer to one
-// than 2^-8 / 510, more than that division's rounding, so the codes are those
-// of exact arithmetic.  A row with an infinity or NaN has s = NaN and reads
-// back as NaN.  A scale belongs to one row: a scale shared by several
-// positions would change what is held of a position with the ones behind it
-// (rejected drafts, a row that is not finite), and an append would round the
-// open block again.  It costs 8 bytes beside a position's 512.
+// For bf16 x no quotient that is not a tie comes closer to one than 2^-8 / 510; the
+// one fma and, next to ties, the one division that take it here (kv8_quantise) round
+// by less, so the codes are those of exact arithmetic.  A row with an infinity or
+// NaN has s = NaN and reads back as NaN.  A scale belongs to one row: a scale shared
+// by several positions would change what is held of a position with the ones behind
+// it (rejected drafts, a row that is not finite), and an append would round the open
+// block again.  It costs 8 bytes beside a position's 512.
 //
 // Layout: per kv head max_len / 32 records of 16,640 bytes, 32 positions each:
 //   [0, 8192)        key codes + 128: position kt, dim d at
@@ -48,25 +46,42 @@ constexpr int kHalfRec = kKv8Half;           // bytes of a record's keys (or val
 constexpr int kRec = kKv8Record;
 static_assert(kRec == 2 * kHalfRec + 2 * kBlk * 4 && kHalfRec == kBlk * kHeadDim, "record");
 
-// One row, dims 4 l .. 4 l + 3 in lane l: the four codes + 128 in a word, the
-// row's scale in every lane.
-__device__ __forceinline__ uint32_t kv8_quantise(const float (&x)[4], float& scale) {
-    const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-    bool bad = false;
+// N elements of a row per lane, the row's largest magnitude a and whether the row
+// holds an infinity or NaN (alike in every lane of the row): the codes + 128, four to
+// a word, and the scale.  127 x / a is taken as x (127 / a) in one fma that adds 2^23 +
+// 2^22 + 128, whose sum's low byte is the code rounded to nearest even: off by at most
+// 127 * 2^-24 before that rounding.  Where some element comes within 2e-5 of a tie, or
+// 127 / a leaves fp32's range, the wave takes the quotients themselves (about one row
+// in fifty).
+template <int N>
+__device__ __forceinline__ void kv8_quantise(const float (&x)[N], float a, bool bad, uint32_t (&w)[N / 4], float& scale) {
+    scale = bad ? __builtin_nanf("") : __fdiv_rn(a, 127.0f);
+    const bool plain = a > 0x1p-100f && a < 0x1p100f;
+    constexpr float kMagic = 12582912.0f + 128.0f;
+    const float inv = plain && !bad ? __fdiv_rn(127.0f, a) : 0.0f;
+    uint32_t t[N];
+    float off = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bad = bad || !(fabsf(x[j]) < INFINITY);
-    const float a = vmi_wave_max(m);
-    if (__any(bad)) {
-        scale = __builtin_nanf("");
-        return 0x80808080u;
+    for (int i = 0; i < N; ++i) {
+        const float m = fmaf(x[i], inv, kMagic);
+        t[i] = __float_as_uint(m);
+        off = fmaxf(off, fabsf(fmaf(x[i], inv, kMagic - m)));
     }
-    scale = __fdiv_rn(a, 127.0f);
-    if (!(a > 0.0f)) return 0x80808080u;
-    const float k = a > 0x1p100f ? 0x1p-7f : 1.0f, den = a * k, num = 127.0f * k;
-    uint32_t w = 0;
+    if (__any(off > 0.49998f || (!plain && a > 0.0f && !bad))) {
+        const float k = a > 0x1p100f ? 0x1p-7f : 1.0f, den = a * k, num = 127.0f * k;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w |= (uint32_t)((int)rintf(__fdiv_rn(x[j] * num, den)) + 128) << (8 * j);
-    return w;
+        for (int i = 0; i < N; ++i) {
+            const int c = a > 0.0f && !bad ? (int)rintf(__fdiv_rn(x[i] * num, den)) : 0;
+            t[i] = (uint32_t)(c + 128);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const uint32_t lo = __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x04000c0cu);
+        w[i] = lo | hi;
+        if (bad) w[i] = 0x80808080u;
+    }
 }
 
 // ------------------------------------------------------------------- store
@@ -78,69 +93,137 @@ struct WriteArgs {
     int max_len;
 };
 
-// grid (records touched, n_kv): one record per workgroup.  Each wave quantises
-// eight positions' keys and values into an image of the record in LDS, which
-// then goes out 16 bytes a thread; bytes of positions outside the call are left
-// as they are (a key's 16 bytes are one position's; eight positions share a
-// value group's 8 bytes, so a group that is not covered goes byte by byte).
-// Bound by the bytes of the rows read.
-__global__ __launch_bounds__(kThreads) void k_kv8_write(WriteArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_rec[kRec];
-    const int lane = threadIdx.x & 63, w = at_wave(), g = blockIdx.y;
+// Sixteen bf16 of a row per lane (two 16-byte pieces), sixteen lanes a row: codes
+// and scale.
+__device__ __forceinline__ void kv8_row16(const vmi_u4& p0, const vmi_u4& p1, uint32_t (&w)[4], float& scale) {
+    uint32_t am = 0;   // largest magnitude, as bf16 bits: infinities and NaN above the finite ones
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        am = max(am, max(p0[i] & 0x7fffu, (p0[i] >> 16) & 0x7fffu));
+        am = max(am, max(p1[i] & 0x7fffu, (p1[i] >> 16) & 0x7fffu));
+    }
+    am = max(am, vmi_dpp_u32<VMI_DPP_XOR1>(am));
+    am = max(am, vmi_dpp_u32<VMI_DPP_XOR2>(am));
+    am = max(am, vmi_dpp_u32<VMI_DPP_HALF_MIRROR>(am));
+    am = max(am, vmi_dpp_u32<VMI_DPP_MIRROR>(am));
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(p0[i] << 16);
+        x[2 * i + 1] = __uint_as_float(p0[i] & 0xffff0000u);
+        x[8 + 2 * i] = __uint_as_float(p1[i] << 16);
+        x[8 + 2 * i + 1] = __uint_as_float(p1[i] & 0xffff0000u);
+    }
+    kv8_quantise<16>(x, __uint_as_float(am << 16), am >= 0x7f80u, w, scale);
+}
+
+// Four words of codes, one position each, four dims a word: four words of one dim,
+// four positions a word.
+__device__ __forceinline__ void kv8_transpose4(const uint32_t (&r)[4], uint32_t (&c)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), b = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u);
+    const uint32_t d = __builtin_amdgcn_perm(r[1], r[0], 0x07030602u), e = __builtin_amdgcn_perm(r[3], r[2], 0x07030602u);
+    c[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    c[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    c[2] = __builtin_amdgcn_perm(e, d, 0x05040100u);
+    c[3] = __builtin_amdgcn_perm(e, d, 0x07060302u);
+}
+
+// Where 16-byte unit u of a record's value codes waits in LDS: the threads write
+// units 64 bytes apart, which spreads them over the banks.
+__device__ __forceinline__ int kv8_unit(int u) { return u ^ (((u >> 4) & 3) << 2) ^ ((u >> 6) & 3); }
+
+// grid (records touched, n_kv, keys | values): half a record per workgroup, sixteen
+// lanes a row.  A key's lane holds the two octets of dims that are stored together, a
+// unit of 16 bytes, which goes out as it is; values turn in LDS, where a thread
+// collects eight positions of four dims and of the four 16 further on, and go out in
+// order, a kilobyte a wave.  Bytes of positions outside the call are left as they are:
+// a key's unit is one position's, and a group of eight positions' values that is not
+// covered goes byte by byte.  Bound by the bytes of the rows and of the cache: 32768
+// positions of two heads, 101 MB, in 27 us (3.7 TB/s; a copy of that size 20); one
+// position 4.6 us with the read back of it, two launches' latency.
+template <bool VALUES>
+__device__ __forceinline__ void kv8_write_record(const WriteArgs& a, uint8_t* s_mem) {
+    constexpr int kPad = kHeadDim + 4;
+    vmi_u4* s_unit = reinterpret_cast<vmi_u4*>(s_mem);                 // units in order (kv8_unit)
+    uint8_t* s_v = s_mem + kHalfRec;                                   // values [positions][kPad]
+    const int lane = threadIdx.x & 63, w = at_wave(), g = blockIdx.y, li = lane & 15, t = threadIdx.x;
     const int blk = a.pos0 / kBlk + blockIdx.x;
     const int lo = max(a.pos0 - blk * kBlk, 0), hi = min(a.pos0 + a.n - blk * kBlk, kBlk);  // positions of the record
-    uint2 raw[2][8];
+    uint8_t* rec = a.cache + ((size_t)g * (a.max_len / kBlk) + blk) * kRec;
+    // the wave's positions 8 w + 4 i + (lane >> 4); a key lane's dims 64 j + 8 o .. and 32 further on, a value lane's 16 li ..
+    const int j = li >> 2, o = li & 3;
+    vmi_u4 r[2][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int kt = 8 * w + i;
-        const int64_t r = (int64_t)(min(max(kt, lo), hi - 1) + blk * kBlk - a.pos0);
+    for (int i = 0; i < 2; ++i) {
+        const int kt = min(max(8 * w + 4 * i + (lane >> 4), lo), hi - 1);
+        const uint16_t* src = a.src[VALUES] + g * a.head[VALUES] + (int64_t)(kt + blk * kBlk - a.pos0) * a.row[VALUES] +
+                              (VALUES ? 16 * li : 64 * j + 8 * o);
+        r[i][0] = *reinterpret_cast<const vmi_u4*>(src);
+        r[i][1] = *reinterpret_cast<const vmi_u4*>(src + (VALUES ? 8 : 32));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (8 * w + 4 * i >= hi || 8 * w + 4 * i + 4 <= lo) continue;   // wave-uniform: none of these four
+        const int kt = 8 * w + 4 * i + (lane >> 4);
+        const bool mine = kt >= lo && kt < hi;
+        uint32_t c[4];
+        float s;
+        kv8_row16(r[i][0], r[i][1], c, s);
+        if (VALUES) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(s_v + kt * kPad + 16 * li + 4 * e) = c[e];
+        } else if (mine) {
+            *reinterpret_cast<vmi_u4*>(rec + kv8_k_off(kt, 64 * j + 8 * o)) = vmi_u4{c[0], c[1], c[2], c[3]};
+        }
+        if (mine && li == 0) *reinterpret_cast<float*>(rec + kv8_scale_off(kt, VALUES)) = s;
+    }
+    if constexpr (!VALUES) return;
+    __syncthreads();
+    if (t < kBlk * kHeadDim / 64) {
+        // positions 8 q .., dims 32 d + 4 e .. and 16 further on
+        const int e = t & 3, d = (t >> 2) & 7, q = t >> 5;
+        uint32_t out[4][4];   // per dim: positions 0..3, 4..7 of it, then of the one 16 further on
 #pragma unroll
         for (int z = 0; z < 2; ++z)
-            raw[z][i] = *reinterpret_cast<const uint2*>(a.src[z] + g * a.head[z] + r * a.row[z] + 4 * lane);
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int kt = 8 * w + i;
+            for (int y = 0; y < 2; ++y) {
+                uint32_t p[4], c[4];
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const float x[4] = {__uint_as_float(raw[z][i].x << 16), __uint_as_float(raw[z][i].x & 0xffff0000u),
-                                __uint_as_float(raw[z][i].y << 16), __uint_as_float(raw[z][i].y & 0xffff0000u)};
-            float s;
-            const uint32_t c = kv8_quantise(x, s);
-            if (z == 0) {
-                *reinterpret_cast<uint32_t*>(s_rec + kv8_k_off(kt, 4 * lane)) = c;
-            } else {
+                for (int i = 0; i < 4; ++i)
+                    p[i] = *reinterpret_cast<const uint32_t*>(s_v + (8 * q + 4 * y + i) * kPad + 32 * d + 16 * z + 4 * e);
+                kv8_transpose4(p, c);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s_rec[kv8_v_off(kt, 4 * lane + j)] = (uint8_t)(c >> (8 * j));
+                for (int i = 0; i < 4; ++i) out[i][2 * z + y] = c[i];
             }
-            if (lane == 0) *reinterpret_cast<float*>(s_rec + kv8_scale_off(kt, z)) = s;
-        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            s_unit[kv8_unit(d * 64 + q * 16 + 4 * e + i)] = vmi_u4{out[i][0], out[i][1], out[i][2], out[i][3]};
     }
     __syncthreads();
-    uint8_t* rec = a.cache + ((size_t)g * (a.max_len / kBlk) + blk) * kRec;
-    const bool whole = lo == 0 && hi == kBlk;
-    for (int i = threadIdx.x; i < kRec / 16; i += kThreads) {
-        const vmi_u4 u = *reinterpret_cast<const vmi_u4*>(s_rec + 16 * i);
-        if (whole) {
-            *reinterpret_cast<vmi_u4*>(rec + 16 * i) = u;
-        } else if (i < kHalfRec / 16) {
-            const int nl = i & 15, kt = 8 * (nl >> 2) + 4 * (i >> 8) + (nl & 3);
-            if (kt >= lo && kt < hi) *reinterpret_cast<vmi_u4*>(rec + 16 * i) = u;
-        } else if (i < 2 * kHalfRec / 16) {
-            const int k0 = 8 * ((i >> 4) & 3);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (k0 + e >= lo && k0 + e < hi) {
-                    rec[16 * i + e] = s_rec[16 * i + e];
-                    rec[16 * i + 8 + e] = s_rec[16 * i + 8 + e];
-                }
+    for (int i = 0; i < kHalfRec / 16 / kThreads; ++i) {
+        const int u = t + kThreads * i, kt = 8 * ((u >> 4) & 3);
+        const vmi_u4 v = s_unit[kv8_unit(u)];
+        uint8_t* dst = rec + kHalfRec + 16 * u;
+        if (kt >= lo && kt + 8 <= hi) {
+            *reinterpret_cast<vmi_u4*>(dst) = v;
         } else {
-            const int k0 = (4 * i) % kBlk;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (k0 + e >= lo && k0 + e < hi) *reinterpret_cast<uint32_t*>(rec + 16 * i + 4 * e) = u[e];
+            for (int y = 0; y < 8; ++y)
+                if (kt + y >= lo && kt + y < hi) {
+                    dst[y] = (uint8_t)(v[y >> 2] >> (8 * (y & 3)));
+                    dst[8 + y] = (uint8_t)(v[2 + (y >> 2)] >> (8 * (y & 3)));
+                }
         }
     }
+}
+
+__global__ __launch_bounds__(kThreads) void k_kv8_write(WriteArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[kHalfRec + kBlk * (kHeadDim + 4)];
+    if (blockIdx.z)
+        kv8_write_record<true>(a, s_mem);
+    else
+        kv8_write_record<false>(a, s_mem);
 }
 
 // -------------------------------------------------------------------- load
@@ -292,7 +375,13 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
             continue;
         }
         float s;
-        const uint32_t c = kv8_quantise(x[i], s);
+        uint32_t cw[1];
+        const float big = fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad = bad || !(fabsf(x[i][j]) < INFINITY);
+        kv8_quantise<4>(x[i], vmi_wave_max(big), __any(bad), cw, s);
+        const uint32_t c = cw[0];
         if (a.tree) {  // plain rows, one record per token
             if (!mine) continue;
             uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * a.T + t) * kKv8TreeRow;
@@ -1365,13 +1454,13 @@ extern "C" int vmi_kv8_write(const uint16_t* keys, int64_t key_head, int64_t key
     vmi::clear_error();
     const int rc = check_cache(cache, n_kv_heads, max_len, pos0, n, nullptr);
     if (rc != VMI_OK) return rc;
-    if (!keys || !values || !aligned(keys, 8) || !aligned(values, 8))
-        return vmi::fail(VMI_ERR_INVALID, "keys or values null or not 8-byte aligned");
-    if ((key_head | key_row | value_head | value_row) & 3)
-        return vmi::fail(VMI_ERR_INVALID, "strides must be multiples of 4 elements");
+    if (!keys || !values || !aligned(keys, 16) || !aligned(values, 16))
+        return vmi::fail(VMI_ERR_INVALID, "keys or values null or not 16-byte aligned");
+    if ((key_head | key_row | value_head | value_row) & 7)
+        return vmi::fail(VMI_ERR_INVALID, "strides must be multiples of 8 elements");
     WriteArgs a{{keys, values}, {key_head, value_head}, {key_row, value_row}, n, pos0, cache, max_len};
     const int recs = (pos0 + n - 1) / kBlk - pos0 / kBlk + 1;
-    hipLaunchKernelGGL(k_kv8_write, dim3(recs, n_kv_heads), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(k_kv8_write, dim3(recs, n_kv_heads, 2), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
     return launched("k_kv8_write launch");
 }
 
