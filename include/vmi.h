@@ -498,7 +498,7 @@ int vmi_tree_commit(const int32_t* result, const vmi_tree_layer* layers, int n_l
  * cache: vmi_kv8_bytes(n_kv_heads, max_len) bytes (0: sizes not taken), 16-byte
  * aligned, max_len a multiple of 32.  Zero-filled it holds zero rows.  Per kv
  * head max_len / 32 records of 16,640 bytes; in a record, position kt and dim d:
- *   key code + 128 at   ((a*4 + (d>>6))*64 + ((d>>3)&3)*16 + nl)*16 + ((d>>5)&1)*8 + (d&7),
+ *   key code (int8) at  ((a*4 + (d>>6))*64 + ((d>>3)&3)*16 + nl)*16 + ((d>>5)&1)*8 + (d&7),
  *                       nl = 4*(kt>>3) + (kt&3), a = (kt>>2)&1
  *   value code + 128 at 8192 + ((d>>5)*64 + (kt>>3)*16 + (d&15))*16 + ((d>>4)&1)*8 + (kt&7)
  *   key scale (fp32) at 16384 + 4 kt, value scale at 16512 + 4 kt
@@ -519,11 +519,15 @@ int vmi_tree_commit(const int32_t* result, const vmi_tree_layer* layers, int n_l
  * vmi_kv8_attention -- out bf16 [T, n_heads, 256] = softmax(q k / 16) v over the
  * cache, query t seeing positions <= pos0 + t; with gate (f32, element strides
  * gate_token and gate_head, 256 contiguous, rows 16-byte aligned) times
- * sigmoid(gate).  q bf16 [T, n_heads, 256], T <= 8192.  Batches of T * n_heads /
- * n_kv_heads <= 64 rows: a token's result does not depend on its batch or on
- * max_len, bit for bit; larger ones equal it up to the order of fp32 sums.
- * Positions behind a query's own never reach its result.  workspace: the
- * query's bytes, 16-byte aligned, nothing kept between calls.
+ * sigmoid(gate).  q bf16 [T, n_heads, 256], T <= 8192; a query is taken as 16-bit
+ * integers of its largest element over 32512 (half a step: 2^-16 of that element,
+ * where a key's codes are within 2^-8 of theirs), so that scores are exact integer
+ * sums.  Batches of T * n_heads / n_kv_heads <= 64 rows: a token's result does not
+ * depend on its batch or on max_len, bit for bit; larger ones equal it up to fp32's
+ * and fp16's rounding.  Positions behind a query's own never reach its result; a query
+ * that sees a row that is not finite, or is not finite itself, is NaN, and one whose
+ * scores pass fp32's range may be.  workspace: the query's bytes (enough for every
+ * smaller T too), 16-byte aligned, nothing kept between calls.
  *
  * pos_device (int32 on the device, or NULL) replaces pos0 when the kernels run;
  * outside [0, max_len - T] it is clamped into it and VMI_STATUS_BAD_POS is OR-ed
@@ -553,7 +557,7 @@ int vmi_kv8_attention(const uint16_t* q, int T, int n_heads, int n_kv_heads, int
  * and a path's rows equal its tokens as a chain, bit for bit), up to 8192 tokens
  * for prompts.  Queries and keys are rounded once, behind norm and rotation.
  * tree: uint8 [paths][n_kv_heads][span] rows of VMI_KV8_TREE_ROW bytes (256 key
- * codes + 128, 256 value codes + 128, the two scales, 8 bytes unused), 16-byte
+ * codes, 256 value codes + 128, the two scales, 8 bytes unused), 16-byte
  * aligned.  A vmi_tree_layer of kind VMI_TREE_ATTENTION_KV8 holds the cache in
  * k_cache and those rows in tree_kv.  status: a caller-owned word or NULL
  * (VMI_STATUS_BAD_POS).  Workspaces keep nothing between calls;

@@ -10,13 +10,18 @@ Bars, from the arithmetic (written here before the first run):
 * appended keys and values: half a code step of the 64-bit row, a / 254, and
   2^-20 a for the same fp32 work (keys) or the division (values).
 * attention, per output o = sum p v with A = sum p |v|: half a bf16 step of o,
-  2^-8 |o|; the probability times value scale in fp16, 2^-11 A (and what lies
-  below fp16's normal range, 2^-25 of 2^14 times the largest value scale times 127
-  summed over the keys: n 2^-39 * max |v|); each score's error d shifts p by d:
-  scores add 256 products of up to (1024 + 255) |q| in eight fp32 steps of a matrix
-  instruction, two roundings of 2^-24 each, so d <= 16 * 2^-24 * 1280 / 16 * sum|q| * s
-  = 2^-24 * 1280 * sum|q| * s on numerator and denominator alike (2 d A); hardware
-  exp2, sums and merge: 2^-16 A.
+  2^-8 |o|; up to three roundings to fp16, 2^-11 A each: a probability times its
+  value's scale, or (prompts) the probability, the scale, and the scale times the
+  code; what lies below fp16's normal range, 2^-25 of 2^14 times the largest value
+  scale times 127 summed over the keys, n 2^-39 max |v|, and (prompts) scales below
+  2^-22 of the largest, held to 2^-25 where that is 2^8: 127 * 2^-25 / (127 * 2^8) =
+  2^-33 max |v|; each score's error d shifts p by d, on numerator and denominator
+  alike, 2 d A.  A query is rounded to integers of its largest element / 32512, so
+  each element is off by at most that / 65024 and a score by max|q| sum|k| / (16 *
+  65024); the integer sums are exact, and their conversion, the key's scale, the row's
+  factor and the subtraction round five times by 2^-24 of scores of at most sum|q|
+  max|k| / 16: d <= max|q| sum|k| / (16 * 65024) + 5 * 2^-24 sum|q| max|k| / 16.
+  Hardware exp2, sums and merge: 2^-16 A.
 """
 import numpy as np
 import pytest
@@ -190,9 +195,11 @@ def attend64(q, k, v, pos0, gate):
         x = torch.matmul(q[:, h], kk.t().contiguous()) / 16.0
         p = torch.softmax(x.masked_fill(~see, -np.inf), -1)
         o, A = torch.matmul(p, vv), torch.matmul(p, vv.abs())
-        d = 2.0 ** -24 * 1280 * q[:, h].abs().sum(-1, keepdim=True) * kk.abs().max() / 127
+        qa = q[:, h].abs()
+        d = qa.amax(-1, keepdim=True) * kk.abs().sum(-1).max() / (16 * 65024) + \
+            5 * 2.0 ** -24 * qa.sum(-1, keepdim=True) * kk.abs().max() / 16
         n = see.sum(-1, keepdim=True)
-        tol[:, h] = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2 * d + 2.0 ** -16) * A + n * 2.0 ** -39 * vv.abs().max()
+        tol[:, h] = 2.0 ** -8 * o.abs() + (3 * 2.0 ** -11 + 2 * d + 2.0 ** -16) * A + (n * 2.0 ** -39 + 2.0 ** -33) * vv.abs().max()
         out[:, h] = o
     if gate is not None:
         s = torch.sigmoid(gate.double().to(dev))

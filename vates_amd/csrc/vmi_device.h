@@ -8,6 +8,7 @@ typedef _Float16 vmi_half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 vmi_bf8 __attribute__((ext_vector_type(8)));
 typedef float vmi_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t vmi_u4 __attribute__((ext_vector_type(4)));
+typedef int32_t vmi_i4 __attribute__((ext_vector_type(4)));
 
 #define VMI_WAVE 64
 
@@ -93,6 +94,10 @@ __device__ __forceinline__ uint32_t vmi_h2_bits(_Float16 lo, _Float16 hi) {
 __device__ __forceinline__ vmi_f4 vmi_mfma_f16(const vmi_u4& a, const vmi_u4& b, const vmi_f4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vmi_half8, a), __builtin_bit_cast(vmi_half8, b),
                                                    c, 0, 0, 0);
+}
+// 64 int8 products a lane pair, summed in int32.
+__device__ __forceinline__ vmi_i4 vmi_mfma_i8(const vmi_u4& a, const vmi_u4& b, const vmi_i4& c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(vmi_i4, a), __builtin_bit_cast(vmi_i4, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ vmi_f4 vmi_mfma_bf16(const vmi_u4& a, const vmi_u4& b, const vmi_f4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vmi_bf8, a), __builtin_bit_cast(vmi_bf8, b), c,
@@ -393,6 +398,35 @@ __device__ __forceinline__ void vmi_lds_dma4_opaque(const void* g, const void* l
                  : "memory", "m0");
 #else
     (void)g;
+    (void)lds;
+#endif
+}
+// The same from base + off, base alike in the wave.
+__device__ __forceinline__ void vmi_lds_dma16_at(const void* base, uint32_t off, const void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(base), "s"(m0)
+                 : "memory", "m0");
+#else
+    (void)base;
+    (void)off;
+    (void)lds;
+#endif
+}
+__device__ __forceinline__ void vmi_lds_dma4_at(const void* base, uint32_t off, const void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(off), "s"(base), "s"(m0)
+                 : "memory", "m0");
+#else
+    (void)base;
+    (void)off;
     (void)lds;
 #endif
 }

@@ -14,7 +14,7 @@
 // block again.  It costs 8 bytes beside a position's 512.
 //
 // Layout: per kv head max_len / 32 records of 16,640 bytes, 32 positions each:
-//   [0, 8192)        key codes + 128: position kt, dim d at
+//   [0, 8192)        key codes (int8): position kt, dim d at
 //                    ((a*4 + (d>>6))*64 + ((d>>3)&3)*16 + nl)*16 + ((d>>5)&1)*8 + (d&7),
 //                    nl = 4*(kt>>3) + (kt&3), a = (kt>>2)&1
 //   [8192, 16384)    value codes + 128: ((d>>5)*64 + (kt>>3)*16 + (d&15))*16 + ((d>>4)&1)*8 + (kt&7)
@@ -29,10 +29,13 @@
 //                  and rotated, q out in bf16, k and v into the cache
 //   k_kv8_split    attention of up to 64 query rows per kv head, the keys dealt
 //                  to the waves of the whole device
-//   k_kv8_flash    attention of more rows, 64 or more to a workgroup
-//   k_kv8_merge    joins the parts, times sigmoid(gate)
+//   k_kv8_flash, k_kv8_flash_short
+//                  attention of more rows, 256 or 128 to a workgroup
+//   k_kv8_merge, k_kv8_merge_rows
+//                  join the parts, times sigmoid(gate)
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vmi_attn_device.h"
 #include "vmi_internal.h"
@@ -45,6 +48,8 @@ constexpr int kBlk = VMI_KV_BLOCK;           // positions per record
 constexpr int kHalfRec = kKv8Half;           // bytes of a record's keys (or values)
 constexpr int kRec = kKv8Record;
 static_assert(kRec == 2 * kHalfRec + 2 * kBlk * 4 && kHalfRec == kBlk * kHeadDim, "record");
+
+constexpr uint32_t kKeySign = 0x80808080u;   // a word's codes + 128 and the codes themselves
 
 // N elements of a row per lane, the row's largest magnitude a and whether the row
 // holds an infinity or NaN (alike in every lane of the row): the codes + 128, four to
@@ -173,7 +178,7 @@ __device__ __forceinline__ void kv8_write_record(const WriteArgs& a, uint8_t* s_
 #pragma unroll
             for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(s_v + kt * kPad + 16 * li + 4 * e) = c[e];
         } else if (mine) {
-            *reinterpret_cast<vmi_u4*>(rec + kv8_k_off(kt, 64 * j + 8 * o)) = vmi_u4{c[0], c[1], c[2], c[3]};
+            *reinterpret_cast<vmi_u4*>(rec + kv8_k_off(kt, 64 * j + 8 * o)) = vmi_u4{c[0], c[1], c[2], c[3]} ^ kKeySign;
         }
         if (mine && li == 0) *reinterpret_cast<float*>(rec + kv8_scale_off(kt, VALUES)) = s;
     }
@@ -251,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void k_kv8_read(ReadArgs a) {
     for (int kt = lo + w; kt < hi; kt += kWaves) {
         uint32_t c;
         if (z == 0) {
-            c = *reinterpret_cast<const uint32_t*>(s_half + kv8_k_off(kt, 4 * lane));
+            c = *reinterpret_cast<const uint32_t*>(s_half + kv8_k_off(kt, 4 * lane)) ^ kKeySign;
         } else {
             c = 0;
 #pragma unroll
@@ -381,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) bad = bad || !(fabsf(x[i][j]) < INFINITY);
         kv8_quantise<4>(x[i], vmi_wave_max(big), __any(bad), cw, s);
-        const uint32_t c = cw[0];
+        const uint32_t c = is_v ? cw[0] : cw[0] ^ kKeySign;
         if (a.tree) {  // plain rows, one record per token
             if (!mine) continue;
             uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * a.T + t) * kKv8TreeRow;
@@ -465,13 +470,34 @@ __device__ __forceinline__ float kv8_sum16(float v) {
     return p.x + p.y;
 }
 
-// A query row's power of two f, max |q| f in (2^13, 2^14]: elements down to
-// 2^-28 of the largest keep their eight bits in fp16.  Rows of magnitudes
-// outside 2^-100 .. 2^100 take the nearest factor.
-__device__ __forceinline__ float kv8_query_scale(float amax) {
-    return vmi_fp16_range_scale(fminf(fmaxf(amax, amax > 0.0f ? 0x1p-100f : 0.0f), 0x1p100f));
+// Scores are sums of int8 products, exact in int32: a query row is held as 16-bit
+// integers of its largest magnitude over 32512, in two signed bytes each, 256 h + l.
+// That is half a step of 2^-16 of the largest element, 128 times finer than a key's
+// codes, and a key's bytes go to the matrix instruction as they are stored.
+constexpr float kQueryTop = 32512.0f;
+constexpr float kScoreUnit = 0.09016844005556021f / kQueryTop;  // log2(e) / sqrt(256) over it
+struct Kv8Unit {
+    float inv, cx;   // integers per unit of the query; powers of two per unit of score (NaN: a row that is not finite)
+};
+// am: the row's largest magnitude as bf16 bits.  Rows below 2^-100 keep fewer bits.
+__device__ __forceinline__ Kv8Unit kv8_query_unit(uint32_t am) {
+    const float top = fmaxf(__uint_as_float(am << 16), 0x1p-100f);
+    const bool bad = am >= 0x7f80u;
+    return {bad ? 0.0f : __fdiv_rn(kQueryTop, top), bad ? __builtin_nanf("") : kScoreUnit * top};
 }
-constexpr float kScoreUnit = 0.09016844005556021f * 0x1p24f;  // log2(e) / sqrt(256), codes in units of 2^-24
+// Four elements' bytes (two words of bf16 pairs), h and l.  The sum's low 16 bits are
+// 256 h + l + 128.
+__device__ __forceinline__ void kv8_digits(uint32_t p0, uint32_t p1, float inv, uint32_t& h, uint32_t& l) {
+    constexpr float kMagic = 12582912.0f + 128.0f;
+    const uint32_t a = __float_as_uint(fmaf(__uint_as_float(p0 << 16), inv, kMagic));
+    const uint32_t b = __float_as_uint(fmaf(__uint_as_float(p0 & 0xffff0000u), inv, kMagic));
+    const uint32_t c = __float_as_uint(fmaf(__uint_as_float(p1 << 16), inv, kMagic));
+    const uint32_t d = __float_as_uint(fmaf(__uint_as_float(p1 & 0xffff0000u), inv, kMagic));
+    const uint32_t u = __builtin_amdgcn_perm(b, a, 0x05010400u), v = __builtin_amdgcn_perm(d, c, 0x05010400u);
+    l = __builtin_amdgcn_perm(v, u, 0x05040100u) ^ kKeySign;
+    h = __builtin_amdgcn_perm(v, u, 0x07060302u);
+}
+__device__ __forceinline__ float kv8_score(int h, int l) { return (float)((int)((uint32_t)h << 8) + l); }
 
 constexpr float kPScale = 16384.0f;            // probabilities times value scales, in fp16: at most this
 constexpr float kSumUnit = 0x1p24f / kPScale;  // of their products' sums, codes in units of 2^-24
@@ -480,20 +506,18 @@ constexpr float kMinRef = 1e-30f;
 // 16 MS query rows of a wave: lane (nl, q4) belongs to row 16 m + nl.
 template <int MS>
 struct Kv8Rows {
-    vmi_u4 q[MS][8];   // fp16 query times a power of two, dims 32 kk + 8 q4 ..
-    float cx[MS];      // score unit over the power of two; NaN for a row that is not finite
-    int last[MS];      // last visible position
+    vmi_u4 q[MS][8];   // h (2 j) and l (2 j + 1) of dims 64 j + 8 q4 .. and 32 further on
+    float cx[MS];      // Kv8Unit
 };
 
-// The wave's query rows, from row r0 of R (rows behind the last repeat it).
+// The wave's query rows, sixteen from each r0 of R (rows behind the last repeat it).
 template <int MS>
-__device__ __forceinline__ void kv8_load_rows(const Kv8Attn& a, const uint16_t* q, int g, int r0, int R, int pos0,
+__device__ __forceinline__ void kv8_load_rows(const Kv8Attn& a, const uint16_t* q, int g, const int (&r0)[MS], int R,
                                               Kv8Rows<MS>& o) {
     const int lane = threadIdx.x & 63, nl = lane & 15, q4 = lane >> 4, G = a.n_heads / a.n_kv;
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
-        const int row = min(r0 + 16 * m + nl, R - 1), t = row / G, h = g * G + row % G;
-        o.last[m] = pos0 + t;
+        const int row = min(r0[m] + nl, R - 1), t = row / G, h = g * G + row % G;
         const vmi_u4* src = reinterpret_cast<const vmi_u4*>(q + ((size_t)t * a.n_heads + h) * kHeadDim + 8 * q4);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) o.q[m][kk] = src[4 * kk];
@@ -507,15 +531,22 @@ __device__ __forceinline__ void kv8_load_rows(const Kv8Attn& a, const uint16_t* 
             for (int i = 0; i < 4; ++i) am = max(am, max(o.q[m][kk][i] & 0x7fffu, (o.q[m][kk][i] >> 16) & 0x7fffu));
         am = max(am, (uint32_t)__shfl_xor((int)am, 16));
         am = max(am, (uint32_t)__shfl_xor((int)am, 32));
-        const float amax = __uint_as_float(am << 16), f = kv8_query_scale(amax);
+        const Kv8Unit f = kv8_query_unit(am);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
+        for (int j = 0; j < 4; ++j) {
+            vmi_u4 h, l;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t u = o.q[m][kk][i];
-                o.q[m][kk][i] = kv8_pack_f16(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f);
+                const vmi_u4& u = o.q[m][2 * j + i / 2];
+                uint32_t x, y;
+                kv8_digits(u[2 * (i % 2)], u[2 * (i % 2) + 1], f.inv, x, y);
+                h[i] = x;
+                l[i] = y;
             }
-        o.cx[m] = amax < 0x1p100f ? kScoreUnit / f : __builtin_nanf("");
+            o.q[m][2 * j] = h;
+            o.q[m][2 * j + 1] = l;
+        }
+        o.cx[m] = f.cx;
     }
 }
 
@@ -609,8 +640,8 @@ struct Kv8Sums {
     }
 };
 
-// One record's 32 keys, the first at position p0, against the rows q (fp16
-// operands in LDS).  S^T = K Q^T: a lane holds the scores of keys 8 q4 + e of its
+// One record's 32 keys, the first at position p0, against the rows q (kv8_digits,
+// in LDS).  S^T = K Q^T: a lane holds the scores of keys 8 q4 + e of its
 // row, which are, as probabilities, already the B operand of O^T = V^T P^T.  A
 // key's scale enters its score, a value's its probability; the product goes to fp16
 // (11 bits) relative to the row's largest value scale so far, and whatever raises
@@ -623,32 +654,25 @@ template <int MS, bool ONCE>
 __device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const float (&cx)[MS], const int (&last)[MS], int p0,
                                          bool mask, __amdgpu_buffer_rsrc_t next, Kv8Sums<MS>& S) {
     const int lane = threadIdx.x & 63, q4 = lane >> 4;
-    vmi_f4 s[MS][2];
+    vmi_i4 s[MS][2][2];   // [tile of 16 keys][h, l]
 #pragma unroll
-    for (int m = 0; m < MS; ++m) s[m][0] = s[m][1] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < MS; ++m) s[m][0][0] = s[m][0][1] = s[m][1][0] = s[m][1][1] = vmi_i4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        vmi_u4 qr[MS][2];
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int m = 0; m < MS; ++m) {
-            qr[m][0] = q[(8 * m + 2 * j) * 64 + lane];
-            qr[m][1] = q[(8 * m + 2 * j + 1) * 64 + lane];
-        }
+        for (int m = 0; m < MS; ++m)
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const vmi_u4 u = rec.k[4 * a + j];
-            const vmi_u4 k0 = kv8_signed(kv8_widen(u[0], u[1])), k1 = kv8_signed(kv8_widen(u[2], u[3]));
+            for (int i = 0; i < 2; ++i) {
+                const vmi_u4 qr = q[(8 * m + 2 * j + i) * 64 + lane];
 #pragma unroll
-            for (int m = 0; m < MS; ++m) s[m][a] = vmi_mfma_f16(k0, qr[m][0], s[m][a]);
-#pragma unroll
-            for (int m = 0; m < MS; ++m) s[m][a] = vmi_mfma_f16(k1, qr[m][1], s[m][a]);
-        }
-    }
+                for (int a = 0; a < 2; ++a) s[m][a][i] = vmi_mfma_i8(rec.k[4 * a + j], qr, s[m][a][i]);
+            }
     float x[MS][8];
 #pragma unroll
     for (int m = 0; m < MS; ++m)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[m][e] = s[m][e >> 2][e & 3] * (rec.ks[e >> 2][e & 3] * cx[m]);
+        for (int e = 0; e < 8; ++e)
+            x[m][e] = kv8_score(s[m][e >> 2][0][e & 3], s[m][e >> 2][1][e & 3]) * (rec.ks[e >> 2][e & 3] * cx[m]);
     kv8_load_keys<ONCE>(rec, next);
     vmi_u4 pb[MS];
 #pragma unroll
@@ -721,15 +745,16 @@ __device__ __forceinline__ void kv8_store_part(__amdgpu_buffer_rsrc_t ro, int ro
 constexpr int kSplitWaves = 4, kSplitThreads = 64 * kSplitWaves;
 
 // grid (S, n_kv, paths * row tiles): record b of a kv head belongs to wave
-// (b / S) % 8 of workgroup b % S, whatever the length, the batch and the capacity,
+// (b / S) % 4 of workgroup b % S, whatever the length, the batch and the capacity,
 // so that a row's sums do not depend on them, a short cache still spreads over the
 // device, and a long one keeps every CU reading.  The workgroup forms the rows'
-// fp16 operands in LDS; a wave then works through its records in registers, two
+// operands in LDS; a wave then works through its records in registers, up to two
 // waves a SIMD (one alone issues an instruction every six cycles), without a barrier
 // until the end, where the waves join in LDS and the workgroup writes one part:
 // maximum, sum and unnormalised output of each row, in fp32.  Bound by the bytes of
-// the cache from some ten thousand positions on, below by the latency of a record
-// and of the two launches.
+// the cache from some ten thousand positions on (one token of 16 heads on 2 at
+// 262,143: 47 us, 5.8 TB/s), below by the latency of a record and of the two launches
+// (at 1000: 8 us; four tokens at 32,764, a record or two a wave: 19).
 template <int MS, bool ONCE>
 __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) float s_o[kSplitWaves * 16 * kHeadDim];   // one row group of each wave
@@ -777,14 +802,16 @@ __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv
             const auto pr = __builtin_amdgcn_permlane16_swap(am, am, false, false);
             am = max((uint32_t)pr[0], (uint32_t)pr[1]);
         }
-        const float amax = __uint_as_float(am << 16), f = kv8_query_scale(amax);
-        vmi_u4 h;
+        const Kv8Unit f = kv8_query_unit(am);
+        uint32_t h[2], l[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            h[e] = kv8_pack_f16(__uint_as_float(qv[i][e] << 16) * f, __uint_as_float(qv[i][e] & 0xffff0000u) * f);
+        for (int e = 0; e < 2; ++e) kv8_digits(qv[i][2 * e], qv[i][2 * e + 1], f.inv, h[e], l[e]);
         const int r = 2 * (NQ * w + i) + (lane >> 5), d8 = lane & 31;   // row of the group, dims 8 d8 ..
-        s_q[(8 * (r >> 4) + (d8 >> 2)) * 64 + (d8 & 3) * 16 + (r & 15)] = h;
-        if (d8 == 0) s_cx[r] = amax < 0x1p100f ? kScoreUnit / f : __builtin_nanf("");
+        uint2* at = reinterpret_cast<uint2*>(s_q + (8 * (r >> 4) + 2 * (d8 >> 3)) * 64 + (d8 & 3) * 16 + (r & 15)) +
+                    ((d8 >> 2) & 1);
+        at[0] = make_uint2(h[0], h[1]);
+        at[2 * 64] = make_uint2(l[0], l[1]);
+        if (d8 == 0) s_cx[r] = f.cx;
     }
     kv8_lds_wait();
     __builtin_amdgcn_s_barrier();   // (not __syncthreads, which would wait for the records too)
@@ -899,9 +926,10 @@ __device__ __forceinline__ uint2 kv8_gated(const vmi_f4& y, float inv_l, const f
     return make_uint2(vmi_pack_bf16x2(o[0], o[1]), vmi_pack_bf16x2(o[2], o[3]));
 }
 
-// k_kv8_split's parts, many of few rows.  grid (rows of all heads, 4): a quarter of a row's dims per workgroup.  Part s is
-// added by slot s % 16 in increasing s, the sixteen slots in a fixed order.  Every
-// row sees position 0, so its sum is positive (or NaN, which it hands on).
+// k_kv8_split's parts, many of few rows.  grid (rows of all heads, 4): a quarter of a
+// row's dims per workgroup.  Part s is added by slot s % 16 in increasing s, the
+// sixteen slots in a fixed order.  Every row sees position 0, so its sum is positive
+// (or NaN, which it hands on).
 constexpr int kMaxParts = 256;
 __global__ __launch_bounds__(kThreads) void k_kv8_merge(Kv8Attn a, int parts) {
     __shared__ float s_f[kMaxParts], s_red[2][kWaves];
@@ -980,7 +1008,7 @@ __global__ __launch_bounds__(kThreads) void k_kv8_merge_rows(Kv8Attn a, int part
     *reinterpret_cast<uint2*>(a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * lane) = kv8_gated(y, __fdiv_rn(1.0f, l), gate);
 }
 
-constexpr int kFlashWaves = 8, kFlashThreads = 64 * kFlashWaves;
+constexpr int kFlashWaves = 8, kFlashThreads = 64 * kFlashWaves, kFlashM = 2, kTileRows = 16 * kFlashWaves;
 
 // Codes of a value record as fp16 integers, exactly (0x6400 is 1024 with a
 // mantissa step of 1), times their positions' factors f.
@@ -996,57 +1024,339 @@ __device__ __forceinline__ vmi_u4 kv8_scaled(uint32_t w0, uint32_t w1, const vmi
     return r;
 }
 
-// Value operands are in units of 2^(E - kValueBits), 2^E the power of two above the
-// record's largest value scale: integers times factors of up to 2^kValueBits.
-constexpr int kValueBits = 8, kMinExp = -100;
-// Probabilities go to fp16 times 2^kProbBits: a row's reference lags its largest
-// score by up to 2^kLazyMax and its largest value scale by up to 2^kLazyExp, so at
-// most 2^14; eleven bits down to 2^-20 of the reference.
-constexpr float kLazyMax = 6.0f;
-constexpr int kLazyExp = 2, kProbBits = 6;
+// The larger of three, of results of arithmetic (fmaxf would quiet each first).
+__device__ __forceinline__ float kv8_max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
-// grid (tiles of 128 M rows, n_kv, key parts): eight waves of 16 M rows share each
-// record.  It comes by DMA, two ahead; one ahead the waves turn it into fp16
-// operands in LDS together (a record's conversion in every wave would cost as
-// much VALU time as the softmax): keys as their codes, values times their scale over
-// the record's largest, in eleven bits.  A position whose value scale is not finite
-// gets zeros for its value and a NaN for its key's scale: the rows that see it end
-// as NaN by their scores, those before it keep theirs.  A wave's own step is matrix
-// instructions on operands as they are read, and the softmax.  One barrier a
-// record.  Part z of P takes an equal run of the tile's records; with P > 1 the
-// parts are written as k_kv8_split's are.
-template <int M>
+// Key scales are held times 2^-18, so that a score stays finite before its row's
+// factor.  Value operands are fp16: codes times their scale over 2^(E - kValueBits),
+// 2^E the power of two above the largest value scale so far, E at least kMinExp: integers
+// times factors of up to 2^kValueBits (eleven bits; a scale below 2^-22 of the largest
+// keeps 2^-33 of the largest value).  Probabilities go to fp16 times 2^kProbBits: a
+// row's reference lags its largest score by up to 2^kLazyMax.
+constexpr float kKeyUnit = 0x1p-18f;
+constexpr int kValueBits = 8, kMinExp = -100, kProbBits = 8;
+constexpr float kLazyMax = 6.0f;
+
+// The lane, computed where it is used: a register that a loop need not keep.
+__device__ __forceinline__ int kv8_lane() {
+    int l = __builtin_amdgcn_mbcnt_lo(~0u, 0u);
+    l = __builtin_amdgcn_mbcnt_hi(~0u, l);
+    asm volatile("" : "+v"(l));
+    return l;
+}
+
+// Row `row` of a flash kernel's sums: o times u, maximum and sum, out or as part z of P.
+__device__ __forceinline__ void kv8_finish_rows(const Kv8Attn& a, const vmi_f4 (&o)[16], float top, float sum, float u,
+                                                int row, int R) {
+    const int q4 = kv8_lane() >> 4, g = blockIdx.y, G = a.n_heads / a.n_kv, P = gridDim.z;
+    if (row >= R) return;
+    const int t = row / G, h = g * G + row % G;
+    if (P > 1) {
+        const size_t at = (size_t)(g * P + blockIdx.z) * a.rp + row;
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+            *reinterpret_cast<vmi_f4*>(a.part_o + at * kHeadDim + 16 * d + 4 * q4) =
+                vmi_f4{o[d][0] * u, o[d][1] * u, o[d][2] * u, o[d][3] * u};
+        if (q4 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, sum);
+    } else {
+        const float inv = __fdiv_rn(1.0f, sum) * u;
+        const float* gate = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + 4 * q4 : nullptr;
+        uint16_t* dst = a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * q4;
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+            *reinterpret_cast<uint2*>(dst + 16 * d) = kv8_gated(o[d], inv, gate ? gate + 16 * d : nullptr);
+    }
+}
+
+// grid (pairs of tiles of 128 rows, n_kv, key parts): eight waves share each record, each
+// with 16 rows of a tile and 16 of the tile as far from the other end, so that every
+// workgroup sees as many keys: the records that both see are taken with 32 rows a wave
+// (every operand read from LDS used twice), the rest with 16.  Records come by DMA.
+// Keys go to the matrix instructions as they are stored; values are turned into fp16 in
+// LDS, an eighth by each wave (in every wave that would cost as much VALU time as the
+// softmax), and the scales are prepared by one.  A position whose value scale is not
+// finite gets zeros for its value and a NaN for its key's scale: the rows that see it
+// end as NaN by their scores, those before it keep theirs.  The sums are rescaled only
+// when a score passes its row's reference by 2^kLazyMax or E rises, so that a step has
+// no reduction over lanes.
+//
+// A SIMD's two waves, w and w + 4, are kept half a step apart: while one feeds the
+// matrix unit (values of record k - 1, keys of record k), the other is in its softmax;
+// a barrier ends each phase.  Waves 0-3 multiply record k in phase 2 k, waves 4-7 in
+// phase 2 k + 1.  Record k + 1 and the scales of k + 2 are asked for in phase 2 k and have
+// come at the end of 2 k + 1; wave 7 prepares the scales of k + 1 in 2 k + 1; values of
+// k + 1 are turned in 2 k + 2 (by waves 4-7) and 2 k + 3 (by waves 0-3).  What is written
+// in a phase was last read in the one before.
+// Part z of P takes an equal run of the tile's records; with P > 1 the parts are written
+// as k_kv8_split's are.
+//
+// 4096 tokens behind 8192, 16 heads on 2: 655 us, 1.05 PFLOP/s (a large bf16 matrix
+// product reaches 1.23); with every wave in step 915, with the tiles unpaired 713.  A phase
+// takes some 1900 cycles, its 64 matrix instructions 1024 of them: what is left is a
+// single wave's instruction issue and the latency of its first LDS reads.  256
+// registers a lane are full; deeper operand prefetch spills.
 __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_raw[2][kRec];
-    __shared__ vmi_u4 s_f16[2][32 * 64];             // keys [a][kk], values [dt], 64 lanes each
+    __shared__ __attribute__((aligned(16))) uint8_t s_rec[2][2 * kHalfRec];   // keys and values, as stored
+    __shared__ float s_scale[2][2 * kBlk];
+    __shared__ vmi_u4 s_f16[2][16 * 64];             // values [dt], 64 lanes each
+    __shared__ __attribute__((aligned(16))) float s_ks[2][kBlk];
+    __shared__ __attribute__((aligned(16))) _Float16 s_vf[2][kBlk];
+    __shared__ int s_exp[2];
+    constexpr int M = kFlashM, kSchedRead = 0x100, kSchedMfma = 0x8;
+    const int w = at_wave(), late = w >> 2;
+    const int g = blockIdx.y, G = a.n_heads / a.n_kv, R = a.span * G, P = gridDim.z, z = blockIdx.z;
+    const int pos0 = kv8_pos0(a.pos0, a.pos_dev, a.span, a.max_len);
+    if (a.pos_dev && a.status && blockIdx.x == 0 && g == 0 && z == 0 && threadIdx.x == 0 && *a.pos_dev != pos0)
+        atomicOr(a.status, VMI_STATUS_BAD_POS);
+    // tile x and, of the other end, its partner: the first sees the fewest keys
+    const int tiles = (R + kTileRows - 1) / kTileRows, part = (int)blockIdx.x, other = tiles - 1 - part;
+    const int r0[M] = {other * kTileRows + 16 * w, part * kTileRows + 16 * w};
+    auto records = [&](int tile) { return (pos0 + (min((tile + 1) * kTileRows, R) - 1) / G) / kBlk + 1; };
+    const int nb = records(other), b0 = (int)((long)nb * z / P), n = (int)((long)nb * (z + 1) / P) - b0;
+    const int nboth = part < other ? min(max(records(part) - b0, 0), n) : 0;   // records that both tiles see
+    const uint8_t* head = a.cache + ((size_t)g * (a.max_len / kBlk) + b0) * kRec;
+    auto issue_scales = [&](int k) {   // every wave the same bytes
+        if (k < n) vmi_lds_dma4_at(head + (size_t)k * kRec + 2 * kHalfRec, 4 * kv8_lane(), s_scale[k & 1]);
+    };
+    auto issue = [&](int k) {   // and the scales of the next
+        if (k >= n) return;
+        const uint8_t* rec = head + (size_t)k * kRec;
+        uint8_t* dst = s_rec[k & 1];
+        const uint32_t at16 = 16 * kv8_lane();
+        vmi_lds_dma16_at(rec + 1024 * w, at16, dst + 1024 * w);
+        vmi_lds_dma16_at(rec + kHalfRec + 1024 * w, at16, dst + kHalfRec + 1024 * w);
+        issue_scales(k + 1);
+    };
+    // the wave's share of a record's values; and the scales
+    auto convert = [&](int k) {
+        if (k >= n) return;
+        const int lane = kv8_lane();
+        const vmi_u4 v = *reinterpret_cast<const vmi_u4*>(s_rec[k & 1] + kHalfRec + 1024 * w + 16 * lane);
+        const vmi_u4 f = *reinterpret_cast<const vmi_u4*>(s_vf[k & 1] + 8 * (lane >> 4));
+        vmi_u4* dst = s_f16[k & 1] + 2 * w * 64 + lane;
+        dst[0] = kv8_scaled(v[0], v[1], f);
+        dst[64] = kv8_scaled(v[2], v[3], f);
+    };
+    int top_exp = kMinExp;   // E, of the wave that prepares the scales
+    auto scales = [&](int k) {
+        if (k >= n || w != kFlashWaves - 1) return;
+        const int lane = kv8_lane();
+        const float ks = s_scale[k & 1][lane & (kBlk - 1)], vs = s_scale[k & 1][kBlk + (lane & (kBlk - 1))];
+        const bool ok = vs == vs;
+        if (__any(vs >= ldexpf(1.0f, top_exp)))
+            top_exp = max(top_exp, (int)(__float_as_uint(vmi_wave_max(ok ? vs : 0.0f)) >> 23) - 126);
+        if (lane < kBlk) {
+            s_ks[k & 1][lane] = ok ? ks * kKeyUnit : vs;
+            s_vf[k & 1][lane] = (_Float16)(ok ? ldexpf(vs, kValueBits - top_exp) : 0.0f);
+            s_exp[k & 1] = top_exp;
+        }
+    };
+    auto phase = [&] {
+        __builtin_amdgcn_sched_barrier(0);
+        kv8_lds_wait();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    issue_scales(0);
+    issue(0);
+    Kv8Rows<M> Q;
+    kv8_load_rows<M>(a, a.q, g, r0, R, Q);
+    vmi_f4 o[M][16];     // in units of 2^(ref - kValueBits - kProbBits)
+    float top[M];        // the reference score, less kProbBits
+    float l[M];          // the lane's share of the probabilities, times 2^kProbBits
+    int ref[M];          // E of the sums
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        Q.cx[i] *= 1.0f / kKeyUnit;
+        top[i] = -3.0e38f;
+        ref[i] = kMinExp;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[i][d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    vmi_u4 pb[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) pb[i] = vmi_u4{0u, 0u, 0u, 0u};
+    s_f16[1][threadIdx.x] = s_f16[1][threadIdx.x + kFlashThreads] = vmi_u4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < M; ++i) pb[i] = vmi_u4{0u, 0u, 0u, 0u};
+    auto values = [&](int k, auto mm) {
+        constexpr int MM = decltype(mm)::value;
+        const vmi_u4* V = s_f16[k & 1] + kv8_lane();
+#pragma unroll
+        for (int d = 0; d < 16; ++d) {
+            const vmi_u4 v = V[d * 64];
+#pragma unroll
+            for (int i = 0; i < MM; ++i) o[i][d] = vmi_mfma_f16(v, pb[i], o[i][d]);
+        }
+        // operands kAhead reads ahead of the matrix instructions that take them
+        constexpr int kAhead = 5;
+        __builtin_amdgcn_sched_group_barrier(kSchedRead, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < 16 - kAhead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, MM, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, MM * kAhead, 0);
+    };
+    float x[M][8];
+    auto scores = [&](int k, auto mm) {
+        constexpr int MM = decltype(mm)::value;
+        {
+            const vmi_u4* K = reinterpret_cast<const vmi_u4*>(s_rec[k & 1] + 16 * kv8_lane());
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                vmi_i4 s[MM][2];   // h, l
+#pragma unroll
+                for (int i = 0; i < MM; ++i) s[i][0] = s[i][1] = vmi_i4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const vmi_u4 key = K[(4 * t + j) * 64];
+#pragma unroll
+                    for (int i = 0; i < MM; ++i)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) s[i][c] = vmi_mfma_i8(key, Q.q[i][2 * j + c], s[i][c]);
+                }
+#pragma unroll
+                for (int i = 0; i < MM; ++i)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) x[i][4 * t + y] = kv8_score(s[i][0][y], s[i][1][y]);
+            }
+        }
+    };
+    auto softmax = [&](int k, auto mm) {
+        constexpr int MM = decltype(mm)::value;
+        const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[k & 1] + 8 * (kv8_lane() >> 4));   // of the lane's keys 8 q4 ..
+        const int e = __builtin_amdgcn_readfirstlane(s_exp[k & 1]);
+        const int p0 = kBlk * (b0 + k);
+        float big[MM];
+        bool raise = false, late_exp = false;
+        {
+            const vmi_f4 k0 = ks[0], k1 = ks[1];
+#pragma unroll
+            for (int i = 0; i < MM; ++i) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    x[i][y] *= k0[y];
+                    x[i][4 + y] *= k1[y];
+                }
+                if (p0 + kBlk - 1 > pos0 + min(r0[i], R - 1) / G) {   // the record reaches past some row's last position
+                    const int lane = kv8_lane();
+                    const int seen = pos0 + min(r0[i] + (lane & 15), R - 1) / G - 8 * (lane >> 4) - p0;   // the lane's keys up to this one
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) x[i][y] = y > seen ? -INFINITY : x[i][y];
+                }
+                big[i] = kv8_max3(kv8_max3(x[i][0], x[i][1], x[i][2]), kv8_max3(x[i][3], x[i][4], x[i][5]),
+                                  kv8_max3(x[i][6], x[i][7], x[i][7]));
+                late_exp = late_exp || e != ref[i];
+                raise = raise || fmaf(big[i], Q.cx[i], -top[i]) > kLazyMax + kProbBits;
+            }
+        }
+        if (late_exp || __any(raise)) {
+#pragma unroll
+            for (int i = 0; i < MM; ++i) {
+                const float nt = fmaxf(top[i], fmaf(kv8_max32(kv8_max16(big[i])), Q.cx[i], -(float)kProbBits));
+                const float f = __builtin_amdgcn_exp2f(top[i] - nt), fo = ldexpf(f, ref[i] - e);
+                l[i] *= f;
+#pragma unroll
+                for (int d = 0; d < 16; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[i][d][r] *= fo;
+                top[i] = nt;
+                ref[i] = e;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MM; ++i) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                x[i][y] = __builtin_amdgcn_exp2f(fmaf(x[i][y], Q.cx[i], -top[i]));
+                l[i] += x[i][y];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pb[i][j] = kv8_pack_f16(x[i][2 * j], x[i][2 * j + 1]);
+        }
+    };
+    constexpr std::integral_constant<int, 2> kBoth{};
+    constexpr std::integral_constant<int, 1> kOne{};
+    vmi_vm_wait_c<0>();
+    phase();
+    scales(0);
+    phase();
+    if (late) {   // phase 0 of the late waves
+        convert(0);
+        issue(1);
+        phase();
+    }
+    // one record: the values of the one before, over vv row groups, and its own scores, over mm
+    auto step = [&](int k, auto vv, auto mm) {
+        if (!late) issue(k + 1);
+        values(k - 1, vv);   // (of record -1: zeros)
+        scores(k, mm);
+        scales(k + 1);
+        if (late) vmi_vm_wait_c<0>();
+        phase();
+        if (late) issue(k + 2);
+        softmax(k, mm);
+        convert(k + late);
+        if (!late) vmi_vm_wait_c<0>();
+        phase();
+    };
+#pragma unroll 1
+    for (int k = 0; k < nboth; ++k) step(k, kBoth, kBoth);
+    if (n > nboth) step(nboth, kBoth, kOne);
+#pragma unroll 1
+    for (int k = nboth + 1; k < n; ++k) step(k, kOne, kOne);
+    if (n > nboth)
+        values(n - 1, kOne);
+    else
+        values(n - 1, kBoth);
+    if (!late) phase();   // the late waves' last
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+        if (i == 0 || part < other)
+            kv8_finish_rows(a, o[i], top[i] + (float)kProbBits, kv8_sum32(kv8_sum16(l[i])) * (1.0f / (float)(1 << kProbBits)),
+                            ldexpf(1.0f, ref[i] - kValueBits - kProbBits), r0[i] + (kv8_lane() & 15), R);
+}
+
+// grid (tiles of 128 rows, n_kv, key parts): k_kv8_flash for little work (flash_plan),
+// where its longer way in and out costs more than its phases give: eight waves of 16
+// rows in step, one barrier a record.  It comes by DMA, two ahead; one ahead the waves
+// turn its values together, over the largest scale of the record.
+__global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_key[3][kHalfRec], s_val[2][kHalfRec];   // as stored
+    __shared__ __attribute__((aligned(16))) float s_scale[2][2 * kBlk];
+    __shared__ vmi_u4 s_v16[2][16 * 64];
     __shared__ __attribute__((aligned(16))) float s_ks[2][kBlk];
     __shared__ int s_exp[2];
-    constexpr int kTile = kFlashWaves * 16 * M;
     const int lane = threadIdx.x & 63, w = at_wave(), nl = lane & 15, q4 = lane >> 4;
     const int g = blockIdx.y, G = a.n_heads / a.n_kv, R = a.span * G, P = gridDim.z, z = blockIdx.z;
     const int pos0 = kv8_pos0(a.pos0, a.pos_dev, a.span, a.max_len);
     if (a.pos_dev && a.status && blockIdx.x == 0 && g == 0 && z == 0 && threadIdx.x == 0 && *a.pos_dev != pos0)
         atomicOr(a.status, VMI_STATUS_BAD_POS);
     const int tile = (int)gridDim.x - 1 - (int)blockIdx.x;   // late tiles see the most keys: first
-    const int r0 = tile * kTile + 16 * M * w, last_row = min(tile * kTile + kTile, R) - 1;
-    const int nb = (pos0 + last_row / G) / kBlk + 1;
+    const int r0[1] = {tile * kTileRows + 16 * w};
+    const int nb = (pos0 + (min((tile + 1) * kTileRows, R) - 1) / G) / kBlk + 1;
     const int b0 = (int)((long)nb * z / P), b1 = (int)((long)nb * (z + 1) / P);
     const uint8_t* head = a.cache + (size_t)g * (a.max_len / kBlk) * kRec;
-    auto issue = [&](int b, int u) {
+    const uint32_t at16 = 16 * lane;
+    auto issue = [&](int b, int uk, int u) {
         const uint8_t* rec = head + (size_t)b * kRec;
-        vmi_lds_dma16_opaque(rec + 1024 * w + 16 * lane, s_raw[u] + 1024 * w);
-        vmi_lds_dma16_opaque(rec + kHalfRec + 1024 * w + 16 * lane, s_raw[u] + kHalfRec + 1024 * w);
-        vmi_lds_dma4_opaque(rec + 2 * kHalfRec + 4 * lane, s_raw[u] + 2 * kHalfRec);   // every wave the same bytes
+        vmi_lds_dma16_at(rec + 1024 * w, at16, s_key[uk] + 1024 * w);
+        vmi_lds_dma16_at(rec + kHalfRec + 1024 * w, at16, s_val[u] + 1024 * w);
+        vmi_lds_dma4_at(rec + 2 * kHalfRec, 4 * lane, s_scale[u]);   // every wave the same bytes
     };
-    // the wave's share of a record: kilobyte w of its keys and of its values
     auto convert = [&](int u) {
-        const uint8_t* raw = s_raw[u];
-        const vmi_u4 k = *reinterpret_cast<const vmi_u4*>(raw + 1024 * w + 16 * lane);
-        const vmi_u4 v = *reinterpret_cast<const vmi_u4*>(raw + kHalfRec + 1024 * w + 16 * lane);
-        const vmi_f4* vs = reinterpret_cast<const vmi_f4*>(raw + 2 * kHalfRec + 4 * kBlk + 32 * q4);
-        const vmi_f4 v0 = vs[0], v1 = vs[1];   // of positions 8 q4 ..
+        const vmi_u4 v = *reinterpret_cast<const vmi_u4*>(s_val[u] + 1024 * w + at16);
+        const vmi_f4* vs = reinterpret_cast<const vmi_f4*>(s_scale[u] + kBlk + 8 * q4);
+        const vmi_f4 v0 = vs[0], v1 = vs[1];
         float top = fmaxf(fmaxf(fmaxf(v0[0], v0[1]), fmaxf(v0[2], v0[3])), fmaxf(fmaxf(v1[0], v1[1]), fmaxf(v1[2], v1[3])));
-        top = kv8_max32(kv8_max16(top));
+        top = fmaxf(kv8_max32(kv8_max16(top)), 0.0f);
         const int e = max((int)(__float_as_uint(top) >> 23) - 126, kMinExp);
         const float unit = ldexpf(1.0f, kValueBits - e);
         vmi_u4 f;
@@ -1055,143 +1365,97 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
             const float x = i < 2 ? v0[2 * i] : v1[2 * i - 4], y = i < 2 ? v0[2 * i + 1] : v1[2 * i - 3];
             f[i] = kv8_pack_f16(x == x ? x * unit : 0.0f, y == y ? y * unit : 0.0f);
         }
-        s_f16[u][2 * w * 64 + lane] = kv8_signed(kv8_widen(k[0], k[1]));
-        s_f16[u][(2 * w + 1) * 64 + lane] = kv8_signed(kv8_widen(k[2], k[3]));
-        s_f16[u][(16 + 2 * w) * 64 + lane] = kv8_scaled(v[0], v[1], f);
-        s_f16[u][(16 + 2 * w + 1) * 64 + lane] = kv8_scaled(v[2], v[3], f);
+        s_v16[u][2 * w * 64 + lane] = kv8_scaled(v[0], v[1], f);
+        s_v16[u][(2 * w + 1) * 64 + lane] = kv8_scaled(v[2], v[3], f);
         if (w == 0 && lane < kBlk) {
-            const float ks = *reinterpret_cast<const float*>(raw + kv8_scale_off(lane, false));
-            const float x = *reinterpret_cast<const float*>(raw + kv8_scale_off(lane, true));
-            s_ks[u][lane] = x == x ? ks : x;
+            const float ks = s_scale[u][lane], x = s_scale[u][kBlk + lane];
+            s_ks[u][lane] = x == x ? ks * kKeyUnit : x;
             if (lane == 0) s_exp[u] = e;
         }
     };
-    Kv8Rows<M> Q;
-    kv8_load_rows<M>(a, a.q, g, r0, R, pos0, Q);
-    const int first = pos0 + min(r0, R - 1) / G;
-    vmi_f4 o[M][16];     // in units of 2^(ref - kValueBits - kProbBits)
-    float m[M], l[M];    // m: the reference score, before cx
-    int ref[M];          // and exponent of the value scales (wave-uniform)
+    if (b0 < b1) issue(b0, 0, 0);
+    if (b0 + 1 < b1) issue(b0 + 1, 1, 1);
+    Kv8Rows<1> Q;
+    kv8_load_rows<1>(a, a.q, g, r0, R, Q);
+    const float cx = Q.cx[0] * (1.0f / kKeyUnit);
+    const int last = pos0 + min(r0[0] + nl, R - 1) / G, first = pos0 + min(r0[0], R - 1) / G;
+    vmi_f4 o[16];                // in units of 2^(ref - kValueBits - kProbBits)
+    float top = -3.0e38f, l = 0.0f;   // the reference score, less kProbBits; probabilities times 2^kProbBits
+    int ref = kMinExp;           // exponent of the value scales
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
-        m[i] = -3.402823466e38f;
-        l[i] = 0.0f;
-        ref[i] = kMinExp;
-#pragma unroll
-        for (int d = 0; d < 16; ++d) o[i][d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
-    }
-    if (b0 < b1) {
-        issue(b0, 0);
-        if (b0 + 1 < b1) {
-            issue(b0 + 1, 1);
-            vmi_vm_wait_c<3>();
-        } else {
-            vmi_vm_wait_c<0>();
-        }
-        __syncthreads();
-        convert(0);
-    }
+    for (int d = 0; d < 16; ++d) o[d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
+    vmi_vm_wait_c<0>();
+    __syncthreads();
+    if (b0 < b1) convert(0);
+    int uk = 0;   // of s_key, the record's
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-        const int u = (b - b0) & 1;
+        const int u = (b - b0) & 1, uk1 = uk == 2 ? 0 : uk + 1;
         vmi_vm_wait_c<0>();
         __syncthreads();   // record b is in operand order, b + 1 in LDS, and nobody reads what is written below
         if (b + 1 < b1) convert(u ^ 1);
-        if (b + 2 < b1) issue(b + 2, u);
-        const vmi_u4* F = s_f16[u];
-        vmi_f4 s[M][2];
+        if (b + 2 < b1) issue(b + 2, uk1 == 2 ? 0 : uk1 + 1, u);
+        const vmi_u4* K = reinterpret_cast<const vmi_u4*>(s_key[uk]) + lane;
+        const vmi_u4* V = s_v16[u] + lane;
+        uk = uk1;
+        vmi_i4 s[2][2];   // [tile of 16 keys][h, l]
+        s[0][0] = s[0][1] = s[1][0] = s[1][1] = vmi_i4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < M; ++i) s[i][0] = s[i][1] = vmi_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const vmi_u4 k = F[(8 * t + kk) * 64 + lane];
+                const vmi_u4 key = K[(4 * t + j) * 64];
 #pragma unroll
-                for (int i = 0; i < M; ++i) s[i][t] = vmi_mfma_f16(k, Q.q[i][kk], s[i][t]);
+                for (int c = 0; c < 2; ++c) s[t][c] = vmi_mfma_i8(key, Q.q[0][2 * j + c], s[t][c]);
             }
         const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[u] + 8 * q4);   // of the lane's keys 8 q4 ..
-        const int e = __builtin_amdgcn_readfirstlane(s_exp[u]);
-        const bool masked = kBlk * b + kBlk - 1 > first;   // the record reaches past some row's last position
-        vmi_u4 pb[M];
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-            float x[8];
+        const int e = max(__builtin_amdgcn_readfirstlane(s_exp[u]), ref);
+        const float down = ldexpf(1.0f, __builtin_amdgcn_readfirstlane(s_exp[u]) - e);   // the record's values to E
+        float x[8];
+        {
             const vmi_f4 k0 = ks[0], k1 = ks[1];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                x[y] = s[i][0][y] * k0[y];
-                x[4 + y] = s[i][1][y] * k1[y];
+                x[y] = kv8_score(s[0][0][y], s[0][1][y]) * k0[y];
+                x[4 + y] = kv8_score(s[1][0][y], s[1][1][y]) * k1[y];
             }
-            if (masked) {
-                const int seen = Q.last[i] - (kBlk * b + 8 * q4);   // the lane's keys up to this one are visible
-#pragma unroll
-                for (int y = 0; y < 8; ++y) x[y] = y > seen ? -INFINITY : x[y];
-            }
-            float nm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            nm = fmaxf(m[i], kv8_max32(kv8_max16(nm)));
-            if (e > ref[i] + kLazyExp || __any((nm - m[i]) * Q.cx[i] > kLazyMax)) {
-                const int ne = max(e, ref[i]);
-                const float f = __builtin_amdgcn_exp2f((m[i] - nm) * Q.cx[i]);
-                l[i] *= f;
-                const float fo = ldexpf(f, ref[i] - ne);
-#pragma unroll
-                for (int d = 0; d < 16; ++d)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[i][d][r] *= fo;
-                m[i] = nm;
-                ref[i] = ne;
-            }
-            const int up = kProbBits + e - ref[i];
-            const float top = fmaxf(m[i] * Q.cx[i], -3.0e38f) - (float)up;
-            float sum = 0.0f;
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                x[y] = __builtin_amdgcn_exp2f(fmaf(x[y], Q.cx[i], -top));
-                sum += x[y];
-            }
-            l[i] = fmaf(sum, ldexpf(1.0f, -up), l[i]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) pb[i][j] = kv8_pack_f16(x[2 * j], x[2 * j + 1]);
         }
+        if (kBlk * b + kBlk - 1 > first) {   // the record reaches past some row's last position
+            const int seen = last - (kBlk * b + 8 * q4);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) {
-            const vmi_u4 v = F[(16 + d) * 64 + lane];
-#pragma unroll
-            for (int i = 0; i < M; ++i) o[i][d] = vmi_mfma_f16(v, pb[i], o[i][d]);
+            for (int y = 0; y < 8; ++y) x[y] = y > seen ? -INFINITY : x[y];
         }
-    }
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-        const float sum = kv8_sum32(kv8_sum16(l[i]));
-        const int row = r0 + 16 * i + nl;
-        if (row >= R) continue;
-        const float u = ldexpf(1.0f, ref[i] - kValueBits - kProbBits);
-        const int t = row / G, h = g * G + row % G;
-        if (P > 1) {
-            const size_t at = (size_t)(g * P + z) * a.rp + row;
+        const float big = kv8_max3(kv8_max3(x[0], x[1], x[2]), kv8_max3(x[3], x[4], x[5]), kv8_max3(x[6], x[7], x[7]));
+        if (e != ref || __any(fmaf(big, cx, -top) > kLazyMax + kProbBits)) {
+            const float nt = fmaxf(top, fmaf(kv8_max32(kv8_max16(big)), cx, -(float)kProbBits));
+            const float f = __builtin_amdgcn_exp2f(top - nt), fo = ldexpf(f, ref - e);
+            l *= f;
 #pragma unroll
             for (int d = 0; d < 16; ++d)
-                *reinterpret_cast<vmi_f4*>(a.part_o + at * kHeadDim + 16 * d + 4 * q4) =
-                    vmi_f4{o[i][d][0] * u, o[i][d][1] * u, o[i][d][2] * u, o[i][d][3] * u};
-            if (q4 == 0)
-                *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(fmaxf(m[i] * Q.cx[i], -3.0e38f), sum);
-        } else {
-            const float inv_l = __fdiv_rn(1.0f, sum);
-            const float* gate = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + 4 * q4 : nullptr;
-            uint16_t* dst = a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * q4;
 #pragma unroll
-            for (int d = 0; d < 16; ++d) {
-                const vmi_f4 y = {o[i][d][0] * u, o[i][d][1] * u, o[i][d][2] * u, o[i][d][3] * u};
-                *reinterpret_cast<uint2*>(dst + 16 * d) = kv8_gated(y, inv_l, gate ? gate + 16 * d : nullptr);
-            }
+                for (int r = 0; r < 4; ++r) o[d][r] *= fo;
+            top = nt;
+            ref = e;
         }
+        vmi_u4 pb;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            x[y] = __builtin_amdgcn_exp2f(fmaf(x[y], cx, -top));
+            l += x[y];
+            x[y] *= down;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pb[j] = kv8_pack_f16(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[d] = vmi_mfma_f16(V[d * 64], pb, o[d]);
     }
+    kv8_finish_rows(a, o, top + (float)kProbBits, kv8_sum32(kv8_sum16(l)) * (1.0f / (float)(1 << kProbBits)),
+                    ldexpf(1.0f, ref - kValueBits - kProbBits), r0[0] + nl, R);
 }
 
 // ------------------------------------------------------------------- host
 constexpr int kSplitRows = 64;   // rows per kv head of k_kv8_split
-constexpr int kMaxTok = 8192;
+constexpr int kMaxTok = 8192, kMaxFlashParts = 64;
 
 // Workgroups per kv head that share its records in k_kv8_split: one per CU
 // over all kv heads.
@@ -1207,18 +1471,29 @@ int split_row_groups(int rows, int records, int groups) {
     return rows > 16 && records >= 3 * kSplitWaves * groups ? 2 : 1;
 }
 
+// Form and grid of more than kSplitRows rows.  k_kv8_flash_short while a CU's share is
+// under sixteen records of a 128-row tile (us, that form and k_kv8_flash: 777 tokens from
+// position 0 39 and 49, 1024 from 0 46 and 55, 200 from 1234 29 and 40, 64 from 0 13 and
+// 28), k_kv8_flash from there (2048 from 0 95 and 90, 300 from 20,000 154 and 127, 4096 from
+// 0 210 and 200, 4096 from 8192 843 and 659).  Parts fill the device where the tiles do
+// not, of four records or more: a part costs its rows' way out and back (100 tokens from
+// 500 in as many parts as records 29, in these 23).
 struct FlashPlan {
-    int tiles, parts;
+    bool paired;
+    int tiles, parts;   // tiles: workgroups per kv head and part
 };
-
-// Tiles of 128 rows and the parts their keys are split into, from the rows and
-// kv heads alone.
-FlashPlan flash_plan(int rows, int n_kv) {
-    const int ncu = vmi::device_cus();
+FlashPlan flash_plan(int rows, int n_kv, int records, bool paired) {
     FlashPlan p;
-    p.tiles = (rows + 127) / 128;
-    p.parts = std::max(1, std::min(ncu / (p.tiles * n_kv), 64));
+    p.paired = paired;
+    p.tiles = (rows + kTileRows - 1) / kTileRows;
+    if (paired) p.tiles = (p.tiles + 1) / 2;
+    p.parts = std::max(1, std::min({vmi::device_cus() / (p.tiles * n_kv), kMaxFlashParts, (records + 3) / 4}));
     return p;
+}
+FlashPlan flash_plan(const Kv8Attn& a, int rows) {
+    const int pos0 = a.pos_dev ? a.max_len - a.span : a.pos0;   // (on the device: by the capacity)
+    const int64_t tiles = (rows + kTileRows - 1) / kTileRows, records = (pos0 + a.span / 2) / kBlk + 1;
+    return flash_plan(rows, a.n_kv, (pos0 + a.span - 1) / kBlk + 1, tiles * a.n_kv * records >= 16 * vmi::device_cus());
 }
 
 }  // namespace
@@ -1234,14 +1509,16 @@ bool vmi::kv8_heads_ok(int n_heads, int n_kv) {
 size_t vmi::kv8_attention_parts_bytes(int paths, int span, int n_heads, int n_kv) {
     if (paths < 1 || span < 1 || paths > 16 || span > kMaxTok || !kv8_heads_ok(n_heads, n_kv)) return 0;
     const int R = span * (n_heads / n_kv);
-    size_t rows;
-    if (R <= kSplitRows) {
-        rows = (size_t)n_kv * split_groups(n_kv) * paths * R;
-    } else {
-        if (paths != 1) return 0;
-        const FlashPlan p = flash_plan(R, n_kv);
-        rows = p.parts > 1 ? (size_t)n_kv * p.parts * R : 1;
-    }
+    if (R > kSplitRows && paths != 1) return 0;
+    // of this span and of every shorter one: a prompt's blocks share a workspace
+    size_t rows = (size_t)n_kv * split_groups(n_kv) * paths * std::min(R, kSplitRows);
+    if (R > kSplitRows)
+        for (int tiles = 1; (tiles - 1) * kTileRows < R; ++tiles) {
+            const int r = std::min(tiles * kTileRows, R);
+            const int parts = std::max(flash_plan(r, n_kv, 1 << 20, false).parts, flash_plan(r, n_kv, 1 << 20, true).parts);
+            if (parts == 1) break;   // and of more tiles
+            rows = std::max(rows, (size_t)n_kv * parts * r);
+        }
     return align256(rows * kHeadDim * 4) + align256(rows * 2 * 4);
 }
 
@@ -1276,12 +1553,15 @@ hipError_t vmi::launch_kv8_attention(Kv8Attn a, void* parts, hipStream_t s) {
         else
             hipLaunchKernelGGL((k_kv8_split<1, false>), grid, blk, 0, s, a);
     } else {
-        const FlashPlan p = flash_plan(R, a.n_kv);
+        const FlashPlan p = flash_plan(a, R);
         n = p.parts;
         rows = n > 1 ? (size_t)a.n_kv * n * R : 1;
         a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(parts) + align256(rows * kHeadDim * 4));
         const dim3 grid(p.tiles, a.n_kv, p.parts), blk(kFlashThreads);
-        hipLaunchKernelGGL(k_kv8_flash<1>, grid, blk, 0, s, a);
+        if (p.paired)
+            hipLaunchKernelGGL(k_kv8_flash, grid, blk, 0, s, a);
+        else
+            hipLaunchKernelGGL(k_kv8_flash_short, grid, blk, 0, s, a);
         if (n == 1) return hipGetLastError();
     }
     const hipError_t e = hipGetLastError();
