@@ -395,11 +395,12 @@ def _trace_moe_calls(fn):
     return {k: [int(np.unique(i.cpu().numpy()).size) for i in v] for k, v in seen.items()}
 
 
-def decode_step_bytes(model, K: int, L: int, U: dict) -> dict:
+def decode_step_bytes(model, K: int, L: int, U: dict, row: int = 512) -> dict:
     """Algorithmic HBM bytes of one speculative step in the [x, d1..dK] layout
     at context L: the verify forward (T = K + 1), K MTP draft steps (T = 1)
     and the MTP update (T = K + 1).  Weights are read once per call, caches
-    as the kernels read them; U: distinct experts per MoE call, traced."""
+    as the kernels read them, `row` bytes a cached key or value; U: distinct
+    experts per MoE call, traced."""
     T = K + 1
     H = model.hidden
     V = model.head.shape[0]
@@ -409,8 +410,8 @@ def decode_step_bytes(model, K: int, L: int, U: dict) -> dict:
     for layer in model.layers:
         if layer.attn is not None:
             a = layer.attn
-            kv_read = 2 * a.n_kv * L * 256 * 2
-            items["verify_attention"] += sum(_proj_bytes(q) for q in a._keep[:4]) + kv_read + 2 * a.n_kv * T * 512
+            kv_read = 2 * a.n_kv * L * row
+            items["verify_attention"] += sum(_proj_bytes(q) for q in a._keep[:4]) + kv_read + 2 * a.n_kv * T * row
         elif layer.gdn is not None:
             g = layer.gdn
             state = g.n_v * 128 * 128 * 4
@@ -420,7 +421,7 @@ def decode_step_bytes(model, K: int, L: int, U: dict) -> dict:
         items["verify_moe"] += u * EXPERT_BYTES + _moe_fixed_bytes(layer.moe)
     w = model.mtp.w
     att = sum(_proj_bytes(q) for q in w.attn._keep[:4])
-    kv = 2 * w.attn.n_kv * L * 256 * 2
+    kv = 2 * w.attn.n_kv * L * row
     mtp_u = U[id(w.moe)]  # K draft calls (T = 1), then the update (T = K + 1)
     for i in range(K):
         items["mtp_drafts"] += _proj_bytes(w.fc) + att + kv + mtp_u[i] * EXPERT_BYTES + _moe_fixed_bytes(w.moe) + head
@@ -509,8 +510,8 @@ def decode_record(args) -> dict:
                              device=dev)
     ctx, N, K = args.context, args.new_tokens, args.K
     max_len = ctx + 2 * N + 4 * (K + 1) + 8
-    caches = model.new_caches(max_len)
-    drafter = MTPDrafter(model.mtp, max_len)
+    caches = model.new_caches(max_len, kv_bits=args.kv_bits)
+    drafter = MTPDrafter(model.mtp, max_len, kv_bits=args.kv_bits)
     torch.cuda.synchronize()
     eprint(f"[bench] decode model resident: {torch.cuda.memory_allocated() / 2**30:.1f} GiB in {time.time() - t0:.1f} s")
     prompt = torch.from_numpy(np.random.default_rng(SEED).integers(0, args.vocab, ctx).astype(np.int32)).to(dev)
@@ -522,8 +523,8 @@ def decode_record(args) -> dict:
         from vates_amd.synth import synth_bf16
         for i, c in enumerate(caches + [drafter.cache]):
             if isinstance(c, KVCache):
-                c.write(0, synth_bf16(SEED, 0xCA000 + 2 * i, (c.k.shape[0], ctx, 256), device=dev),
-                        synth_bf16(SEED, 0xCA001 + 2 * i, (c.v.shape[0], ctx, 256), device=dev))
+                c.write(0, synth_bf16(SEED, 0xCA000 + 2 * i, (c.n_kv, ctx, 256), device=dev),
+                        synth_bf16(SEED, 0xCA001 + 2 * i, (c.n_kv, ctx, 256), device=dev))
             elif c is not None:
                 c.length = ctx
         drafter.cache.length = ctx - 1
@@ -550,7 +551,7 @@ def decode_record(args) -> dict:
     # distinct experts of every MoE call of one step, traced on an eager step
     reset()
     U = _trace_moe_calls(lambda: speculative_decode(model, drafter, caches, x0, h0, ctx, 1, K=K))
-    step_bytes = decode_step_bytes(model, K, ctx + K + 1, U)
+    step_bytes = decode_step_bytes(model, K, ctx + K + 1, U, 512 if args.kv_bits == 16 else 260)
 
     def graph_spec(planted=None, **kw):
         reset()
@@ -622,7 +623,7 @@ def decode_record(args) -> dict:
         "value": round(tps, 2), "unit": "tokens/s", "n_gpus": 1,
         "steps": st.steps, "warmup": args.warmup, "ms_per_step": round(ms_step, 4),
         "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-        "dtype": "u4 experts/projections, bf16 head and KV, f32 accumulate", "data": "synthetic",
+        "dtype": "u4 experts/projections, bf16 head" + (" and KV" if args.kv_bits == 16 else ", 8-bit KV") + ", f32 accumulate", "data": "synthetic",
         "config": {"workload": f"{args.layers}-layer random-init Qwen3-Next-shaped model ({args.layers // args.attn_every}"
                                f" full-attention and {args.layers - args.layers // args.attn_every} Gated DeltaNet "
                                f"layers, every layer MoE 512x top-{args.top_k} + shared expert), MTP K={K}, "
@@ -776,6 +777,7 @@ def main() -> int:
     ap.add_argument("--new-tokens", type=int, default=512)
     ap.add_argument("--K", type=int, default=3)
     ap.add_argument("--attn-every", type=int, default=4)
+    ap.add_argument("--kv-bits", type=int, choices=[16, 8], default=16, help="decode: bits of the attention caches")
     ap.add_argument("--tau", type=float, default=0.3, help="decode: adaptive-depth confidence threshold")
     ap.add_argument("--no-decode", action="store_true", help="default path: skip the decode record")
     ap.add_argument("--synthetic-cache", action="store_true",

@@ -216,13 +216,13 @@ class KVCache8(KVCache):
             raise VmiError(f"dtype {dtype} is not bfloat16 or float32")
         if not 0 <= start <= stop <= self.max_len:
             raise VmiError(f"positions {start}..{stop} outside the capacity {self.max_len}")
-        _on_current(self.data)
+        dev = _on_current(self.data)
         rows = _like(self.data, (self.n_kv, stop - start, 256), dtype, stream)
         k = rows if want_k else None
         v = (rows if not want_k else _like(rows, None, dtype, stream)) if want_v else None
         if stop > start:
             check(load().vmi_kv8_read(self.data.data_ptr(), self.n_kv, self.max_len, start, stop - start, _ptr(k),
-                                      _ptr(v), VMI_F32 if dtype is torch.float32 else VMI_BF16, _stream_handle(stream)),
+                                      _ptr(v), VMI_F32 if dtype is torch.float32 else VMI_BF16, _stream_on(dev, stream)),
                   "vmi_kv8_read")
         return k, v
 
@@ -240,7 +240,7 @@ class KVCache8(KVCache):
         if n:
             check(load().vmi_kv8_write(keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(),
                                        values.stride(0), values.stride(1), self.n_kv, start, n, self.data.data_ptr(),
-                                       self.max_len, _stream_handle(stream)), "vmi_kv8_write")
+                                       self.max_len, _stream_on(dev, stream)), "vmi_kv8_write")
 
 
 def _like(t: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
@@ -255,9 +255,17 @@ def _like(t: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
 def _on_current(t: torch.Tensor) -> torch.device:
     """The tensor's device, which has to be the one that the calls go to."""
     dev = t.device
-    if dev.type != "cuda" or dev.index != torch.cuda.current_device():
+    # (torch.cuda.current_device without its check that the device is initialised: t is on one)
+    if dev.type != "cuda" or dev.index != torch._C._cuda_getDevice():
         raise VmiError(f"tensors on {dev} are not on the current HIP device")
     return dev
+
+
+def _stream_on(dev: torch.device, stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
+
+
+_ATTEND_BYTES: dict = {}   # (device, T, query heads, kv heads) -> bytes of vmi_kv8_attention's workspace
 
 
 def _position(cache: KVCache8, T: int, pos0: Optional[int], pos_device: Optional[torch.Tensor], dev) -> int:
@@ -300,7 +308,7 @@ def norm_rope_append(qkv: torch.Tensor, cache: KVCache8, q_norm: torch.Tensor, k
     if T:
         check(load().vmi_kv8_append(qkv.data_ptr(), T, n_heads, cache.n_kv, q_norm.data_ptr(), k_norm.data_ptr(), eps,
                                     rope_dim, rope_theta, pos, _ptr(pos_device), cache.data.data_ptr(), cache.max_len,
-                                    out.data_ptr(), cache.status.data_ptr(), _stream_handle(stream)), "vmi_kv8_append")
+                                    out.data_ptr(), cache.status.data_ptr(), _stream_on(dev, stream)), "vmi_kv8_append")
     if pos_device is None:
         cache.length = pos + T
     return out
@@ -337,12 +345,15 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
         _rows_bf16(out, "out", (T, n_heads, 256), dev)
     if T:
         lib = load()
-        nbytes = lib.vmi_kv8_attention_workspace_bytes(T, n_heads, cache.n_kv)
+        key = (dev.index, T, n_heads, cache.n_kv)
+        nbytes = _ATTEND_BYTES.get(key)
+        if nbytes is None:
+            nbytes = _ATTEND_BYTES[key] = lib.vmi_kv8_attention_workspace_bytes(T, n_heads, cache.n_kv)
         ws = _like(cache.data, (nbytes,), torch.uint8, stream)
         check(lib.vmi_kv8_attention(q.data_ptr(), T, n_heads, cache.n_kv, pos, _ptr(pos_device), cache.data.data_ptr(),
                                     cache.max_len, _ptr(gate), 0 if gate is None else gate.stride(0),
                                     0 if gate is None else gate.stride(1), out.data_ptr(), cache.status.data_ptr(),
-                                    ws.data_ptr(), nbytes, _stream_handle(stream)), "vmi_kv8_attention")
+                                    ws.data_ptr(), nbytes, _stream_on(dev, stream)), "vmi_kv8_attention")
     return out
 
 

@@ -1088,13 +1088,13 @@ __device__ __forceinline__ void kv8_finish_rows(const Kv8Attn& a, const vmi_f4 (
 // matrix unit (values of record k - 1, keys of record k), the other is in its softmax;
 // a barrier ends each phase.  Waves 0-3 multiply record k in phase 2 k, waves 4-7 in
 // phase 2 k + 1.  Record k + 1 and the scales of k + 2 are asked for in phase 2 k and have
-// come at the end of 2 k + 1; wave 7 prepares the scales of k + 1 in 2 k + 1; values of
-// k + 1 are turned in 2 k + 2 (by waves 4-7) and 2 k + 3 (by waves 0-3).  What is written
-// in a phase was last read in the one before.
+// come at the end of 2 k + 1; wave 0 prepares the scales of k + 1 in 2 k (three slots: waves
+// 4-7 use those of k - 1 in it); values of k + 1 are turned in 2 k + 2 (by waves 4-7) and
+// 2 k + 3 (by waves 0-3).  What is written in a phase was last read in the one before.
 // Part z of P takes an equal run of the tile's records; with P > 1 the parts are written
 // as k_kv8_split's are.
 //
-// 4096 tokens behind 8192, 16 heads on 2: 655 us, 1.05 PFLOP/s (a large bf16 matrix
+// 4096 tokens behind 8192, 16 heads on 2: 640 us, 1.07 PFLOP/s (a large bf16 matrix
 // product reaches 1.23); with every wave in step 915, with the tiles unpaired 713.  A phase
 // takes some 1900 cycles, its 64 matrix instructions 1024 of them: what is left is a
 // single wave's instruction issue and the latency of its first LDS reads.  256
@@ -1103,9 +1103,9 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_rec[2][2 * kHalfRec];   // keys and values, as stored
     __shared__ float s_scale[2][2 * kBlk];
     __shared__ vmi_u4 s_f16[2][16 * 64];             // values [dt], 64 lanes each
-    __shared__ __attribute__((aligned(16))) float s_ks[2][kBlk];
-    __shared__ __attribute__((aligned(16))) _Float16 s_vf[2][kBlk];
-    __shared__ int s_exp[2];
+    __shared__ __attribute__((aligned(16))) float s_ks[3][kBlk];
+    __shared__ __attribute__((aligned(16))) _Float16 s_vf[3][kBlk];
+    __shared__ int s_exp[3];
     constexpr int M = kFlashM, kSchedRead = 0x100, kSchedMfma = 0x8;
     const int w = at_wave(), late = w >> 2;
     const int g = blockIdx.y, G = a.n_heads / a.n_kv, R = a.span * G, P = gridDim.z, z = blockIdx.z;
@@ -1136,23 +1136,23 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
         if (k >= n) return;
         const int lane = kv8_lane();
         const vmi_u4 v = *reinterpret_cast<const vmi_u4*>(s_rec[k & 1] + kHalfRec + 1024 * w + 16 * lane);
-        const vmi_u4 f = *reinterpret_cast<const vmi_u4*>(s_vf[k & 1] + 8 * (lane >> 4));
+        const vmi_u4 f = *reinterpret_cast<const vmi_u4*>(s_vf[k % 3] + 8 * (lane >> 4));
         vmi_u4* dst = s_f16[k & 1] + 2 * w * 64 + lane;
         dst[0] = kv8_scaled(v[0], v[1], f);
         dst[64] = kv8_scaled(v[2], v[3], f);
     };
     int top_exp = kMinExp;   // E, of the wave that prepares the scales
     auto scales = [&](int k) {
-        if (k >= n || w != kFlashWaves - 1) return;
+        if (k >= n || w != 0) return;
         const int lane = kv8_lane();
         const float ks = s_scale[k & 1][lane & (kBlk - 1)], vs = s_scale[k & 1][kBlk + (lane & (kBlk - 1))];
         const bool ok = vs == vs;
         if (__any(vs >= ldexpf(1.0f, top_exp)))
             top_exp = max(top_exp, (int)(__float_as_uint(vmi_wave_max(ok ? vs : 0.0f)) >> 23) - 126);
         if (lane < kBlk) {
-            s_ks[k & 1][lane] = ok ? ks * kKeyUnit : vs;
-            s_vf[k & 1][lane] = (_Float16)(ok ? ldexpf(vs, kValueBits - top_exp) : 0.0f);
-            s_exp[k & 1] = top_exp;
+            s_ks[k % 3][lane] = ok ? ks * kKeyUnit : vs;
+            s_vf[k % 3][lane] = (_Float16)(ok ? ldexpf(vs, kValueBits - top_exp) : 0.0f);
+            s_exp[k % 3] = top_exp;
         }
     };
     auto phase = [&] {
@@ -1231,8 +1231,8 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     };
     auto softmax = [&](int k, auto mm) {
         constexpr int MM = decltype(mm)::value;
-        const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[k & 1] + 8 * (kv8_lane() >> 4));   // of the lane's keys 8 q4 ..
-        const int e = __builtin_amdgcn_readfirstlane(s_exp[k & 1]);
+        const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[k % 3] + 8 * (kv8_lane() >> 4));   // of the lane's keys 8 q4 ..
+        const int e = __builtin_amdgcn_readfirstlane(s_exp[k % 3]);
         const int p0 = kBlk * (b0 + k);
         float big[MM];
         bool raise = false, late_exp = false;
@@ -1475,7 +1475,7 @@ int split_row_groups(int rows, int records, int groups) {
 // under sixteen records of a 128-row tile (us, that form and k_kv8_flash: 777 tokens from
 // position 0 39 and 49, 1024 from 0 46 and 55, 200 from 1234 29 and 40, 64 from 0 13 and
 // 28), k_kv8_flash from there (2048 from 0 95 and 90, 300 from 20,000 154 and 127, 4096 from
-// 0 210 and 200, 4096 from 8192 843 and 659).  Parts fill the device where the tiles do
+// 0 210 and 200, 4096 from 8192 843 and 640).  Parts fill the device where the tiles do
 // not, of four records or more: a part costs its rows' way out and back (100 tokens from
 // 500 in as many parts as records 29, in these 23).
 struct FlashPlan {
