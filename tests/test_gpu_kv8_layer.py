@@ -212,3 +212,16 @@ def test_prompt_blocks_and_batches_agree(gpu, model, monkeypatch):
     for h, v in ends[1:]:
         assert float((h - ends[0][0]).norm() / ends[0][0].norm()) <= 0.03
         assert float((v - ends[0][1]).norm() / ends[0][1].norm()) <= 0.03
+
+
+def test_a_cache_of_another_layer_is_refused(gpu):
+    import torch
+    from vates_amd._lib import VmiError
+    layer = make_layer(gpu, 41)
+    other = make_layer(gpu, 42, H=512, n_heads=4, n_kv=1).new_cache(128, 8)
+    x = torch.zeros((40, layer.hidden), dtype=torch.bfloat16, device=gpu)
+    for call in (lambda: layer(x[:1], other), lambda: layer.prompt(x, other, pos0=0), lambda: layer.tree(x[:4], other, 2),
+                 lambda: layer(x[:9], layer.new_cache(128, 8)), lambda: layer.prompt(x, layer.new_cache(32, 8), pos0=0),
+                 lambda: layer(x[:4], layer.new_cache(32, 8), pos0=29), lambda: layer.new_cache(64, 4)):
+        with pytest.raises(VmiError):
+            call()

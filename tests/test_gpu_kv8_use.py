@@ -342,3 +342,18 @@ def test_a_cache_past_four_gib(gpu):
             assert bool(((got[t, h].double().cpu() - want).abs() <= tol).all()), (h, t)
     del cache
     torch.cuda.empty_cache()
+
+
+def test_strides_that_no_step_takes(gpu):
+    """One kv head, one position, one token: the stride between them may be anything."""
+    from vates_amd.attention import attend
+    k, v = rows(110, 1, 4, gpu)
+    a, b = new_cache(1, 64, gpu), new_cache(1, 64, gpu)
+    a.write(0, k, v)
+    b.write(0, k.as_strided((1, 4, DIM), (3, DIM, 1)), v)
+    for t in range(4):
+        b.write(t, k[:, t:t + 1].as_strided((1, 1, DIM), (5, 7, 1), t * DIM), v[:, t:t + 1])
+    assert torch.equal(a.data, b.data)
+    q, gate = queries(111, 1, 8, gpu)
+    want = attend(q, a, pos0=3, gate=gate)
+    assert torch.equal(attend(q, a, pos0=3, gate=gate.as_strided((1, 8, DIM), (1, DIM, 1))), want)

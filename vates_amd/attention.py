@@ -229,7 +229,8 @@ class KVCache8(KVCache):
     def write(self, start: int, keys: torch.Tensor, values: torch.Tensor, *, stream=None) -> None:
         """Stores bfloat16 [n_kv_heads, n, 256] keys and values at positions
         start..start+n-1.  Rows of 256 are contiguous; heads and positions may
-        be strided (a transposed view of token-major rows)."""
+        be strided (a transposed view of token-major rows; 16-byte aligned).  The
+        committed length is the caller's to set."""
         dev = _on_current(self.data)
         n = keys.shape[1] if keys.dim() == 3 else 0
         for name, t in (("keys", keys), ("values", values)):
@@ -238,9 +239,10 @@ class KVCache8(KVCache):
         if start < 0 or start + n > self.max_len:
             raise VmiError(f"positions {start}..{start + n} outside the capacity {self.max_len}")
         if n:
-            check(load().vmi_kv8_write(keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(),
-                                       values.stride(0), values.stride(1), self.n_kv, start, n, self.data.data_ptr(),
-                                       self.max_len, _stream_on(dev, stream)), "vmi_kv8_write")
+            a, b = int(self.n_kv > 1), int(n > 1)   # (one head, or one position, may have any stride)
+            check(load().vmi_kv8_write(keys.data_ptr(), keys.stride(0) * a, keys.stride(1) * b, values.data_ptr(),
+                                       values.stride(0) * a, values.stride(1) * b, self.n_kv, start, n,
+                                       self.data.data_ptr(), self.max_len, _stream_on(dev, stream)), "vmi_kv8_write")
 
 
 def _like(t: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
@@ -351,8 +353,8 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
             nbytes = _ATTEND_BYTES[key] = lib.vmi_kv8_attention_workspace_bytes(T, n_heads, cache.n_kv)
         ws = _like(cache.data, (nbytes,), torch.uint8, stream)
         check(lib.vmi_kv8_attention(q.data_ptr(), T, n_heads, cache.n_kv, pos, _ptr(pos_device), cache.data.data_ptr(),
-                                    cache.max_len, _ptr(gate), 0 if gate is None else gate.stride(0),
-                                    0 if gate is None else gate.stride(1), out.data_ptr(), cache.status.data_ptr(),
+                                    cache.max_len, _ptr(gate), 0 if gate is None or T == 1 else gate.stride(0),
+                                    0 if gate is None or n_heads == 1 else gate.stride(1), out.data_ptr(), cache.status.data_ptr(),
                                     ws.data_ptr(), nbytes, _stream_on(dev, stream)), "vmi_kv8_attention")
     return out
 
@@ -463,7 +465,8 @@ class AttentionLayer:
         if ws is None:
             ws = scratch(self.prompt_workspace_bytes(T, cache), self.device, stream)
         if isinstance(cache, KVCache8):
-            _on_current(cache.data)
+            if _on_current(cache.data) != self.device or cache.n_kv != self.n_kv:
+                raise VmiError(f"a cache of {cache.n_kv} kv heads on {cache.device} does not fit the layer")
             check(load().vmi_attention_prompt_kv8(ctypes.byref(self.desc), x.data_ptr(), T, pos0, cache.data.data_ptr(),
                                                   cache.max_len, _ptr(out), ws.data_ptr(), ws.numel(), sh),
                   "vmi_attention_prompt_kv8")
