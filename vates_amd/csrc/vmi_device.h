@@ -95,7 +95,7 @@ __device__ __forceinline__ vmi_f4 vmi_mfma_f16(const vmi_u4& a, const vmi_u4& b,
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vmi_half8, a), __builtin_bit_cast(vmi_half8, b),
                                                    c, 0, 0, 0);
 }
-// 64 int8 products a lane pair, summed in int32.
+// Sums of 64 int8 products in int32.
 __device__ __forceinline__ vmi_i4 vmi_mfma_i8(const vmi_u4& a, const vmi_u4& b, const vmi_i4& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(vmi_i4, a), __builtin_bit_cast(vmi_i4, b), c, 0, 0, 0);
 }

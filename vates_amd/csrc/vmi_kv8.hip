@@ -1183,8 +1183,6 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
 #pragma unroll
     for (int i = 0; i < M; ++i) pb[i] = vmi_u4{0u, 0u, 0u, 0u};
     s_f16[1][threadIdx.x] = s_f16[1][threadIdx.x + kFlashThreads] = vmi_u4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < M; ++i) pb[i] = vmi_u4{0u, 0u, 0u, 0u};
     auto values = [&](int k, auto mm) {
         constexpr int MM = decltype(mm)::value;
         const vmi_u4* V = s_f16[k & 1] + kv8_lane();
@@ -1207,26 +1205,24 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     float x[M][8];
     auto scores = [&](int k, auto mm) {
         constexpr int MM = decltype(mm)::value;
-        {
-            const vmi_u4* K = reinterpret_cast<const vmi_u4*>(s_rec[k & 1] + 16 * kv8_lane());
+        const vmi_u4* K = reinterpret_cast<const vmi_u4*>(s_rec[k & 1] + 16 * kv8_lane());
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                vmi_i4 s[MM][2];   // h, l
+        for (int t = 0; t < 2; ++t) {
+            vmi_i4 s[MM][2];   // h, l
 #pragma unroll
-                for (int i = 0; i < MM; ++i) s[i][0] = s[i][1] = vmi_i4{0, 0, 0, 0};
+            for (int i = 0; i < MM; ++i) s[i][0] = s[i][1] = vmi_i4{0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const vmi_u4 key = K[(4 * t + j) * 64];
-#pragma unroll
-                    for (int i = 0; i < MM; ++i)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) s[i][c] = vmi_mfma_i8(key, Q.q[i][2 * j + c], s[i][c]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                const vmi_u4 key = K[(4 * t + j) * 64];
 #pragma unroll
                 for (int i = 0; i < MM; ++i)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) x[i][4 * t + y] = kv8_score(s[i][0][y], s[i][1][y]);
+                    for (int c = 0; c < 2; ++c) s[i][c] = vmi_mfma_i8(key, Q.q[i][2 * j + c], s[i][c]);
             }
+#pragma unroll
+            for (int i = 0; i < MM; ++i)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) x[i][4 * t + y] = kv8_score(s[i][0][y], s[i][1][y]);
         }
     };
     auto softmax = [&](int k, auto mm) {
@@ -1247,7 +1243,8 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
                 }
                 if (p0 + kBlk - 1 > pos0 + min(r0[i], R - 1) / G) {   // the record reaches past some row's last position
                     const int lane = kv8_lane();
-                    const int seen = pos0 + min(r0[i] + (lane & 15), R - 1) / G - 8 * (lane >> 4) - p0;   // the lane's keys up to this one
+                    // the lane's keys up to this one are visible
+                    const int seen = pos0 + min(r0[i] + (lane & 15), R - 1) / G - 8 * (lane >> 4) - p0;
 #pragma unroll
                     for (int y = 0; y < 8; ++y) x[i][y] = y > seen ? -INFINITY : x[i][y];
                 }
