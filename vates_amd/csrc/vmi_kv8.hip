@@ -578,13 +578,15 @@ __device__ __forceinline__ void kv8_load_keys(Kv8Rec& r, __amdgpu_buffer_rsrc_t 
         r.ks[j] = __builtin_bit_cast(vmi_f4, kv8_bload<ONCE>(rs, 2 * kHalfRec + 32 * (lane >> 4) + 16 * j, 0));
 }
 template <bool ONCE>
-__device__ __forceinline__ void kv8_load_values(Kv8Rec& r, __amdgpu_buffer_rsrc_t rs) {
+__device__ __forceinline__ void kv8_load_value_scales(Kv8Rec& r, __amdgpu_buffer_rsrc_t rs) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
         r.vs[j] = __builtin_bit_cast(vmi_f4, kv8_bload<ONCE>(rs, 2 * kHalfRec + 128 + 32 * (lane >> 4) + 16 * j, 0));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r.v[j] = kv8_bload<ONCE>(rs, 16 * lane, kHalfRec + 1024 * j);
+}
+template <bool ONCE>
+__device__ __forceinline__ void kv8_load_value(Kv8Rec& r, __amdgpu_buffer_rsrc_t rs, int j) {
+    r.v[j] = kv8_bload<ONCE>(rs, 16 * (threadIdx.x & 63), kHalfRec + 1024 * j);
 }
 
 // Position kt of the record from a tree token's row.
@@ -649,7 +651,7 @@ struct Kv8Sums {
 // reaches past the visible positions of some row; masked scores count as minus
 // infinity and masked scales as zero, so that nothing stored behind a row's last
 // position reaches it.  The next record's keys are asked for once these are used,
-// its values at the end.
+// each of its value operands once this record's is.
 template <int MS, bool ONCE>
 __device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const float (&cx)[MS], const int (&last)[MS], int p0,
                                          bool mask, __amdgpu_buffer_rsrc_t next, Kv8Sums<MS>& S) {
@@ -717,6 +719,7 @@ __device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const flo
 #pragma unroll
         for (int i = 0; i < 4; ++i) pb[m][i] = kv8_pack_f16(x[m][2 * i], x[m][2 * i + 1]);
     }
+    kv8_load_value_scales<ONCE>(rec, next);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const vmi_u4 u = rec.v[j];
@@ -725,8 +728,8 @@ __device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const flo
         for (int m = 0; m < MS; ++m) S.o[m][2 * j] = vmi_mfma_f16(v0, pb[m], S.o[m][2 * j]);
 #pragma unroll
         for (int m = 0; m < MS; ++m) S.o[m][2 * j + 1] = vmi_mfma_f16(v1, pb[m], S.o[m][2 * j + 1]);
+        kv8_load_value<ONCE>(rec, next, j);
     }
-    kv8_load_values<ONCE>(rec, next);
 }
 
 // Waits for the wave's own LDS operations.
@@ -779,16 +782,10 @@ __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv
         qv[i] = *reinterpret_cast<const vmi_u4*>(a.q + ((size_t)(path * T + t) * a.n_heads + g * G + row % G) * kHeadDim +
                                                  8 * (lane & 31));
     }
-    // a CU returns loads in the order they were issued: every wave's rows before any wave's record
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     Kv8Rec rec;
-    {
-        const __amdgpu_buffer_rsrc_t rs = kv8_rsrc(head, first, first < nblk);
-        kv8_load_keys<ONCE>(rec, rs);
-        kv8_load_values<ONCE>(rec, rs);
-    }
+    const __amdgpu_buffer_rsrc_t rs0 = kv8_rsrc(head, first, first < nblk);
+    kv8_load_keys<ONCE>(rec, rs0);
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
         uint32_t am = 0;   // largest magnitude, as bf16 bits
@@ -813,6 +810,10 @@ __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv
         at[2 * 64] = make_uint2(l[0], l[1]);
         if (d8 == 0) s_cx[r] = f.cx;
     }
+    asm volatile("" ::: "memory");   // the values behind the forming: a full memory queue would hold it up
+    kv8_load_value_scales<ONCE>(rec, rs0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) kv8_load_value<ONCE>(rec, rs0, j);
     kv8_lds_wait();
     __builtin_amdgcn_s_barrier();   // (not __syncthreads, which would wait for the records too)
     asm volatile("" ::: "memory");
