@@ -1032,6 +1032,12 @@ __device__ __forceinline__ float kv8_max3(float a, float b, float c) {
     return r;
 }
 
+// Two probabilities as they are multiplied, in fp16, added to s in fp32.
+__device__ __forceinline__ float kv8_sum2(uint32_t p, float s) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), h2{(_Float16)1.0f, (_Float16)1.0f}, s, false);
+}
+
 // Key scales are held times 2^-18, so that a score stays finite before its row's
 // factor.  Value operands are fp16: codes times their scale over 2^(E - kValueBits),
 // 2^E the power of two above the largest value scale so far, E at least kMinExp: integers
@@ -1272,12 +1278,12 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
 #pragma unroll
         for (int i = 0; i < MM; ++i) {
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                x[i][y] = __builtin_amdgcn_exp2f(fmaf(x[i][y], Q.cx[i], -top[i]));
-                l[i] += x[i][y];
-            }
+            for (int y = 0; y < 8; ++y) x[i][y] = __builtin_amdgcn_exp2f(fmaf(x[i][y], Q.cx[i], -top[i]));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) pb[i][j] = kv8_pack_f16(x[i][2 * j], x[i][2 * j + 1]);
+            for (int j = 0; j < 4; ++j) {
+                pb[i][j] = kv8_pack_f16(x[i][2 * j], x[i][2 * j + 1]);
+                l[i] = kv8_sum2(pb[i][j], l[i]);
+            }
         }
     };
     constexpr std::integral_constant<int, 2> kBoth{};
@@ -1461,10 +1467,10 @@ int split_groups(int n_kv) { return std::min(std::max(1, vmi::device_cus() / n_k
 
 // 16-row groups of a k_kv8_split workgroup.  Two for more than 16 rows over a cache
 // that gives a wave three records or more: the groups' workgroups read the cache once
-// each, which costs nothing while its records come from L2 (four tokens at 16,000
-// positions 15.6 us in one-group workgroups, 15.9 in two-group ones, at 32,764 18.9 and
-// 18.9; eight at 16,000 22.2 and 27.1) and the rate of HBM beyond (four at 64,000 28.8
-// and 23.4, at 262,000 89 and 56; eight at 64,000 49 and 43).  The results are the same.
+// each, which costs nothing while its records come from L2 (us, one group and two: four
+// tokens at 17,000 positions 14.7 and 16.8, at 32,764 18.0 and 18.0; eight 21.0 and 25.4,
+// 26.9 and 30.8) and the rate of HBM beyond (four at 64,000 26.6 and 23.0, eight at
+// 50,000 38.2 and 36.5).  The results are the same.
 int split_row_groups(int rows, int records, int groups) {
     return rows > 16 && records >= 3 * kSplitWaves * groups ? 2 : 1;
 }
