@@ -5,13 +5,11 @@
 // A row (one position's key or value of one kv head, 256 dims) is held as
 // codes c in [-127, 127] and one fp32 scale s, and stands for s c:
 //   a = max |x|,  s = a / 127,  c = RNE(127 x / a)     (a = 0: s = 0, c = 0)
-// For bf16 x no quotient that is not a tie comes closer to one than 2^-8 / 510; the
-// one fma and, next to ties, the one division that take it here (kv8_quantise) round
-// by less, so the codes are those of exact arithmetic.  A row with an infinity or
-// NaN has s = NaN and reads back as NaN.  A scale belongs to one row: a scale shared
-// by several positions would change what is held of a position with the ones behind
-// it (rejected drafts, a row that is not finite), and an append would round the open
-// block again.  It costs 8 bytes beside a position's 512.
+// For bf16 x the codes are those of exact arithmetic (kv8_quantise).  A row with an
+// infinity or NaN has s = NaN and reads back as NaN.  A scale belongs to one row: a scale
+// shared by several positions would change what is held of a position with the ones
+// behind it (rejected drafts, a row that is not finite), and an append would round the
+// open block again.  It costs 8 bytes beside a position's 512.
 //
 // Layout: per kv head max_len / 32 records of 16,640 bytes, 32 positions each:
 //   [0, 8192)        key codes (int8): position kt, dim d at
@@ -53,39 +51,37 @@ constexpr uint32_t kKeySign = 0x80808080u;   // a word's codes + 128 and the cod
 
 // N elements of a row per lane, the row's largest magnitude a and whether the row
 // holds an infinity or NaN (alike in every lane of the row): the codes + 128, four to
-// a word, and the scale.  127 x / a is taken as x (127 / a) in one fma that adds 2^23 +
-// 2^22 + 128, whose sum's low byte is the code rounded to nearest even: off by at most
-// 127 * 2^-24 before that rounding.  Where some element comes within 2e-5 of a tie, or
-// 127 / a leaves fp32's range, the wave takes the quotients themselves (about one row
-// in fifty).
-template <int N>
-__device__ __forceinline__ void kv8_quantise(const float (&x)[N], float a, bool bad, uint32_t (&w)[N / 4], float& scale) {
+// a word, and the scale.  127 x / a is taken as x (127 / a), off by at most three parts in
+// 2^24, and rounded by adding 2^23 + 2^22 + 128, whose sum's low byte is the code.  BF16:
+// x has eight bits, and its quotient is a tie or 2^-17 of itself and more away from
+// one (|254 x - (2 n + 1) a| is a multiple of x's last bit): rounded to twenty bits
+// first, it goes to the even code exactly where it should (checked for every pair of
+// mantissas).  A tie is no rare case, one element in some six hundred: a division where
+// a wave has one took twice the instructions, and the store 30 us in place of 20.
+template <int N, bool BF16>
+__device__ __forceinline__ void kv8_quantise(float (&x)[N], float a, bool bad, uint32_t (&w)[N / 4], float& scale) {
     scale = bad ? __builtin_nanf("") : __fdiv_rn(a, 127.0f);
-    const bool plain = a > 0x1p-100f && a < 0x1p100f;
-    constexpr float kMagic = 12582912.0f + 128.0f;
-    const float inv = plain && !bad ? __fdiv_rn(127.0f, a) : 0.0f;
+    if (__any(a < 0x1p-100f && a > 0.0f)) {   // 127 / a would leave fp32
+        const float k = a < 0x1p-100f ? 0x1p64f : 1.0f;
+        a *= k;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= k;
+    }
+    const float inv = a > 0.0f && !bad ? __fdiv_rn(127.0f, a) : 0.0f;
     uint32_t t[N];
-    float off = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float m = fmaf(x[i], inv, kMagic);
-        t[i] = __float_as_uint(m);
-        off = fmaxf(off, fabsf(fmaf(x[i], inv, kMagic - m)));
-    }
-    if (__any(off > 0.49998f || (!plain && a > 0.0f && !bad))) {
-        const float k = a > 0x1p100f ? 0x1p-7f : 1.0f, den = a * k, num = 127.0f * k;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = a > 0.0f && !bad ? (int)rintf(__fdiv_rn(x[i] * num, den)) : 0;
-            t[i] = (uint32_t)(c + 128);
-        }
+        constexpr float kMagic = 12582912.0f + 128.0f;
+        if constexpr (BF16)
+            t[i] = __float_as_uint(__uint_as_float((__float_as_uint(x[i] * inv) + 8u) & ~15u) + kMagic);
+        else
+            t[i] = __float_as_uint(fmaf(x[i], inv, kMagic));
     }
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
         const uint32_t lo = __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0c0c0400u);
         const uint32_t hi = __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x04000c0cu);
-        w[i] = lo | hi;
-        if (bad) w[i] = 0x80808080u;
+        w[i] = bad ? 0x80808080u : lo | hi;
     }
 }
 
@@ -101,12 +97,14 @@ struct WriteArgs {
 // Sixteen bf16 of a row per lane (two 16-byte pieces), sixteen lanes a row: codes
 // and scale.
 __device__ __forceinline__ void kv8_row16(const vmi_u4& p0, const vmi_u4& p1, uint32_t (&w)[4], float& scale) {
-    uint32_t am = 0;   // largest magnitude, as bf16 bits: infinities and NaN above the finite ones
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+    us2 pm = {0, 0};   // largest magnitude, as bf16 bits: infinities and NaN above the finite ones
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        am = max(am, max(p0[i] & 0x7fffu, (p0[i] >> 16) & 0x7fffu));
-        am = max(am, max(p1[i] & 0x7fffu, (p1[i] >> 16) & 0x7fffu));
+        pm = __builtin_elementwise_max(pm, __builtin_bit_cast(us2, (uint32_t)p0[i] & 0x7fff7fffu));
+        pm = __builtin_elementwise_max(pm, __builtin_bit_cast(us2, (uint32_t)p1[i] & 0x7fff7fffu));
     }
+    uint32_t am = max((uint32_t)pm[0], (uint32_t)pm[1]);
     am = max(am, vmi_dpp_u32<VMI_DPP_XOR1>(am));
     am = max(am, vmi_dpp_u32<VMI_DPP_XOR2>(am));
     am = max(am, vmi_dpp_u32<VMI_DPP_HALF_MIRROR>(am));
@@ -119,7 +117,7 @@ __device__ __forceinline__ void kv8_row16(const vmi_u4& p0, const vmi_u4& p1, ui
         x[8 + 2 * i] = __uint_as_float(p1[i] << 16);
         x[8 + 2 * i + 1] = __uint_as_float(p1[i] & 0xffff0000u);
     }
-    kv8_quantise<16>(x, __uint_as_float(am << 16), am >= 0x7f80u, w, scale);
+    kv8_quantise<16, true>(x, __uint_as_float(am << 16), am >= 0x7f80u, w, scale);
 }
 
 // Four words of codes, one position each, four dims a word: four words of one dim,
@@ -144,8 +142,8 @@ __device__ __forceinline__ int kv8_unit(int u) { return u ^ (((u >> 4) & 3) << 2
 // order, a kilobyte a wave.  Bytes of positions outside the call are left as they are:
 // a key's unit is one position's, and a group of eight positions' values that is not
 // covered goes byte by byte.  Bound by the bytes of the rows and of the cache: 32768
-// positions of two heads, 101 MB, in 27 us (3.7 TB/s; a copy of that size 20); one
-// position 4.6 us with the read back of it, two launches' latency.
+// positions of two heads, 101 MB, in 19.6 us (5.2 TB/s; a large copy's rate is 5.1), 131072
+// in 70.5 (5.7).
 template <bool VALUES>
 __device__ __forceinline__ void kv8_write_record(const WriteArgs& a, uint8_t* s_mem) {
     constexpr int kPad = kHeadDim + 4;
@@ -385,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) bad = bad || !(fabsf(x[i][j]) < INFINITY);
-        kv8_quantise<4>(x[i], vmi_wave_max(big), __any(bad), cw, s);
+        kv8_quantise<4, false>(x[i], vmi_wave_max(big), __any(bad), cw, s);
         const uint32_t c = is_v ? cw[0] : cw[0] ^ kKeySign;
         if (a.tree) {  // plain rows, one record per token
             if (!mine) continue;
