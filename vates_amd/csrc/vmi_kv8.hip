@@ -281,6 +281,27 @@ __device__ __forceinline__ int kv8_pos0(int pos0, const int32_t* pos_dev, int sp
     return min(max(p, 0), max_len - span);
 }
 
+// (cos, sin) of pos * base^fi, base = theta^(-2/rd), fi < half: the angle in quarter
+// turns in double, to the nearest axis, then Taylor's series over an eighth of a turn (to
+// x^9 and x^10: within 2^-28).  The general functions took as many instructions as the
+// rest of the heads' kernel, which they bound.
+__device__ __forceinline__ float2 kv8_rotary_cs(int pos, int fi, int half, double base) {
+    double f = 1.0, b = base;
+    for (int k = 0; (half - 1) >> k; ++k) {   // wave-uniform
+        f = (fi >> k) & 1 ? f * b : f;
+        b *= b;
+    }
+    const double quarters = (double)pos * (f * 0.6366197723675814);   // 2 / pi
+    const double axis = rint(quarters);
+    const float x = (float)((quarters - axis) * 1.5707963267948966), z = x * x;
+    const int n = (int)axis;
+    const float sn = fmaf(x * z, fmaf(z, fmaf(z, fmaf(z, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -1.6666667e-1f), x);
+    const float cs = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -2.7557319e-7f, 2.4801587e-5f), -1.3888889e-3f), 4.1666667e-2f), -0.5f), 1.0f);
+    const float c = n & 1 ? sn : cs, d = n & 1 ? cs : sn;
+    return make_float2(__uint_as_float(__float_as_uint(c) ^ (uint32_t)((n + 1) & 2) << 30),
+                       __uint_as_float(__float_as_uint(d) ^ (uint32_t)(n & 2) << 30));
+}
+
 // One row, dims 4 l .. in lane l: RMSNorm times the weight, then the rotary
 // pairs (i, i + rd/2), in fp32.
 __device__ __forceinline__ void kv8_norm_rope(float (&x)[4], const float (&nw)[4], float eps, const float2* cs, int rd,
@@ -290,7 +311,9 @@ __device__ __forceinline__ void kv8_norm_rope(float (&x)[4], const float (&nw)[4
 #pragma unroll
     for (int j = 0; j < 4; ++j) ss = fmaf(x[j], x[j], ss);
     ss = vmi_wave_sum_canon(ss);
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / (float)kHeadDim) + eps));
+    // the hardware's reciprocal square root and one Newton step (a sum past fp32 gives 0)
+    const float var = fmaf(ss, 1.0f / (float)kHeadDim, eps), r = __builtin_amdgcn_rsqf(var);
+    const float inv = var < INFINITY ? fmaf(0.5f * r, fmaf(-var * r, r, 1.0f), r) : r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (x[j] * inv) * nw[j];
     float pr[4];
@@ -357,10 +380,9 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) nw[j] = vmi_bf16_to_f32(nwp[4 * lane + j]);
         const int half = a.rope_dim / 2;
-        for (int i = threadIdx.x; i < kHeadTok * half; i += kThreads) {
-            const int kt = i / half, f = i - kt * half;
-            if (kt >= lo && kt < hi) s_cs[kt][f] = rotary_cs(p0 + kt, f, a.rope_base);
-        }
+        const int kt = threadIdx.x / (kThreads / kHeadTok);
+        for (int f = threadIdx.x % (kThreads / kHeadTok); f < half; f += kThreads / kHeadTok)
+            if (kt >= lo && kt < hi) s_cs[kt][f] = kv8_rotary_cs(p0 + kt, f, half, a.rope_base);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
