@@ -303,6 +303,32 @@ __global__ __launch_bounds__(kThreads) void k_kv8_read(ReadArgs a) {
     }
 }
 
+// Lane l and lane l ^ 32 (l ^ 16): both lanes' values, the lower lane's first.
+__device__ __forceinline__ float2 kv8_pair32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float2 kv8_pair16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float kv8_max32(float v) {
+    const float2 p = kv8_pair32(v);
+    return fmaxf(p.x, p.y);
+}
+__device__ __forceinline__ float kv8_max16(float v) {
+    const float2 p = kv8_pair16(v);
+    return fmaxf(p.x, p.y);
+}
+__device__ __forceinline__ float kv8_sum32(float v) {
+    const float2 p = kv8_pair32(v);
+    return p.x + p.y;
+}
+__device__ __forceinline__ float kv8_sum16(float v) {
+    const float2 p = kv8_pair16(v);
+    return p.x + p.y;
+}
+
 // ------------------------------------------------------------------- heads
 using vmi::Kv8Heads;
 
@@ -332,59 +358,79 @@ __device__ __forceinline__ float2 kv8_rotary_cs(int pos, int fi, int half, doubl
                        __uint_as_float(__float_as_uint(d) ^ (uint32_t)(n & 2) << 30));
 }
 
-// One row, dims 4 l .. in lane l: RMSNorm times the weight, then the rotary
-// pairs (i, i + rd/2), in fp32.
-__device__ __forceinline__ void kv8_norm_rope(float (&x)[4], const float (&nw)[4], float eps, const float2* cs, int rd,
+// A row in half a wave, dims 8 l .. in lane l of it: its sum, its largest (as bits of a
+// magnitude), alike in every lane.
+__device__ __forceinline__ float kv8_row_sum(float v) {
+    v += __uint_as_float(vmi_dpp_u32<VMI_DPP_XOR1>(__float_as_uint(v)));
+    v += __uint_as_float(vmi_dpp_u32<VMI_DPP_XOR2>(__float_as_uint(v)));
+    v += __uint_as_float(vmi_dpp_u32<VMI_DPP_HALF_MIRROR>(__float_as_uint(v)));
+    v += __uint_as_float(vmi_dpp_u32<VMI_DPP_MIRROR>(__float_as_uint(v)));
+    return kv8_sum16(v);
+}
+__device__ __forceinline__ uint32_t kv8_row_max(uint32_t v) {
+    v = max(v, vmi_dpp_u32<VMI_DPP_XOR1>(v));
+    v = max(v, vmi_dpp_u32<VMI_DPP_XOR2>(v));
+    v = max(v, vmi_dpp_u32<VMI_DPP_HALF_MIRROR>(v));
+    v = max(v, vmi_dpp_u32<VMI_DPP_MIRROR>(v));
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+
+// Such a row: RMSNorm times the weight, then the rotary pairs (i, i + rd/2), in fp32.
+// srow: 256 floats of the row's own.
+__device__ __forceinline__ void kv8_norm_rope(float (&x)[8], const float (&nw)[8], float eps, const float2* cs, int rd,
                                               float* srow) {
-    const int lane = threadIdx.x & 63, half = rd / 2;
+    const int l = threadIdx.x & 31, half = rd / 2;
     float ss = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ss = fmaf(x[j], x[j], ss);
-    ss = vmi_wave_sum_canon(ss);
+    for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+    ss = kv8_row_sum(ss);
     // the hardware's reciprocal square root and one Newton step (a sum past fp32 gives 0)
     const float var = fmaf(ss, 1.0f / (float)kHeadDim, eps), r = __builtin_amdgcn_rsqf(var);
     const float inv = var < INFINITY ? fmaf(0.5f * r, fmaf(-var * r, r, 1.0f), r) : r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (x[j] * inv) * nw[j];
-    float pr[4];
-    if (rd % 8 == 0) {  // wave-uniform: the partners of a lane's dims are another lane's
-        const int src = (4 * lane < half ? lane + half / 4 : lane - half / 4) & 63;
+    for (int j = 0; j < 8; ++j) x[j] = (x[j] * inv) * nw[j];
+    float pr[8];
+    if (rd % 16 == 0) {  // wave-uniform: the partners of a lane's dims are another lane's
+        const int src = (8 * l < half ? l + half / 8 : l - half / 8) & 31;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pr[j] = __shfl(x[j], src, 64);
+        for (int j = 0; j < 8; ++j) pr[j] = __shfl(x[j], src, 32);
     } else {
-        *reinterpret_cast<float4*>(srow + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4)
+            *reinterpret_cast<float4*>(srow + 8 * l + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();  // srow is this wave's own
+        __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int d = 4 * lane + j;
+        for (int j = 0; j < 8; ++j) {
+            const int d = 8 * l + j;
             pr[j] = srow[d < half ? d + half : d < rd ? d - half : d];
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();  // read before the next row is written
     }
+    if (8 * l < rd) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int d = 4 * lane + j;
-        if (d < rd) {
-            const float2 c = cs[d < half ? d : d - half];
-            x[j] = fmaf(x[j], c.x, (d < half ? -pr[j] : pr[j]) * c.y);
+        for (int j = 0; j < 8; ++j) {
+            const int d = 8 * l + j;
+            if (rd % 16 == 0 || d < rd) {
+                const float2 c = cs[d < half ? d : d - half];
+                x[j] = fmaf(x[j], c.x, (d < half ? -pr[j] : pr[j]) * c.y);
+            }
         }
     }
 }
 
 constexpr int kHeadTok = 8;  // positions of a workgroup: one value group of a record
 
-// grid (groups of eight positions, heads (q, then k, then v), paths): a wave
-// takes the group's tokens w and w + 4 of one head.  Keys go out 4 bytes a lane;
-// a value group's eight positions are collected in LDS and go out together.
-// Bound by the bytes of the projections on a prompt, by latency on a batch.
+// grid (groups of eight positions, heads (q, then k, then v), paths): half a wave takes
+// one of the group's tokens of one head, sixteen bytes a lane in and out.  A value
+// group's eight positions are collected in LDS and go out together.  Bound by the
+// bytes of the projections on a prompt, by latency on a batch.
 __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
     __shared__ float2 s_cs[kHeadTok][kHeadDim / 2];
-    __shared__ float s_row[kWaves][kHeadDim];
+    __shared__ __attribute__((aligned(16))) float s_row[kHeadTok][kHeadDim];
     __shared__ __attribute__((aligned(16))) uint8_t s_v[kHeadDim][kHeadTok];
-    const int lane = threadIdx.x & 63, w = at_wave(), path = blockIdx.z;
+    const int l = threadIdx.x & 31, row = threadIdx.x >> 5, path = blockIdx.z;
     const int pos0 = kv8_pos0(a.pos0, a.pos_dev, a.T, a.max_len);
     if (a.pos_dev && a.status && blockIdx.x == 0 && blockIdx.y == 0 && path == 0 && threadIdx.x == 0 && *a.pos_dev != pos0)
         atomicOr(a.status, VMI_STATUS_BAD_POS);
@@ -395,73 +441,72 @@ __global__ __launch_bounds__(kThreads) void k_kv8_heads(Kv8Heads a) {
     const bool is_q = hh < a.n_heads, is_v = hh >= a.n_heads + a.n_kv;
     const int stride = (a.n_heads + a.n_kv) * 2 * kHeadDim;
     const int col = is_q ? hh * 2 * kHeadDim : a.n_heads * 2 * kHeadDim + (hh - a.n_heads) * kHeadDim;
-    const float* rows = a.qkv + (size_t)path * a.T * stride + col + 4 * lane;
-    float x[2][4];
+    const int kt = min(max(row, lo), hi - 1);
+    const bool mine = kt == row;
+    const int t = p0 + kt - pos0, tb = (p0 + kt) % kBlk;
+    const float* src = a.qkv + ((size_t)path * a.T + t) * stride + col + 8 * l;
+    float x[8];
+    {
+        const vmi_f4 u = *reinterpret_cast<const vmi_f4*>(src), v = *reinterpret_cast<const vmi_f4*>(src + 4);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int kt = min(max(w + kWaves * i, lo), hi - 1);
-        const vmi_f4 v = *reinterpret_cast<const vmi_f4*>(rows + (size_t)(p0 + kt - pos0) * stride);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = v[j];
+        for (int j = 0; j < 4; ++j) {
+            x[j] = u[j];
+            x[4 + j] = v[j];
+        }
     }
     if (!is_v) {
         const uint16_t* nwp = is_q ? a.q_norm : a.k_norm;
-        float nw[4];
+        float nw[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) nw[j] = vmi_bf16_to_f32(nwp[4 * lane + j]);
+        for (int j = 0; j < 8; ++j) nw[j] = vmi_bf16_to_f32(nwp[8 * l + j]);
         const int half = a.rope_dim / 2;
-        const int kt = threadIdx.x / (kThreads / kHeadTok);
-        for (int f = threadIdx.x % (kThreads / kHeadTok); f < half; f += kThreads / kHeadTok)
-            if (kt >= lo && kt < hi) s_cs[kt][f] = kv8_rotary_cs(p0 + kt, f, half, a.rope_base);
+        if (mine)
+            for (int f = l; f < half; f += 32) s_cs[row][f] = kv8_rotary_cs(p0 + row, f, half, a.rope_base);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            kv8_norm_rope(x[i], nw, a.eps, s_cs[min(max(w + kWaves * i, lo), hi - 1)], a.rope_dim, s_row[w]);
+        kv8_norm_rope(x, nw, a.eps, s_cs[kt], a.rope_dim, s_row[row]);
+    }
+    if (is_q) {
+        if (mine)
+            *reinterpret_cast<vmi_u4*>(a.q + ((size_t)(path * a.T + t) * a.n_heads + hh) * kHeadDim + 8 * l) =
+                vmi_u4{vmi_pack_bf16x2(x[0], x[1]), vmi_pack_bf16x2(x[2], x[3]), vmi_pack_bf16x2(x[4], x[5]),
+                       vmi_pack_bf16x2(x[6], x[7])};
+        return;
     }
     const int g = is_v ? hh - a.n_heads - a.n_kv : hh - a.n_heads;
+    uint32_t am = 0;   // largest magnitude, as bits: infinities and NaN above the finite ones
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int kt = w + kWaves * i, t = p0 + kt - pos0, tb = (p0 + kt) % kBlk;
-        const bool mine = kt >= lo && kt < hi;   // wave-uniform
-        if (is_q) {
-            if (mine)
-                *reinterpret_cast<uint2*>(a.q + ((size_t)(path * a.T + t) * a.n_heads + hh) * kHeadDim + 4 * lane) =
-                    make_uint2(vmi_pack_bf16x2(x[i][0], x[i][1]), vmi_pack_bf16x2(x[i][2], x[i][3]));
-            continue;
-        }
-        float s;
-        uint32_t cw[1];
-        const float big = fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bad = bad || !(fabsf(x[i][j]) < INFINITY);
-        kv8_quantise<4, false>(x[i], vmi_wave_max(big), __any(bad), cw, s);
-        const uint32_t c = is_v ? cw[0] : cw[0] ^ kKeySign;
-        if (a.tree) {  // plain rows, one record per token
-            if (!mine) continue;
-            uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * a.T + t) * kKv8TreeRow;
-            *reinterpret_cast<uint32_t*>(side + (is_v ? kHeadDim : 0) + 4 * lane) = c;
-            if (lane == 0) *reinterpret_cast<float*>(side + 2 * kHeadDim + (is_v ? 4 : 0)) = s;
-            continue;
-        }
-        uint8_t* rec = a.cache + ((size_t)g * (a.max_len / kBlk) + p0 / kBlk) * kRec;
-        if (mine && lane == 0) *reinterpret_cast<float*>(rec + kv8_scale_off(tb, is_v)) = s;
-        if (!is_v) {
-            if (mine) *reinterpret_cast<uint32_t*>(rec + kv8_k_off(tb, 4 * lane)) = c;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s_v[4 * lane + j][kt] = (uint8_t)(c >> (8 * j));
-        }
+    for (int j = 0; j < 8; ++j) am = max(am, __float_as_uint(x[j]) & 0x7fffffffu);
+    am = kv8_row_max(am);
+    float s;
+    uint32_t c[2];
+    kv8_quantise<8, false>(x, __uint_as_float(am), am >= 0x7f800000u, c, s);
+    if (!is_v) {
+        c[0] ^= kKeySign;
+        c[1] ^= kKeySign;
     }
-    if (!is_v || a.tree) return;
+    if (a.tree) {  // plain rows, one record per token
+        if (!mine) return;
+        uint8_t* side = a.tree + ((size_t)(path * a.n_kv + g) * a.T + t) * kKv8TreeRow;
+        *reinterpret_cast<uint2*>(side + (is_v ? kHeadDim : 0) + 8 * l) = make_uint2(c[0], c[1]);
+        if (l == 0) *reinterpret_cast<float*>(side + 2 * kHeadDim + (is_v ? 4 : 0)) = s;
+        return;
+    }
+    uint8_t* rec = a.cache + ((size_t)g * (a.max_len / kBlk) + p0 / kBlk) * kRec;
+    if (mine && l == 0) *reinterpret_cast<float*>(rec + kv8_scale_off(tb, is_v)) = s;
+    if (!is_v) {
+        if (mine) *reinterpret_cast<uint2*>(rec + kv8_k_off(tb, 8 * l)) = make_uint2(c[0], c[1]);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_v[8 * l + j][row] = (uint8_t)(c[j >> 2] >> (8 * (j & 3)));
     __syncthreads();
     // thread d: dim d of the group's eight positions
     const int d = threadIdx.x;
-    uint8_t* dst = a.cache + ((size_t)g * (a.max_len / kBlk) + p0 / kBlk) * kRec + kv8_v_off(p0 % kBlk, d);
+    uint8_t* dst = rec + kv8_v_off(p0 % kBlk, d);
     if (lo == 0 && hi == kHeadTok) {
         *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(s_v[d]);
     } else {
-        for (int kt = lo; kt < hi; ++kt) dst[kt] = s_v[d][kt];
+        for (int i = lo; i < hi; ++i) dst[i] = s_v[d][i];
     }
 }
 
@@ -492,32 +537,6 @@ __device__ __forceinline__ uint32_t kv8_pack_f16(float a, float b) {  // one con
     typedef float f2 __attribute__((ext_vector_type(2)));
     const f2 v = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
-}
-
-// Lane l and lane l ^ 32 (l ^ 16): both lanes' values, the lower lane's first.
-__device__ __forceinline__ float2 kv8_pair32(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float2 kv8_pair16(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float kv8_max32(float v) {
-    const float2 p = kv8_pair32(v);
-    return fmaxf(p.x, p.y);
-}
-__device__ __forceinline__ float kv8_max16(float v) {
-    const float2 p = kv8_pair16(v);
-    return fmaxf(p.x, p.y);
-}
-__device__ __forceinline__ float kv8_sum32(float v) {
-    const float2 p = kv8_pair32(v);
-    return p.x + p.y;
-}
-__device__ __forceinline__ float kv8_sum16(float v) {
-    const float2 p = kv8_pair16(v);
-    return p.x + p.y;
 }
 
 // Scores are sums of int8 products, exact in int32: a query row is held as 16-bit
