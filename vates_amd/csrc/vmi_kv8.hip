@@ -826,7 +826,7 @@ constexpr int kSplitWaves = 4, kSplitThreads = 64 * kSplitWaves;
 // maximum, sum and unnormalised output of each row, in fp32.  Bound by the bytes of
 // the cache from some ten thousand positions on (one token of 16 heads on 2 at
 // 262,143: 47 us, 5.8 TB/s), below by the latency of a record and of the two launches
-// (at 1000: 8 us; four tokens at 32,764, a record or two a wave: 19).
+// (at 1000: 7.4 us; four tokens at 32,764, two records a wave: 17.9).
 template <int MS, bool ONCE>
 __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) float s_o[kSplitWaves * 16 * kHeadDim];   // one row group of each wave
@@ -1170,9 +1170,9 @@ __device__ __forceinline__ void kv8_finish_rows(const Kv8Attn& a, const vmi_f4 (
 // Part z of P takes an equal run of the tile's records; with P > 1 the parts are written
 // as k_kv8_split's are.
 //
-// 4096 tokens behind 8192, 16 heads on 2: 640 us, 1.07 PFLOP/s (a large bf16 matrix
+// 4096 tokens behind 8192, 16 heads on 2: 630 us, 1.09 PFLOP/s (a large bf16 matrix
 // product reaches 1.23); with every wave in step 915, with the tiles unpaired 713.  A phase
-// takes some 1900 cycles, its 64 matrix instructions 1024 of them: what is left is a
+// takes some 1850 cycles, its 64 matrix instructions 1024 of them: what is left is a
 // single wave's instruction issue and the latency of its first LDS reads.  256
 // registers a lane are full; deeper operand prefetch spills.
 __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
