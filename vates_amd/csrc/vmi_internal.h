@@ -107,7 +107,7 @@ struct Kv8Attn {
     int64_t gate_tok, gate_head;
     uint16_t* o;           // [paths * span, n_heads, 256]
     uint32_t* status;      // or null
-    int rp;                // set by the launch: rows of a part, and the parts
+    int rp, run;           // set by the launch: rows of a part, records of one, and the parts
     float *part_o, *part_ml;
 };
 bool kv8_heads_ok(int n_heads, int n_kv);

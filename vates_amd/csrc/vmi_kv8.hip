@@ -1054,18 +1054,34 @@ __global__ __launch_bounds__(kThreads) void k_kv8_merge(Kv8Attn a, int parts) {
     *reinterpret_cast<uint2*>(a.o + ((size_t)t * a.n_heads + h) * kHeadDim + d0) = kv8_gated(y, __fdiv_rn(1.0f, l), gp);
 }
 
-// k_kv8_flash's parts, few of many rows: a wave per row, four dims a lane, the parts
-// in order.  A part may hold nothing of a row (its maximum is then the lowest).
+constexpr int kFlashWaves = 8, kFlashThreads = 64 * kFlashWaves, kFlashM = 2, kTileRows = 16 * kFlashWaves;
+
+// Records that a tile of 128 rows of R sees.
+__device__ __forceinline__ int kv8_tile_records(int pos0, int tile, int R, int G) {
+    return (pos0 + (min((tile + 1) * kTileRows, R) - 1) / G) / kBlk + 1;
+}
+
+// The flash kernels' parts, few of many rows: a wave per row, four dims a lane, the parts
+// in order.  A part may hold nothing of a row (its maximum is then the lowest).  With
+// a.run k_kv8_flash_short's, as many as a row's tile has; rows that have one are out
+// already.
 __global__ __launch_bounds__(kThreads) void k_kv8_merge_rows(Kv8Attn a, int parts) {
     const int lane = threadIdx.x & 63, r = blockIdx.x * kWaves + at_wave();
     const int t = r / a.n_heads, h = r % a.n_heads, G = a.n_heads / a.n_kv, g = h / G;
     if (t >= a.span) return;
-    const size_t at = (size_t)g * parts * a.rp + t * G + h % G;
+    const int row = t * G + h % G;
+    int n = parts;
+    if (a.run) {
+        const int pos0 = kv8_pos0(a.pos0, a.pos_dev, a.span, a.max_len);
+        n = (kv8_tile_records(pos0, row / kTileRows, a.span * G, G) + a.run - 1) / a.run;
+        if (n == 1) return;
+    }
+    const size_t at = (size_t)g * parts * a.rp + row;
     float M = -3.402823466e38f, l = 0.0f;
-    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[(at + (size_t)s * a.rp) * 2]);
+    for (int s = 0; s < n; ++s) M = fmaxf(M, a.part_ml[(at + (size_t)s * a.rp) * 2]);
     vmi_f4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
+    for (int s = 0; s < n; ++s) {
         const size_t p = at + (size_t)s * a.rp;
         const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
         const vmi_f4 z = *reinterpret_cast<const vmi_f4*>(a.part_o + p * kHeadDim + 4 * lane);
@@ -1077,8 +1093,6 @@ __global__ __launch_bounds__(kThreads) void k_kv8_merge_rows(Kv8Attn a, int part
     const float* gate = a.gate ? a.gate + t * a.gate_tok + h * a.gate_head + 4 * lane : nullptr;
     *reinterpret_cast<uint2*>(a.o + ((size_t)t * a.n_heads + h) * kHeadDim + 4 * lane) = kv8_gated(y, __fdiv_rn(1.0f, l), gate);
 }
-
-constexpr int kFlashWaves = 8, kFlashThreads = 64 * kFlashWaves, kFlashM = 2, kTileRows = 16 * kFlashWaves;
 
 // Codes of a value record as fp16 integers, exactly (0x6400 is 1024 with a
 // mantissa step of 1), times their positions' factors f.
@@ -1125,13 +1139,13 @@ __device__ __forceinline__ int kv8_lane() {
     return l;
 }
 
-// Row `row` of a flash kernel's sums: o times u, maximum and sum, out or as part z of P.
+// Row `row` of a flash kernel's sums: o times u, maximum and sum, out or as part z.
 __device__ __forceinline__ void kv8_finish_rows(const Kv8Attn& a, const vmi_f4 (&o)[16], float top, float sum, float u,
-                                                int row, int R) {
+                                                int row, int R, bool out) {
     const int q4 = kv8_lane() >> 4, g = blockIdx.y, G = a.n_heads / a.n_kv, P = gridDim.z;
     if (row >= R) return;
     const int t = row / G, h = g * G + row % G;
-    if (P > 1) {
+    if (!out) {
         const size_t at = (size_t)(g * P + blockIdx.z) * a.rp + row;
 #pragma unroll
         for (int d = 0; d < 16; ++d)
@@ -1191,9 +1205,8 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     // tile x and, of the other end, its partner: the first sees the fewest keys
     const int tiles = (R + kTileRows - 1) / kTileRows, part = (int)blockIdx.x, other = tiles - 1 - part;
     const int r0[M] = {other * kTileRows + 16 * w, part * kTileRows + 16 * w};
-    auto records = [&](int tile) { return (pos0 + (min((tile + 1) * kTileRows, R) - 1) / G) / kBlk + 1; };
-    const int nb = records(other), b0 = (int)((long)nb * z / P), n = (int)((long)nb * (z + 1) / P) - b0;
-    const int nboth = part < other ? min(max(records(part) - b0, 0), n) : 0;   // records that both tiles see
+    const int nb = kv8_tile_records(pos0, other, R, G), b0 = (int)((long)nb * z / P), n = (int)((long)nb * (z + 1) / P) - b0;
+    const int nboth = part < other ? min(max(kv8_tile_records(pos0, part, R, G) - b0, 0), n) : 0;   // records that both tiles see
     const uint8_t* head = a.cache + ((size_t)g * (a.max_len / kBlk) + b0) * kRec;
     auto issue_scales = [&](int k) {   // every wave the same bytes
         if (k < n) vmi_lds_dma4_at(head + (size_t)k * kRec + 2 * kHalfRec, 4 * kv8_lane(), s_scale[k & 1]);
@@ -1394,13 +1407,15 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     for (int i = 0; i < M; ++i)
         if (i == 0 || part < other)
             kv8_finish_rows(a, o[i], top[i] + (float)kProbBits, kv8_sum32(kv8_sum16(l[i])) * (1.0f / (float)(1 << kProbBits)),
-                            ldexpf(1.0f, ref[i] - kValueBits - kProbBits), r0[i] + (kv8_lane() & 15), R);
+                            ldexpf(1.0f, ref[i] - kValueBits - kProbBits), r0[i] + (kv8_lane() & 15), R, P == 1);
 }
 
 // grid (tiles of 128 rows, n_kv, key parts): k_kv8_flash for little work (flash_plan),
 // where its longer way in and out costs more than its phases give: eight waves of 16
 // rows in step, one barrier a record.  It comes by DMA, two ahead; one ahead the waves
-// turn its values together, over the largest scale of the record.
+// turn its values together, over the largest scale of the record.  A part takes the
+// same number of records in every tile (a.run), so that the last tiles, which see
+// the most, have the most parts; a tile of one part goes out at once.
 __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_key[3][kHalfRec], s_val[2][kHalfRec];   // as stored
     __shared__ __attribute__((aligned(16))) float s_scale[2][2 * kBlk];
@@ -1414,8 +1429,9 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
         atomicOr(a.status, VMI_STATUS_BAD_POS);
     const int tile = (int)gridDim.x - 1 - (int)blockIdx.x;   // late tiles see the most keys: first
     const int r0[1] = {tile * kTileRows + 16 * w};
-    const int nb = (pos0 + (min((tile + 1) * kTileRows, R) - 1) / G) / kBlk + 1;
-    const int b0 = (int)((long)nb * z / P), b1 = (int)((long)nb * (z + 1) / P);
+    const int nb = kv8_tile_records(pos0, tile, R, G);
+    const int b0 = z * a.run, b1 = min(b0 + a.run, nb);
+    if (b0 >= nb) return;   // whole workgroup: a part that this tile does not have
     const uint8_t* head = a.cache + (size_t)g * (a.max_len / kBlk) * kRec;
     const uint32_t at16 = 16 * lane;
     auto issue = [&](int b, int uk, int u) {
@@ -1523,7 +1539,7 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
         for (int d = 0; d < 16; ++d) o[d] = vmi_mfma_f16(V[d * 64], pb, o[d]);
     }
     kv8_finish_rows(a, o, top + (float)kProbBits, kv8_sum32(kv8_sum16(l)) * (1.0f / (float)(1 << kProbBits)),
-                    ldexpf(1.0f, ref - kValueBits - kProbBits), r0[0] + nl, R);
+                    ldexpf(1.0f, ref - kValueBits - kProbBits), r0[0] + nl, R, nb <= a.run);
 }
 
 // ------------------------------------------------------------------- host
@@ -1546,27 +1562,42 @@ int split_row_groups(int rows, int records, int groups) {
 
 // Form and grid of more than kSplitRows rows.  k_kv8_flash_short while a CU's share is
 // under sixteen records of a 128-row tile (us, that form and k_kv8_flash: 777 tokens from
-// position 0 39 and 49, 1024 from 0 46 and 55, 200 from 1234 29 and 40, 64 from 0 13 and
+// position 0 35 and 49, 1024 from 0 48 and 55, 200 from 1234 29 and 40, 64 from 0 13 and
 // 28), k_kv8_flash from there (2048 from 0 95 and 90, 300 from 20,000 154 and 127, 4096 from
 // 0 210 and 200, 4096 from 8192 843 and 640).  Parts fill the device where the tiles do
 // not, of four records or more: a part costs its rows' way out and back (100 tokens from
 // 500 in as many parts as records 29, in these 23).
 struct FlashPlan {
     bool paired;
-    int tiles, parts;   // tiles: workgroups per kv head and part
+    int tiles, parts, run;   // workgroups per kv head and part; records of a part of the short form
 };
-FlashPlan flash_plan(int rows, int n_kv, int records, bool paired) {
-    FlashPlan p;
-    p.paired = paired;
-    p.tiles = (rows + kTileRows - 1) / kTileRows;
-    if (paired) p.tiles = (p.tiles + 1) / 2;
-    p.parts = std::max(1, std::min({vmi::device_cus() / (p.tiles * n_kv), kMaxFlashParts, (records + 3) / 4}));
-    return p;
+// The most parts of a form, at any position.
+int flash_max_parts(int tiles, int n_kv, bool paired) {
+    const int ncu = vmi::device_cus();
+    return std::max(1, std::min((paired ? ncu : 2 * ncu) / (tiles * n_kv), kMaxFlashParts));
+}
+int flash_tiles(int rows, bool paired) {
+    const int tiles = (rows + kTileRows - 1) / kTileRows;
+    return paired ? (tiles + 1) / 2 : tiles;
 }
 FlashPlan flash_plan(const Kv8Attn& a, int rows) {
-    const int pos0 = a.pos_dev ? a.max_len - a.span : a.pos0;   // (on the device: by the capacity)
-    const int64_t tiles = (rows + kTileRows - 1) / kTileRows, records = (pos0 + a.span / 2) / kBlk + 1;
-    return flash_plan(rows, a.n_kv, (pos0 + a.span - 1) / kBlk + 1, tiles * a.n_kv * records >= 16 * vmi::device_cus());
+    const int ncu = vmi::device_cus(), pos0 = a.pos_dev ? a.max_len - a.span : a.pos0;   // (on the device: by the capacity)
+    const int64_t all = (int64_t)flash_tiles(rows, false) * a.n_kv;   // tiles of all heads
+    const int mean = (pos0 + a.span / 2) / kBlk + 1, last = (pos0 + a.span - 1) / kBlk + 1;
+    FlashPlan p;
+    p.paired = all * mean >= 16 * ncu;
+    p.tiles = flash_tiles(rows, p.paired);
+    const int most = flash_max_parts(p.tiles, a.n_kv, p.paired);
+    int run = 4;   // records of a part
+    if (!p.paired) {
+        // workgroups: records over run and half a part a tile, of seven eighths of the CUs (the XCDs' shares differ)
+        const int64_t room = 7 * ncu / 8 - all / 2;
+        run = room > 0 ? (int)std::max<int64_t>(run, (all * mean + room - 1) / room) : last;
+        run = std::max(run, (last + most - 1) / most);
+    }
+    p.parts = std::min((last + run - 1) / run, most);
+    p.run = p.paired ? 0 : run;
+    return p;
 }
 
 }  // namespace
@@ -1587,10 +1618,9 @@ size_t vmi::kv8_attention_parts_bytes(int paths, int span, int n_heads, int n_kv
     size_t rows = (size_t)n_kv * split_groups(n_kv) * paths * std::min(R, kSplitRows);
     if (R > kSplitRows)
         for (int tiles = 1; (tiles - 1) * kTileRows < R; ++tiles) {
-            const int r = std::min(tiles * kTileRows, R);
-            const int parts = std::max(flash_plan(r, n_kv, 1 << 20, false).parts, flash_plan(r, n_kv, 1 << 20, true).parts);
+            const int parts = std::max(flash_max_parts(tiles, n_kv, false), flash_max_parts((tiles + 1) / 2, n_kv, true));
             if (parts == 1) break;   // and of more tiles
-            rows = std::max(rows, (size_t)n_kv * parts * r);
+            rows = std::max(rows, (size_t)n_kv * parts * std::min(tiles * kTileRows, R));
         }
     return align256(rows * kHeadDim * 4) + align256(rows * 2 * 4);
 }
@@ -1604,6 +1634,7 @@ hipError_t vmi::launch_kv8_heads(const Kv8Heads& h, int paths, hipStream_t s) {
 hipError_t vmi::launch_kv8_attention(Kv8Attn a, void* parts, hipStream_t s) {
     const int R = a.span * (a.n_heads / a.n_kv);
     a.rp = R;
+    a.run = 0;
     a.part_o = static_cast<float*>(parts);
     int n;
     size_t rows;
@@ -1628,6 +1659,7 @@ hipError_t vmi::launch_kv8_attention(Kv8Attn a, void* parts, hipStream_t s) {
     } else {
         const FlashPlan p = flash_plan(a, R);
         n = p.parts;
+        a.run = p.run;
         rows = n > 1 ? (size_t)a.n_kv * n * R : 1;
         a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(parts) + align256(rows * kHeadDim * 4));
         const dim3 grid(p.tiles, a.n_kv, p.parts), blk(kFlashThreads);
