@@ -357,3 +357,17 @@ def test_strides_that_no_step_takes(gpu):
     q, gate = queries(111, 1, 8, gpu)
     want = attend(q, a, pos0=3, gate=gate)
     assert torch.equal(attend(q, a, pos0=3, gate=gate.as_strided((1, 8, DIM), (1, DIM, 1))), want)
+
+
+@pytest.mark.parametrize("T,pos0", [(9, 40), (100, 0), (100, 5000), (700, 31)])
+def test_device_position_far_below_the_capacity(gpu, T, pos0):
+    """The form and its parts are chosen by the capacity, the work by the position."""
+    log(f"case: kv8 T={T} at {pos0} of 200,000")
+    from vates_amd.attention import attend
+    cache = new_cache(2, 200000, gpu)
+    cache.data.fill_(255)
+    cache.write(0, *rows(120, 2, pos0 + T, gpu))
+    q, gate = queries(121, T, 16, gpu)
+    pos = torch.tensor([pos0], dtype=torch.int32, device=gpu)
+    check_attend(attend(q, cache, pos_device=pos, gate=gate), q, cache, pos0, gate)
+    assert int(cache.status) == 0
