@@ -1561,9 +1561,9 @@ int split_groups(int n_kv) { return std::min(std::max(1, vmi::device_cus() / n_k
 // 16-row groups of a k_kv8_split workgroup.  Two for more than 16 rows over a cache
 // that gives a wave three records or more: the groups' workgroups read the cache once
 // each, which costs nothing while its records come from L2 (us, one group and two: four
-// tokens at 17,000 positions 14.7 and 16.8, at 32,764 18.0 and 18.0; eight 21.0 and 25.4,
-// 26.9 and 30.8) and the rate of HBM beyond (four at 64,000 26.6 and 23.0, eight at
-// 50,000 38.2 and 36.5).  The results are the same.
+// tokens at 17,000 positions 14.6 and 17.2, at 32,764 17.7 and 18.2; eight 21.5 and 26.1,
+// 26.7 and 31.1) and the rate of HBM beyond (four at 64,000 26.5 and 23.1, eight at
+// 50,000 37.9 and 36.8).  The results are the same.
 int split_row_groups(int rows, int records, int groups) {
     return rows > 16 && records >= 3 * kSplitWaves * groups ? 2 : 1;
 }
