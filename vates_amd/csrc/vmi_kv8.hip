@@ -1134,7 +1134,13 @@ __device__ __forceinline__ float kv8_sum2(uint32_t p, float s) {
 // 2^E the power of two above the largest value scale so far, E at least kMinExp: integers
 // times factors of up to 2^kValueBits (eleven bits; a scale below 2^-22 of the largest
 // keeps 2^-33 of the largest value).  Probabilities go to fp16 times 2^kProbBits: a
-// row's reference lags its largest score by up to 2^kLazyMax.
+// row's reference lags its largest score by up to 2^kLazyMax.  A record that some row
+// of its workgroup does not see to its end has no E that is every row's: its value
+// operands are the codes times 2^kValueBits, which is exact, and a position's scale, over
+// the 2^E of the scales that the row itself has seen, enters the row's probability, zero
+// where the row does not see the position.  (With the record's own E there, a later token's row
+// 2^22 times larger took bits from the tokens before it, one 2^34 times larger all.)
+// Costs little: 64 tokens from 0, every record such a one, 13.2 -> 13.6 us, 777 34.3 -> 34.5.
 constexpr float kKeyUnit = 0x1p-18f;
 constexpr int kValueBits = 8, kMinExp = -100, kProbBits = 8;
 constexpr float kLazyMax = 6.0f;
@@ -1170,6 +1176,53 @@ __device__ __forceinline__ void kv8_finish_rows(const Kv8Attn& a, const vmi_f4 (
     }
 }
 
+// The records that every row of a tile of 128 sees to their ends.
+__device__ __forceinline__ int kv8_tile_seen(int pos0, int tile, int R, int G) {
+    return (pos0 + min(tile * kTileRows, R - 1) / G + 1) / kBlk;
+}
+
+// A row's step over a record that it may not see to its end: scores x (before the
+// row's factor cx) of the lane's eight keys, of which those up to `seen` are visible, and
+// their positions' value scales.  Brings the row's reference top and its exponent ref up,
+// the sums o and l with them, and gives the probabilities times their scales, as they
+// are multiplied: below 2^(kProbBits + kLazyMax).
+__device__ __forceinline__ vmi_u4 kv8_masked_weights(float (&x)[8], const vmi_f4 (&vs)[2], int seen, float cx, float& top,
+                                                     int& ref, float& l, vmi_f4 (&o)[16]) {
+    float v[8], big = -INFINITY, vm = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+        x[y] = y > seen ? -INFINITY : x[y];
+        v[y] = y > seen ? 0.0f : vs[y >> 2][y & 3];
+        big = fmaxf(big, x[y]);
+        vm = fmaxf(vm, v[y]);
+    }
+    constexpr float kRaise = kLazyMax + kProbBits;
+    if (__any(fmaf(big, cx, -top) > kRaise || (int)(__float_as_uint(vm) >> 23) - 126 > ref)) {
+        // each row by its own scores and scales: another row's change nothing of it
+        big = kv8_max32(kv8_max16(big));
+        const float nt = fmaf(big, cx, -top) > kRaise ? fmaf(big, cx, -(float)kProbBits) : top;
+        const int e = max(ref, (int)(__float_as_uint(kv8_max32(kv8_max16(vm))) >> 23) - 126);
+        const float f = __builtin_amdgcn_exp2f(top - nt), fo = ldexpf(f, ref - e);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[d][r] *= fo;
+        top = nt;
+        ref = e;
+    }
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+        x[y] = __builtin_amdgcn_exp2f(fmaf(x[y], cx, -top));
+        l += x[y];
+        x[y] *= ldexpf(v[y], -ref);
+    }
+    vmi_u4 pb;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pb[j] = kv8_pack_f16(x[2 * j], x[2 * j + 1]);
+    return pb;
+}
+
 // grid (pairs of tiles of 128 rows, n_kv, key parts): eight waves share each record, each
 // with 16 rows of a tile and 16 of the tile as far from the other end, so that every
 // workgroup sees as many keys: the records that both see are taken with 32 rows a wave
@@ -1192,7 +1245,7 @@ __device__ __forceinline__ void kv8_finish_rows(const Kv8Attn& a, const vmi_f4 (
 // Part z of P takes an equal run of the tile's records; with P > 1 the parts are written
 // as k_kv8_split's are.
 //
-// 4096 tokens behind 8192, 16 heads on 2: 630 us, 1.09 PFLOP/s (a large bf16 matrix
+// 4096 tokens behind 8192, 16 heads on 2: 619 us, 1.11 PFLOP/s (a large bf16 matrix
 // product reaches 1.23); with every wave in step 915, with the tiles unpaired 713.  A phase
 // takes some 1850 cycles, its 64 matrix instructions 1024 of them: what is left is a
 // single wave's instruction issue and the latency of its first LDS reads.  256
@@ -1201,7 +1254,7 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_rec[2][2 * kHalfRec];   // keys and values, as stored
     __shared__ float s_scale[2][2 * kBlk];
     __shared__ vmi_u4 s_f16[2][16 * 64];             // values [dt], 64 lanes each
-    __shared__ __attribute__((aligned(16))) float s_ks[3][kBlk];
+    __shared__ __attribute__((aligned(16))) float s_ks[3][kBlk], s_vs[3][kBlk];
     __shared__ __attribute__((aligned(16))) _Float16 s_vf[3][kBlk];
     __shared__ int s_exp[3];
     constexpr int M = kFlashM, kSchedRead = 0x100, kSchedMfma = 0x8;
@@ -1215,6 +1268,9 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     const int r0[M] = {other * kTileRows + 16 * w, part * kTileRows + 16 * w};
     const int nb = kv8_tile_records(pos0, other, R, G), b0 = (int)((long)nb * z / P), n = (int)((long)nb * (z + 1) / P) - b0;
     const int nboth = part < other ? min(max(kv8_tile_records(pos0, part, R, G) - b0, 0), n) : 0;   // records that both tiles see
+    // of those, and of all, the first that some row does not see to its end
+    const int mboth = min(max(kv8_tile_seen(pos0, part, R, G) - b0, 0), nboth);
+    const int mone = min(max(kv8_tile_seen(pos0, other, R, G) - b0, nboth), n);
     const uint8_t* head = a.cache + ((size_t)g * (a.max_len / kBlk) + b0) * kRec;
     auto issue_scales = [&](int k) {   // every wave the same bytes
         if (k < n) vmi_lds_dma4_at(head + (size_t)k * kRec + 2 * kHalfRec, 4 * kv8_lane(), s_scale[k & 1]);
@@ -1244,11 +1300,14 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
         const int lane = kv8_lane();
         const float ks = s_scale[k & 1][lane & (kBlk - 1)], vs = s_scale[k & 1][kBlk + (lane & (kBlk - 1))];
         const bool ok = vs == vs;
+        // (what a masked record raises E by that a row does not see, no unmasked one of that row's follows)
         if (__any(vs >= ldexpf(1.0f, top_exp)))
             top_exp = max(top_exp, (int)(__float_as_uint(vmi_wave_max(ok ? vs : 0.0f)) >> 23) - 126);
         if (lane < kBlk) {
             s_ks[k % 3][lane] = ok ? ks * kKeyUnit : vs;
-            s_vf[k % 3][lane] = (_Float16)(ok ? ldexpf(vs, kValueBits - top_exp) : 0.0f);
+            s_vs[k % 3][lane] = ok ? vs : 0.0f;
+            const bool masked = k < nboth ? k >= mboth : k >= mone;
+            s_vf[k % 3][lane] = (_Float16)(masked ? (float)(1 << kValueBits) : ok ? ldexpf(vs, kValueBits - top_exp) : 0.0f);
             s_exp[k % 3] = top_exp;
         }
     };
@@ -1322,36 +1381,46 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
                 for (int y = 0; y < 4; ++y) x[i][4 * t + y] = kv8_score(s[i][0][y], s[i][1][y]);
         }
     };
-    auto softmax = [&](int k, auto mm) {
-        constexpr int MM = decltype(mm)::value;
+    auto scaled = [&](int k, int mm) {   // the scores times their keys' scales
         const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[k % 3] + 8 * (kv8_lane() >> 4));   // of the lane's keys 8 q4 ..
-        const int e = __builtin_amdgcn_readfirstlane(s_exp[k % 3]);
-        const int p0 = kBlk * (b0 + k);
-        float big[MM];
-        bool raise = false, late_exp = false;
-        {
-            const vmi_f4 k0 = ks[0], k1 = ks[1];
+        const vmi_f4 k0 = ks[0], k1 = ks[1];
 #pragma unroll
-            for (int i = 0; i < MM; ++i) {
+        for (int i = 0; i < M; ++i)
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
+            for (int y = 0; y < 4; ++y)
+                if (i < mm) {
                     x[i][y] *= k0[y];
                     x[i][4 + y] *= k1[y];
                 }
-                if (p0 + kBlk - 1 > pos0 + min(r0[i], R - 1) / G) {   // the record reaches past some row's last position
-                    const int lane = kv8_lane();
-                    // the lane's keys up to this one are visible
-                    const int seen = pos0 + min(r0[i] + (lane & 15), R - 1) / G - 8 * (lane >> 4) - p0;
+    };
+    // a record that some row may not see to its end
+    auto softmax_masked = [&](int k, auto mm) {
+        constexpr int MM = decltype(mm)::value;
+        scaled(k, MM);
+        const vmi_f4* v = reinterpret_cast<const vmi_f4*>(s_vs[k % 3] + 8 * (kv8_lane() >> 4));
+        const vmi_f4 vs[2] = {v[0], v[1]};
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) x[i][y] = y > seen ? -INFINITY : x[i][y];
-                }
+        for (int i = 0; i < MM; ++i) {
+            const int lane = kv8_lane();
+            const int seen = pos0 + min(r0[i] + (lane & 15), R - 1) / G - 8 * (lane >> 4) - kBlk * (b0 + k);
+            pb[i] = kv8_masked_weights(x[i], vs, seen, Q.cx[i], top[i], ref[i], l[i], o[i]);
+        }
+    };
+    auto softmax = [&](int k, auto mm) {
+        constexpr int MM = decltype(mm)::value;
+        scaled(k, MM);
+        const int e = __builtin_amdgcn_readfirstlane(s_exp[k % 3]);
+        float big[MM];
+        bool raise = false;
+        {
+#pragma unroll
+            for (int i = 0; i < MM; ++i) {
                 big[i] = kv8_max3(kv8_max3(x[i][0], x[i][1], x[i][2]), kv8_max3(x[i][3], x[i][4], x[i][5]),
                                   kv8_max3(x[i][6], x[i][7], x[i][7]));
-                late_exp = late_exp || e != ref[i];
-                raise = raise || fmaf(big[i], Q.cx[i], -top[i]) > kLazyMax + kProbBits;
+                raise = raise || e != ref[i] || fmaf(big[i], Q.cx[i], -top[i]) > kLazyMax + kProbBits;
             }
         }
-        if (late_exp || __any(raise)) {
+        if (__any(raise)) {
 #pragma unroll
             for (int i = 0; i < MM; ++i) {
                 const float nt = fmaxf(top[i], fmaf(kv8_max32(kv8_max16(big[i])), Q.cx[i], -(float)kProbBits));
@@ -1387,29 +1456,37 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
         issue(1);
         phase();
     }
-    // one record: the values of the one before, over vv row groups, and its own scores, over mm
-    auto step = [&](int k, auto vv, auto mm) {
+    // one record: the values of the one before and its own scores, over mm row groups
+    auto step = [&](int k, auto mm, auto masked) {
         if (!late) issue(k + 1);
-        values(k - 1, vv);   // (of record -1: zeros)
+        values(k - 1, mm);   // (of record -1: zeros)
         scores(k, mm);
         scales(k + 1);
         if (late) vmi_vm_wait_c<0>();
         phase();
         if (late) issue(k + 2);
-        softmax(k, mm);
+        if constexpr (masked)
+            softmax_masked(k, mm);
+        else
+            softmax(k, mm);
         convert(k + late);
         if (!late) vmi_vm_wait_c<0>();
         phase();
     };
 #pragma unroll 1
-    for (int k = 0; k < nboth; ++k) step(k, kBoth, kBoth);
-    if (n > nboth) step(nboth, kBoth, kOne);
+    for (int k = 0; k < mboth; ++k) step(k, kBoth, std::false_type{});
 #pragma unroll 1
-    for (int k = nboth + 1; k < n; ++k) step(k, kOne, kOne);
-    if (n > nboth)
-        values(n - 1, kOne);
-    else
-        values(n - 1, kBoth);
+    for (int k = mboth; k < nboth; ++k) step(k, kBoth, std::true_type{});
+    if (nboth) {   // the first tile's last values
+        const vmi_u4* V = s_f16[(nboth - 1) & 1] + kv8_lane();
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[1][d] = vmi_mfma_f16(V[d * 64], pb[1], o[1][d]);
+    }
+#pragma unroll 1
+    for (int k = nboth; k < mone; ++k) step(k, kOne, std::false_type{});
+#pragma unroll 1
+    for (int k = mone; k < n; ++k) step(k, kOne, std::true_type{});
+    values(n - 1, kOne);
     if (!late) phase();   // the late waves' last
 #pragma unroll
     for (int i = 0; i < M; ++i)
@@ -1421,14 +1498,14 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
 // grid (tiles of 128 rows, n_kv, key parts): k_kv8_flash for little work (flash_plan),
 // where its longer way in and out costs more than its phases give: eight waves of 16
 // rows in step, one barrier a record.  It comes by DMA, two ahead; one ahead the waves
-// turn its values together, over the largest scale of the record.  A part takes the
+// turn its values together, over the largest scale of a record that all rows see.  A part takes the
 // same number of records in every tile (a.run), so that the last tiles, which see
 // the most, have the most parts; a tile of one part goes out at once.
 __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_key[3][kHalfRec], s_val[2][kHalfRec];   // as stored
     __shared__ __attribute__((aligned(16))) float s_scale[2][2 * kBlk];
     __shared__ vmi_u4 s_v16[2][16 * 64];
-    __shared__ __attribute__((aligned(16))) float s_ks[2][kBlk];
+    __shared__ __attribute__((aligned(16))) float s_ks[2][kBlk], s_vs[2][kBlk];
     __shared__ int s_exp[2];
     const int lane = threadIdx.x & 63, w = at_wave(), nl = lane & 15, q4 = lane >> 4;
     const int g = blockIdx.y, G = a.n_heads / a.n_kv, R = a.span * G, P = gridDim.z, z = blockIdx.z;
@@ -1440,6 +1517,7 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
     const int nb = kv8_tile_records(pos0, tile, R, G);
     const int b0 = z * a.run, b1 = min(b0 + a.run, nb);
     if (b0 >= nb) return;   // whole workgroup: a part that this tile does not have
+    const int bm = min(max(kv8_tile_seen(pos0, tile, R, G), b0), b1);   // the first that some row does not see to its end
     const uint8_t* head = a.cache + (size_t)g * (a.max_len / kBlk) * kRec;
     const uint32_t at16 = 16 * lane;
     auto issue = [&](int b, int uk, int u) {
@@ -1448,25 +1526,30 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
         vmi_lds_dma16_at(rec + kHalfRec + 1024 * w, at16, s_val[u] + 1024 * w);
         vmi_lds_dma4_at(rec + 2 * kHalfRec, 4 * lane, s_scale[u]);   // every wave the same bytes
     };
-    auto convert = [&](int u) {
+    auto convert = [&](int b, int u) {
         const vmi_u4 v = *reinterpret_cast<const vmi_u4*>(s_val[u] + 1024 * w + at16);
         const vmi_f4* vs = reinterpret_cast<const vmi_f4*>(s_scale[u] + kBlk + 8 * q4);
-        const vmi_f4 v0 = vs[0], v1 = vs[1];
-        float top = fmaxf(fmaxf(fmaxf(v0[0], v0[1]), fmaxf(v0[2], v0[3])), fmaxf(fmaxf(v1[0], v1[1]), fmaxf(v1[2], v1[3])));
-        top = fmaxf(kv8_max32(kv8_max16(top)), 0.0f);
-        const int e = max((int)(__float_as_uint(top) >> 23) - 126, kMinExp);
-        const float unit = ldexpf(1.0f, kValueBits - e);
+        int e = kMinExp;
         vmi_u4 f;
+        f[0] = f[1] = f[2] = f[3] = kv8_pack_f16((float)(1 << kValueBits), (float)(1 << kValueBits));
+        if (b < bm) {
+            const vmi_f4 v0 = vs[0], v1 = vs[1];
+            float top = fmaxf(fmaxf(fmaxf(v0[0], v0[1]), fmaxf(v0[2], v0[3])), fmaxf(fmaxf(v1[0], v1[1]), fmaxf(v1[2], v1[3])));
+            top = fmaxf(kv8_max32(kv8_max16(top)), 0.0f);
+            e = max((int)(__float_as_uint(top) >> 23) - 126, kMinExp);
+            const float unit = ldexpf(1.0f, kValueBits - e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = i < 2 ? v0[2 * i] : v1[2 * i - 4], y = i < 2 ? v0[2 * i + 1] : v1[2 * i - 3];
-            f[i] = kv8_pack_f16(x == x ? x * unit : 0.0f, y == y ? y * unit : 0.0f);
+            for (int i = 0; i < 4; ++i) {
+                const float x = i < 2 ? v0[2 * i] : v1[2 * i - 4], y = i < 2 ? v0[2 * i + 1] : v1[2 * i - 3];
+                f[i] = kv8_pack_f16(x == x ? x * unit : 0.0f, y == y ? y * unit : 0.0f);
+            }
         }
         s_v16[u][2 * w * 64 + lane] = kv8_scaled(v[0], v[1], f);
         s_v16[u][(2 * w + 1) * 64 + lane] = kv8_scaled(v[2], v[3], f);
         if (w == 0 && lane < kBlk) {
             const float ks = s_scale[u][lane], x = s_scale[u][kBlk + lane];
             s_ks[u][lane] = x == x ? ks * kKeyUnit : x;
+            s_vs[u][lane] = x == x ? x : 0.0f;
             if (lane == 0) s_exp[u] = e;
         }
     };
@@ -1475,7 +1558,7 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
     Kv8Rows<1> Q;
     kv8_load_rows<1>(a, a.q, g, r0, R, Q);
     const float cx = Q.cx[0] * (1.0f / kKeyUnit);
-    const int last = pos0 + min(r0[0] + nl, R - 1) / G, first = pos0 + min(r0[0], R - 1) / G;
+    const int last = pos0 + min(r0[0] + nl, R - 1) / G;
     vmi_f4 o[16];                // in units of 2^(ref - kValueBits - kProbBits)
     float top = -3.0e38f, l = 0.0f;   // the reference score, less kProbBits; probabilities times 2^kProbBits
     int ref = kMinExp;           // exponent of the value scales
@@ -1483,14 +1566,13 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
     for (int d = 0; d < 16; ++d) o[d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
     vmi_vm_wait_c<0>();
     __syncthreads();
-    if (b0 < b1) convert(0);
+    if (b0 < b1) convert(b0, 0);
     int uk = 0;   // of s_key, the record's
-#pragma unroll 1
-    for (int b = b0; b < b1; ++b) {
+    auto step = [&](int b, auto masked) {
         const int u = (b - b0) & 1, uk1 = uk == 2 ? 0 : uk + 1;
         vmi_vm_wait_c<0>();
         __syncthreads();   // record b is in operand order, b + 1 in LDS, and nobody reads what is written below
-        if (b + 1 < b1) convert(u ^ 1);
+        if (b + 1 < b1) convert(b + 1, u ^ 1);
         if (b + 2 < b1) issue(b + 2, uk1 == 2 ? 0 : uk1 + 1, u);
         const vmi_u4* K = reinterpret_cast<const vmi_u4*>(s_key[uk]) + lane;
         const vmi_u4* V = s_v16[u] + lane;
@@ -1506,8 +1588,6 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
                 for (int c = 0; c < 2; ++c) s[t][c] = vmi_mfma_i8(key, Q.q[0][2 * j + c], s[t][c]);
             }
         const vmi_f4* ks = reinterpret_cast<const vmi_f4*>(s_ks[u] + 8 * q4);   // of the lane's keys 8 q4 ..
-        const int e = max(__builtin_amdgcn_readfirstlane(s_exp[u]), ref);
-        const float down = ldexpf(1.0f, __builtin_amdgcn_readfirstlane(s_exp[u]) - e);   // the record's values to E
         float x[8];
         {
             const vmi_f4 k0 = ks[0], k1 = ks[1];
@@ -1517,35 +1597,42 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a)
                 x[4 + y] = kv8_score(s[1][0][y], s[1][1][y]) * k1[y];
             }
         }
-        if (kBlk * b + kBlk - 1 > first) {   // the record reaches past some row's last position
-            const int seen = last - (kBlk * b + 8 * q4);
-#pragma unroll
-            for (int y = 0; y < 8; ++y) x[y] = y > seen ? -INFINITY : x[y];
-        }
-        const float big = kv8_max3(kv8_max3(x[0], x[1], x[2]), kv8_max3(x[3], x[4], x[5]), kv8_max3(x[6], x[7], x[7]));
-        if (e != ref || __any(fmaf(big, cx, -top) > kLazyMax + kProbBits)) {
-            const float nt = fmaxf(top, fmaf(kv8_max32(kv8_max16(big)), cx, -(float)kProbBits));
-            const float f = __builtin_amdgcn_exp2f(top - nt), fo = ldexpf(f, ref - e);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < 16; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[d][r] *= fo;
-            top = nt;
-            ref = e;
-        }
         vmi_u4 pb;
+        if constexpr (masked) {
+            const vmi_f4* v = reinterpret_cast<const vmi_f4*>(s_vs[u] + 8 * q4);
+            const vmi_f4 vs[2] = {v[0], v[1]};
+            pb = kv8_masked_weights(x, vs, last - (kBlk * b + 8 * q4), cx, top, ref, l, o);
+        } else {
+            const int e = max(__builtin_amdgcn_readfirstlane(s_exp[u]), ref);
+            const float down = ldexpf(1.0f, __builtin_amdgcn_readfirstlane(s_exp[u]) - e);   // the record's values to E
+            const float big = kv8_max3(kv8_max3(x[0], x[1], x[2]), kv8_max3(x[3], x[4], x[5]), kv8_max3(x[6], x[7], x[7]));
+            if (e != ref || __any(fmaf(big, cx, -top) > kLazyMax + kProbBits)) {
+                const float nt = fmaxf(top, fmaf(kv8_max32(kv8_max16(big)), cx, -(float)kProbBits));
+                const float f = __builtin_amdgcn_exp2f(top - nt), fo = ldexpf(f, ref - e);
+                l *= f;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-            x[y] = __builtin_amdgcn_exp2f(fmaf(x[y], cx, -top));
-            l += x[y];
-            x[y] *= down;
+                for (int d = 0; d < 16; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] *= fo;
+                top = nt;
+                ref = e;
+            }
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                x[y] = __builtin_amdgcn_exp2f(fmaf(x[y], cx, -top));
+                l += x[y];
+                x[y] *= down;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pb[j] = kv8_pack_f16(x[2 * j], x[2 * j + 1]);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) pb[j] = kv8_pack_f16(x[2 * j], x[2 * j + 1]);
 #pragma unroll
         for (int d = 0; d < 16; ++d) o[d] = vmi_mfma_f16(V[d * 64], pb, o[d]);
-    }
+    };
+#pragma unroll 1
+    for (int b = b0; b < bm; ++b) step(b, std::false_type{});
+#pragma unroll 1
+    for (int b = bm; b < b1; ++b) step(b, std::true_type{});
     kv8_finish_rows(a, o, top + (float)kProbBits, kv8_sum32(kv8_sum16(l)) * (1.0f / (float)(1 << kProbBits)),
                     ldexpf(1.0f, ref - kValueBits - kProbBits), r0[0] + nl, R, nb <= a.run);
 }
