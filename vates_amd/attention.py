@@ -108,7 +108,8 @@ class KVCache:
         self.length = 0  # committed positions
         self.n_kv = n_kv_heads
         self.tree_kv = None  # [paths, n_kv, 2, span, 256] bf16: a draft tree's new keys and values
-        self._tree_flat = None
+        # (made here, not by the first tree: that one's stream would not wait for the fill)
+        self._tree_flat = torch.zeros(16 * n_kv_heads * 2 * 256, dtype=torch.bfloat16, device=device)
 
     @property
     def device(self) -> torch.device:
@@ -120,8 +121,6 @@ class KVCache:
         for different (paths, span) see the same address."""
         if paths * span > 16:
             raise VmiError(f"a tree of {paths} x {span} tokens exceeds 16")
-        if self._tree_flat is None:
-            self._tree_flat = torch.zeros(16 * self.n_kv * 2 * 256, dtype=torch.bfloat16, device=self.k.device)
         self.tree_kv = self._tree_flat[:paths * self.n_kv * 2 * span * 256].view(paths, self.n_kv, 2, span, 256)
         return self.tree_kv
 
@@ -180,7 +179,7 @@ class KVCache8(KVCache):
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.length = 0
         self.tree_kv = None   # uint8: a draft tree's new rows
-        self._tree_flat = None
+        self._tree_flat = torch.zeros(16 * n_kv_heads * VMI_KV8_TREE_ROW, dtype=torch.uint8, device=device)
 
     @property
     def device(self) -> torch.device:
@@ -191,8 +190,6 @@ class KVCache8(KVCache):
         allocation for every tree of at most 16 tokens, as KVCache's."""
         if paths * span > 16:
             raise VmiError(f"a tree of {paths} x {span} tokens exceeds 16")
-        if self._tree_flat is None:
-            self._tree_flat = torch.zeros(16 * self.n_kv * VMI_KV8_TREE_ROW, dtype=torch.uint8, device=self.data.device)
         self.tree_kv = self._tree_flat[:paths * self.n_kv * span * VMI_KV8_TREE_ROW].view(paths, self.n_kv, span,
                                                                                           VMI_KV8_TREE_ROW)
         return self.tree_kv
