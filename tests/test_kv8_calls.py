@@ -1,5 +1,7 @@
 """Calls around the 8-bit KV cache that need no device: what a call makes by itself,
 and objects with methods of their own beside it."""
+import types
+
 import pytest
 import torch
 
@@ -18,3 +20,44 @@ def test_a_tree_buffer_is_made_with_its_cache(monkeypatch, bits):
         monkeypatch.setattr(torch, name, refuse)
     a, b = cache.tree_buffer(2, 3), cache.tree_buffer(4, 4)
     assert a.data_ptr() == b.data_ptr() and b.shape[:2] == (4, 2) and not bool(b.any())
+
+
+class OwnAttention:
+    """An attention object of a program's own, as bf16 caches use it."""
+    n_heads, n_kv = 4, 2
+
+    def __init__(self):
+        self.made = []
+
+    def prompt_workspace_bytes(self, T):
+        return 100 * T
+
+
+def test_a_layer_whose_prompt_workspace_takes_tokens_alone(monkeypatch):
+    """The MTP layer's query for its cache's fill, and the layer's own prompt call, ask it as before."""
+    from vates_amd import attention, mtp
+    from vates_amd.attention import AttentionLayer, KVCache
+
+    layer = mtp.MTPLayer.__new__(mtp.MTPLayer)
+    layer.hidden, layer.w = 512, types.SimpleNamespace(fc=None, attn=OwnAttention())
+    monkeypatch.setattr(mtp, "qgemm_workspace_bytes", lambda w, T, K: 7)
+    cache = KVCache(2, 64, "cpu")
+    assert layer.fill_workspace_bytes(5) == 500 and layer.fill_workspace_bytes(5, cache) == 500
+
+    class Sized(AttentionLayer):
+        def prompt_workspace_bytes(self, T):
+            return 100 * T
+
+    asked = []
+
+    def scratch(nbytes, device, stream=None):
+        asked.append(nbytes)
+        raise MemoryError
+
+    sized = Sized.__new__(Sized)
+    sized.__dict__.update(hidden=512, n_kv=2, n_heads=4, device=torch.device("cpu"))
+    monkeypatch.setattr(attention, "scratch", scratch)
+    monkeypatch.setattr(attention, "_stream_handle", lambda stream: 0)
+    with pytest.raises(MemoryError):
+        sized.prompt(torch.zeros((5, 512), dtype=torch.bfloat16), cache, pos0=0)
+    assert asked == [500]

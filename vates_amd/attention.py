@@ -356,6 +356,12 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
     return out
 
 
+def prompt_bytes(attn, T: int, cache: Optional[KVCache]) -> int:
+    """An attention layer's prompt workspace for this kind of cache.  Layers whose own
+    ``prompt_workspace_bytes`` takes T alone serve bf16 caches."""
+    return attn.prompt_workspace_bytes(T, cache) if isinstance(cache, KVCache8) else attn.prompt_workspace_bytes(T)
+
+
 class AttentionLayer:
     def __init__(self, q_proj: QuantizedProj, k_proj: QuantizedProj, v_proj: QuantizedProj, o_proj: QuantizedProj,
                  input_norm: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, *, n_heads: int = 16,
@@ -460,7 +466,7 @@ class AttentionLayer:
         out = None if keys_only else torch.empty_like(x)
         sh = _stream_handle(stream)
         if ws is None:
-            ws = scratch(self.prompt_workspace_bytes(T, cache), self.device, stream)
+            ws = scratch(prompt_bytes(self, T, cache), self.device, stream)
         if isinstance(cache, KVCache8):
             if _on_current(cache.data) != self.device or cache.n_kv != self.n_kv:
                 raise VmiError(f"a cache of {cache.n_kv} kv heads on {cache.device} does not fit the layer")

@@ -33,7 +33,7 @@ import torch
 
 from ._lib import VmiError, check, load
 from .accept import accept_greedy, accept_stochastic, raise_sampling_status, sample_top_p, spec_commit
-from .attention import AttentionLayer, KVCache, KVCache8
+from .attention import AttentionLayer, KVCache, KVCache8, prompt_bytes
 from .gdn import GatedDeltaNetLayer, GdnCache
 from .head import TiledHead, lm_head
 from .moe import MoELayer, scratch
@@ -227,11 +227,6 @@ def _own(obj, name: str, cls) -> bool:
     return method is getattr(cls, name) and name not in getattr(obj, "__dict__", {})
 
 
-def _prompt_bytes(attn: AttentionLayer, T: int, cache) -> int:
-    """The attention layer's prompt workspace for this kind of cache."""
-    return attn.prompt_workspace_bytes(T, cache) if isinstance(cache, KVCache8) else attn.prompt_workspace_bytes(T)
-
-
 def _fill_bytes(drafter: MTPDrafter, T: int) -> int:
     cache = getattr(drafter, "cache", None)
     return (drafter.mtp.fill_workspace_bytes(T, cache) if isinstance(cache, KVCache8) else
@@ -264,7 +259,7 @@ def _prompt_blocks(model: SpecModel, prompt: torch.Tensor, caches, drafter: Opti
         if layer.attn is not None:
             ok = (isinstance(cache, KVCache) and P <= cache.max_len and
                   chunk * (layer.attn.n_heads // layer.attn.n_kv) <= 64 and
-                  _prompt_bytes(layer.attn, step, cache))
+                  prompt_bytes(layer.attn, step, cache))
         elif layer.gdn is not None:
             ok = (isinstance(cache, GdnCache) and cache.n_slots > chunk and layer.gdn.prompt_workspace_bytes(step))
         else:
@@ -287,7 +282,7 @@ def _prompt_scratch(model: SpecModel, prompt: torch.Tensor, blocks: list, drafte
     while blocks:
         step = blocks[0][1]
         need = [l.moe.prompt_workspace_bytes(step) for l in model.layers]
-        need += [_prompt_bytes(l.attn, step, c) if l.attn else l.gdn.prompt_workspace_bytes(step)
+        need += [prompt_bytes(l.attn, step, c) if l.attn else l.gdn.prompt_workspace_bytes(step)
                  for l, c in zip(model.layers, caches or [None] * len(model.layers)) if l.attn or l.gdn]
         if drafter is not None:
             need.append(_fill_bytes(drafter, step))

@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from ._lib import VmiError, check, load
-from .attention import AttentionLayer, KVCache, qgemm, qgemm_workspace_bytes, qgemv
+from .attention import AttentionLayer, KVCache, prompt_bytes, qgemm, qgemm_workspace_bytes, qgemv
 from .head import TiledHead, lm_head
 from .moe import MoELayer, QuantizedProj, _require, _stream_handle
 
@@ -107,7 +107,7 @@ class MTPLayer:
     def fill_workspace_bytes(self, T: int, cache: Optional[KVCache] = None) -> int:
         """Workspace of ``fill`` on T tokens (0: a form it is not built for)
         into the cache (None: a bf16 one)."""
-        parts = qgemm_workspace_bytes(self.w.fc, T, 2 * self.hidden), self.w.attn.prompt_workspace_bytes(T, cache)
+        parts = qgemm_workspace_bytes(self.w.fc, T, 2 * self.hidden), prompt_bytes(self.w.attn, T, cache)
         return max(parts) if all(parts) else 0
 
     def fill(self, hidden: torch.Tensor, tokens: torch.Tensor, cache: KVCache, stream=None,
