@@ -61,3 +61,25 @@ def test_a_layer_whose_prompt_workspace_takes_tokens_alone(monkeypatch):
     with pytest.raises(MemoryError):
         sized.prompt(torch.zeros((5, 512), dtype=torch.bfloat16), cache, pos0=0)
     assert asked == [500]
+
+
+def test_a_layer_whose_new_cache_takes_the_length_alone():
+    """Models and drafters ask for bf16 caches as before, for 8-bit ones by name."""
+    from vates_amd.decode import DecoderLayer, SpecModel
+    from vates_amd.mtp import MTPDrafter
+
+    class Own:
+        def new_cache(self, max_len):
+            return ("own", max_len)
+
+    class Both:
+        def new_cache(self, max_len, bits=16):
+            return ("both", max_len, bits)
+
+    model = SpecModel.__new__(SpecModel)
+    model.layers = [DecoderLayer(None, attn=Own()), DecoderLayer(None, attn=Both()), DecoderLayer(None)]
+    assert model.new_caches(64) == [("own", 64), ("both", 64, 16), None]
+    model.layers = model.layers[1:]
+    assert model.new_caches(64, kv_bits=8) == [("both", 64, 8), None]
+    for attn, kw, want in ((Own(), {}, ("own", 9)), (Both(), dict(kv_bits=8), ("both", 9, 8))):
+        assert MTPDrafter(types.SimpleNamespace(w=types.SimpleNamespace(attn=attn)), 9, **kw).cache == want

@@ -356,6 +356,12 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
     return out
 
 
+def layer_cache(attn, max_len: int, bits: int) -> KVCache:
+    """A cache of an attention layer.  Layers whose own ``new_cache`` takes the length
+    alone give bf16 ones."""
+    return attn.new_cache(max_len) if bits == 16 else attn.new_cache(max_len, bits)
+
+
 def prompt_bytes(attn, T: int, cache: Optional[KVCache]) -> int:
     """An attention layer's prompt workspace for this kind of cache.  Layers whose own
     ``prompt_workspace_bytes`` takes T alone serve bf16 caches."""

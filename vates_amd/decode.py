@@ -33,7 +33,7 @@ import torch
 
 from ._lib import VmiError, check, load
 from .accept import accept_greedy, accept_stochastic, raise_sampling_status, sample_top_p, spec_commit
-from .attention import AttentionLayer, KVCache, KVCache8, prompt_bytes
+from .attention import AttentionLayer, KVCache, KVCache8, layer_cache, prompt_bytes
 from .gdn import GatedDeltaNetLayer, GdnCache
 from .head import TiledHead, lm_head
 from .moe import MoELayer, scratch
@@ -99,7 +99,7 @@ class SpecModel:
         """Per layer: a KVCache (full attention; with kv_bits=8 a KVCache8, half
         the bytes), a GdnCache (linear attention, verify batches up to max_batch
         tokens) or None."""
-        return [l.attn.new_cache(max_len, kv_bits) if l.attn is not None else
+        return [layer_cache(l.attn, max_len, kv_bits) if l.attn is not None else
                 l.gdn.new_cache(max_batch) if l.gdn is not None else None for l in self.layers]
 
     def forward(self, ids: torch.Tensor, caches: list, pos0: int, *, want_logits: bool = False,

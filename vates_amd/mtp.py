@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from ._lib import VmiError, check, load
-from .attention import AttentionLayer, KVCache, prompt_bytes, qgemm, qgemm_workspace_bytes, qgemv
+from .attention import AttentionLayer, KVCache, layer_cache, prompt_bytes, qgemm, qgemm_workspace_bytes, qgemv
 from .head import TiledHead, lm_head
 from .moe import MoELayer, QuantizedProj, _require, _stream_handle
 
@@ -128,7 +128,7 @@ class MTPDrafter:
     def __init__(self, mtp: MTPLayer, max_len: int, *, kv_bits: int = 16):
         """kv_bits=8: the MTP layer's cache is a KVCache8."""
         self.mtp = mtp
-        self.cache = mtp.w.attn.new_cache(max_len, kv_bits)
+        self.cache = layer_cache(mtp.w.attn, max_len, kv_bits)
 
     def draft(self, H_last: torch.Tensor, x_tok: torch.Tensor, K: int) -> torch.Tensor:
         """K greedy drafts (int32 [K] on the device) from the main model's last
