@@ -40,3 +40,22 @@ def test_first_tree_of_a_cache(gpu, layer):
     TreeCommit([b], P, S)(rec, pos0=pos0)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and torch.equal(a.data, b.data)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_prompt_output_is_of_the_call_s_stream(gpu, layer, bits):
+    """Memory that the current stream gave up may still be in use there: the output
+    of a call on another stream does not take it."""
+    from vates_amd.synth import synth_bf16
+    log(f"case: prompt output on a stream, {bits} bits")
+    x = synth_bf16(51, 31, (40, layer.hidden), device=gpu)
+    st = torch.cuda.Stream()
+    want = layer.prompt(x, layer.new_cache(64, bits), pos0=0)
+    cache = layer.new_cache(64, bits)
+    torch.cuda.synchronize()
+    given = torch.empty_like(x)
+    at = given.data_ptr()
+    del given
+    got = layer.prompt(x, cache, pos0=0, stream=st)
+    torch.cuda.synchronize()
+    assert got.data_ptr() != at and torch.equal(got, want)

@@ -469,7 +469,7 @@ class AttentionLayer:
             raise VmiError(f"x {tuple(x.shape)} or a cache of {cache.n_kv} kv heads does not fit the layer")
         T = x.shape[0]
         _require(x, "x", 2, self.device)
-        out = None if keys_only else torch.empty_like(x)
+        out = None if keys_only else _like(x, None, x.dtype, stream)
         sh = _stream_handle(stream)
         if ws is None:
             ws = scratch(prompt_bytes(self, T, cache), self.device, stream)
