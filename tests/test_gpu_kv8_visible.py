@@ -24,8 +24,9 @@ from test_gpu_kv8 import DIM, log, new_cache, queries, rows
 pytestmark = pytest.mark.gpu
 
 
-def attend64(q, k, v, pos0):
-    """(outputs, bars) for fp32 rows k, v [n_kv, L, 256]; every maximum over the row's own positions."""
+def attend64(q, k, v, pos0, roundings=3, scales=2.0 ** -33):
+    """(outputs, bars) for fp32 rows k, v [n_kv, L, 256]; every maximum over the row's own positions.
+    roundings: to fp16; scales: of V, where scales are held by themselves."""
     T, nh, _ = q.shape
     G = nh // k.shape[0]
     dev = k.device
@@ -44,7 +45,7 @@ def attend64(q, k, v, pos0):
         o, A = torch.matmul(p, vv), torch.matmul(p, vv.abs())
         d = qq.abs().amax(-1, keepdim=True) * ksum / (16 * 65024) + 5 * 2.0 ** -24 * qq.abs().sum(-1, keepdim=True) * kmax / 16
         out[:, h] = o
-        tol[:, h] = 2.0 ** -8 * o.abs() + (3 * 2.0 ** -11 + 2 * d + 2.0 ** -16) * A + (n * 2.0 ** -39 + 2.0 ** -33) * vmax
+        tol[:, h] = 2.0 ** -8 * o.abs() + (roundings * 2.0 ** -11 + 2 * d + 2.0 ** -16) * A + (n * 2.0 ** -39 + scales) * vmax
     return out, tol
 
 

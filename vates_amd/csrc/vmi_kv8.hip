@@ -523,6 +523,15 @@ __device__ __forceinline__ vmi_u4 kv8_widen(uint32_t w0, uint32_t w1) {
     r[3] = __builtin_amdgcn_perm(0u, w1, 0x0c030c02u);
     return r;
 }
+// The codes themselves, c 2^-24 (exact).
+__device__ __forceinline__ vmi_u4 kv8_signed(const vmi_u4& u) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 off = {(_Float16)(-0x1p-17f), (_Float16)(-0x1p-17f)};
+    vmi_u4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (uint32_t)u[i]) + off);
+    return r;
+}
 __device__ __forceinline__ uint32_t kv8_pack_f16(float a, float b) {  // one conversion of both, to nearest even
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     typedef float f2 __attribute__((ext_vector_type(2)));
@@ -686,8 +695,7 @@ __device__ __forceinline__ void kv8_insert(Kv8Rec& r, const uint8_t* row, int kt
 // Running softmax of a wave's 16 MS rows.  o is in units of s kSumUnit.
 template <int MS>
 struct Kv8Sums {
-    vmi_f4 o[MS][16];  // dims 16 dt + 4 q4 + r of row 16 m + nl, of codes + 128
-    vmi_f4 c[MS];      // the probabilities' sum, as multiplied, in every element
+    vmi_f4 o[MS][16];  // dims 16 dt + 4 q4 + r of row 16 m + nl
     float m[MS];       // maximum score, in powers of two
     float l[MS];       // the lane's share of sum 2^(score - m)
     float s[MS];       // largest value scale seen
@@ -697,7 +705,6 @@ struct Kv8Sums {
             m[i] = -3.402823466e38f;
             l[i] = 0.0f;
             s[i] = kMinRef;
-            c[i] = vmi_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < 16; ++d) o[i][d] = vmi_f4{0.f, 0.f, 0.f, 0.f};
         }
@@ -709,10 +716,7 @@ struct Kv8Sums {
 // row, which are, as probabilities, already the B operand of O^T = V^T P^T.  A
 // key's scale enters its score, a value's its probability; the product goes to fp16
 // (11 bits) relative to the row's largest value scale so far, and whatever raises
-// that or the running maximum rescales the sums.  Values are multiplied as codes + 128,
-// as they are widened, and the products' own sum, one more row of ones, takes the 128
-// off at the end: fp32 roundings of up to 128 times a code's, a hundredth of the
-// product's, for half of the widening's instructions.  mask (wave-uniform): the record
+// that or the running maximum rescales the sums.  mask (wave-uniform): the record
 // reaches past the visible positions of some row; masked scores count as minus
 // infinity and masked scales as zero, so that nothing stored behind a row's last
 // position reaches it.  The next record's keys are asked for once these are used,
@@ -771,8 +775,6 @@ __device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const flo
             for (int d = 0; d < 16; ++d)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) S.o[m][d][r] *= fo;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S.c[m][r] *= fo;
             S.m[m] = nm;
             S.s[m] = ns;
         }
@@ -787,13 +789,10 @@ __device__ __forceinline__ void kv8_step(Kv8Rec& rec, const vmi_u4* q, const flo
         for (int i = 0; i < 4; ++i) pb[m][i] = kv8_pack_f16(x[m][2 * i], x[m][2 * i + 1]);
     }
     kv8_load_value_scales<ONCE>(rec, next);
-    const vmi_u4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-#pragma unroll
-    for (int m = 0; m < MS; ++m) S.c[m] = vmi_mfma_f16(ones, pb[m], S.c[m]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const vmi_u4 u = rec.v[j];
-        const vmi_u4 v0 = kv8_widen(u[0], u[1]), v1 = kv8_widen(u[2], u[3]);
+        const vmi_u4 v0 = kv8_signed(kv8_widen(u[0], u[1])), v1 = kv8_signed(kv8_widen(u[2], u[3]));
 #pragma unroll
         for (int m = 0; m < MS; ++m) S.o[m][2 * j] = vmi_mfma_f16(v0, pb[m], S.o[m][2 * j]);
 #pragma unroll
@@ -906,13 +905,6 @@ __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv
         }
         kv8_step<MS, ONCE>(rec, s_q, cx, last, kBlk * b, kBlk * b + kBlk - 1 > pos0, kv8_rsrc(head, b + step, b + step < nblk), Y);
     }
-    // codes + 128 were multiplied: 128 times the probabilities come off
-#pragma unroll
-    for (int m = 0; m < MS; ++m)
-#pragma unroll
-        for (int d = 0; d < 16; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) Y.o[m][d][r] = fmaf(Y.c[m][r], -0x1p-17f, Y.o[m][d][r]);
     const size_t part = ((size_t)(g * S + wg) * a.paths + path) * a.rp;
     const __amdgpu_buffer_rsrc_t ro = vmi_rsrc(a.part_o + part * kHeadDim, (uint32_t)R * kHeadDim * 4);
     float l[MS];
