@@ -515,7 +515,8 @@ int vmi_tree_commit(const int32_t* result, const vmi_tree_layer* layers, int n_l
  * as vmi_attention_layer's q_proj, k_proj and v_proj emit them) the queries and
  * keys with their per-head RMSNorm (weights bf16 [256]) and rotary embedding on
  * the first rope_dim dims at positions pos0 .., all in fp32: q_out bf16 [T,
- * n_heads, 256] (NULL: not formed), keys and values into the cache.
+ * n_heads, 256] (NULL: not formed), keys and values into the cache.  rope_theta > 0; below
+ * 1 (later pairs turn faster) max_len * rope_theta^(2/rope_dim - 1) must stay below 2^31.
  * vmi_kv8_attention -- out bf16 [T, n_heads, 256] = softmax(q k / 16) v over the
  * cache, query t seeing positions <= pos0 + t; with gate (f32, element strides
  * gate_token and gate_head, 256 contiguous, rows 16-byte aligned) times

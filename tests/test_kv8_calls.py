@@ -83,3 +83,38 @@ def test_a_layer_whose_new_cache_takes_the_length_alone():
     assert model.new_caches(64, kv_bits=8) == [("both", 64, 8), None]
     for attn, kw, want in ((Own(), {}, ("own", 9)), (Both(), dict(kv_bits=8), ("both", 9, 8))):
         assert MTPDrafter(types.SimpleNamespace(w=types.SimpleNamespace(attn=attn)), 9, **kw).cache == want
+
+
+def test_rotations_past_the_counted_turns_are_refused():
+    """The heads' kernel counts quarter turns in 32 bits: with a theta below 1 the last
+    pair turns by theta^(2/rope_dim - 1) a position, which passes them."""
+    import ctypes
+
+    from vates_amd._lib import QMat, load
+    from vates_amd.attention import AttnDesc
+    lib, P, big = load(), 1 << 20, 1 << 40
+
+    def append(theta, rd, max_len, q_norm=P):
+        return lib.vmi_kv8_append(P, 1, 4, 2, q_norm, P, 1e-6, rd, theta, 0, None, P, max_len, P, None, None)
+
+    def layers(theta, rd, max_len, x=P):
+        d = AttnDesc()
+        d.hidden, d.n_heads, d.n_kv_heads, d.head_dim, d.rope_dim, d.bits, d.group = 2048, 16, 2, 256, rd, 4, 64
+        d.q_proj = d.k_proj = d.v_proj = d.o_proj = QMat(P, P, P)
+        d.input_norm = d.q_norm = d.k_norm = P
+        d.rope_theta, d.norm_eps = theta, 1e-6
+        r = ctypes.byref(d)
+        # (the workspace a byte short, so that what is not refused for its angles is for that)
+        return (lib.vmi_attention_layer_kv8(r, x, 1, 0, None, P, max_len, P, None, P, 16, None),
+                lib.vmi_attention_tree_kv8(r, x, 2, 2, 0, None, P, max_len, P, P, None, P, 16, None),
+                lib.vmi_attention_prompt_kv8(r, x, 20, 0, P, max_len, P, P, 16, None))
+
+    invalid, short = -1, -4
+    for theta, rd, max_len in ((1e-6, 64, 262144), (1e-30, 256, 64), (1e-7, 4, 1 << 30), (float("nan"), 0, 64), (-1.0, 0, 64)):
+        assert append(theta, rd, max_len) == invalid and b"rope_theta" in lib.vmi_last_error()
+        for rc in layers(theta, rd, max_len):
+            assert rc in (invalid, -2)
+    # what can be formed still goes on to the next check
+    for theta, rd, max_len in ((1e7, 64, 1 << 30), (1.0, 256, 1 << 30), (0.5, 64, 262144), (1e-30, 2, 262144), (1e-30, 0, 64)):
+        assert append(theta, rd, max_len, q_norm=None) == invalid and b"null" in lib.vmi_last_error()
+        assert layers(theta, rd, max_len) == (short, short, short)

@@ -94,6 +94,8 @@ struct Kv8Heads {
     uint32_t* status;      // or null (VMI_STATUS_BAD_POS)
 };
 double kv8_rope_base(float theta, int rope_dim);
+// Whether the rotation of every position below max_len is formed (rope_dim even, in [0, 256]).
+bool kv8_rope_ok(float theta, int rope_dim, int max_len);
 hipError_t launch_kv8_heads(const Kv8Heads& h, int paths, hipStream_t s);
 
 // Attention over the cache: paths sequences of span tokens at positions pos0 ..

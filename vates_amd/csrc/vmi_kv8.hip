@@ -1693,6 +1693,12 @@ double vmi::kv8_rope_base(float theta, int rope_dim) {
     return rope_dim ? pow((double)theta, -2.0 / (double)rope_dim) : 1.0;
 }
 
+// The quarter turns are counted in an int; the fastest pair is the first, or with theta below 1 the last.
+bool vmi::kv8_rope_ok(float theta, int rope_dim, int max_len) {
+    if (!(theta > 0.0f)) return false;
+    return rope_dim == 0 || max_len * std::max(1.0, pow(kv8_rope_base(theta, rope_dim), rope_dim / 2 - 1)) < 0x1p31;
+}
+
 bool vmi::kv8_heads_ok(int n_heads, int n_kv) {
     return n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && n_heads <= 1024;
 }
@@ -1833,7 +1839,7 @@ int layer_impl(const vmi_attn_layer_desc* desc, const uint16_t* x, int paths, in
     if (!layer_shape_ok(paths, span, D.hidden, D.n_heads, D.n_kv_heads))
         return vmi::fail(VMI_ERR_UNSUPPORTED, "paths=%d span=%d hidden=%d heads=%d/%d not built", paths, span, D.hidden,
                          D.n_heads, D.n_kv_heads);
-    if (D.rope_dim < 0 || D.rope_dim > kHeadDim || D.rope_dim % 2 || !(D.rope_theta > 0.0f))
+    if (D.rope_dim < 0 || D.rope_dim > kHeadDim || D.rope_dim % 2 || !vmi::kv8_rope_ok(D.rope_theta, D.rope_dim, max_len))
         return vmi::fail(VMI_ERR_INVALID, "rope_dim=%d rope_theta=%g", D.rope_dim, (double)D.rope_theta);
     const int rc = check_cache(cache, D.n_kv_heads, max_len, pos0, span, pos_device);
     if (rc != VMI_OK) return rc;
@@ -1963,7 +1969,7 @@ extern "C" int vmi_kv8_append(const float* qkv, int T, int n_heads, int n_kv_hea
     if (rc != VMI_OK) return rc;
     if (!vmi::kv8_heads_ok(n_heads, n_kv_heads))
         return vmi::fail(VMI_ERR_INVALID, "n_heads=%d n_kv_heads=%d", n_heads, n_kv_heads);
-    if (rope_dim < 0 || rope_dim > kHeadDim || rope_dim % 2 || !(rope_theta > 0.0f))
+    if (rope_dim < 0 || rope_dim > kHeadDim || rope_dim % 2 || !vmi::kv8_rope_ok(rope_theta, rope_dim, max_len))
         return vmi::fail(VMI_ERR_INVALID, "rope_dim=%d rope_theta=%g", rope_dim, (double)rope_theta);
     if (!qkv || !aligned(qkv, 16) || !k_norm || (q_out && !q_norm) || !aligned(q_out, 16))
         return vmi::fail(VMI_ERR_INVALID, "null or misaligned qkv, norm weights or q");

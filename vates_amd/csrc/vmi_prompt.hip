@@ -1263,6 +1263,8 @@ extern "C" int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const u
     if (!x || !cache) return vmi::fail(VMI_ERR_INVALID, "null x/cache");
     if (pos0 < 0 || max_len % VMI_KV_BLOCK || T > max_len || pos0 > max_len - T)
         return vmi::fail(VMI_ERR_INVALID, "pos0=%d T=%d max_len=%d", pos0, T, max_len);
+    if (!vmi::kv8_rope_ok(D.rope_theta, D.rope_dim, max_len))
+        return vmi::fail(VMI_ERR_INVALID, "rope_dim=%d rope_theta=%g", D.rope_dim, (double)D.rope_theta);
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache) |
          reinterpret_cast<uintptr_t>(workspace)) & 15)
         return vmi::fail(VMI_ERR_INVALID, "x, out, cache and workspace must be 16-byte aligned");
