@@ -520,15 +520,22 @@ int vmi_tree_commit(const int32_t* result, const vmi_tree_layer* layers, int n_l
  * vmi_kv8_attention -- out bf16 [T, n_heads, 256] = softmax(q k / 16) v over the
  * cache, query t seeing positions <= pos0 + t; with gate (f32, element strides
  * gate_token and gate_head, 256 contiguous, rows 16-byte aligned) times
- * sigmoid(gate).  q bf16 [T, n_heads, 256], T <= 8192; a query is taken as 16-bit
- * integers of its largest element over 32512 (half a step: 2^-16 of that element,
- * where a key's codes are within 2^-8 of theirs), so that scores are exact integer
- * sums.  Batches of T * n_heads / n_kv_heads <= 64 rows: a token's result does not
- * depend on its batch or on max_len, bit for bit; larger ones equal it up to fp32's
- * and fp16's rounding.  Positions behind a query's own never reach its result; a query
- * that sees a row that is not finite, or is not finite itself, is NaN, and one whose
- * scores pass fp32's range may be.  workspace: the query's bytes (enough for every
- * smaller T too), 16-byte aligned, nothing kept between calls.
+ * sigmoid(gate).  q bf16 [T, n_heads, 256], T <= 8192.  Batches of T * n_heads /
+ * n_kv_heads <= 64 rows: a token's result does not depend on its batch or on max_len,
+ * bit for bit; larger ones (prompts) equal it up to the roundings named here.
+ * Positions behind a query's own never reach its result, whatever lies there: their
+ * keys and values change no bit of it.  A query that sees a row that is not finite,
+ * or is not finite itself, is NaN, and one whose scores pass fp32's range may be.
+ *   What is rounded: a query to 16-bit integers of its largest element over 32512
+ * (half a step: 2^-16 of that element, where a key's codes are within 2^-8 of theirs;
+ * elements below 2^-7 of the largest keep fewer bits than their bf16), so that
+ * scores are exact integer sums; a batch's probability times its value's scale to fp16, a
+ * prompt's probability, scale, and scale times code to fp16 each (11 bits).  Scales
+ * are held relative to the largest that the query sees, whatever that one's probability:
+ * beside one 2^22 times larger a value keeps fewer bits in a prompt, beside one 2^33 (in a
+ * batch 2^38) times larger none.  Maxima and sums are fp32, out is rounded once.
+ *   workspace: the query's bytes (enough for every smaller T too), 16-byte aligned,
+ * nothing kept between calls.
  *
  * pos_device (int32 on the device, or NULL) replaces pos0 when the kernels run;
  * outside [0, max_len - T] it is clamped into it and VMI_STATUS_BAD_POS is OR-ed

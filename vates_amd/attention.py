@@ -326,7 +326,10 @@ def attend(q: torch.Tensor, cache: KVCache8, *, pos0: Optional[int] = None, gate
     ones), each seeing the positions up to its own; with gate (float32 [T, n_heads,
     256], rows of 256 contiguous) times sigmoid(gate).  Returns bfloat16 [T,
     n_heads, 256].  The result of a token of a batch of T * n_heads / n_kv <= 64
-    does not depend on the batch.  pos_device as for ``norm_rope_append``."""
+    does not depend on the batch, and no token's on the keys and values behind it.
+    Queries count as 16-bit integers, probabilities and value scales as fp16, a scale relative
+    to the largest that the query sees (include/vmi.h).  pos_device as for
+    ``norm_rope_append``."""
     dev = _on_current(cache.data)
     if q.dim() != 3 or q.shape[1] % cache.n_kv or not q.shape[1]:
         raise VmiError(f"q {tuple(q.shape)} does not fit a cache of {cache.n_kv} kv heads")

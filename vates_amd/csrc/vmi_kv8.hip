@@ -716,7 +716,10 @@ struct Kv8Sums {
 // row, which are, as probabilities, already the B operand of O^T = V^T P^T.  A
 // key's scale enters its score, a value's its probability; the product goes to fp16
 // (11 bits) relative to the row's largest value scale so far, and whatever raises
-// that or the running maximum rescales the sums.  mask (wave-uniform): the record
+// that or the running maximum rescales the sums.  The codes themselves are multiplied: codes +
+// 128, as they are widened, with the 128 taken off at the end, would save half of the
+// widening's instructions (1 % of four tokens at 32,764) and leave 2^-24 of a row's
+// scale in every dim, also where its code is zero.  mask (wave-uniform): the record
 // reaches past the visible positions of some row; masked scores count as minus
 // infinity and masked scales as zero, so that nothing stored behind a row's last
 // position reaches it.  The next record's keys are asked for once these are used,
@@ -826,7 +829,7 @@ constexpr int kSplitWaves = 4, kSplitThreads = 64 * kSplitWaves;
 // maximum, sum and unnormalised output of each row, in fp32.  Bound by the bytes of
 // the cache from some ten thousand positions on (one token of 16 heads on 2 at
 // 262,143: 47 us, 5.8 TB/s), below by the latency of a record and of the two launches
-// (at 1000: 7.4 us; four tokens at 32,764, two records a wave: 17.9).
+// (at 1000: 7.7 us; four tokens at 32,764, two records a wave: 18.2).
 template <int MS, bool ONCE>
 __global__ __launch_bounds__(kSplitThreads, MS == 1 ? 2 : 1) void k_kv8_split(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) float s_o[kSplitWaves * 16 * kHeadDim];   // one row group of each wave
@@ -1237,11 +1240,12 @@ __device__ __forceinline__ vmi_u4 kv8_masked_weights(float (&x)[8], const vmi_f4
 // Part z of P takes an equal run of the tile's records; with P > 1 the parts are written
 // as k_kv8_split's are.
 //
-// 4096 tokens behind 8192, 16 heads on 2: 619 us, 1.11 PFLOP/s (a large bf16 matrix
-// product reaches 1.23); with every wave in step 915, with the tiles unpaired 713.  A phase
-// takes some 1850 cycles, its 64 matrix instructions 1024 of them: what is left is a
-// single wave's instruction issue and the latency of its first LDS reads.  256
-// registers a lane are full; deeper operand prefetch spills.
+// 4096 tokens behind 8192, 16 heads on 2: 619 to 645 us by the inputs, 1.07 to 1.11 PFLOP/s (a
+// large bf16 matrix product reaches 1.23); with every wave in step 915, with the tiles
+// unpaired 713; with the mask's branch in every record 626 to 652.  A phase takes some
+// 1850 cycles, its 64 matrix instructions 1024 of them: what is left is a single wave's
+// instruction issue and the latency of its first LDS reads.  256 registers a lane are
+// full; deeper operand prefetch spills.
 __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_rec[2][2 * kHalfRec];   // keys and values, as stored
     __shared__ float s_scale[2][2 * kBlk];
@@ -1490,9 +1494,9 @@ __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash(Kv8Attn a) {
 // grid (tiles of 128 rows, n_kv, key parts): k_kv8_flash for little work (flash_plan),
 // where its longer way in and out costs more than its phases give: eight waves of 16
 // rows in step, one barrier a record.  It comes by DMA, two ahead; one ahead the waves
-// turn its values together, over the largest scale of a record that all rows see.  A part takes the
-// same number of records in every tile (a.run), so that the last tiles, which see
-// the most, have the most parts; a tile of one part goes out at once.
+// turn its values together, over the largest scale of a record that all rows see.  A
+// part takes the same number of records in every tile (a.run), so that the last tiles,
+// which see the most, have the most parts; a tile of one part goes out at once.
 __global__ __launch_bounds__(kFlashThreads, 2) void k_kv8_flash_short(Kv8Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_key[3][kHalfRec], s_val[2][kHalfRec];   // as stored
     __shared__ __attribute__((aligned(16))) float s_scale[2][2 * kBlk];
@@ -1640,20 +1644,23 @@ int split_groups(int n_kv) { return std::min(std::max(1, vmi::device_cus() / n_k
 // 16-row groups of a k_kv8_split workgroup.  Two for more than 16 rows over a cache
 // that gives a wave three records or more: the groups' workgroups read the cache once
 // each, which costs nothing while its records come from L2 (us, one group and two: four
-// tokens at 17,000 positions 14.6 and 17.2, at 32,764 17.7 and 18.2; eight 21.5 and 26.1,
-// 26.7 and 31.1) and the rate of HBM beyond (four at 64,000 26.5 and 23.1, eight at
-// 50,000 37.9 and 36.8).  The results are the same.
+// tokens at 17,000 positions 15.1 and 17.0, at 32,764 18.3 and 18.3; eight 21.1 and 25.7,
+// 26.6 and 30.6) and the rate of HBM beyond (four at 64,000 26.8 and 22.9, eight at
+// 50,000 38.2 and 36.4).  32 heads on 4: four at 10,000 15.7 and 17.5, at 30,000 26.1 and
+// 23.0; 64 on 8: eight at 8000 27.1 and 29.5, at 16,000 48.4 and 40.6.  The results are the same.
 int split_row_groups(int rows, int records, int groups) {
     return rows > 16 && records >= 3 * kSplitWaves * groups ? 2 : 1;
 }
 
 // Form and grid of more than kSplitRows rows.  k_kv8_flash_short while a CU's share is
 // under sixteen records of a 128-row tile (us, that form and k_kv8_flash: 777 tokens from
-// position 0 35 and 49, 1024 from 0 48 and 55, 200 from 1234 29 and 40, 64 from 0 13 and
-// 28), k_kv8_flash from there (2048 from 0 95 and 90, 300 from 20,000 154 and 127, 4096 from
-// 0 210 and 200, 4096 from 8192 843 and 640).  Parts fill the device where the tiles do
-// not, of four records or more: a part costs its rows' way out and back (100 tokens from
-// 500 in as many parts as records 29, in these 23).
+// position 0 34 and 45, 1024 from 0 42 and 50, 1400 from 0 60 and 60, 200 from 1234 29
+// and 38, 64 from 0 13 and 24), k_kv8_flash from there (2048 from 0 95 and 79, 300 from
+// 20,000 171 and 122, 4096 from 0 207 and 181, 4096 from 8192 860 and 642).  With more kv
+// heads of eight query heads each: on 4, 777 from 0 50 and 52, 1024 from 0 54 and 59, 300 from
+// 4000 90 and 72; on 8, 400 from 0 38 and 43, 200 from 2000 72 and 61.  Parts fill the
+// device where the tiles do not, of four records or more: a part costs its rows' way out
+// and back (100 tokens from 500 in as many parts as records 29, in these 23).
 struct FlashPlan {
     bool paired;
     int tiles, parts, run;   // workgroups per kv head and part; records of a part of the short form
