@@ -45,6 +45,7 @@ enum vmi_dtype { VMI_F32 = 0, VMI_BF16 = 1 };
 #define VMI_STATUS_BAD_RECORD 0x8u /* an acceptance record outside what vmi_spec_commit allows */
 #define VMI_STATUS_WAIT_GAVE_UP 0x10u /* a wait of vmi_accept_stochastic / vmi_sample_top_p outlasted its bound */
 #define VMI_STATUS_BAD_LOGITS 0x20u   /* a logit row of those calls had no finite value */
+#define VMI_STATUS_BAD_TARGET 0x40u   /* a target of vmi_head_loss outside the vocabulary */
 
 /* Last error message of the calling thread ("" when none). */
 const char* vmi_last_error(void);
@@ -583,6 +584,74 @@ int vmi_attention_tree_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, i
 size_t vmi_attention_prompt_kv8_workspace_bytes(const vmi_attn_layer_desc* desc, int T);
 int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x, int T, int pos0, uint8_t* cache,
                              int max_len, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * vmi_head_loss -- the softmax cross entropy of tokens under a head, without
+ * the logits in memory (no counterpart in the reference, which neither scores
+ * texts nor trains): for x bf16 [T, hidden] (behind the final norm), weight bf16
+ * [vocab, hidden] and targets int64 [T]
+ *   z = x . weight (fp32 sums of bf16 products), lse[t] = log sum_v exp z[t][v],
+ *   loss[t] = lse[t] - z[t][target],  both f32 [T].
+ * A token whose target is ignore_index has loss and lse 0 and is not read
+ * beyond that; a target outside [0, vocab) gives NaN in both and ORs
+ * VMI_STATUS_BAD_TARGET into *status (uint32 on the device, or NULL).  A token with
+ * a logit that is NaN or plus infinity has NaN.
+ * vmi_head_loss_grad -- its gradients, from the lse that it wrote:
+ *   g[t][v] = (d_loss[t] + d_lse[t]) exp(z[t][v] - lse[t]) - d_loss[t] [v == target],
+ *   dx = g . weight  (bf16 [T, hidden], or NULL),
+ *   dweight = g^T . x  (dweight_dtype VMI_BF16 or VMI_F32 [vocab, hidden], or NULL).
+ * d_loss, d_lse f32 [T] (d_lse may be NULL: zeros).  Tokens left out of the loss
+ * (ignore_index, or outside the vocabulary) have no gradient and add none.  z is
+ * formed again, a piece of the vocabulary at a time; g is rounded to bf16 as
+ * the operand of the two products, whose sums are fp32, rounded once.  Sums
+ * run in a fixed order: the same call gives the same bits.
+ * T <= 65536 (0: nothing but a dweight of zeros), hidden a multiple of 64 up to
+ * 8192, vocab <= 2^21, pointers 16-byte aligned (targets 8).  workspace: the query's bytes
+ * (0: a form that is not built), 256-byte aligned, nothing kept between calls.
+ * ------------------------------------------------------------------------ */
+size_t vmi_head_loss_workspace_bytes(int T, int hidden, int vocab);
+int vmi_head_loss(const uint16_t* x, int T, int hidden, const uint16_t* weight, int vocab, const int64_t* targets,
+                  int64_t ignore_index, float* loss, float* lse, uint32_t* status, void* workspace,
+                  size_t workspace_bytes, void* stream);
+size_t vmi_head_loss_grad_workspace_bytes(int T, int hidden, int vocab);
+int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const uint16_t* weight, int vocab, const int64_t* targets,
+                       int64_t ignore_index, const float* lse, const float* d_loss, const float* d_lse, uint16_t* dx,
+                       void* dweight, int dweight_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Routes sorted by expert, and back, for experts of a caller's own between a
+ * router's choice (vmi_moe_layer's ids_out, scores_out) and the residual: the
+ * gathers and the weighted scatter of FileStreamingMoeBlock._expert_major_forward
+ * (mlx_streaming/core/moe/block.py:111-243) as operators, with gradients.
+ * Route p = t k + j is token t's j-th.
+ *
+ * vmi_expert_plan -- from ids int32 [T, k]: the routes in the order of their
+ * experts, stable.  source int32 [T k]: the route of each row; place int32 [T, k]:
+ * the row of each route; offsets int32 [num_experts + 1]: expert e's rows are
+ * offsets[e] .. offsets[e + 1] - 1.  A route with id -1 has no expert: its row
+ * comes behind all others and its place is ~row; so has one with another
+ * id outside [0, num_experts), which also ORs VMI_STATUS_BAD_SLOT into *status (may be
+ * NULL).  num_experts <= 1024; workspace: the query's bytes (0: sizes not taken).
+ * vmi_expert_rows -- rows[place[t][j]] = x[t]; rows of routes without an expert
+ * are zeros.
+ * vmi_expert_combine -- out[t] = sum_j scores[t][j] y[place[t][j]] (+ residual[t]), over
+ * the routes with an expert in rank order in fp32, rounded once; scores f32
+ * [T, k], NULL: ones (the gradient of vmi_expert_rows).
+ * vmi_expert_combine_grad -- d_y[place[t][j]] = scores[t][j] d_out[t] (zeros in rows of routes
+ * without an expert), d_scores[t][j] = d_out[t] . y[place[t][j]] (0 there) in fp32, in a fixed
+ * order; d_y or d_scores may be NULL (y is read for d_scores only).
+ * x, out, residual, d_out [T, hidden] and rows, y, d_y [T k, hidden] of dtype (VMI_BF16,
+ * hidden a multiple of 8, or VMI_F32, of 4), 16-byte aligned; k <= 32, T k <= 2^24; T may be 0.
+ * Outputs must not overlap inputs.  A place past T k reads and writes nothing.
+ * ------------------------------------------------------------------------ */
+size_t vmi_expert_plan_workspace_bytes(int T, int k, int num_experts);
+int vmi_expert_plan(const int32_t* ids, int T, int k, int num_experts, int32_t* offsets, int32_t* source,
+                    int32_t* place, uint32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+int vmi_expert_rows(const void* x, int dtype, int T, int k, int hidden, const int32_t* place, void* rows, void* stream);
+int vmi_expert_combine(const void* y, int dtype, int T, int k, int hidden, const int32_t* place, const float* scores,
+                       const void* residual, void* out, void* stream);
+int vmi_expert_combine_grad(const void* d_out, const void* y, int dtype, int T, int k, int hidden, const int32_t* place,
+                            const float* scores, void* d_y, float* d_scores, void* stream);
 
 /* ------------------------------------------------------------------------
  * vmi_rmsnorm -- out = bf16(x * 1/sqrt(mean(x^2) + eps) * weight) per token

@@ -1,0 +1,306 @@
+"""The loss of tokens under a head and its gradients (vmi_head_loss, vmi_head_loss_grad)
+against the same formulas in 64 bits.
+
+Bars, written before the first run (u = 2^-24, S = sum |x w| of a logit):
+  logit       |e| <= H u S =: ez (H fp32 additions of exact products)
+  lse         ez + u (8 + |lse|) + 2^-17: a probability's exponent is a product and a
+              difference of numbers up to 2^8 in powers of two (2^-16 of itself at most, half
+              of that on average over a sum of them), the sums add up to V/64/4 terms a lane
+  loss        the lse's and the target's logit's
+  g           2^-8 |g| (bf16) + a p (2 ez + 2^-15)
+  dx, dW      the sums of |g|'s bounds times |w| (|x|), the additions' n u sum |g w|, and the
+              output's own rounding, 2^-8 of it (bf16)
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def log(msg):
+    print(msg, flush=True)
+
+
+def _inputs(dev, T, H, V, seed=0, ignored=0, foreseen=8.0):
+    import torch
+    g = torch.Generator(device=dev).manual_seed(1000 * seed + T + H + V)
+    w = (torch.randn((V, H), generator=g, device=dev) * (0.9 / H ** 0.5)).to(torch.bfloat16)
+    y = torch.randint(0, V, (T,), generator=g, device=dev)
+    x = torch.randn((T, H), generator=g, device=dev) + foreseen * torch.rand((T, 1), generator=g, device=dev) * w[y].float()
+    if ignored:
+        y[torch.randperm(T, generator=g, device=dev)[:ignored]] = -100
+    a = (torch.rand(T, generator=g, device=dev) + 0.5) / T
+    b = torch.rand(T, generator=g, device=dev) * 0.1 / T
+    return x.to(torch.bfloat16), w, y, a, b
+
+
+def _reference(x, w, y, d_loss, d_lse, V):
+    """64-bit loss, lse, dx, dW and the bounds of each."""
+    import torch
+    x, w = x.double(), w.double()
+    H = x.shape[1]
+    keep = (y >= 0) & (y < V)
+    z = x @ w.t().contiguous()
+    ez = H * U * (x.abs() @ w.abs().t().contiguous())
+    lse = torch.logsumexp(z, -1)
+    at = torch.where(keep, y, 0)
+    zero = torch.zeros_like(lse)
+    loss = torch.where(keep, lse - z.gather(1, at[:, None])[:, 0], zero)
+    top = ez.amax(-1)
+    e_lse = top + U * (8 + lse.abs()) + 2.0 ** -17
+    out = {"loss": (loss, e_lse + top), "lse": (torch.where(keep, lse, zero), e_lse)}
+    a = torch.where(keep, d_loss.double() + d_lse.double(), zero)[:, None]
+    p = torch.exp(z - lse[:, None])
+    g = a * p
+    g.scatter_add_(1, at[:, None], -torch.where(keep, d_loss.double(), zero)[:, None])
+    eg = 2.0 ** -8 * g.abs() + a * p * (2 * ez + 2.0 ** -15)
+    x = torch.where(keep[:, None], x, torch.zeros_like(x))
+    dx, dw = g @ w, g.t().contiguous() @ x
+    out["dx"] = (dx, eg @ w.abs() + V * U * (g.abs() @ w.abs()) + 2.0 ** -8 * dx.abs())
+    out["dw"] = (dw, eg.t().contiguous() @ x.abs() + len(y) * U * (g.abs().t().contiguous() @ x.abs()))
+    return out
+
+
+def _within(got, want, name, rounding=0.0):
+    ref, bound = want
+    err = (got.double() - ref).abs()
+    bound = bound + rounding * ref.abs() + 1e-30
+    worst = (err / bound).max().item() if err.numel() else 0.0
+    log(f"  {name}: error over bound {worst:.3f}")
+    assert (err <= bound).all(), f"{name}: {worst:.3g} of the bound"
+
+
+CASES = [(1, 64, 1), (1, 512, 16), (3, 64, 257), (5, 512, 4099), (16, 2048, 1601), (63, 192, 1000), (64, 1024, 1003),
+         (65, 320, 2048), (130, 512, 777), (256, 64, 70), (257, 2048, 3001), (777, 512, 8200), (300, 8192, 129)]
+
+
+@pytest.mark.parametrize("T,H,V", CASES)
+def test_loss_and_gradients(gpu, T, H, V):
+    import torch
+    from vates_amd.head import head_loss, head_loss_grad
+    log(f"case: head_loss T={T} H={H} V={V}")
+    x, w, y, a, b = _inputs(gpu, T, H, V, ignored=T // 5)
+    loss, lse = head_loss(x, w, y)
+    torch.cuda.synchronize()
+    ref = _reference(x, w, y, a, b, V)
+    _within(loss, ref["loss"], "loss")
+    _within(lse, ref["lse"], "lse")
+    dx, dw = head_loss_grad(x, w, y, lse, a, b)
+    torch.cuda.synchronize()
+    _within(dx, ref["dx"], "dx")
+    _within(dw, ref["dw"], "dweight bf16", 2.0 ** -8)
+    none, dw32 = head_loss_grad(x, w, y, lse, a, b, want_dx=False, dweight_dtype=torch.float32)
+    assert none is None and torch.equal(dw32.to(torch.bfloat16), dw)
+    _within(dw32, ref["dw"], "dweight f32")
+    dx2, none = head_loss_grad(x, w, y, lse, a, b, want_dweight=False)
+    assert none is None and torch.equal(dx2, dx)
+
+
+def test_several_pieces(gpu, monkeypatch):
+    """A vocabulary of several pieces, the last one short: tokens enough that g of all
+    of it passes 256 MB."""
+    import torch
+    from vates_amd.head import head_loss, head_loss_grad
+    T, H, V = 4100, 64, 33000
+    log(f"case: pieces T={T} H={H} V={V}")
+    x, w, y, a, b = _inputs(gpu, T, H, V, ignored=9)
+    loss, lse = head_loss(x, w, y)
+    dx, dw = head_loss_grad(x, w, y, lse, a, b)
+    ref = _reference(x, w, y, a, b, V)
+    _within(loss, ref["loss"], "loss")
+    _within(dx, ref["dx"], "dx")
+    _within(dw, ref["dw"], "dweight", 2.0 ** -8)
+
+
+def test_whole_vocabulary(gpu):
+    import torch
+    from vates_amd.head import head_loss, lm_head
+    T, H, V = 16, 2048, 151936
+    log("case: V=151936 against lm_head's logits")
+    x, w, y, _, _ = _inputs(gpu, T, H, V, ignored=2)
+    loss, lse = head_loss(x, w, y)
+    z = lm_head(x, w)[0].double()
+    keep = y >= 0
+    want = torch.logsumexp(z, -1)
+    hit = z.gather(1, y.clamp(min=0)[:, None])[:, 0]
+    # both sides' logits are off by H u S at most; S is below |x| |w| = 0.9 |x|
+    bound = 3 * H * U * 0.95 * x.double().norm(dim=-1) + 2.0 ** -17 + 32 * U
+    assert ((loss.double() - (want - hit)).abs()[keep] <= bound[keep]).all()
+    assert (loss[~keep] == 0).all() and (lse[~keep] == 0).all()
+
+
+def test_tokens_left_out(gpu):
+    """Ignored tokens and targets outside the vocabulary: what their rows hold reaches
+    nothing, their gradients are zeros; a batch without any token in the loss."""
+    import torch
+    from vates_amd._lib import VMI_STATUS_BAD_TARGET
+    from vates_amd.head import head_loss, head_loss_grad
+    T, H, V = 70, 512, 1003
+    log("case: tokens left out")
+    x, w, y, a, b = _inputs(gpu, T, H, V)
+    y[::3] = -100
+    keep = y >= 0
+    loss, lse = head_loss(x, w, y)
+    dx, dw = head_loss_grad(x, w, y, lse, a, b)
+    x2, a2, b2 = x.clone(), a.clone(), b.clone()
+    x2[::3] = float("nan")
+    x2[3] = float("inf")
+    a2[::3] = float("nan")
+    b2[::3] = float("inf")
+    got = head_loss(x2, w, y)
+    assert torch.equal(got[0], loss) and torch.equal(got[1], lse)
+    dx2, dw2 = head_loss_grad(x2, w, y, lse, a2, b2)
+    assert torch.equal(dx2, dx) and torch.equal(dw2, dw) and not dx[::3].any()
+    # the same tokens without the others
+    few = head_loss(x[keep].contiguous(), w, y[keep].contiguous())
+    assert torch.equal(few[0], loss[keep]) and torch.equal(few[1], lse[keep])
+    status = torch.zeros(1, dtype=torch.int32, device=gpu)
+    bad = y.clone()
+    bad[1], bad[2] = V, -7
+    l2, s2 = head_loss(x, w, bad, status=status)
+    assert status.item() == VMI_STATUS_BAD_TARGET and l2[1:3].isnan().all() and s2[1:3].isnan().all()
+    assert not l2[3:].isnan().any()
+    dx3, dw3 = head_loss_grad(x, w, bad, s2, a, b)
+    assert not dx3[1:3].any() and torch.isfinite(dw3).all()
+    # another index to ignore, a token of the vocabulary
+    z = head_loss(x, w, y.clamp(min=0), ignore_index=0)
+    assert (z[0][~keep] == 0).all() and torch.equal(z[0][keep & (y != 0)], loss[keep & (y != 0)])
+    none = torch.full_like(y, -100)
+    l4, s4 = head_loss(x2, w, none)
+    dx4, dw4 = head_loss_grad(x2, w, none, s4, a2, b2)
+    assert not l4.any() and not s4.any() and not dx4.any() and not dw4.any()
+    empty = head_loss(x[:0], w, y[:0])
+    dx5, dw5 = head_loss_grad(x[:0], w, y[:0], empty[1], a[:0], b[:0])
+    assert empty[0].shape == (0,) and dx5.shape == (0, H) and not dw5.any()
+
+
+def test_rows_that_are_not_finite(gpu):
+    """A token whose logits are not finite is NaN, the others' losses and dx are not."""
+    import torch
+    from vates_amd.head import head_loss, head_loss_grad
+    T, H, V = 9, 512, 1003
+    log("case: rows that are not finite")
+    x, w, y, a, b = _inputs(gpu, T, H, V)
+    loss, lse = head_loss(x, w, y)
+    dx, _ = head_loss_grad(x, w, y, lse, a, b)
+    x2 = x.clone()
+    x2[4, 7] = float("inf")
+    x2[6] = float("nan")
+    l2, s2 = head_loss(x2, w, y)
+    dx2, dw2 = head_loss_grad(x2, w, y, s2, a, b)
+    rest = [0, 1, 2, 3, 5, 7, 8]
+    assert l2[[4, 6]].isnan().all() and torch.equal(l2[rest], loss[rest])
+    assert torch.equal(dx2[rest], dx[rest]) and dx2[[4, 6]].isnan().all()
+    # equal logits, and logits far apart
+    flat = head_loss(x, torch.zeros_like(w), y)
+    assert (flat[0] - np.log(V)).abs().max().item() <= 32 * U * np.log(V)
+    far = head_loss((x * 1e4), w, y)
+    assert torch.isfinite(far[0]).all() and (far[0] >= 0).all()
+
+
+@pytest.mark.parametrize("T,H,V", [(37, 512, 1003), (300, 320, 2000)])
+def test_autograd_and_differences(gpu, T, H, V):
+    """The gradients that autograd gives are the entry's, and follow differences of
+    the loss: over a step d both ways, sum dx d against the loss's change, within dx's
+    bound, the losses' own and the third derivative's h^3."""
+    import torch
+    from vates_amd.head import head_loss, head_loss_grad
+    log(f"case: autograd T={T}")
+    x, w, y, a, b = _inputs(gpu, T, H, V, ignored=4)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss, lse = head_loss(xl, wl, y)
+    ((loss * a).sum() + (lse * b).sum()).backward()
+    dx, dw = head_loss_grad(x, w, y, lse.detach(), a, b)
+    assert torch.equal(xl.grad, dx) and torch.equal(wl.grad, dw)
+    # the mean over the tokens (gradients with stride 0), only one output, only one leaf
+    xl.grad = None
+    loss, _ = head_loss(xl, w, y)
+    loss.mean().backward()
+    ones = torch.full((T,), 1.0 / T, device=gpu)
+    assert torch.equal(xl.grad, head_loss_grad(x, w, y, lse.detach(), ones, want_dweight=False)[0])
+    _, only = head_loss(x, wl, y.int())
+    gw, = torch.autograd.grad(only, wl, b)
+    assert torch.equal(gw, head_loss_grad(x, w, y, lse.detach(), torch.zeros_like(a), b, want_dx=False)[1])
+    ref = _reference(x, w, y, a, b, V)
+    for name, base, grad, other in (("x", x, dx, w), ("w", w, dw, x)):
+        d = grad.float().sign() * (2.0 ** -5 if name == "x" else 2.0 ** -9)     # uphill, so that the change is large
+        hi, lo = (base.float() + d).to(torch.bfloat16), (base.float() - d).to(torch.bfloat16)
+        step = hi.double() - lo.double()
+
+        def total(v):
+            out = head_loss(v, w, y) if name == "x" else head_loss(x, v, y)
+            return (out[0].double() * a.double() + out[1].double() * b.double()).sum().item()
+
+        change = total(hi) - total(lo)
+        along = (grad.double() * step).sum().item()
+        wobble = (ref["dx" if name == "x" else "dw"][1] * step.abs()).sum().item() + 2.0 ** -8 * (grad.double() * step).abs().sum().item()
+        own = 2 * ((a + b).double() * (ref["loss"][1] + ref["lse"][1])).sum().item()
+        dz = (step @ other.double().t().contiguous()).abs().amax(-1) if name == "x" else (other.double() @ step.t().contiguous()).abs().amax(-1)
+        # f(+) - f(-) - f' (hi - lo): the third derivative of a log-sum-exp along dz is below dz^3, the second below dz^2
+        # (dz over the whole step; the middle of hi and lo, which are bf16, is off base by ez)
+        off = (hi.double() + lo.double()) / 2 - base.double()
+        ez = (off @ other.double().t().contiguous()).abs().amax(-1) if name == "x" else (other.double() @ off.t().contiguous()).abs().amax(-1)
+        curve = ((a + b).double() * (dz ** 3 / 12 + dz * ez)).sum().item()
+        log(f"  {name}: change {change:.6g} along {along:.6g} bounds {wobble:.2g} {own:.2g} {curve:.2g}")
+        assert abs(change - along) <= wobble + own + curve
+        assert wobble + own + curve <= 0.25 * change
+
+
+def test_same_bits_streams_and_graphs(gpu):
+    """The same call gives the same bits: again, on another stream, two at once on two
+    streams, and captured and replayed on new inputs."""
+    import torch
+    from vates_amd.head import head_loss, head_loss_grad
+    T, H, V = 130, 512, 4099
+    log("case: streams and graphs")
+    sets = [_inputs(gpu, T, H, V, seed=s, ignored=11) for s in range(3)]
+    want = []
+    for x, w, y, a, b in sets:
+        loss, lse = head_loss(x, w, y)
+        want.append((loss, lse, *head_loss_grad(x, w, y, lse, a, b)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for s, (x, w, y, a, b) in zip(streams, sets):
+            loss, lse = head_loss(x, w, y, stream=s)
+            got.append((loss, lse, *head_loss_grad(x, w, y, lse, a, b, stream=s)))
+        torch.cuda.synchronize()
+        for g, r in zip(got, want):
+            assert all(torch.equal(i, j) for i, j in zip(g, r))
+    # two captured graphs, each a training step of its own inputs, replayed in turn
+    held = [[t.clone() for t in sets[i]] for i in (0, 1)]
+    for h in held:
+        h[0].requires_grad_()
+        h[1].requires_grad_()
+
+    def step(h):
+        loss, lse = head_loss(*h[:3])
+        return (loss, lse, *torch.autograd.grad((loss, lse), h[:2], h[3:]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for h in held:
+            step(h)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for h in held:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(h))
+        graphs.append(g)
+    for order in ((0, 1), (1, 2), (2, 0), (0, 0)):
+        for h, n in zip(held, order):
+            with torch.no_grad():
+                for dst, src in zip(h, sets[n]):
+                    dst.copy_(src)
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for o, n in zip(outs, order):
+            assert all(torch.equal(i.detach(), j) for i, j in zip(o, want[n]))

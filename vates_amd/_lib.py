@@ -24,6 +24,7 @@ VMI_STATUS_BAD_POS = 0x4
 VMI_STATUS_BAD_RECORD = 0x8
 VMI_STATUS_WAIT_GAVE_UP = 0x10
 VMI_STATUS_BAD_LOGITS = 0x20
+VMI_STATUS_BAD_TARGET = 0x40
 
 
 class VmiError(RuntimeError):
@@ -152,6 +153,20 @@ _SIGNATURES = {
                             c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "vmi_head_tiles_bytes": (c_size_t, [c_int, c_int]),
     "vmi_head_tiles": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "vmi_head_loss_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vmi_head_loss": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_size_t, c_void_p]),
+    "vmi_head_loss_grad_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vmi_head_loss_grad": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "vmi_expert_plan_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vmi_expert_plan": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_size_t, c_void_p]),
+    "vmi_expert_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "vmi_expert_combine": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p]),
+    "vmi_expert_combine_grad": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p]),
     "vmi_lm_head_tiled": (c_int, [c_void_p, c_int, c_int, c_void_p, c_float, c_void_p, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
 }

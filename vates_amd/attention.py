@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 
 from ._lib import VMI_BF16, VMI_F32, VMI_KV8_TREE_ROW, QMat, VmiError, check, load
-from .moe import QuantizedProj, _ptr, _require, _stream_handle, scratch, workspace
+from .moe import QuantizedProj, _like, _on_current, _ptr, _require, _stream_handle, _stream_on, scratch, workspace
 
 
 class AttnDesc(ctypes.Structure):
@@ -240,28 +240,6 @@ class KVCache8(KVCache):
             check(load().vmi_kv8_write(keys.data_ptr(), keys.stride(0) * a, keys.stride(1) * b, values.data_ptr(),
                                        values.stride(0) * a, values.stride(1) * b, self.n_kv, start, n,
                                        self.data.data_ptr(), self.max_len, _stream_on(dev, stream)), "vmi_kv8_write")
-
-
-def _like(t: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
-    """An output of a call on `stream`, on t's device (shape None: and of its
-    shape), allocated in that stream's order."""
-    if stream is not None:
-        with torch.cuda.stream(stream):
-            return _like(t, shape, dtype, None)
-    return torch.empty_like(t) if shape is None else t.new_empty(shape, dtype=dtype)
-
-
-def _on_current(t: torch.Tensor) -> torch.device:
-    """The tensor's device, which has to be the one that the calls go to."""
-    dev = t.device
-    # (torch.cuda.current_device without its check that the device is initialised: t is on one)
-    if dev.type != "cuda" or dev.index != torch._C._cuda_getDevice():
-        raise VmiError(f"tensors on {dev} are not on the current HIP device")
-    return dev
-
-
-def _stream_on(dev: torch.device, stream) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
 
 
 _ATTEND_BYTES: dict = {}   # (device, T, query heads, kv heads) -> bytes of vmi_kv8_attention's workspace

@@ -1,4 +1,5 @@
-"""lm_head over the vocabulary with the argmax fused in (libvmi ``vmi_lm_head``).
+"""lm_head over the vocabulary with the argmax fused in (libvmi ``vmi_lm_head``), and
+the loss of tokens under a head with its gradients (``head_loss``).
 
 The analogue of the verify forward's tail ``logits = model.lm_head(inner.norm(h))``
 followed by ``preds = mx.argmax(logits, -1)`` (mlx_streaming/mtp/generate.py:208-217,
@@ -11,8 +12,8 @@ from typing import Optional
 
 import torch
 
-from ._lib import VmiError, check, load
-from .moe import _require, _stream_handle, workspace
+from ._lib import VMI_BF16, VMI_F32, VmiError, check, load
+from .moe import _like, _matches, _on_current, _on_stream, _ptr, _require, _stream_handle, _stream_on, scratch, workspace
 
 
 class TiledHead:
@@ -92,3 +93,105 @@ def lm_head(x: torch.Tensor, weight, norm_weight: Optional[torch.Tensor] = None,
                          ws.numel(), sh)
     check(rc, "vmi_lm_head_tiled" if tiled else "vmi_lm_head")
     return logits, argmax, max_logit
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, ignore_index, status):
+        loss, lse = _head_loss(x, weight, targets, ignore_index, status)
+        ctx.save_for_backward(x, weight, targets, lse)
+        ctx.ignore_index = ignore_index
+        ctx.set_materialize_grads(False)
+        return loss, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, d_lse):
+        x, weight, targets, lse = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if d_loss is None and d_lse is None:
+            return None, None, None, None, None
+        d_loss = torch.zeros_like(lse) if d_loss is None else d_loss.contiguous()
+        dx, dw = head_loss_grad(x, weight, targets, lse, d_loss, None if d_lse is None else d_lse.contiguous(),
+                                want_dx=need_x, want_dweight=need_w, ignore_index=ctx.ignore_index)
+        return dx, dw, None, None, None
+
+
+def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor) -> torch.device:
+    dev = _on_current(x)
+    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
+        raise VmiError(f"x must be [T, hidden] and weight [vocab, hidden], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _matches(x, "x", x.shape, torch.bfloat16, dev)
+    _matches(weight, "weight", weight.shape, torch.bfloat16, dev)
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise VmiError(f"targets must be int64 or int32 (got {targets.dtype})")
+    _matches(targets, "targets", (x.shape[0],), targets.dtype, dev)
+    return dev
+
+
+def _head_loss(x, weight, targets, ignore_index, status):
+    T, H = x.shape
+    V = weight.shape[0]
+    loss, lse = x.new_empty(T, dtype=torch.float32), x.new_empty(T, dtype=torch.float32)
+    lib = load()
+    ws = scratch(lib.vmi_head_loss_workspace_bytes(T, H, V), x.device)
+    check(lib.vmi_head_loss(x.data_ptr(), T, H, weight.data_ptr(), V, targets.data_ptr(), ignore_index, loss.data_ptr(),
+                            lse.data_ptr(), _ptr(status), ws.data_ptr(), ws.numel(), _stream_on(x.device, None)),
+          "vmi_head_loss")
+    return loss, lse
+
+
+def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
+              status: Optional[torch.Tensor] = None, stream=None):
+    """(loss f32 [T], lse f32 [T]): the softmax cross entropy of every token under a
+    head, lse - z[target] with z = x . weight and lse = log sum exp z, without the
+    logits in memory (``vmi_head_loss``).  The likelihood of a text is -loss.sum().
+
+    x bf16 [T, hidden] behind the final norm (T <= 65536, hidden a multiple of 64
+    up to 8192), weight bf16 [vocab, hidden] (the row-major head), targets int64 or
+    int32 [T].  A token with target ignore_index has loss and lse 0 and is not read;
+    a target outside the vocabulary gives NaN and ORs VMI_STATUS_BAD_TARGET into
+    status (int32 [1] on the device).  Differentiable in x and weight through
+    both outputs (``head_loss_grad``; a weight that needs no gradient costs none);
+    tokens left out of the loss have zeros and add nothing."""
+    dev = _check_loss(x, weight, targets)
+    if status is not None:
+        _matches(status, "status", (1,), torch.int32, dev)
+    return _on_stream(stream, _head_loss_on, x, weight, targets, ignore_index, status)
+
+
+def _head_loss_on(x, weight, targets, ignore_index, status):
+    targets = targets.long()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _HeadLoss.apply(x, weight, targets, ignore_index, status)
+    return _head_loss(x, weight, targets, ignore_index, status)
+
+
+def head_loss_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, d_loss: torch.Tensor,
+                   d_lse: Optional[torch.Tensor] = None, *, want_dx: bool = True, want_dweight: bool = True,
+                   dweight_dtype: torch.dtype = torch.bfloat16, ignore_index: int = -100, stream=None):
+    """(dx bf16 [T, hidden] or None, dweight [vocab, hidden] or None): the gradients
+    of ``head_loss`` from the lse that it returned and those of its outputs, f32
+    [T] (``vmi_head_loss_grad``).  dweight_dtype: bf16, or f32 for gradients that a
+    caller adds up itself.  The same call gives the same bits."""
+    dev = _check_loss(x, weight, targets)
+    T, H = x.shape
+    V = weight.shape[0]
+    for t, name in ((lse, "lse"), (d_loss, "d_loss"), (d_lse, "d_lse")):
+        if t is not None or name != "d_lse":
+            _matches(t, name, (T,), torch.float32, dev)
+    if dweight_dtype not in (torch.bfloat16, torch.float32):
+        raise VmiError(f"dweight_dtype must be bf16 or f32 (got {dweight_dtype})")
+    if not (want_dx or want_dweight):
+        raise VmiError("neither dx nor dweight wanted")
+    lib = load()
+    if targets.dtype is not torch.int64:
+        targets = _on_stream(stream, targets.long)
+    dx = _like(x, None, x.dtype, stream) if want_dx else None
+    dw = _like(weight, (V, H), dweight_dtype, stream) if want_dweight else None
+    ws = scratch(lib.vmi_head_loss_grad_workspace_bytes(T, H, V), dev, stream)
+    check(lib.vmi_head_loss_grad(x.data_ptr(), T, H, weight.data_ptr(), V, targets.data_ptr(), ignore_index, lse.data_ptr(),
+                                 d_loss.data_ptr(), _ptr(d_lse), _ptr(dx), _ptr(dw),
+                                 VMI_F32 if dweight_dtype is torch.float32 else VMI_BF16, ws.data_ptr(), ws.numel(),
+                                 _stream_on(dev, stream)), "vmi_head_loss_grad")
+    return dx, dw

@@ -73,6 +73,28 @@ def scratch(nbytes: int, device: torch.device, stream=None) -> torch.Tensor:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _like(t: torch.Tensor, shape, dtype: torch.dtype, stream) -> torch.Tensor:
+    """An output of a call on `stream`, on t's device (shape None: and of its
+    shape), allocated in that stream's order."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _like(t, shape, dtype, None)
+    return torch.empty_like(t) if shape is None else t.new_empty(shape, dtype=dtype)
+
+
+def _on_current(t: torch.Tensor) -> torch.device:
+    """The tensor's device, which has to be the one that the calls go to."""
+    dev = t.device
+    # (torch.cuda.current_device without its check that the device is initialised: t is on one)
+    if dev.type != "cuda" or dev.index != torch._C._cuda_getDevice():
+        raise VmiError(f"tensors on {dev} are not on the current HIP device")
+    return dev
+
+
+def _stream_on(dev: torch.device, stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
+
+
 @dataclass
 class QuantizedProj:
     """One affine-quantised projection stack: weight uint32-bits
@@ -450,3 +472,175 @@ class MoELayer:
                                _ptr(ids_out), _ptr(scores_out), ws.data_ptr(), ws.numel(), sh)
         check(rc, "vmi_moe_layer")
         return out
+
+
+# ------------------------------------------------ routes sorted by expert, and back
+@dataclass
+class ExpertPlan:
+    """Where the routes of a batch go when they are sorted by expert, each
+    expert's in the order of their tokens (``expert_plan``).  Route t*k + j is
+    token t's j-th; expert e's rows are offsets[e] .. offsets[e + 1] - 1."""
+
+    offsets: torch.Tensor   # int32 [experts + 1]; the last: how many rows have an expert
+    source: torch.Tensor    # int32 [T * k]: the route of each row
+    place: torch.Tensor     # int32 [T, k]: the row of each route, ~row where it has no expert (those come last)
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.numel() - 1
+
+    @property
+    def tokens(self) -> int:
+        return self.place.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.place.shape[1]
+
+
+def _on_stream(stream, fn, *args):
+    """fn(*args) on `stream`: what autograd records then runs backward there too."""
+    if stream is None:
+        return fn(*args)
+    with torch.cuda.stream(stream):
+        return fn(*args)
+
+
+def _rows_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype is torch.bfloat16:
+        return _lib.VMI_BF16
+    if t.dtype is torch.float32:
+        return _lib.VMI_F32
+    raise VmiError(f"{name} must be bf16 or f32 (got {t.dtype})")
+
+
+def _matches(t: torch.Tensor, name: str, shape, dtype: torch.dtype, dev: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+        raise VmiError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {dev}")
+
+
+def expert_plan(ids: torch.Tensor, num_experts: int, *, status: Optional[torch.Tensor] = None,
+                stream=None) -> ExpertPlan:
+    """The plan that sorts a batch's routes by expert, stably (``vmi_expert_plan``).
+
+    ids int32 [T, k], a router's choice of experts (``MoELayer``'s ids_out); -1
+    is a route without an expert (padding, or past an expert's capacity), and so
+    is any other id outside [0, num_experts), which also ORs
+    VMI_STATUS_BAD_SLOT into status (int32 [1] on the device)."""
+    dev = _on_current(ids)
+    if ids.dim() != 2 or ids.shape[1] == 0:
+        raise VmiError(f"ids must be [T, k], got {tuple(ids.shape)}")
+    _matches(ids, "ids", ids.shape, torch.int32, dev)
+    if status is not None:
+        _matches(status, "status", (1,), torch.int32, dev)
+    T, k = ids.shape
+    lib = load()
+    nbytes = lib.vmi_expert_plan_workspace_bytes(T, k, num_experts)
+    buf = _like(ids, (num_experts + 1 + 2 * T * k if nbytes else 0,), torch.int32, stream)
+    offsets, source, place = buf.split([num_experts + 1, T * k, T * k]) if nbytes else (buf, buf, buf)
+    ws = scratch(nbytes, dev, stream)
+    check(lib.vmi_expert_plan(ids.data_ptr(), T, k, num_experts, offsets.data_ptr(), source.data_ptr(), place.data_ptr(),
+                              _ptr(status), ws.data_ptr(), ws.numel(), _stream_on(dev, stream)), "vmi_expert_plan")
+    return ExpertPlan(offsets, source, place.view(T, k))
+
+
+def _sorted_rows(x: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
+    T, k = place.shape
+    rows = x.new_empty((T * k, x.shape[1]))
+    check(load().vmi_expert_rows(x.data_ptr(), _rows_dtype(x, "x"), T, k, x.shape[1], place.data_ptr(), rows.data_ptr(),
+                                 _stream_on(x.device, None)), "vmi_expert_rows")
+    return rows
+
+
+def _combined(y: torch.Tensor, place: torch.Tensor, scores: Optional[torch.Tensor],
+              residual: Optional[torch.Tensor]) -> torch.Tensor:
+    T, k = place.shape
+    out = y.new_empty((T, y.shape[1]))
+    check(load().vmi_expert_combine(y.data_ptr(), _rows_dtype(y, "y"), T, k, y.shape[1], place.data_ptr(), _ptr(scores),
+                                    _ptr(residual), out.data_ptr(), _stream_on(y.device, None)), "vmi_expert_combine")
+    return out
+
+
+class _SortByExpert(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, place):
+        ctx.save_for_backward(place)
+        return _sorted_rows(x, place)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_rows):
+        place, = ctx.saved_tensors
+        return _combined(d_rows.contiguous(), place, None, None), None
+
+
+class _CombineExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, place, scores, residual):
+        ctx.save_for_backward(y if scores is not None and scores.requires_grad else None, place, scores)
+        return _combined(y, place, scores, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        y, place, scores = ctx.saved_tensors
+        need_y, _, need_scores, need_residual = ctx.needs_input_grad
+        d_out = d_out.contiguous()
+        T, k = place.shape
+        d_y = d_out.new_empty((T * k, d_out.shape[1])) if need_y else None
+        d_scores = torch.empty_like(scores) if need_scores else None
+        if need_y or need_scores:
+            check(load().vmi_expert_combine_grad(d_out.data_ptr(), _ptr(y), _rows_dtype(d_out, "d_out"), T, k,
+                                                 d_out.shape[1], place.data_ptr(), _ptr(scores), _ptr(d_y),
+                                                 _ptr(d_scores), _stream_on(d_out.device, None)),
+                  "vmi_expert_combine_grad")
+        return d_y, None, d_scores, d_out if need_residual else None
+
+
+def _check_plan(plan: ExpertPlan, dev: torch.device) -> None:
+    if not isinstance(plan, ExpertPlan):
+        raise VmiError("plan must be an ExpertPlan")
+    _matches(plan.place, "plan.place", plan.place.shape, torch.int32, dev)
+
+
+def sort_by_expert(x: torch.Tensor, plan: ExpertPlan, *, stream=None) -> torch.Tensor:
+    """The tokens' rows in the plan's order: row plan.place[t, j] is x[t], for
+    experts of the caller's own (expert e's rows are plan.offsets[e] ..).
+
+    x bf16 or f32 [T, hidden] (hidden a multiple of 8, f32 of 4); returns
+    [T * k, hidden], rows behind the last expert's are zeros.  Differentiable: a
+    token's gradient is the sum of its rows', in rank order in fp32, rounded once."""
+    dev = _on_current(x)
+    _check_plan(plan, dev)
+    if x.dim() != 2 or x.shape[0] != plan.tokens:
+        raise VmiError(f"x must be [{plan.tokens}, hidden], got {tuple(x.shape)}")
+    _rows_dtype(x, "x")
+    _matches(x, "x", x.shape, x.dtype, dev)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _on_stream(stream, _SortByExpert.apply, x, plan.place)
+    return _on_stream(stream, _sorted_rows, x, plan.place)
+
+
+def combine_experts(y: torch.Tensor, plan: ExpertPlan, scores: Optional[torch.Tensor] = None, *,
+                    residual: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """out[t] = residual[t] + sum_j scores[t, j] * y[plan.place[t, j]], in rank
+    order in fp32, rounded once; routes without an expert add nothing, whatever
+    their rows hold.
+
+    y bf16 or f32 [T * k, hidden] in the plan's order, scores f32 [T, k] (None:
+    ones), residual [T, hidden] of y's type or None.  Differentiable in y,
+    scores and residual (rows without an expert get zeros)."""
+    dev = _on_current(y)
+    _check_plan(plan, dev)
+    T, k = plan.place.shape
+    if y.dim() != 2 or y.shape[0] != T * k:
+        raise VmiError(f"y must be [{T * k}, hidden], got {tuple(y.shape)}")
+    _rows_dtype(y, "y")
+    _matches(y, "y", y.shape, y.dtype, dev)
+    if scores is not None:
+        _matches(scores, "scores", (T, k), torch.float32, dev)
+    if residual is not None:
+        _matches(residual, "residual", (T, y.shape[1]), y.dtype, dev)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, scores, residual)):
+        return _on_stream(stream, _CombineExperts.apply, y, plan.place, scores, residual)
+    return _on_stream(stream, _combined, y, plan.place, scores, residual)
