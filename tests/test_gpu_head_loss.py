@@ -153,9 +153,12 @@ def test_tokens_left_out(gpu):
     assert torch.equal(got[0], loss) and torch.equal(got[1], lse)
     dx2, dw2 = head_loss_grad(x2, w, y, lse, a2, b2)
     assert torch.equal(dx2, dx) and torch.equal(dw2, dw) and not dx[::3].any()
-    # the same tokens without the others
+    # the same tokens without the others: another count of tokens cuts the vocabulary into other strips, so the sums run
+    # in another order; both results are within the bars of the 64-bit one, hence within twice that of each other
     few = head_loss(x[keep].contiguous(), w, y[keep].contiguous())
-    assert torch.equal(few[0], loss[keep]) and torch.equal(few[1], lse[keep])
+    ref = _reference(x, w, y, a, b, V)
+    for got, old, name in zip(few, (loss, lse), ("loss", "lse")):
+        assert ((got.double() - old[keep].double()).abs() <= 2 * ref[name][1][keep]).all()
     status = torch.zeros(1, dtype=torch.int32, device=gpu)
     bad = y.clone()
     bad[1], bad[2] = V, -7

@@ -50,9 +50,9 @@ def test_loss_workspaces(lib):
         for bad in ((-1, 512, 1000), (65537, 512, 1000), (4, 100, 1000), (4, 8256, 1000), (4, 512, 0), (4, 512, (1 << 21) + 1)):
             assert q(*bad) == 0
         assert q(0, 512, 1000) > 0
-    # no logits: the loss of a long block takes a few MB, its gradients' pieces a bounded part of V
+    # no logits (2.5 GB of bf16 at 8192 tokens): the loss takes a few MB, its gradients a piece of half a GB beside x and dx
     assert lib.vmi_head_loss_workspace_bytes(8192, 2048, 151936) < 8 << 20
-    assert lib.vmi_head_loss_grad_workspace_bytes(8192, 2048, 151936) < 512 << 20
+    assert lib.vmi_head_loss_grad_workspace_bytes(8192, 2048, 151936) < 768 << 20
     assert lib.vmi_head_loss_grad_workspace_bytes(65536, 2048, 151936) < 3 << 30
 
 

@@ -416,6 +416,21 @@ __device__ __forceinline__ void vmi_lds_dma16_at(const void* base, uint32_t off,
     (void)lds;
 #endif
 }
+// Nontemporal form.
+__device__ __forceinline__ void vmi_lds_dma16_at_nt(const void* base, uint32_t off, const void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(off), "s"(base), "s"(m0)
+                 : "memory", "m0");
+#else
+    (void)base;
+    (void)off;
+    (void)lds;
+#endif
+}
 __device__ __forceinline__ void vmi_lds_dma4_at(const void* base, uint32_t off, const void* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane(

@@ -43,22 +43,23 @@ __device__ __forceinline__ int ls_wave() { return __builtin_amdgcn_readfirstlane
 
 // ------------------------------------------------------------------ products
 // One workgroup's tile: BM x BN, waves WM x WN.  SLOW operands have k as the slow
-// index (rows of BM or BN = 256 values).
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_, bool ASLOW_, bool BSLOW_>
+// index (rows of BM or BN = 256 values).  ONCE: A is read by this workgroup alone.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, bool ASLOW_, bool BSLOW_, bool ONCE_ = false>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
-    static constexpr bool ASLOW = ASLOW_, BSLOW = BSLOW_;
+    static constexpr bool ASLOW = ASLOW_, BSLOW = BSLOW_, ONCE = ONCE_;
     static constexpr int MB = BM / WM / 16, NB = BN / WN / 16;
     static constexpr int kA = BM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
-    static constexpr int DA = kA / 1024 / kWaves, DB = kB / 1024 / kWaves;   // DMA instructions of a wave a step
-    static_assert(WM * WN == kWaves && DA >= 1 && DB >= 1, "shape");
+    // kilobytes, one DMA instruction each, dealt to the waves in turn
+    static constexpr int DA = kA / 1024 / kWaves, DB = (kB / 1024 + kWaves - 1) / kWaves, RB = kB / 1024 % kWaves;
+    static_assert(WM * WN == kWaves && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && kA % (1024 * kWaves) == 0, "shape");
     static_assert((!ASLOW || BM == 256) && (!BSLOW || BN == 256), "slow operands have rows of 512 bytes");
 };
 
-// Row and 16-byte piece of a lane in DMA instruction i of D of its wave.
-template <int D, bool SLOW>
+// Row and 16-byte piece of a lane in the wave's DMA instruction i.
+template <bool SLOW>
 __device__ __forceinline__ void ls_slot(int i, int& row, int& piece) {
-    const int lane = threadIdx.x & 63, u = ls_wave() * D + i;
+    const int lane = threadIdx.x & 63, u = ls_wave() + kWaves * i;
     if constexpr (SLOW) {   // two rows of 32 pieces
         row = 2 * u + (lane >> 5);
         const int s = lane & 31;
@@ -68,10 +69,27 @@ __device__ __forceinline__ void ls_slot(int i, int& row, int& piece) {
         piece = (lane & 7) ^ (row & 7);
     }
 }
-template <int D>
+// D instructions, the last for the first R waves only (R: 0, all).
+template <int D, int R, bool ONCE>
 __device__ __forceinline__ void ls_dma(const void* base, const uint32_t (&off)[D], uint8_t* lds) {
+    const int w = ls_wave();
 #pragma unroll
-    for (int i = 0; i < D; ++i) vmi_lds_dma16_at(base, off[i], lds + (ls_wave() * D + i) * 1024);
+    for (int i = 0; i < D; ++i) {
+        if (R && i == D - 1 && w >= R) continue;
+        if constexpr (ONCE)
+            vmi_lds_dma16_at_nt(base, off[i], lds + (w + kWaves * i) * 1024);
+        else
+            vmi_lds_dma16_at(base, off[i], lds + (w + kWaves * i) * 1024);
+    }
+}
+// Until the wave's oldest step is there (STAGES - 1 are in flight).
+template <class S>
+__device__ __forceinline__ void ls_wait() {
+    constexpr int n = S::STAGES - 2;
+    if (S::RB == 0 || n == 0 || ls_wave() < S::RB)
+        vmi_vm_wait_c<n * (S::DA + S::DB)>();
+    else
+        vmi_vm_wait_c<n * (S::DA + S::DB - 1)>();
 }
 
 // Operand of block b (16 of m or n, from `first` on) and k = 32 kk ..
@@ -134,7 +152,7 @@ __device__ __forceinline__ void ls_run(uint8_t* lds, Job& job, int total) {
     for (int s = 0; s < S::STAGES - 1; ++s) job.issue(lds + s * S::kStage);
     int in = S::STAGES - 1, out = 0;
     for (int s = 0; s < total; ++s) {
-        vmi_vm_wait_c<(S::STAGES - 2) * (S::DA + S::DB)>();
+        ls_wait<S>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -158,37 +176,49 @@ struct Coef {
     int32_t target;
 };
 
+// What k_loss_rows leaves for the kernels behind it.
+struct Meta {
+    int32_t nv;          // tokens in the loss
+    int32_t bn;          // tokens of a tile
+    int32_t strips;      // of the vocabulary, or of a whole piece of it
+    int32_t last;        // of the last piece
+    int32_t splits;      // sums of dx over the columns of a piece
+};
+__device__ __forceinline__ Meta ls_meta(const Meta* m) {
+    const int32_t* p = &m->nv;
+    return {vmi_sload_i32(p), vmi_sload_i32(p + 1), vmi_sload_i32(p + 2), vmi_sload_i32(p + 3), vmi_sload_i32(p + 4)};
+}
+
 struct LogitArgs {
     const uint16_t *x, *w;
-    const int32_t *idx, *meta;   // meta[0]: nv
+    const int32_t* idx;
+    const Meta* meta;
     const Coef* coef;
     int H, V;
     // score
     float2* part;                // [item][BN] maximum, sum
     float* hit;                  // [nv] the target's logit
     // gradient
-    int v0, v1;                  // the piece (v1 past V: columns of zeros)
+    int v0, v1, last;            // the piece (v1 past V: columns of zeros), whether it is the last
     uint16_t* g;                 // [tokens][ldg]
     int64_t ldg;
 };
 
-// The strips that the vocabulary is cut into for nrb blocks of tokens.
-__device__ __host__ __forceinline__ int ls_strips(int nrb, int grid) { return 8 * nrb <= grid ? grid / nrb : 8; }
-
-template <class S, bool GRAD>
+// GRAD: 0 loss, 1 g, 2 g and, BN rows behind it, what its rounding left.
+template <class S, int GRAD>
 struct LogitJob {
     const LogitArgs& a;
+    const Coef* coef;                 // LDS: the block's tokens
     int nv, rb, v1;                   // tokens, block, end of the strip
     int tile;                         // first row of the tile being multiplied
     int next, k, nk;                  // first row of the tile being asked for, its step, steps of one
     int kd;                           // step being multiplied
     uint32_t offa[S::DA], offb[S::DB];
-    Coef c[S::NB];
     float m[S::NB], l[S::NB];
     int m0, n0;
 
-    __device__ __forceinline__ LogitJob(const LogitArgs& a_, int rb_, int v0_, int v1_) : a(a_), rb(rb_), v1(v1_) {
-        nv = vmi_sload_i32(a.meta);
+    __device__ __forceinline__ LogitJob(const LogitArgs& a_, Coef* coef_, int nv_, int rb_, int v0_, int v1_)
+        : a(a_), coef(coef_), nv(nv_), rb(rb_), v1(v1_) {
         nk = a.H / kBK;
         tile = v0_;
         next = min(v0_, a.V - 1);   // (a piece's last tile may lie behind the vocabulary: its columns are zeros)
@@ -199,16 +229,17 @@ struct LogitJob {
 #pragma unroll
         for (int i = 0; i < S::DB; ++i) {
             int row, piece;
-            ls_slot<S::DB, false>(i, row, piece);
-            const int c0 = min(rb * S::BN + row, nv - 1);
-            offb[i] = (uint32_t)(a.idx ? a.idx[c0] : c0) * (uint32_t)(2 * a.H) + 16 * piece;
+            ls_slot<false>(i, row, piece);
+            const int c = min(rb * S::BN + row, nv - 1);
+            offb[i] = (uint32_t)(a.idx ? a.idx[c] : c) * (uint32_t)(2 * a.H) + 16 * piece;
         }
         rows();
+        if (threadIdx.x < S::BN) {
+            const int t = rb * S::BN + threadIdx.x;
+            coef_[threadIdx.x] = t < nv ? a.coef[t] : Coef{0.0f, 0.0f, __builtin_inff(), -1};
+        }
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
-            const int t = rb * S::BN + n0 + 16 * n;
-            c[n] = a.coef[min(t, nv - 1)];
-            if (t >= nv) c[n] = Coef{0.0f, 0.0f, __builtin_inff(), -1};
             m[n] = kLowest;
             l[n] = 0.0f;
         }
@@ -217,13 +248,13 @@ struct LogitJob {
 #pragma unroll
         for (int i = 0; i < S::DA; ++i) {
             int row, piece;
-            ls_slot<S::DA, false>(i, row, piece);
+            ls_slot<false>(i, row, piece);
             offa[i] = (uint32_t)min(row, min(v1, a.V) - 1 - next) * (uint32_t)(2 * a.H) + 16 * piece;
         }
     }
     __device__ __forceinline__ void issue(uint8_t* lds) {
-        ls_dma<S::DA>(a.w + (size_t)next * a.H + (size_t)k * kBK, offa, lds);
-        ls_dma<S::DB>(a.x + (size_t)k * kBK, offb, lds + S::kA);
+        ls_dma<S::DA, 0, S::ONCE>(a.w + (size_t)next * a.H + (size_t)k * kBK, offa, lds);
+        ls_dma<S::DB, S::RB, false>(a.x + (size_t)k * kBK, offb, lds + S::kA);
         if (++k == nk) {
             if (next + S::BM < min(v1, a.V)) {
                 next += S::BM;
@@ -237,7 +268,7 @@ struct LogitJob {
     __device__ __forceinline__ void done(vmi_f4 (&acc)[S::MB][S::NB]) {
         if (++kd < nk) return;
         kd = 0;
-        if constexpr (GRAD)
+        if constexpr (GRAD != 0)
             store(acc);
         else
             sum(acc);
@@ -258,7 +289,7 @@ struct LogitJob {
         }
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
-            const int d = c[n].target - tile - m0;
+            const int d = coef[n0 + 16 * n].target - tile - m0;
             if (__any((uint32_t)d < (uint32_t)(16 * S::MB))) {
 #pragma unroll
                 for (int mb = 0; mb < S::MB; ++mb)
@@ -271,11 +302,12 @@ struct LogitJob {
             for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[mb][n][r]);
-            float s = l[n] * __builtin_amdgcn_exp2f((m[n] - top) * kLog2e);   // (a product's rounding before the difference would
+            // (a product's rounding before the difference would grow with the logits)
+            float s = l[n] * __builtin_amdgcn_exp2f((m[n] - top) * kLog2e);
 #pragma unroll
             for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[mb][n][r] - top) * kLog2e);   // grow with the logits)
+                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[mb][n][r] - top) * kLog2e);
             m[n] = top;
             l[n] = s;
         }
@@ -283,18 +315,25 @@ struct LogitJob {
     __device__ __forceinline__ void store(vmi_f4 (&acc)[S::MB][S::NB]) {
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
-            const int t = rb * S::BN + n0 + 16 * n, d = c[n].target - tile - m0;
+            const Coef c = coef[n0 + 16 * n];
+            const int t = rb * S::BN + n0 + 16 * n, d = c.target - tile - m0;
             uint16_t* dst = a.g + (int64_t)t * a.ldg + (tile - a.v0) + m0;
 #pragma unroll
             for (int mb = 0; mb < S::MB; ++mb) {
+                if (tile + m0 + 16 * mb >= v1) continue;   // another strip's
                 float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    v[r] = c[n].a * __builtin_amdgcn_exp2f((acc[mb][n][r] - c[n].lse) * kLog2e);
-                    if (d == 16 * mb + r) v[r] -= c[n].b;
+                    v[r] = c.a * __builtin_amdgcn_exp2f((acc[mb][n][r] - c.lse) * kLog2e);
+                    if (d == 16 * mb + r) v[r] -= c.b;
                     if (t >= nv || tile + m0 + 16 * mb + r >= a.V) v[r] = 0.0f;
                 }
-                *reinterpret_cast<uint2*>(dst + 16 * mb) = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
+                const uint2 u = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
+                *reinterpret_cast<uint2*>(dst + 16 * mb) = u;
+                if constexpr (GRAD == 2)
+                    *reinterpret_cast<uint2*>(dst + S::BN * a.ldg + 16 * mb) =
+                        make_uint2(vmi_pack_bf16x2(v[0] - __uint_as_float(u.x << 16), v[1] - __uint_as_float(u.x & 0xffff0000u)),
+                                   vmi_pack_bf16x2(v[2] - __uint_as_float(u.y << 16), v[3] - __uint_as_float(u.y & 0xffff0000u)));
             }
         }
     }
@@ -309,19 +348,16 @@ __device__ __forceinline__ void ls_join(float& m, float& l, float m2, float l2) 
 // A workgroup takes a block of tokens and a strip of the vocabulary, whose tiles follow
 // each other without a pause of the DMA.
 template <class S>
-__global__ __launch_bounds__(kThreads) void k_loss_score(LogitArgs a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::STAGES * S::kStage];
-    const int nv = vmi_sload_i32(a.meta), nrb = (nv + S::BN - 1) / S::BN;
-    if (nrb == 0) return;
-    const int strips = ls_strips(nrb, gridDim.x), per = ((a.V + strips - 1) / strips + 15) & ~15;
-    for (int item = blockIdx.x; item < nrb * strips; item += gridDim.x) {
+__device__ __forceinline__ void ls_score(const LogitArgs& a, const Meta& me, uint8_t* lds, Coef* coef) {
+    const int nrb = (me.nv + S::BN - 1) / S::BN, per = ((a.V + me.strips - 1) / me.strips + 15) & ~15;
+    for (int item = blockIdx.x; item < nrb * me.strips; item += gridDim.x) {
         const int rb = item % nrb, v0 = (item / nrb) * per, v1 = min(a.V, v0 + per);
         float2* part = a.part + (size_t)item * S::BN;
         if (v0 >= v1) {
             if (threadIdx.x < S::BN) part[threadIdx.x] = make_float2(kLowest, 0.0f);
             continue;
         }
-        LogitJob<S, false> job(a, rb, v0, v1);
+        LogitJob<S, 0> job(a, coef, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
         float2* s_ml = reinterpret_cast<float2*>(lds);   // [WM][BN]
 #pragma unroll
@@ -342,35 +378,68 @@ __global__ __launch_bounds__(kThreads) void k_loss_score(LogitArgs a) {
 }
 
 // The same tiles of one piece of the vocabulary as rows of g.
-template <class S>
-__global__ __launch_bounds__(kThreads) void k_loss_g(LogitArgs a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::STAGES * S::kStage];
-    const int nv = vmi_sload_i32(a.meta), nrb = (nv + S::BN - 1) / S::BN;
-    if (nrb == 0) return;
-    const int tiles = (a.v1 - a.v0 + S::BM - 1) / S::BM, strips = min(ls_strips(nrb, gridDim.x), tiles);
-    const int per = (tiles + strips - 1) / strips * S::BM;
+template <class S, int GRAD>
+__device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, uint8_t* lds, Coef* coef) {
+    const int nrb = (me.nv + S::BN - 1) / S::BN, strips = a.last ? me.last : me.strips;
+    const int per = ((a.v1 - a.v0 + strips - 1) / strips + 15) & ~15;
     for (int item = blockIdx.x; item < nrb * strips; item += gridDim.x) {
         const int rb = item % nrb, v0 = a.v0 + (item / nrb) * per, v1 = min(a.v1, v0 + per);
         if (v0 >= v1) continue;
-        LogitJob<S, true> job(a, rb, v0, v1);
+        LogitJob<S, GRAD> job(a, coef, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
+    }
+}
+
+// Tiles by tokens of a block.  Up to 64 tokens the head is read once, by one workgroup each
+// part of it, and its bytes bound the call; above, five widths, of which k_loss_rows takes the one with the least work.
+constexpr int kFew = 64, kFewest = 32;
+using Score32 = Tile<256, 32, 8, 1, 4, false, false, true>;
+using Score64 = Tile<256, 64, 4, 2, 3, false, false, true>;
+template <int BN>
+using ScoreN = Tile<256, BN, 4, 2, BN <= 160 ? 3 : 2, false, false>;
+template <class S>
+constexpr int kLds = S::STAGES * S::kStage;
+
+// WHICH: 32, 64, or 0 for the widths above.
+template <int WHICH, int GRAD>
+__global__ __launch_bounds__(kThreads) void k_loss_logits(LogitArgs a) {
+    constexpr int kBytes = WHICH == 32 ? kLds<Score32> : WHICH == 64 ? kLds<Score64> : kLds<ScoreN<160>>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
+    __shared__ Coef coef[WHICH ? WHICH : 256];
+    const Meta me = ls_meta(a.meta);
+    if (me.nv == 0) return;
+    auto go = [&](auto s) {
+        using S = decltype(s);
+        static_assert(kLds<S> <= kBytes, "LDS");
+        if constexpr (GRAD)
+            ls_g<S, GRAD>(a, me, lds, coef);
+        else
+            ls_score<S>(a, me, lds, coef);
+    };
+    if constexpr (WHICH == 32) {
+        go(Score32{});
+    } else if constexpr (WHICH == 64) {
+        go(Score64{});
+    } else {
+        switch (me.bn) {
+            case 128: go(ScoreN<128>{}); break;
+            case 160: go(ScoreN<160>{}); break;
+            case 192: go(ScoreN<192>{}); break;
+            case 224: go(ScoreN<224>{}); break;
+            default: go(ScoreN<256>{}); break;
+        }
     }
 }
 
 // ------------------------------------------------------------------------ dx
 struct DxArgs {
     const uint16_t *w, *g;
-    const int32_t* meta;
+    const Meta* meta;
     int H, V, v0, cols;      // the piece's first row, its columns of g (a multiple of 64)
     int64_t ldg;
     float* sum;              // [split][token block rows][H]
     int add;                 // a later piece than the first: added to the sums
-    int short_steps;         // steps of the shortest piece: no split without columns
 };
-
-__device__ __forceinline__ int ls_dx_splits(int nrb, int nht, int grid, int steps) {
-    return min(max(grid / (nrb * nht), 1), steps);
-}
 
 template <class S>
 struct DxJob {
@@ -385,7 +454,7 @@ struct DxJob {
 #pragma unroll
         for (int i = 0; i < S::DB; ++i) {
             int row, piece;
-            ls_slot<S::DB, false>(i, row, piece);
+            ls_slot<false>(i, row, piece);
             offb[i] = (uint32_t)row * (uint32_t)(2 * a.ldg) + 16 * piece;
         }
     }
@@ -396,12 +465,12 @@ struct DxJob {
 #pragma unroll
         for (int i = 0; i < S::DA; ++i) {
             int row, piece;
-            ls_slot<S::DA, true>(i, row, piece);
+            ls_slot<true>(i, row, piece);
             const int col = min(ht * S::BM + 8 * piece, a.H - 8);
             offa[i] = (uint32_t)(max(min(row, rows - 1), 0)) * (uint32_t)(2 * a.H) + 2 * col;
         }
-        ls_dma<S::DA>(a.w + (size_t)(a.v0 + base) * a.H, offa, lds);
-        ls_dma<S::DB>(a.g + (int64_t)rb * S::BN * a.ldg + kn, offb, lds + S::kA);
+        ls_dma<S::DA, 0, false>(a.w + (size_t)(a.v0 + base) * a.H, offa, lds);
+        ls_dma<S::DB, S::RB, false>(a.g + (int64_t)rb * S::BN * a.ldg + kn, offb, lds + S::kA);
         if (--left > 0) kn += kBK;
     }
     __device__ __forceinline__ void done(vmi_f4 (&acc)[S::MB][S::NB]) {
@@ -425,11 +494,8 @@ struct DxJob {
 // Tiles of 256 hidden values by a block of tokens; where these leave CUs idle the
 // piece's columns are split over several workgroups, each with sums of its own.
 template <class S>
-__global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::STAGES * S::kStage];
-    const int nv = vmi_sload_i32(a.meta), nrb = (nv + S::BN - 1) / S::BN, nht = (a.H + S::BM - 1) / S::BM, steps = a.cols / kBK;
-    if (nrb == 0) return;
-    const int splits = ls_dx_splits(nrb, nht, gridDim.x, a.short_steps);
+__device__ __forceinline__ void ls_dx(const DxArgs& a, int nrb, int splits, uint8_t* lds) {
+    const int nht = (a.H + S::BM - 1) / S::BM, steps = a.cols / kBK;
     for (int item = blockIdx.x; item < splits * nht * nrb; item += gridDim.x) {
         const int rb = item % nrb, ht = item / nrb % nht, sp = item / nrb / nht;
         const int k0 = (int)((int64_t)steps * sp / splits), k1 = (int)((int64_t)steps * (sp + 1) / splits);
@@ -438,10 +504,43 @@ __global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
     }
 }
 
+// Up to 64 tokens: g and its rest side by side as tokens of one block.
+using Dx32 = Tile<256, 64, 4, 2, 3, true, false>;
+using Dx64 = Tile<256, 128, 4, 2, 3, true, false>;
+template <int BN>
+using DxN = Tile<256, BN, 4, 2, BN <= 160 ? 3 : 2, true, false>;
+
+template <int WHICH>
+__global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
+    constexpr int kBytes = WHICH == 32 ? kLds<Dx32> : WHICH == 64 ? kLds<Dx64> : kLds<DxN<160>>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
+    const Meta me = ls_meta(a.meta);
+    if (me.nv == 0) return;
+    if constexpr (WHICH == 32) {
+        ls_dx<Dx32>(a, 1, me.splits, lds);
+    } else if constexpr (WHICH == 64) {
+        ls_dx<Dx64>(a, 1, me.splits, lds);
+    } else {
+        auto go = [&](auto s) {
+            using S = decltype(s);
+            static_assert(kLds<S> <= kBytes, "LDS");
+            ls_dx<S>(a, (me.nv + S::BN - 1) / S::BN, me.splits, lds);
+        };
+        switch (me.bn) {
+            case 128: go(DxN<128>{}); break;
+            case 160: go(DxN<160>{}); break;
+            case 192: go(DxN<192>{}); break;
+            case 224: go(DxN<224>{}); break;
+            default: go(DxN<256>{}); break;
+        }
+    }
+}
+
 // ------------------------------------------------------------------------ dW
 struct DwArgs {
     const uint16_t *x, *g;
-    const int32_t* meta;
+    const Meta* meta;
+    int fold;                // rows of g (and of x) where it is in two parts, else 0
     int H, V, v0, cols;
     int64_t ldg;
     void* dw;
@@ -463,19 +562,19 @@ struct DwJob {
 #pragma unroll
         for (int i = 0; i < S::DA; ++i) {
             int row, piece;
-            ls_slot<S::DA, true>(i, row, piece);
+            ls_slot<true>(i, row, piece);
             offa[i] = (uint32_t)row * (uint32_t)(2 * a.H) + 2 * min(ht * S::BM + 8 * piece, a.H - 8);
         }
 #pragma unroll
         for (int i = 0; i < S::DB; ++i) {
             int row, piece;
-            ls_slot<S::DB, true>(i, row, piece);
+            ls_slot<true>(i, row, piece);
             offb[i] = (uint32_t)row * (uint32_t)(2 * a.ldg) + 2 * (vt * S::BN + 8 * piece);
         }
     }
     __device__ __forceinline__ void issue(uint8_t* lds) {
-        ls_dma<S::DA>(a.x + (size_t)step * kBK * a.H, offa, lds);
-        ls_dma<S::DB>(a.g + (int64_t)step * kBK * a.ldg, offb, lds + S::kA);
+        ls_dma<S::DA, 0, false>(a.x + (size_t)step * kBK * a.H, offa, lds);
+        ls_dma<S::DB, S::RB, false>(a.g + (int64_t)step * kBK * a.ldg, offb, lds + S::kA);
         if (++step == nk) {
             if (item + (int)gridDim.x < items) {
                 item += gridDim.x;
@@ -515,11 +614,14 @@ struct DwJob {
     }
 };
 
-template <class S, bool F32>
+using DwTile = Tile<256, 256, 2, 4, 2, true, true>;
+
+template <bool F32>
 __global__ __launch_bounds__(kThreads) void k_loss_dw(DwArgs a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::STAGES * S::kStage];
-    const int nv = vmi_sload_i32(a.meta), nk = (nv + kBK - 1) / kBK, nht = (a.H + S::BM - 1) / S::BM;
-    const int items = nht * ((a.cols + S::BN - 1) / S::BN);
+    using S = DwTile;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds<S>];
+    const int nv = vmi_sload_i32(&a.meta->nv), nk = nv ? ((a.fold ? a.fold : nv) + kBK - 1) / kBK : 0;
+    const int nht = (a.H + S::BM - 1) / S::BM, items = nht * ((a.cols + S::BN - 1) / S::BN);
     if ((int)blockIdx.x >= items) return;
     DwJob<S, F32> job(a, max(nk, 1), nht, items);
     const int mine = (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;
@@ -539,70 +641,122 @@ __global__ __launch_bounds__(kThreads) void k_loss_dw(DwArgs a) {
 struct RowsArgs {
     const int64_t* target;
     int64_t ignore;
-    int T, Tp, V;
-    int32_t *idx, *pos, *meta;     // tokens in the loss, each token's place among them or -1, their number
-    Coef* coef;                    // [Tp]
+    int T, V;
+    int32_t *idx, *pos;            // tokens in the loss, each token's place among them or -1
+    Meta* meta;
+    Coef* coef;                    // of the tokens in the loss
     float *loss, *lse_out;         // score: written for tokens left out
     uint32_t* status;
     const float *lse, *dloss, *dlse;
+    int grid, few;                 // workgroups of the products; their block of tokens where there are few, else 0
+    int tiles, last, nht, steps;   // vocabulary tiles of a piece and of the last one, hidden tiles, dx's steps of the last piece
 };
 
-// One workgroup: a thread takes a run of tokens.  Bound by latency, 3 to 5 us up to 8192 tokens.
+constexpr int kMaxItems = 4;       // workgroups' turns at most that the strips are cut for
+
+// The least work, in tokens' widths of a tile, of `tiles` cut into s strips by blocks of
+// bn tokens: turns of the grid times a turn's tiles (a tile's own cost beside its
+// products about 16 tokens, a turn's 24); lane l tries s = l + 1, l + 65, ..  Returns work * 2^16 + s.
+__device__ __forceinline__ uint64_t ls_plan(int nv, int bn, int tiles, int grid) {
+    const int lane = threadIdx.x & 63, nrb = (nv + bn - 1) / bn;
+    const int most = min(tiles, max(1, kMaxItems * grid / nrb));
+    uint64_t best = ~0ull;
+    for (int s = lane + 1; s <= most; s += 64) {
+        const uint64_t turns = (nrb * s + grid - 1) / grid;
+        const uint64_t work = turns * ((uint64_t)((tiles + s - 1) / s) * (bn + 16) + 24);
+        best = min(best, work << 16 | (uint64_t)s);
+    }
+    return ~vmi_wave_max_u64(~best);
+}
+
+// One workgroup: a wave takes a run of tokens, 64 at a time, eight such groups' loads together.
 __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
     __shared__ int s_sum[16];
-    const int lane = threadIdx.x & 63, w = ls_wave(), run = (a.T + 1023) / 1024;
-    const int t0 = min(a.T, (int)threadIdx.x * run), t1 = min(a.T, t0 + run);
+    const int lane = threadIdx.x & 63, w = ls_wave(), run = (a.T + 1023) / 1024 * 64;
+    const int t0 = min(a.T, w * run), t1 = min(a.T, t0 + run);
+    constexpr int kAhead = 8;
     int n = 0;
     bool bad = false;
-    for (int t = t0; t < t1; ++t) {
-        const int64_t y = a.target[t];
-        const bool in = y >= 0 && y < a.V && y != a.ignore;
-        n += in;
-        bad |= !in && y != a.ignore;
-    }
-    if (a.status && __any(bad) && lane == 0) atomicOr(a.status, VMI_STATUS_BAD_TARGET);
-    int v = n;
+    for (int t = t0; t < t1; t += 64 * kAhead) {
+        int64_t y[kAhead];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d);
-        if (lane >= d) v += u;
-    }
-    if (lane == 63) s_sum[w] = v;
-    __syncthreads();
-    int c = v - n, all = 0;
-    for (int i = 0; i < 16; ++i) {
-        c += i < w ? s_sum[i] : 0;
-        all += s_sum[i];
-    }
-    for (int t = t0; t < t1; ++t) {
-        const int64_t y = a.target[t];
-        const bool in = y >= 0 && y < a.V && y != a.ignore;
-        a.pos[t] = in ? c : -1;
-        if (in) {
-            a.idx[c] = t;
-            Coef k{0.0f, 0.0f, 0.0f, (int32_t)y};
-            if (a.dloss) {
-                k.b = a.dloss[t];
-                k.a = k.b + (a.dlse ? a.dlse[t] : 0.0f);
-                k.lse = a.lse[t];
-            }
-            a.coef[c++] = k;
-        } else if (a.loss) {
-            a.loss[t] = a.lse_out[t] = y == a.ignore ? 0.0f : __builtin_nanf("");
+        for (int i = 0; i < kAhead; ++i) y[i] = a.target[min(t + 64 * i + lane, a.T - 1)];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const bool here = t + 64 * i + lane < t1, in = here && y[i] >= 0 && y[i] < a.V && y[i] != a.ignore;
+            n += __builtin_popcountll(__ballot(in));
+            bad |= here && !in && y[i] != a.ignore;
         }
     }
-    if (threadIdx.x == 0) a.meta[0] = all;
+    if (a.status && __any(bad) && lane == 0) atomicOr(a.status, VMI_STATUS_BAD_TARGET);
+    if (lane == 0) s_sum[w] = n;
+    __syncthreads();
+    int c = 0, nv = 0;
+    for (int i = 0; i < 16; ++i) {
+        c += i < w ? s_sum[i] : 0;
+        nv += s_sum[i];
+    }
+    for (int t = t0; t < t1; t += 64 * kAhead) {
+        int64_t y[kAhead];
+        Coef k[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int at = min(t + 64 * i + lane, a.T - 1);
+            y[i] = a.target[at];
+            k[i] = Coef{0.0f, 0.0f, 0.0f, 0};
+            if (a.dloss) k[i] = Coef{a.dlse ? a.dlse[at] : 0.0f, a.dloss[at], a.lse[at], 0};
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int at = t + 64 * i + lane;
+            const bool here = at < t1, in = here && y[i] >= 0 && y[i] < a.V && y[i] != a.ignore;
+            const uint64_t all = __ballot(in);
+            const int mine = c + __builtin_popcountll(all & ((1ull << lane) - 1));
+            c += __builtin_popcountll(all);
+            if (here) a.pos[at] = in ? mine : -1;
+            if (in) {
+                a.idx[mine] = at;
+                k[i].a += k[i].b;
+                k[i].target = (int32_t)y[i];
+                a.coef[mine] = k[i];
+            } else if (here && a.loss) {
+                a.loss[at] = a.lse_out[at] = y[i] == a.ignore ? 0.0f : __builtin_nanf("");
+            }
+        }
+    }
+    if (w != 0) return;
+    Meta me{nv, a.few, 1, 1, 1};
+    if (nv) {
+        uint64_t best = ~0ull;
+        if (a.few) {   // one strip a workgroup: bytes bound it
+            me.strips = me.last = a.grid;
+        } else {
+            for (int bn = 256; bn >= 128; bn -= 32) {
+                const uint64_t p = ls_plan(nv, bn, a.tiles, a.grid);
+                if (p >> 16 < best >> 16) {
+                    best = p;
+                    me.bn = bn;
+                }
+            }
+            me.strips = (int)(best & 0xffffu);
+            me.last = (int)(ls_plan(nv, me.bn, a.last, a.grid) & 0xffffu);
+        }
+        const int nrb = (nv + me.bn - 1) / me.bn;
+        me.splits = min(max(a.grid / max(nrb * a.nht, 1), 1), max(a.steps / 4, 1));
+    }
+    if (lane == 0) *a.meta = me;
 }
 
 // A wave per token: its strips' maxima and sums, in a fixed order.
-__global__ __launch_bounds__(256) void k_loss_merge(const int32_t* meta, const int32_t* idx, const float2* part,
-                                                    const float* hit, int bn, int grid, float* loss, float* lse) {
-    const int c = blockIdx.x * 4 + ls_wave(), lane = threadIdx.x & 63, nv = meta[0];
-    if (c >= nv) return;
-    const int nrb = (nv + bn - 1) / bn, strips = ls_strips(nrb, grid), rb = c / bn;
+__global__ __launch_bounds__(256) void k_loss_merge(const Meta* meta, const int32_t* idx, const float2* part,
+                                                    const float* hit, float* loss, float* lse) {
+    const Meta me = ls_meta(meta);
+    const int c = blockIdx.x * 4 + ls_wave(), lane = threadIdx.x & 63;
+    if (c >= me.nv) return;
+    const int nrb = (me.nv + me.bn - 1) / me.bn, rb = c / me.bn;
     float m = kLowest, l = 0.0f;
-    for (int s = lane; s < strips; s += 64) {
-        const float2 p = part[((size_t)s * nrb + rb) * bn + c % bn];
+    for (int s = lane; s < me.strips; s += 64) {
+        const float2 p = part[((size_t)s * nrb + rb) * me.bn + c % me.bn];
         ls_join(m, l, p.x, p.y);
     }
 #pragma unroll
@@ -614,50 +768,47 @@ __global__ __launch_bounds__(256) void k_loss_merge(const int32_t* meta, const i
     }
 }
 
-// Row c of the tokens in the loss, zeros from nv on.
-__global__ __launch_bounds__(256) void k_loss_compact(const int32_t* meta, const int32_t* idx, const vmi_u4* x, int U,
+// Row c (of c and c + fold alike) of the tokens in the loss, zeros from nv on.
+__global__ __launch_bounds__(256) void k_loss_compact(const Meta* meta, const int32_t* idx, int fold, const vmi_u4* x, int U,
                                                       vmi_u4* out) {
-    const int c = blockIdx.x;
-    const bool in = c < meta[0];
+    const int c = fold && (int)blockIdx.x >= fold ? blockIdx.x - fold : blockIdx.x;
+    const bool in = c < meta->nv;
     const size_t src = in ? (size_t)idx[c] * U : 0;
-    for (int u = threadIdx.x; u < U; u += 256) out[(size_t)c * U + u] = in ? x[src + u] : vmi_u4{0, 0, 0, 0};
+    for (int u = threadIdx.x; u < U; u += 256) out[(size_t)blockIdx.x * U + u] = in ? x[src + u] : vmi_u4{0, 0, 0, 0};
 }
 
-// dx of a token: its splits' sums in order, zeros for a token left out.
-__global__ __launch_bounds__(256) void k_loss_dx_out(const int32_t* meta, const int32_t* pos, const float* sum, int H, int bn,
-                                                     int bm, int grid, int steps, uint16_t* dx) {
-    const int t = blockIdx.x, c = pos[t], nrb = (meta[0] + bn - 1) / bn;
-    const int splits = nrb ? ls_dx_splits(nrb, (H + bm - 1) / bm, grid, steps) : 0;
+// dx of a token: its splits' sums in order (fold: those of the two parts of g, fold rows
+// apart), zeros for a token left out.
+__global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int32_t* pos, const float* sum, int H, int fold,
+                                                     uint16_t* dx) {
+    const Meta me = ls_meta(meta);
+    const int t = blockIdx.x, c = pos[t], rows = fold ? 2 * fold : (me.nv + me.bn - 1) / me.bn * me.bn;
+    constexpr int kAhead = 8;
     for (int h = 4 * threadIdx.x; h < H; h += 1024) {
         vmi_f4 v = {0.f, 0.f, 0.f, 0.f};
-        if (c >= 0)
-            for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const vmi_f4*>(sum + ((size_t)s * nrb * bn + c) * H + h);
+        if (c >= 0) {
+            const int n = fold ? 2 * me.splits : me.splits;
+            for (int i0 = 0; i0 < n; i0 += kAhead) {
+                vmi_f4 u[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const int j = min(i0 + i, n - 1), s = fold ? j >> 1 : j;
+                    u[i] = *reinterpret_cast<const vmi_f4*>(sum + ((size_t)s * rows + c + (fold && (j & 1) ? fold : 0)) * H + h);
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+                    if (i0 + i < n) v += u[i];
+            }
+        }
         *reinterpret_cast<uint2*>(dx + (size_t)t * H + h) = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
     }
 }
 
 // ---------------------------------------------------------------------- host
-template <int BN>
-struct Shapes;
-template <>
-struct Shapes<256> {
-    using Logit = Tile<256, 256, 2, 4, 2, false, false>;
-    using Dx = Tile<256, 256, 2, 4, 2, true, false>;
-};
-template <>
-struct Shapes<64> {
-    using Logit = Tile<128, 64, 4, 2, 4, false, false>;
-    using Dx = Tile<256, 64, 4, 2, 3, true, false>;
-};
-using DwTile = Tile<256, 256, 2, 4, 2, true, true>;
-
-// Tokens of a tile.
-int token_block(int T) { return T <= 64 ? 64 : 256; }
-
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 
 struct Layout {
-    int bn, Tp, piece;                // tokens of a block, T in whole blocks, vocabulary rows of a piece
+    int few, rows, piece;             // tokens of the one block where there are few, rows of g, vocabulary rows of a piece
     int64_t ldg;
     size_t idx, pos, meta, coef, part, hit, x, g, sum, bytes;
 };
@@ -668,8 +819,8 @@ bool form_ok(int T, int H, int V) {
 
 Layout carve(int T, int H, int V, bool grad) {
     Layout l{};
-    l.bn = token_block(T);
-    l.Tp = std::max(1, (T + l.bn - 1) / l.bn) * l.bn;
+    l.few = T <= kFewest ? kFewest : T <= kFew ? kFew : 0;
+    l.rows = l.few ? 2 * l.few : (T + 255 + 63) / 64 * 64;   // whole blocks of any width end below T + 256
     const int cus = vmi::device_cus();
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -677,24 +828,24 @@ Layout carve(int T, int H, int V, bool grad) {
         at += vmi::align256(n);
         return p;
     };
-    l.meta = take(256);
-    l.idx = take((size_t)l.Tp * 4);
-    l.pos = take((size_t)l.Tp * 4);
-    l.coef = take((size_t)l.Tp * sizeof(Coef));
+    l.meta = take(sizeof(Meta));
+    l.idx = take((size_t)T * 4);
+    l.pos = take((size_t)T * 4);
+    l.coef = take((size_t)T * sizeof(Coef));
     if (!grad) {
-        const size_t nrb = l.Tp / l.bn;
-        l.part = take(std::max<size_t>(cus, 8 * nrb) * l.bn * sizeof(float2));
-        l.hit = take((size_t)l.Tp * 4);
+        // items: a strip for every block at least, kMaxItems turns at most
+        const size_t blocks = (T + 127) / 128;
+        l.part = take(std::max<size_t>((size_t)kMaxItems * cus, blocks) * (l.few ? l.few : 256) * sizeof(float2));
+        l.hit = take((size_t)l.rows * 4);
     } else {
         const int64_t all = ((int64_t)V + 255) / 256 * 256;
-        const int64_t fit = std::max<int64_t>(8192, kPieceBytes / (2 * l.Tp) / 256 * 256);
+        const int64_t fit = std::max<int64_t>(8192, kPieceBytes / (2 * l.rows) / 256 * 256);
         l.piece = (int)std::min(all, fit);
         l.ldg = l.piece + 64;         // off a power of two
-        l.x = take((size_t)l.Tp * H * 2);
-        l.g = take((size_t)l.Tp * l.ldg * 2);
+        l.x = take((size_t)l.rows * H * 2);
+        l.g = take((size_t)l.rows * l.ldg * 2);
         const int nht = (H + 255) / 256;
-        const size_t rows = std::max<size_t>(l.Tp, (size_t)std::max(cus / nht, 1) * l.bn);
-        l.sum = take(rows * H * 4);
+        l.sum = take(((size_t)l.rows + (size_t)std::max(cus / nht, 1) * (l.few ? 2 * l.few : 256)) * H * 4);
     }
     l.bytes = at;
     return l;
@@ -718,14 +869,23 @@ bool aligned(std::initializer_list<const void*> ps, uintptr_t to) {
     return !(m & (to - 1));
 }
 
-template <int BN>
-void launch_score(const LogitArgs& a, int grid, hipStream_t s) {
-    hipLaunchKernelGGL((k_loss_score<typename Shapes<BN>::Logit>), dim3(grid), dim3(kThreads), 0, s, a);
+template <int GRAD>
+void launch_logits(const LogitArgs& a, int few, int grid, hipStream_t s) {
+    constexpr int kSmall = GRAD ? 2 : 0;   // few tokens: g in two parts
+    if (few == 32)
+        hipLaunchKernelGGL((k_loss_logits<32, kSmall>), dim3(grid), dim3(kThreads), 0, s, a);
+    else if (few == 64)
+        hipLaunchKernelGGL((k_loss_logits<64, kSmall>), dim3(grid), dim3(kThreads), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_loss_logits<0, GRAD>), dim3(grid), dim3(kThreads), 0, s, a);
 }
-template <int BN>
-void launch_piece(const LogitArgs& a, const DxArgs* dx, int grid, hipStream_t s) {
-    hipLaunchKernelGGL((k_loss_g<typename Shapes<BN>::Logit>), dim3(grid), dim3(kThreads), 0, s, a);
-    if (dx) hipLaunchKernelGGL((k_loss_dx<typename Shapes<BN>::Dx>), dim3(grid), dim3(kThreads), 0, s, *dx);
+void launch_dx(const DxArgs& a, int few, int grid, hipStream_t s) {
+    if (few == 32)
+        hipLaunchKernelGGL((k_loss_dx<32>), dim3(grid), dim3(kThreads), 0, s, a);
+    else if (few == 64)
+        hipLaunchKernelGGL((k_loss_dx<64>), dim3(grid), dim3(kThreads), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_loss_dx<0>), dim3(grid), dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
@@ -753,15 +913,18 @@ extern "C" int vmi_head_loss(const uint16_t* x, int T, int hidden, const uint16_
     r.target = targets;
     r.ignore = ignore_index;
     r.T = T;
-    r.Tp = l.Tp;
     r.V = vocab;
+    r.grid = grid;
+    r.few = l.few;
     r.idx = reinterpret_cast<int32_t*>(ws + l.idx);
     r.pos = reinterpret_cast<int32_t*>(ws + l.pos);
-    r.meta = reinterpret_cast<int32_t*>(ws + l.meta);
+    r.meta = reinterpret_cast<Meta*>(ws + l.meta);
     r.coef = reinterpret_cast<Coef*>(ws + l.coef);
     r.loss = loss;
     r.lse_out = lse;
     r.status = status;
+    r.tiles = r.last = (vocab + 255) / 256;
+    r.nht = r.steps = 1;
     hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
     LogitArgs a{};
     a.x = x;
@@ -773,11 +936,8 @@ extern "C" int vmi_head_loss(const uint16_t* x, int T, int hidden, const uint16_
     a.V = vocab;
     a.part = reinterpret_cast<float2*>(ws + l.part);
     a.hit = reinterpret_cast<float*>(ws + l.hit);
-    if (l.bn == 64)
-        launch_score<64>(a, grid, s);
-    else
-        launch_score<256>(a, grid, s);
-    hipLaunchKernelGGL(k_loss_merge, dim3((T + 3) / 4), dim3(256), 0, s, r.meta, r.idx, a.part, a.hit, l.bn, grid, loss, lse);
+    launch_logits<0>(a, l.few, grid, s);
+    hipLaunchKernelGGL(k_loss_merge, dim3((T + 3) / 4), dim3(256), 0, s, r.meta, r.idx, a.part, a.hit, loss, lse);
     return launched("k_loss_merge launch");
 }
 
@@ -808,20 +968,25 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     r.target = targets;
     r.ignore = ignore_index;
     r.T = T;
-    r.Tp = l.Tp;
     r.V = vocab;
+    r.grid = grid;
+    r.few = l.few;
     r.idx = reinterpret_cast<int32_t*>(ws + l.idx);
     r.pos = reinterpret_cast<int32_t*>(ws + l.pos);
-    r.meta = reinterpret_cast<int32_t*>(ws + l.meta);
+    r.meta = reinterpret_cast<Meta*>(ws + l.meta);
     r.coef = reinterpret_cast<Coef*>(ws + l.coef);
     r.lse = lse;
     r.dloss = d_loss;
     r.dlse = d_lse;
+    r.tiles = l.piece / 256;
+    r.last = ((vocab - 1) % l.piece + 256) / 256;
+    r.nht = (hidden + 255) / 256;
+    r.steps = r.last * 256 / kBK;
     hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
     uint16_t* xc = reinterpret_cast<uint16_t*>(ws + l.x);
     if (T)
-        hipLaunchKernelGGL(k_loss_compact, dim3(l.Tp), dim3(256), 0, s, r.meta, r.idx, reinterpret_cast<const vmi_u4*>(x),
-                           hidden / 8, reinterpret_cast<vmi_u4*>(xc));
+        hipLaunchKernelGGL(k_loss_compact, dim3(l.rows), dim3(256), 0, s, r.meta, r.idx, l.few,
+                           reinterpret_cast<const vmi_u4*>(x), hidden / 8, reinterpret_cast<vmi_u4*>(xc));
     LogitArgs a{};
     a.x = xc;
     a.w = weight;
@@ -847,29 +1012,27 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     u.V = vocab;
     u.ldg = l.ldg;
     u.dw = dweight;
-    const int steps = (int)(((int64_t)vocab - 1) % l.piece / 256 + 1) * 256 / kBK;   // of the last piece, the shortest
+    u.fold = 2 * l.few;
     for (int v0 = 0; v0 < vocab; v0 += l.piece) {
         const int cols = std::min(l.piece, (vocab - v0 + 255) / 256 * 256);
         a.v0 = v0;
         a.v1 = v0 + cols;
+        a.last = v0 + l.piece >= vocab;
         d.v0 = u.v0 = v0;
         d.cols = u.cols = cols;
         d.add = v0 != 0;
-        d.short_steps = steps;
         if (T) {
-            if (l.bn == 64)
-                launch_piece<64>(a, dx ? &d : nullptr, grid, s);
-            else
-                launch_piece<256>(a, dx ? &d : nullptr, grid, s);
+            launch_logits<1>(a, l.few, grid, s);
+            if (dx) launch_dx(d, l.few, grid, s);
         }
         if (dweight) {
             if (dweight_dtype == VMI_F32)
-                hipLaunchKernelGGL((k_loss_dw<DwTile, true>), dim3(grid), dim3(kThreads), 0, s, u);
+                hipLaunchKernelGGL(k_loss_dw<true>, dim3(grid), dim3(kThreads), 0, s, u);
             else
-                hipLaunchKernelGGL((k_loss_dw<DwTile, false>), dim3(grid), dim3(kThreads), 0, s, u);
+                hipLaunchKernelGGL(k_loss_dw<false>, dim3(grid), dim3(kThreads), 0, s, u);
         }
     }
     if (dx && T)
-        hipLaunchKernelGGL(k_loss_dx_out, dim3(T), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden, l.bn, 256, grid, steps, dx);
+        hipLaunchKernelGGL(k_loss_dx_out, dim3(T), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden, l.few, dx);
     return launched("vmi_head_loss_grad launch");
 }

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from ._lib import VMI_BF16, VMI_F32, VmiError, check, load
-from .moe import _like, _matches, _on_current, _on_stream, _ptr, _require, _stream_handle, _stream_on, scratch, workspace
+from .moe import _matches, _on_current, _on_stream, _once, _ptr, _require, _stream_handle, _stream_on, scratch, workspace
 
 
 class TiledHead:
@@ -105,15 +105,15 @@ class _HeadLoss(torch.autograd.Function):
         return loss, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_loss, d_lse):
         x, weight, targets, lse = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         if d_loss is None and d_lse is None:
             return None, None, None, None, None
         d_loss = torch.zeros_like(lse) if d_loss is None else d_loss.contiguous()
-        dx, dw = head_loss_grad(x, weight, targets, lse, d_loss, None if d_lse is None else d_lse.contiguous(),
-                                want_dx=need_x, want_dweight=need_w, ignore_index=ctx.ignore_index)
+        dx, dw = _head_loss_grad(x, weight, targets, lse, d_loss, None if d_lse is None else d_lse.contiguous(), need_x,
+                                 torch.bfloat16 if need_w else None, ctx.ignore_index)
         return dx, dw, None, None, None
 
 
@@ -175,8 +175,7 @@ def head_loss_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
     [T] (``vmi_head_loss_grad``).  dweight_dtype: bf16, or f32 for gradients that a
     caller adds up itself.  The same call gives the same bits."""
     dev = _check_loss(x, weight, targets)
-    T, H = x.shape
-    V = weight.shape[0]
+    T = x.shape[0]
     for t, name in ((lse, "lse"), (d_loss, "d_loss"), (d_lse, "d_lse")):
         if t is not None or name != "d_lse":
             _matches(t, name, (T,), torch.float32, dev)
@@ -184,14 +183,20 @@ def head_loss_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
         raise VmiError(f"dweight_dtype must be bf16 or f32 (got {dweight_dtype})")
     if not (want_dx or want_dweight):
         raise VmiError("neither dx nor dweight wanted")
+    return _on_stream(stream, _head_loss_grad, x, weight, targets, lse, d_loss, d_lse,
+                      want_dx, dweight_dtype if want_dweight else None, ignore_index)
+
+
+def _head_loss_grad(x, weight, targets, lse, d_loss, d_lse, want_dx, dweight_dtype, ignore_index):
+    T, H = x.shape
+    V = weight.shape[0]
     lib = load()
-    if targets.dtype is not torch.int64:
-        targets = _on_stream(stream, targets.long)
-    dx = _like(x, None, x.dtype, stream) if want_dx else None
-    dw = _like(weight, (V, H), dweight_dtype, stream) if want_dweight else None
-    ws = scratch(lib.vmi_head_loss_grad_workspace_bytes(T, H, V), dev, stream)
+    targets = targets.long()
+    dx = torch.empty_like(x) if want_dx else None
+    dw = None if dweight_dtype is None else weight.new_empty((V, H), dtype=dweight_dtype)
+    ws = scratch(lib.vmi_head_loss_grad_workspace_bytes(T, H, V), x.device)
     check(lib.vmi_head_loss_grad(x.data_ptr(), T, H, weight.data_ptr(), V, targets.data_ptr(), ignore_index, lse.data_ptr(),
                                  d_loss.data_ptr(), _ptr(d_lse), _ptr(dx), _ptr(dw),
                                  VMI_F32 if dweight_dtype is torch.float32 else VMI_BF16, ws.data_ptr(), ws.numel(),
-                                 _stream_on(dev, stream)), "vmi_head_loss_grad")
+                                 _stream_on(x.device, None)), "vmi_head_loss_grad")
     return dx, dw

@@ -506,6 +506,16 @@ def _on_stream(stream, fn, *args):
         return fn(*args)
 
 
+def _once(backward):
+    """torch's once_differentiable, whose own cost (5 us) is paid only where a graph of
+    the gradients is asked for."""
+    twice = torch.autograd.function.once_differentiable(backward)
+
+    def either(ctx, *grads):
+        return (twice if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return either
+
+
 def _rows_dtype(t: torch.Tensor, name: str) -> int:
     if t.dtype is torch.bfloat16:
         return _lib.VMI_BF16
@@ -568,7 +578,7 @@ class _SortByExpert(torch.autograd.Function):
         return _sorted_rows(x, place)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_rows):
         place, = ctx.saved_tensors
         return _combined(d_rows.contiguous(), place, None, None), None
@@ -581,7 +591,7 @@ class _CombineExperts(torch.autograd.Function):
         return _combined(y, place, scores, residual)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_out):
         y, place, scores = ctx.saved_tensors
         need_y, _, need_scores, need_residual = ctx.needs_input_grad
