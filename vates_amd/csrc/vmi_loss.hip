@@ -41,6 +41,16 @@ constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ int ls_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
+// Two blocks' values, 4 q .. 4 q + 3 of 16 as two words each: eight in a row per lane, as
+// rows 0 and 2 (16 lanes each) of the first block's and rows 1 and 3 of the second's.
+__device__ __forceinline__ vmi_u4 ls_pair8(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
+    return vmi_u4{x[0], y[0], x[1], y[1]};
+}
+// Where a lane's eight begin among the two blocks' 32.
+__device__ __forceinline__ int ls_pair8_at() { return 16 * ((threadIdx.x >> 4) & 1) + 8 * ((threadIdx.x >> 5) & 1); }
+
 // ------------------------------------------------------------------ products
 // One workgroup's tile: BM x BN, waves WM x WN.  SLOW operands have k as the slow
 // index (rows of BM or BN = 256 values).  ONCE: A is read by this workgroup alone.
@@ -55,6 +65,21 @@ struct Tile {
     static_assert(WM * WN == kWaves && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && kA % (1024 * kWaves) == 0, "shape");
     static_assert((!ASLOW || BM == 256) && (!BSLOW || BN == 256), "slow operands have rows of 512 bytes");
 };
+
+// This workgroup's item in turn `turn` of n, or -1.  Workgroups go to the eight XCDs in
+// turn, and each of these takes a run of consecutive items, which share operands in its L2.
+__device__ __forceinline__ int ls_item(int turn, int n) {
+    const int grid = gridDim.x, at = turn * grid, count = min(grid, n - at), chunk = (count + 7) / 8;
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3, i = x * chunk + j;
+    return j < chunk && i < count ? at + i : -1;
+}
+// The block of tokens and the strip of item i: eight blocks by all strips after another,
+// so that a run of items is some blocks by some strips.
+__device__ __forceinline__ void ls_pair(int i, int nrb, int strips, int& rb, int& strip) {
+    const int group = i / (8 * strips), wide = min(8, nrb - 8 * group), j = i - group * 8 * strips;
+    rb = 8 * group + j % wide;
+    strip = j / wide;
+}
 
 // Row and 16-byte piece of a lane in the wave's DMA instruction i.
 template <bool SLOW>
@@ -82,14 +107,17 @@ __device__ __forceinline__ void ls_dma(const void* base, const uint32_t (&off)[D
             vmi_lds_dma16_at(base, off[i], lds + (w + kWaves * i) * 1024);
     }
 }
-// Until the wave's oldest step is there (STAGES - 1 are in flight).
-template <class S>
+// Until the wave's oldest step is there: STAGES - 1 are in flight, and behind them the
+// STORES instructions of the step before, where it ended a tile (vector memory
+// operations of a wave end in the order of their issue).
+template <class S, int STORES>
 __device__ __forceinline__ void ls_wait() {
     constexpr int n = S::STAGES - 2;
+    static_assert(n * (S::DA + S::DB) + STORES < 64, "the counter's range");
     if (S::RB == 0 || n == 0 || ls_wave() < S::RB)
-        vmi_vm_wait_c<n * (S::DA + S::DB)>();
+        vmi_vm_wait_c<n * (S::DA + S::DB) + STORES>();
     else
-        vmi_vm_wait_c<n * (S::DA + S::DB - 1)>();
+        vmi_vm_wait_c<n * (S::DA + S::DB - 1) + STORES>();
 }
 
 // Operand of block b (16 of m or n, from `first` on) and k = 32 kk ..
@@ -144,15 +172,20 @@ __device__ __forceinline__ void ls_clear(vmi_f4 (&acc)[S::MB][S::NB]) {
 
 // The steps 0 .. total - 1 of a workgroup's tiles, one after another: job.issue(lds) asks
 // for the next step's operands (behind the last, again for the last's, so that every
-// wait counts alike), job.done(acc) ends a step and takes a tile that is complete.
+// wait counts alike), job.done(acc) ends a step, takes a tile that is complete and says
+// whether it has issued its STORES stores (all of them, whatever they cover).
 template <class S, class Job>
 __device__ __forceinline__ void ls_run(uint8_t* lds, Job& job, int total) {
     vmi_f4 acc[S::MB][S::NB];
     ls_clear<S>(acc);
     for (int s = 0; s < S::STAGES - 1; ++s) job.issue(lds + s * S::kStage);
     int in = S::STAGES - 1, out = 0;
+    bool stored = false;
     for (int s = 0; s < total; ++s) {
-        ls_wait<S>();
+        if (Job::STORES && stored)
+            ls_wait<S, Job::STORES>();
+        else
+            ls_wait<S, 0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -160,7 +193,7 @@ __device__ __forceinline__ void ls_run(uint8_t* lds, Job& job, int total) {
         in = in + 1 == S::STAGES ? 0 : in + 1;
         ls_multiply<S>(lds + out * S::kStage, acc);
         out = out + 1 == S::STAGES ? 0 : out + 1;
-        job.done(acc);
+        stored = job.done(acc);
     }
     // nothing in flight, and no wave reading, when the next run begins
     vmi_vm_wait_c<0>();
@@ -212,6 +245,7 @@ struct LogitJob {
     int nv, rb, v1;                   // tokens, block, end of the strip
     int tile;                         // first row of the tile being multiplied
     int next, k, nk;                  // first row of the tile being asked for, its step, steps of one
+    int turn;                         // step at which the tiles' rows are begun
     int kd;                           // step being multiplied
     uint32_t offa[S::DA], offb[S::DB];
     float m[S::NB], l[S::NB];
@@ -220,6 +254,9 @@ struct LogitJob {
     __device__ __forceinline__ LogitJob(const LogitArgs& a_, Coef* coef_, int nv_, int rb_, int v0_, int v1_)
         : a(a_), coef(coef_), nv(nv_), rb(rb_), v1(v1_) {
         nk = a.H / kBK;
+        // Rows of a few KB put the pieces that all workgroups ask for at one time on few memory channels; begun at
+        // steps of their own, strips spread over them all (one token 129 -> 109 us, 100 tokens 156 -> 129).
+        turn = nv <= 4 * S::BN ? v0_ / 16 % nk : 0;
         tile = v0_;
         next = min(v0_, a.V - 1);   // (a piece's last tile may lie behind the vocabulary: its columns are zeros)
         k = kd = 0;
@@ -253,8 +290,9 @@ struct LogitJob {
         }
     }
     __device__ __forceinline__ void issue(uint8_t* lds) {
-        ls_dma<S::DA, 0, S::ONCE>(a.w + (size_t)next * a.H + (size_t)k * kBK, offa, lds);
-        ls_dma<S::DB, S::RB, false>(a.x + (size_t)k * kBK, offb, lds + S::kA);
+        const int kk = k + turn >= nk ? k + turn - nk : k + turn;
+        ls_dma<S::DA, 0, S::ONCE>(a.w + (size_t)next * a.H + (size_t)kk * kBK, offa, lds);
+        ls_dma<S::DB, S::RB, false>(a.x + (size_t)kk * kBK, offb, lds + S::kA);
         if (++k == nk) {
             if (next + S::BM < min(v1, a.V)) {
                 next += S::BM;
@@ -265,8 +303,9 @@ struct LogitJob {
             }
         }
     }
-    __device__ __forceinline__ void done(vmi_f4 (&acc)[S::MB][S::NB]) {
-        if (++kd < nk) return;
+    static constexpr int STORES = GRAD * S::MB * S::NB / (S::MB % 2 ? 1 : 2);
+    __device__ __forceinline__ bool done(vmi_f4 (&acc)[S::MB][S::NB]) {
+        if (++kd < nk) return false;
         kd = 0;
         if constexpr (GRAD != 0)
             store(acc);
@@ -274,6 +313,7 @@ struct LogitJob {
             sum(acc);
         ls_clear<S>(acc);
         tile += S::BM;
+        return true;
     }
     // Running maximum and sum of a lane's own rows of the tiles, joined over lanes at the end only.
     __device__ __forceinline__ void sum(vmi_f4 (&acc)[S::MB][S::NB]) {
@@ -313,27 +353,45 @@ struct LogitJob {
         }
     }
     __device__ __forceinline__ void store(vmi_f4 (&acc)[S::MB][S::NB]) {
+        constexpr int W = S::MB % 2 ? 1 : 2;      // blocks of a store
+        const int q = (threadIdx.x & 63) >> 4;
+        // the block's rows of g from the tile's first column on (and, GRAD 2, those of the rest)
+        const __amdgpu_buffer_rsrc_t rs = vmi_rsrc(a.g + (int64_t)rb * S::BN * a.ldg + (tile - a.v0), 0x7fffffffu);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const Coef c = coef[n0 + 16 * n];
-            const int t = rb * S::BN + n0 + 16 * n, d = c.target - tile - m0;
-            uint16_t* dst = a.g + (int64_t)t * a.ldg + (tile - a.v0) + m0;
+            const int d = c.target - tile - m0;
+            const bool in = rb * S::BN + n0 + 16 * n < nv;
+            const uint32_t row = (uint32_t)(n0 + 16 * n) * (uint32_t)(2 * a.ldg);
 #pragma unroll
-            for (int mb = 0; mb < S::MB; ++mb) {
-                if (tile + m0 + 16 * mb >= v1) continue;   // another strip's
-                float v[4];
+            for (int mb = 0; mb < S::MB; mb += W) {
+                uint32_t u[W][2], e[W][2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v[r] = c.a * __builtin_amdgcn_exp2f((acc[mb][n][r] - c.lse) * kLog2e);
-                    if (d == 16 * mb + r) v[r] -= c.b;
-                    if (t >= nv || tile + m0 + 16 * mb + r >= a.V) v[r] = 0.0f;
+                for (int j = 0; j < W; ++j) {
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        v[r] = c.a * __builtin_amdgcn_exp2f((acc[mb + j][n][r] - c.lse) * kLog2e);
+                        if (d == 16 * (mb + j) + r) v[r] -= c.b;
+                        if (!in || tile + m0 + 16 * (mb + j) + r >= a.V) v[r] = 0.0f;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        u[j][r] = vmi_pack_bf16x2(v[2 * r], v[2 * r + 1]);
+                        e[j][r] = vmi_pack_bf16x2(v[2 * r] - __uint_as_float(u[j][r] << 16),
+                                                  v[2 * r + 1] - __uint_as_float(u[j][r] & 0xffff0000u));
+                    }
                 }
-                const uint2 u = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
-                *reinterpret_cast<uint2*>(dst + 16 * mb) = u;
-                if constexpr (GRAD == 2)
-                    *reinterpret_cast<uint2*>(dst + S::BN * a.ldg + 16 * mb) =
-                        make_uint2(vmi_pack_bf16x2(v[0] - __uint_as_float(u.x << 16), v[1] - __uint_as_float(u.x & 0xffff0000u)),
-                                   vmi_pack_bf16x2(v[2] - __uint_as_float(u.y << 16), v[3] - __uint_as_float(u.y & 0xffff0000u)));
+                const int at = W == 2 ? m0 - 4 * q + 16 * mb + ls_pair8_at() : m0 + 16 * mb;
+                const uint32_t off = tile + at < v1 ? row + 2 * at : VMI_OOB;   // (else another strip's)
+                const uint32_t rest = off == VMI_OOB ? off : off + (uint32_t)S::BN * (uint32_t)(2 * a.ldg);
+                if constexpr (W == 2) {
+                    vmi_bstore_b128(ls_pair8(u[0][0], u[0][1], u[1][0], u[1][1]), rs, off, 0);
+                    if (GRAD == 2) vmi_bstore_b128(ls_pair8(e[0][0], e[0][1], e[1][0], e[1][1]), rs, rest, 0);
+                } else {
+                    vmi_bstore_b64(make_uint2(u[0][0], u[0][1]), rs, off, 0);
+                    if (GRAD == 2) vmi_bstore_b64(make_uint2(e[0][0], e[0][1]), rs, rest, 0);
+                }
             }
         }
     }
@@ -350,9 +408,13 @@ __device__ __forceinline__ void ls_join(float& m, float& l, float m2, float l2) 
 template <class S>
 __device__ __forceinline__ void ls_score(const LogitArgs& a, const Meta& me, uint8_t* lds, Coef* coef) {
     const int nrb = (me.nv + S::BN - 1) / S::BN, per = ((a.V + me.strips - 1) / me.strips + 15) & ~15;
-    for (int item = blockIdx.x; item < nrb * me.strips; item += gridDim.x) {
-        const int rb = item % nrb, v0 = (item / nrb) * per, v1 = min(a.V, v0 + per);
-        float2* part = a.part + (size_t)item * S::BN;
+    for (int turn = 0; turn * (int)gridDim.x < nrb * me.strips; ++turn) {
+        const int item = ls_item(turn, nrb * me.strips);
+        if (item < 0) break;
+        int rb, strip;
+        ls_pair(item, nrb, me.strips, rb, strip);
+        const int v0 = strip * per, v1 = min(a.V, v0 + per);
+        float2* part = a.part + ((size_t)strip * nrb + rb) * S::BN;
         if (v0 >= v1) {
             if (threadIdx.x < S::BN) part[threadIdx.x] = make_float2(kLowest, 0.0f);
             continue;
@@ -382,8 +444,12 @@ template <class S, int GRAD>
 __device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, uint8_t* lds, Coef* coef) {
     const int nrb = (me.nv + S::BN - 1) / S::BN, strips = a.last ? me.last : me.strips;
     const int per = ((a.v1 - a.v0 + strips - 1) / strips + 15) & ~15;
-    for (int item = blockIdx.x; item < nrb * strips; item += gridDim.x) {
-        const int rb = item % nrb, v0 = a.v0 + (item / nrb) * per, v1 = min(a.v1, v0 + per);
+    for (int turn = 0; turn * (int)gridDim.x < nrb * strips; ++turn) {
+        const int item = ls_item(turn, nrb * strips);
+        if (item < 0) break;
+        int rb, strip;
+        ls_pair(item, nrb, strips, rb, strip);
+        const int v0 = a.v0 + strip * per, v1 = min(a.v1, v0 + per);
         if (v0 >= v1) continue;
         LogitJob<S, GRAD> job(a, coef, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
@@ -393,8 +459,8 @@ __device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, uint8_t
 // Tiles by tokens of a block.  Up to 64 tokens the head is read once, by one workgroup each
 // part of it, and its bytes bound the call; above, five widths, of which k_loss_rows takes the one with the least work.
 constexpr int kFew = 64, kFewest = 32;
-using Score32 = Tile<256, 32, 8, 1, 4, false, false, true>;
-using Score64 = Tile<256, 64, 4, 2, 3, false, false, true>;
+using Score32 = Tile<128, 32, 8, 1, 4, false, false, true>;
+using Score64 = Tile<128, 64, 4, 2, 4, false, false, true>;
 template <int BN>
 using ScoreN = Tile<256, BN, 4, 2, BN <= 160 ? 3 : 2, false, false>;
 template <class S>
@@ -469,12 +535,13 @@ struct DxJob {
             const int col = min(ht * S::BM + 8 * piece, a.H - 8);
             offa[i] = (uint32_t)(max(min(row, rows - 1), 0)) * (uint32_t)(2 * a.H) + 2 * col;
         }
-        ls_dma<S::DA, 0, false>(a.w + (size_t)(a.v0 + base) * a.H, offa, lds);
+        ls_dma<S::DA, 0, S::ONCE>(a.w + (size_t)(a.v0 + base) * a.H, offa, lds);
         ls_dma<S::DB, S::RB, false>(a.g + (int64_t)rb * S::BN * a.ldg + kn, offb, lds + S::kA);
         if (--left > 0) kn += kBK;
     }
-    __device__ __forceinline__ void done(vmi_f4 (&acc)[S::MB][S::NB]) {
-        if (++kd < steps) return;
+    static constexpr int STORES = 0;   // (its tiles end the run)
+    __device__ __forceinline__ bool done(vmi_f4 (&acc)[S::MB][S::NB]) {
+        if (++kd < steps) return false;
         const int w = ls_wave(), lane = threadIdx.x & 63;
         const int m0 = ht * S::BM + (w / S::WN) * (S::BM / S::WM) + 4 * (lane >> 4);
         const int n0 = rb * S::BN + (w % S::WN) * (S::BN / S::WN) + (lane & 15);
@@ -488,6 +555,7 @@ struct DxJob {
                 *dst = a.add ? *dst + acc[mb][n] : acc[mb][n];
             }
         }
+        return false;
     }
 };
 
@@ -496,7 +564,9 @@ struct DxJob {
 template <class S>
 __device__ __forceinline__ void ls_dx(const DxArgs& a, int nrb, int splits, uint8_t* lds) {
     const int nht = (a.H + S::BM - 1) / S::BM, steps = a.cols / kBK;
-    for (int item = blockIdx.x; item < splits * nht * nrb; item += gridDim.x) {
+    for (int turn = 0; turn * (int)gridDim.x < splits * nht * nrb; ++turn) {
+        const int item = ls_item(turn, splits * nht * nrb);
+        if (item < 0) break;
         const int rb = item % nrb, ht = item / nrb % nht, sp = item / nrb / nht;
         const int k0 = (int)((int64_t)steps * sp / splits), k1 = (int)((int64_t)steps * (sp + 1) / splits);
         DxJob<S> job(a, ht, rb, sp, nrb, k0, k1);
@@ -505,8 +575,8 @@ __device__ __forceinline__ void ls_dx(const DxArgs& a, int nrb, int splits, uint
 }
 
 // Up to 64 tokens: g and its rest side by side as tokens of one block.
-using Dx32 = Tile<256, 64, 4, 2, 3, true, false>;
-using Dx64 = Tile<256, 128, 4, 2, 3, true, false>;
+using Dx32 = Tile<256, 64, 4, 2, 3, true, false, true>;
+using Dx64 = Tile<256, 128, 4, 2, 3, true, false, true>;
 template <int BN>
 using DxN = Tile<256, BN, 4, 2, BN <= 160 ? 3 : 2, true, false>;
 
@@ -540,7 +610,8 @@ __global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
 struct DwArgs {
     const uint16_t *x, *g;
     const Meta* meta;
-    int fold;                // rows of g (and of x) where it is in two parts, else 0
+    int few;                 // tokens of g's two parts (x: their rows by idx), or 0 (x: those tokens' rows side by side)
+    const int32_t* idx;
     int H, V, v0, cols;
     int64_t ldg;
     void* dw;
@@ -549,12 +620,13 @@ struct DwArgs {
 template <class S, bool F32>
 struct DwJob {
     const DwArgs& a;
-    int nk, nht, step, item, items;      // asked for
-    int kd, at;                          // being multiplied
+    int nv, nk, nht, items;
+    int turn, item, step;                // asked for
+    int kd, done_turn;                   // being multiplied
     uint32_t offa[S::DA], offb[S::DB];
 
-    __device__ __forceinline__ DwJob(const DwArgs& a_, int nk_, int nht_, int items_)
-        : a(a_), nk(nk_), nht(nht_), step(0), item(blockIdx.x), items(items_), kd(0), at(blockIdx.x) {
+    __device__ __forceinline__ DwJob(const DwArgs& a_, int nv_, int nk_, int nht_, int items_)
+        : a(a_), nv(nv_), nk(nk_), nht(nht_), items(items_), turn(0), item(ls_item(0, items_)), step(0), kd(0), done_turn(0) {
         rows();
     }
     __device__ __forceinline__ void rows() {
@@ -563,7 +635,8 @@ struct DwJob {
         for (int i = 0; i < S::DA; ++i) {
             int row, piece;
             ls_slot<true>(i, row, piece);
-            offa[i] = (uint32_t)row * (uint32_t)(2 * a.H) + 2 * min(ht * S::BM + 8 * piece, a.H - 8);
+            const int r = a.few ? a.idx[min(row & (a.few - 1), nv - 1)] : row;   // (g is zero behind the last token)
+            offa[i] = (uint32_t)r * (uint32_t)(2 * a.H) + 2 * min(ht * S::BM + 8 * piece, a.H - 8);
         }
 #pragma unroll
         for (int i = 0; i < S::DB; ++i) {
@@ -573,11 +646,13 @@ struct DwJob {
         }
     }
     __device__ __forceinline__ void issue(uint8_t* lds) {
-        ls_dma<S::DA, 0, false>(a.x + (size_t)step * kBK * a.H, offa, lds);
+        ls_dma<S::DA, 0, false>(a.x + (a.few ? 0 : (size_t)step * kBK * a.H), offa, lds);
         ls_dma<S::DB, S::RB, false>(a.g + (int64_t)step * kBK * a.ldg, offb, lds + S::kA);
         if (++step == nk) {
-            if (item + (int)gridDim.x < items) {
-                item += gridDim.x;
+            const int next = (turn + 1) * (int)gridDim.x < items ? ls_item(turn + 1, items) : -1;
+            if (next >= 0) {
+                ++turn;
+                item = next;
                 step = 0;
                 rows();
             } else {
@@ -585,32 +660,33 @@ struct DwJob {
             }
         }
     }
-    __device__ __forceinline__ void done(vmi_f4 (&acc)[S::MB][S::NB]) {
-        if (++kd < nk) return;
+    static constexpr int STORES = S::MB * S::NB / (F32 ? 1 : 2);
+    __device__ __forceinline__ bool done(vmi_f4 (&acc)[S::MB][S::NB]) {
+        if (++kd < nk) return false;
         kd = 0;
         write(acc);
         ls_clear<S>(acc);
-        at += gridDim.x;
+        return true;
     }
     __device__ __forceinline__ void write(vmi_f4 (&acc)[S::MB][S::NB]) {
-        const int w = ls_wave(), lane = threadIdx.x & 63;
+        const int w = ls_wave(), lane = threadIdx.x & 63, at = ls_item(done_turn++, items);
+        constexpr int e = F32 ? 4 : 2;
         const int m0 = at % nht * S::BM + (w / S::WN) * (S::BM / S::WM) + 4 * (lane >> 4);
-        const int n0 = a.v0 + at / nht * S::BN + (w % S::WN) * (S::BN / S::WN) + (lane & 15);
+        const int first = a.v0 + at / nht * S::BN, n0 = (w % S::WN) * (S::BN / S::WN) + (lane & 15);
+        const __amdgpu_buffer_rsrc_t rs = vmi_rsrc(static_cast<uint8_t*>(a.dw) + (size_t)first * a.H * e, 0x7fffffffu);
 #pragma unroll
-        for (int n = 0; n < S::NB; ++n) {
-            if (n0 + 16 * n >= a.V) continue;
-            const size_t row = (size_t)(n0 + 16 * n) * a.H + m0;
+        for (int n = 0; n < S::NB; ++n)
 #pragma unroll
-            for (int mb = 0; mb < S::MB; ++mb) {
-                if (m0 + 16 * mb >= a.H) continue;
-                const vmi_f4 v = acc[mb][n];
+            for (int mb = 0; mb < S::MB; mb += F32 ? 1 : 2) {
+                const int h = F32 ? m0 + 16 * mb : m0 - 4 * (lane >> 4) + 16 * mb + ls_pair8_at();
+                const uint32_t off = first + n0 + 16 * n < a.V && h < a.H ? (uint32_t)((n0 + 16 * n) * a.H + h) * e : VMI_OOB;
+                const vmi_f4 v = acc[mb][n], u = acc[mb + (F32 ? 0 : 1)][n];
                 if constexpr (F32)
-                    *reinterpret_cast<vmi_f4*>(static_cast<float*>(a.dw) + row + 16 * mb) = v;
+                    vmi_bstore_b128(__builtin_bit_cast(vmi_u4, v), rs, off, 0);
                 else
-                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dw) + row + 16 * mb) =
-                        make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
+                    vmi_bstore_b128(ls_pair8(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]),
+                                             vmi_pack_bf16x2(u[0], u[1]), vmi_pack_bf16x2(u[2], u[3])), rs, off, 0);
             }
-        }
     }
 };
 
@@ -620,18 +696,16 @@ template <bool F32>
 __global__ __launch_bounds__(kThreads) void k_loss_dw(DwArgs a) {
     using S = DwTile;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds<S>];
-    const int nv = vmi_sload_i32(&a.meta->nv), nk = nv ? ((a.fold ? a.fold : nv) + kBK - 1) / kBK : 0;
+    const int nv = vmi_sload_i32(&a.meta->nv), nk = nv ? ((a.few ? 2 * a.few : nv) + kBK - 1) / kBK : 0;
     const int nht = (a.H + S::BM - 1) / S::BM, items = nht * ((a.cols + S::BN - 1) / S::BN);
-    if ((int)blockIdx.x >= items) return;
-    DwJob<S, F32> job(a, max(nk, 1), nht, items);
-    const int mine = (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;
+    if (ls_item(0, items) < 0) return;
+    DwJob<S, F32> job(a, max(nv, 1), max(nk, 1), nht, items);
+    const int whole = items / (int)gridDim.x;    // turns in which every workgroup has an item; the last may leave some out
+    const int mine = whole + (whole * (int)gridDim.x < items && ls_item(whole, items) >= 0 ? 1 : 0);
     if (nk == 0) {   // no token in the loss: zeros
         vmi_f4 acc[S::MB][S::NB];
         ls_clear<S>(acc);
-        for (int i = 0; i < mine; ++i) {
-            job.write(acc);
-            job.at += gridDim.x;
-        }
+        for (int i = 0; i < mine; ++i) job.write(acc);
         return;
     }
     ls_run<S>(lds, job, mine * nk);
@@ -654,17 +728,17 @@ struct RowsArgs {
 
 constexpr int kMaxItems = 4;       // workgroups' turns at most that the strips are cut for
 
-// The least work, in tokens' widths of a tile, of `tiles` cut into s strips by blocks of
-// bn tokens: turns of the grid times a turn's tiles (a tile's own cost beside its
+// The least work, in tokens' widths of a tile, of `tiles` cut into s strips by nrb blocks
+// of bn tokens: turns of the grid times a turn's tiles (a tile's own cost beside its
 // products about 16 tokens, a turn's 24); lane l tries s = l + 1, l + 65, ..  Returns work * 2^16 + s.
-__device__ __forceinline__ uint64_t ls_plan(int nv, int bn, int tiles, int grid) {
-    const int lane = threadIdx.x & 63, nrb = (nv + bn - 1) / bn;
+__device__ __forceinline__ uint64_t ls_plan(int nrb, int bn, int tiles, int grid) {
     const int most = min(tiles, max(1, kMaxItems * grid / nrb));
+    const float per_grid = (float)nrb / (float)grid;
     uint64_t best = ~0ull;
-    for (int s = lane + 1; s <= most; s += 64) {
-        const uint64_t turns = (nrb * s + grid - 1) / grid;
-        const uint64_t work = turns * ((uint64_t)((tiles + s - 1) / s) * (bn + 16) + 24);
-        best = min(best, work << 16 | (uint64_t)s);
+    for (int s = (threadIdx.x & 63) + 1; s <= most; s += 64) {
+        // rounded up, whole quotients off by a division's rounding left whole
+        const float turns = ceilf((float)s * per_grid - 1e-3f), deep = ceilf((float)tiles * __builtin_amdgcn_rcpf((float)s) - 1e-3f);
+        best = min(best, (uint64_t)(turns * fmaf(deep, (float)(bn + 16), 24.0f)) << 16 | (uint64_t)s);
     }
     return ~vmi_wave_max_u64(~best);
 }
@@ -672,6 +746,8 @@ __device__ __forceinline__ uint64_t ls_plan(int nv, int bn, int tiles, int grid)
 // One workgroup: a wave takes a run of tokens, 64 at a time, eight such groups' loads together.
 __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
     __shared__ int s_sum[16];
+    __shared__ uint64_t s_work[5];
+    __shared__ uint32_t s_cut[5];
     const int lane = threadIdx.x & 63, w = ls_wave(), run = (a.T + 1023) / 1024 * 64;
     const int t0 = min(a.T, w * run), t1 = min(a.T, t0 + run);
     constexpr int kAhead = 8;
@@ -724,27 +800,28 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
             }
         }
     }
-    if (w != 0) return;
-    Meta me{nv, a.few, 1, 1, 1};
-    if (nv) {
-        uint64_t best = ~0ull;
-        if (a.few) {   // one strip a workgroup: bytes bound it
-            me.strips = me.last = a.grid;
-        } else {
-            for (int bn = 256; bn >= 128; bn -= 32) {
-                const uint64_t p = ls_plan(nv, bn, a.tiles, a.grid);
-                if (p >> 16 < best >> 16) {
-                    best = p;
-                    me.bn = bn;
-                }
-            }
-            me.strips = (int)(best & 0xffffu);
-            me.last = (int)(ls_plan(nv, me.bn, a.last, a.grid) & 0xffffu);
+    // waves 0 to 4 weigh a width each
+    const int bn = a.few ? a.few : 256 - 32 * w, nrb = max((nv + bn - 1) / bn, 1);
+    if (!a.few && nv && bn >= 128) {
+        const uint64_t p = ls_plan(nrb, bn, a.tiles, a.grid), q = ls_plan(nrb, bn, a.last, a.grid);
+        if (lane == 0) {
+            s_work[w] = p >> 16;
+            s_cut[w] = (uint32_t)(p & 0xffffu) | (uint32_t)(q & 0xffffu) << 16;
         }
-        const int nrb = (nv + me.bn - 1) / me.bn;
-        me.splits = min(max(a.grid / max(nrb * a.nht, 1), 1), max(a.steps / 4, 1));
     }
-    if (lane == 0) *a.meta = me;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    Meta me{nv, bn, a.grid, a.grid, 1};   // few: one strip a workgroup, bytes bound it
+    if (!a.few && nv) {
+        int best = 0;
+        for (int i = 1; i < 5; ++i) best = s_work[i] < s_work[best] ? i : best;
+        me.bn = 256 - 32 * best;
+        me.strips = (int)(s_cut[best] & 0xffffu);
+        me.last = (int)(s_cut[best] >> 16);
+    }
+    const int blocks = max((nv + me.bn - 1) / me.bn, 1);
+    me.splits = min(max(a.grid / (blocks * a.nht), 1), max(a.steps / 4, 1));
+    *a.meta = me;
 }
 
 // A wave per token: its strips' maxima and sums, in a fixed order.
@@ -768,40 +845,48 @@ __global__ __launch_bounds__(256) void k_loss_merge(const Meta* meta, const int3
     }
 }
 
-// Row c (of c and c + fold alike) of the tokens in the loss, zeros from nv on.
-__global__ __launch_bounds__(256) void k_loss_compact(const Meta* meta, const int32_t* idx, int fold, const vmi_u4* x, int U,
-                                                      vmi_u4* out) {
-    const int c = fold && (int)blockIdx.x >= fold ? blockIdx.x - fold : blockIdx.x;
+// Row c of the tokens in the loss, zeros from nv on.
+__global__ __launch_bounds__(256) void k_loss_compact(const Meta* meta, const int32_t* idx, const vmi_u4* x, int U, vmi_u4* out) {
+    const int c = blockIdx.x;
     const bool in = c < meta->nv;
     const size_t src = in ? (size_t)idx[c] * U : 0;
-    for (int u = threadIdx.x; u < U; u += 256) out[(size_t)blockIdx.x * U + u] = in ? x[src + u] : vmi_u4{0, 0, 0, 0};
+    for (int u = threadIdx.x; u < U; u += 256) out[(size_t)c * U + u] = in ? x[src + u] : vmi_u4{0, 0, 0, 0};
 }
 
-// dx of a token: its splits' sums in order (fold: those of the two parts of g, fold rows
-// apart), zeros for a token left out.
-__global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int32_t* pos, const float* sum, int H, int fold,
+// dx of a token: its splits' sums in a fixed order (few: those of g's two parts, few rows
+// apart), zeros for a token left out.  A wave takes 256 hidden values; SPREAD: the
+// workgroup's four waves share one such piece's sums (few tokens, many splits: 22 -> 7 us).
+template <bool SPREAD>
+__global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int32_t* pos, const float* sum, int H, int few,
                                                      uint16_t* dx) {
+    __shared__ vmi_f4 s_part[3][64];
     const Meta me = ls_meta(meta);
-    const int t = blockIdx.x, c = pos[t], rows = fold ? 2 * fold : (me.nv + me.bn - 1) / me.bn * me.bn;
-    constexpr int kAhead = 8;
-    for (int h = 4 * threadIdx.x; h < H; h += 1024) {
-        vmi_f4 v = {0.f, 0.f, 0.f, 0.f};
-        if (c >= 0) {
-            const int n = fold ? 2 * me.splits : me.splits;
-            for (int i0 = 0; i0 < n; i0 += kAhead) {
-                vmi_f4 u[kAhead];
+    const int t = blockIdx.x, c = pos[t], rows = few ? 2 * few : (me.nv + me.bn - 1) / me.bn * me.bn, w = ls_wave();
+    const int lane = threadIdx.x & 63, h = 256 * (SPREAD ? blockIdx.y : 4 * blockIdx.y + w) + 4 * lane;
+    vmi_f4 v = {0.f, 0.f, 0.f, 0.f};
+    if (c >= 0 && h < H) {
+        constexpr int kAhead = 8;
+        const int n = few ? 2 * me.splits : me.splits, i0 = SPREAD ? n * w / 4 : 0, i1 = SPREAD ? n * (w + 1) / 4 : n;
+        for (int i = i0; i < i1; i += kAhead) {
+            vmi_f4 u[kAhead];
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    const int j = min(i0 + i, n - 1), s = fold ? j >> 1 : j;
-                    u[i] = *reinterpret_cast<const vmi_f4*>(sum + ((size_t)s * rows + c + (fold && (j & 1) ? fold : 0)) * H + h);
-                }
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i)
-                    if (i0 + i < n) v += u[i];
+            for (int j = 0; j < kAhead; ++j) {
+                const int p = min(i + j, i1 - 1), s = few ? p >> 1 : p;
+                u[j] = *reinterpret_cast<const vmi_f4*>(sum + ((size_t)s * rows + c + (few && (p & 1) ? few : 0)) * H + h);
             }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (i + j < i1) v += u[j];
         }
-        *reinterpret_cast<uint2*>(dx + (size_t)t * H + h) = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
     }
+    if constexpr (SPREAD) {
+        if (w) s_part[w - 1][lane] = v;
+        __syncthreads();
+        if (w) return;
+        for (int i = 0; i < 3; ++i) v += s_part[i][lane];
+    }
+    if (h < H)
+        *reinterpret_cast<uint2*>(dx + (size_t)t * H + h) = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
 }
 
 // ---------------------------------------------------------------------- host
@@ -842,7 +927,7 @@ Layout carve(int T, int H, int V, bool grad) {
         const int64_t fit = std::max<int64_t>(8192, kPieceBytes / (2 * l.rows) / 256 * 256);
         l.piece = (int)std::min(all, fit);
         l.ldg = l.piece + 64;         // off a power of two
-        l.x = take((size_t)l.rows * H * 2);
+        l.x = take(l.few ? 0 : (size_t)l.rows * H * 2);
         l.g = take((size_t)l.rows * l.ldg * 2);
         const int nht = (H + 255) / 256;
         l.sum = take(((size_t)l.rows + (size_t)std::max(cus / nht, 1) * (l.few ? 2 * l.few : 256)) * H * 4);
@@ -984,12 +1069,14 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     r.steps = r.last * 256 / kBK;
     hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
     uint16_t* xc = reinterpret_cast<uint16_t*>(ws + l.x);
-    if (T)
-        hipLaunchKernelGGL(k_loss_compact, dim3(l.rows), dim3(256), 0, s, r.meta, r.idx, l.few,
-                           reinterpret_cast<const vmi_u4*>(x), hidden / 8, reinterpret_cast<vmi_u4*>(xc));
+    const bool compact = dweight && !l.few;   // (the other products take x's rows by idx)
+    if (compact)
+        hipLaunchKernelGGL(k_loss_compact, dim3(l.rows), dim3(256), 0, s, r.meta, r.idx, reinterpret_cast<const vmi_u4*>(x),
+                           hidden / 8, reinterpret_cast<vmi_u4*>(xc));
     LogitArgs a{};
-    a.x = xc;
+    a.x = x;
     a.w = weight;
+    a.idx = r.idx;
     a.meta = r.meta;
     a.coef = r.coef;
     a.H = hidden;
@@ -1005,14 +1092,15 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     d.ldg = l.ldg;
     d.sum = reinterpret_cast<float*>(ws + l.sum);
     DwArgs u{};
-    u.x = xc;
+    u.x = compact ? xc : x;
+    u.idx = r.idx;
+    u.few = l.few;
     u.g = a.g;
     u.meta = r.meta;
     u.H = hidden;
     u.V = vocab;
     u.ldg = l.ldg;
     u.dw = dweight;
-    u.fold = 2 * l.few;
     for (int v0 = 0; v0 < vocab; v0 += l.piece) {
         const int cols = std::min(l.piece, (vocab - v0 + 255) / 256 * 256);
         a.v0 = v0;
@@ -1032,7 +1120,13 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
                 hipLaunchKernelGGL(k_loss_dw<false>, dim3(grid), dim3(kThreads), 0, s, u);
         }
     }
-    if (dx && T)
-        hipLaunchKernelGGL(k_loss_dx_out, dim3(T), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden, l.few, dx);
+    if (dx && T) {
+        if (T <= 1024)
+            hipLaunchKernelGGL(k_loss_dx_out<true>, dim3(T, (hidden + 255) / 256), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden,
+                               l.few, dx);
+        else
+            hipLaunchKernelGGL(k_loss_dx_out<false>, dim3(T, (hidden + 1023) / 1024), dim3(256), 0, s, r.meta, r.pos, d.sum,
+                               hidden, l.few, dx);
+    }
     return launched("vmi_head_loss_grad launch");
 }
