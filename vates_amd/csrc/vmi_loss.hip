@@ -24,7 +24,7 @@
 // Kernels beside them:
 //   k_loss_rows     the tokens in the loss, and their coefficients
 //   k_loss_merge    the strips' maxima and sums of a token joined
-//   k_loss_compact  those tokens' rows of x side by side
+//   k_loss_turn     those tokens' x turned
 //   k_loss_dx_out   the split sums of dx joined
 
 #include <algorithm>
@@ -172,7 +172,8 @@ __device__ __forceinline__ void ls_clear(vmi_f4 (&acc)[S::MB][S::NB]) {
 
 // The steps 0 .. total - 1 of a workgroup's tiles, one after another: job.issue(lds) asks
 // for the next step's operands (behind the last, again for the last's, so that every
-// wait counts alike), job.done(acc) ends a step, takes a tile that is complete and says
+// wait counts alike), job.wanted() says whether the wave's part of the tile has any row,
+// job.done(acc) ends a step, takes a tile that is complete and says
 // whether it has issued its STORES stores (all of them, whatever they cover).
 template <class S, class Job>
 __device__ __forceinline__ void ls_run(uint8_t* lds, Job& job, int total) {
@@ -191,7 +192,7 @@ __device__ __forceinline__ void ls_run(uint8_t* lds, Job& job, int total) {
         asm volatile("" ::: "memory");
         job.issue(lds + in * S::kStage);
         in = in + 1 == S::STAGES ? 0 : in + 1;
-        ls_multiply<S>(lds + out * S::kStage, acc);
+        if (job.wanted()) ls_multiply<S>(lds + out * S::kStage, acc);
         out = out + 1 == S::STAGES ? 0 : out + 1;
         stored = job.done(acc);
     }
@@ -256,7 +257,8 @@ struct LogitJob {
         nk = a.H / kBK;
         // Rows of a few KB put the pieces that all workgroups ask for at one time on few memory channels; begun at
         // steps of their own, strips spread over them all (one token 129 -> 109 us, 100 tokens 156 -> 129).
-        turn = nv <= 4 * S::BN ? v0_ / 16 % nk : 0;
+        // Where blocks of tokens share a strip in an XCD's L2, groups of them do (8192 tokens 4014 -> 3965 us).
+        turn = nv <= 4 * S::BN ? v0_ / 16 % nk : (rb >> 3) * 11 % nk;
         tile = v0_;
         next = min(v0_, a.V - 1);   // (a piece's last tile may lie behind the vocabulary: its columns are zeros)
         k = kd = 0;
@@ -304,6 +306,7 @@ struct LogitJob {
         }
     }
     static constexpr int STORES = GRAD * S::MB * S::NB / (S::MB % 2 ? 1 : 2);
+    __device__ __forceinline__ bool wanted() const { return tile + (ls_wave() / S::WN) * (S::BM / S::WM) < v1; }
     __device__ __forceinline__ bool done(vmi_f4 (&acc)[S::MB][S::NB]) {
         if (++kd < nk) return false;
         kd = 0;
@@ -540,6 +543,7 @@ struct DxJob {
         if (--left > 0) kn += kBK;
     }
     static constexpr int STORES = 0;   // (its tiles end the run)
+    __device__ __forceinline__ bool wanted() const { return true; }
     __device__ __forceinline__ bool done(vmi_f4 (&acc)[S::MB][S::NB]) {
         if (++kd < steps) return false;
         const int w = ls_wave(), lane = threadIdx.x & 63;
@@ -578,7 +582,7 @@ __device__ __forceinline__ void ls_dx(const DxArgs& a, int nrb, int splits, uint
 using Dx32 = Tile<256, 64, 4, 2, 3, true, false, true>;
 using Dx64 = Tile<256, 128, 4, 2, 3, true, false, true>;
 template <int BN>
-using DxN = Tile<256, BN, 4, 2, BN <= 160 ? 3 : 2, true, false>;
+using DxN = Tile<256, BN, 4, 2, BN <= 160 ? 3 : 2, true, false, true>;
 
 template <int WHICH>
 __global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
@@ -607,14 +611,15 @@ __global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
 }
 
 // ------------------------------------------------------------------------ dW
+// x as [hidden][token] of the tokens in the loss (ldx values a row), its own rows by idx where there are few.
 struct DwArgs {
     const uint16_t *x, *g;
     const Meta* meta;
-    int few;                 // tokens of g's two parts (x: their rows by idx), or 0 (x: those tokens' rows side by side)
-    const int32_t* idx;
     int H, V, v0, cols;
-    int64_t ldg;
+    int64_t ldg, ldx;
     void* dw;
+    int few;                 // tokens of g's two parts, or 0
+    const int32_t* idx;
 };
 
 template <class S, bool F32>
@@ -634,9 +639,12 @@ struct DwJob {
 #pragma unroll
         for (int i = 0; i < S::DA; ++i) {
             int row, piece;
-            ls_slot<true>(i, row, piece);
-            const int r = a.few ? a.idx[min(row & (a.few - 1), nv - 1)] : row;   // (g is zero behind the last token)
-            offa[i] = (uint32_t)r * (uint32_t)(2 * a.H) + 2 * min(ht * S::BM + 8 * piece, a.H - 8);
+            ls_slot<S::ASLOW>(i, row, piece);
+            if constexpr (S::ASLOW)   // few tokens, by idx (g is zero behind the last)
+                offa[i] = (uint32_t)a.idx[min(row & (a.few - 1), nv - 1)] * (uint32_t)(2 * a.H) +
+                          2 * min(ht * S::BM + 8 * piece, a.H - 8);
+            else
+                offa[i] = (uint32_t)min(ht * S::BM + row, a.H - 1) * (uint32_t)(2 * a.ldx) + 16 * piece;
         }
 #pragma unroll
         for (int i = 0; i < S::DB; ++i) {
@@ -646,7 +654,7 @@ struct DwJob {
         }
     }
     __device__ __forceinline__ void issue(uint8_t* lds) {
-        ls_dma<S::DA, 0, false>(a.x + (a.few ? 0 : (size_t)step * kBK * a.H), offa, lds);
+        ls_dma<S::DA, 0, false>(a.x + (S::ASLOW ? 0 : step * kBK), offa, lds);
         ls_dma<S::DB, S::RB, false>(a.g + (int64_t)step * kBK * a.ldg, offb, lds + S::kA);
         if (++step == nk) {
             const int next = (turn + 1) * (int)gridDim.x < items ? ls_item(turn + 1, items) : -1;
@@ -661,6 +669,7 @@ struct DwJob {
         }
     }
     static constexpr int STORES = S::MB * S::NB / (F32 ? 1 : 2);
+    __device__ __forceinline__ bool wanted() const { return true; }
     __device__ __forceinline__ bool done(vmi_f4 (&acc)[S::MB][S::NB]) {
         if (++kd < nk) return false;
         kd = 0;
@@ -690,13 +699,11 @@ struct DwJob {
     }
 };
 
-using DwTile = Tile<256, 256, 2, 4, 2, true, true>;
-
-template <bool F32>
+template <bool FEW, bool F32>
 __global__ __launch_bounds__(kThreads) void k_loss_dw(DwArgs a) {
-    using S = DwTile;
+    using S = Tile<256, 256, 2, 4, 2, FEW, true>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds<S>];
-    const int nv = vmi_sload_i32(&a.meta->nv), nk = nv ? ((a.few ? 2 * a.few : nv) + kBK - 1) / kBK : 0;
+    const int nv = vmi_sload_i32(&a.meta->nv), nk = nv ? ((FEW ? 2 * a.few : nv) + kBK - 1) / kBK : 0;
     const int nht = (a.H + S::BM - 1) / S::BM, items = nht * ((a.cols + S::BN - 1) / S::BN);
     if (ls_item(0, items) < 0) return;
     DwJob<S, F32> job(a, max(nv, 1), max(nk, 1), nht, items);
@@ -729,15 +736,16 @@ struct RowsArgs {
 constexpr int kMaxItems = 4;       // workgroups' turns at most that the strips are cut for
 
 // The least work, in tokens' widths of a tile, of `tiles` cut into s strips by nrb blocks
-// of bn tokens: turns of the grid times a turn's tiles (a tile's own cost beside its
-// products about 16 tokens, a turn's 24); lane l tries s = l + 1, l + 65, ..  Returns work * 2^16 + s.
+// of bn tokens: turns of the grid times a turn's tiles in quarters, which the waves behind a strip's end leave out (a tile's own
+// cost beside its products about 16 tokens, a turn's 24); lane l tries s = l + 1, l + 65, ..  Returns work * 2^16 + s.
 __device__ __forceinline__ uint64_t ls_plan(int nrb, int bn, int tiles, int grid) {
     const int most = min(tiles, max(1, kMaxItems * grid / nrb));
     const float per_grid = (float)nrb / (float)grid;
     uint64_t best = ~0ull;
     for (int s = (threadIdx.x & 63) + 1; s <= most; s += 64) {
         // rounded up, whole quotients off by a division's rounding left whole
-        const float turns = ceilf((float)s * per_grid - 1e-3f), deep = ceilf((float)tiles * __builtin_amdgcn_rcpf((float)s) - 1e-3f);
+        const float turns = ceilf((float)s * per_grid - 1e-3f);
+        const float deep = 0.25f * ceilf(4.0f * (float)tiles * __builtin_amdgcn_rcpf((float)s) - 1e-3f);
         best = min(best, (uint64_t)(turns * fmaf(deep, (float)(bn + 16), 24.0f)) << 16 | (uint64_t)s);
     }
     return ~vmi_wave_max_u64(~best);
@@ -845,12 +853,28 @@ __global__ __launch_bounds__(256) void k_loss_merge(const Meta* meta, const int3
     }
 }
 
-// Row c of the tokens in the loss, zeros from nv on.
-__global__ __launch_bounds__(256) void k_loss_compact(const Meta* meta, const int32_t* idx, const vmi_u4* x, int U, vmi_u4* out) {
-    const int c = blockIdx.x;
-    const bool in = c < meta->nv;
-    const size_t src = in ? (size_t)idx[c] * U : 0;
-    for (int u = threadIdx.x; u < U; u += 256) out[(size_t)c * U + u] = in ? x[src + u] : vmi_u4{0, 0, 0, 0};
+// x of the tokens in the loss turned, out[h][c], zeros from nv on: the head's gradient then
+// reads one operand of its two along memory (both turned as they were read, LDS took longer than the
+// products: 4096 tokens 2.5 -> 2.1 ms).  64 tokens by 64 hidden values a workgroup.
+__global__ __launch_bounds__(256) void k_loss_turn(const Meta* meta, const int32_t* idx, const uint16_t* x, int H, int64_t ldx,
+                                                   uint16_t* out) {
+    __shared__ uint32_t s_x[64][33];
+    const int nv = vmi_sload_i32(&meta->nv), c0 = blockIdx.x * 64, h0 = blockIdx.y * 64, t = threadIdx.x;
+    if (c0 >= (nv + kBK - 1) / kBK * kBK) return;
+    for (int i = t; i < 64 * 8; i += 256) {
+        const int c = i >> 3, u = i & 7;
+        vmi_u4 v = {0, 0, 0, 0};
+        if (c0 + c < nv) v = *reinterpret_cast<const vmi_u4*>(x + (size_t)idx[c0 + c] * H + h0 + 8 * u);
+        for (int j = 0; j < 4; ++j) s_x[c][4 * u + j] = v[j];
+    }
+    __syncthreads();
+    for (int i = t; i < 64 * 8; i += 256) {
+        const int h = i >> 3, u = i & 7, sh = 16 * (h & 1);
+        vmi_u4 v;
+        for (int j = 0; j < 4; ++j)
+            v[j] = ((s_x[8 * u + 2 * j][h >> 1] >> sh) & 0xffffu) | ((s_x[8 * u + 2 * j + 1][h >> 1] >> sh) << 16);
+        *reinterpret_cast<vmi_u4*>(out + (int64_t)(h0 + h) * ldx + c0 + 8 * u) = v;
+    }
 }
 
 // dx of a token: its splits' sums in a fixed order (few: those of g's two parts, few rows
@@ -894,7 +918,7 @@ constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 
 struct Layout {
     int few, rows, piece;             // tokens of the one block where there are few, rows of g, vocabulary rows of a piece
-    int64_t ldg;
+    int64_t ldg, ldx;
     size_t idx, pos, meta, coef, part, hit, x, g, sum, bytes;
 };
 
@@ -927,7 +951,8 @@ Layout carve(int T, int H, int V, bool grad) {
         const int64_t fit = std::max<int64_t>(8192, kPieceBytes / (2 * l.rows) / 256 * 256);
         l.piece = (int)std::min(all, fit);
         l.ldg = l.piece + 64;         // off a power of two
-        l.x = take(l.few ? 0 : (size_t)l.rows * H * 2);
+        l.ldx = l.rows + 64;
+        l.x = take(l.few ? 0 : (size_t)l.ldx * H * 2);
         l.g = take((size_t)l.rows * l.ldg * 2);
         const int nht = (H + 255) / 256;
         l.sum = take(((size_t)l.rows + (size_t)std::max(cus / nht, 1) * (l.few ? 2 * l.few : 256)) * H * 4);
@@ -1068,11 +1093,9 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     r.nht = (hidden + 255) / 256;
     r.steps = r.last * 256 / kBK;
     hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
-    uint16_t* xc = reinterpret_cast<uint16_t*>(ws + l.x);
-    const bool compact = dweight && !l.few;   // (the other products take x's rows by idx)
-    if (compact)
-        hipLaunchKernelGGL(k_loss_compact, dim3(l.rows), dim3(256), 0, s, r.meta, r.idx, reinterpret_cast<const vmi_u4*>(x),
-                           hidden / 8, reinterpret_cast<vmi_u4*>(xc));
+    uint16_t* xt = reinterpret_cast<uint16_t*>(ws + l.x);
+    if (dweight && !l.few)
+        hipLaunchKernelGGL(k_loss_turn, dim3(l.rows / 64, hidden / 64), dim3(256), 0, s, r.meta, r.idx, x, hidden, l.ldx, xt);
     LogitArgs a{};
     a.x = x;
     a.w = weight;
@@ -1092,7 +1115,8 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     d.ldg = l.ldg;
     d.sum = reinterpret_cast<float*>(ws + l.sum);
     DwArgs u{};
-    u.x = compact ? xc : x;
+    u.x = l.few ? x : xt;
+    u.ldx = l.ldx;
     u.idx = r.idx;
     u.few = l.few;
     u.g = a.g;
@@ -1114,10 +1138,15 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
             if (dx) launch_dx(d, l.few, grid, s);
         }
         if (dweight) {
-            if (dweight_dtype == VMI_F32)
-                hipLaunchKernelGGL(k_loss_dw<true>, dim3(grid), dim3(kThreads), 0, s, u);
+            const bool f32 = dweight_dtype == VMI_F32;
+            if (l.few && f32)
+                hipLaunchKernelGGL((k_loss_dw<true, true>), dim3(grid), dim3(kThreads), 0, s, u);
+            else if (l.few)
+                hipLaunchKernelGGL((k_loss_dw<true, false>), dim3(grid), dim3(kThreads), 0, s, u);
+            else if (f32)
+                hipLaunchKernelGGL((k_loss_dw<false, true>), dim3(grid), dim3(kThreads), 0, s, u);
             else
-                hipLaunchKernelGGL(k_loss_dw<false>, dim3(grid), dim3(kThreads), 0, s, u);
+                hipLaunchKernelGGL((k_loss_dw<false, false>), dim3(grid), dim3(kThreads), 0, s, u);
         }
     }
     if (dx && T) {
