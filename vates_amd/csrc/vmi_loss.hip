@@ -948,8 +948,8 @@ Layout carve(int T, int H, int V, bool grad) {
         l.hit = take((size_t)l.rows * 4);
     } else {
         const int64_t all = ((int64_t)V + 255) / 256 * 256;
-        const int64_t fit = std::max<int64_t>(8192, kPieceBytes / (2 * l.rows) / 256 * 256);
-        l.piece = (int)std::min(all, fit);
+        const int64_t fit = std::max<int64_t>(8192, kPieceBytes / (2 * l.rows)), n = (all + fit - 1) / fit;
+        l.piece = (int)((all / 256 + n - 1) / n * 256);   // pieces alike
         l.ldg = l.piece + 64;         // off a power of two
         l.ldx = l.rows + 64;
         l.x = take(l.few ? 0 : (size_t)l.ldx * H * 2);
