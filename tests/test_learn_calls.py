@@ -62,7 +62,7 @@ def test_expert_refusals(lib):
         assert plan(**kw) == L.VMI_ERR_INVALID, kw
     for E in (0, -1, 1025):
         assert plan(E=E) == L.VMI_ERR_UNSUPPORTED and lib.vmi_expert_plan_workspace_bytes(4, 2, E) == 0
-    assert plan(ws=None) == L.VMI_ERR_WORKSPACE and plan(n=4) == L.VMI_ERR_WORKSPACE
+    assert plan(T=4097, ws=None) == L.VMI_ERR_WORKSPACE and plan(T=4097, n=4) == L.VMI_ERR_WORKSPACE
     assert lib.vmi_expert_plan_workspace_bytes(4, 33, 8) == 0
 
     def rows(T=4, k=2, H=64, dt=L.VMI_BF16, x=P, p=P, r=P):

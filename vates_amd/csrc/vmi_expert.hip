@@ -23,7 +23,8 @@ namespace {
 
 constexpr int kMaxE = 1024, kMaxK = 32;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kMaxSegments = 64;
+constexpr int kChunks = 8;                               // groups of 64 routes of a wave
+constexpr int kWhole = kSortThreads * kChunks;           // routes of a workgroup at most
 
 struct PlanArgs {
     const int32_t* ids;
@@ -35,20 +36,31 @@ struct PlanArgs {
 
 __device__ __forceinline__ int ex_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
-// The route's bin: its expert, or E.
-__device__ __forceinline__ int ex_bin(const PlanArgs& a, int p, bool& odd) {
-    const int id = a.ids[p];
-    odd |= id < -1 || id >= a.E;
-    return (uint32_t)id < (uint32_t)a.E ? id : a.E;
+// The bins of the lane's route in each of the wave's kChunks groups of 64, all asked for
+// together: its expert, E for none, -1 behind the segment.
+__device__ __forceinline__ void ex_bins(const PlanArgs& a, int p0, int p1, int (&b)[kChunks], bool& odd) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) b[i] = p0 + 64 * i < p1 ? a.ids[min(p0 + 64 * i + lane, a.n - 1)] : 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+        const bool in = p0 + 64 * i + lane < p1;
+        odd |= in && (b[i] < -1 || b[i] >= a.E);
+        b[i] = !in ? -1 : (uint32_t)b[i] < (uint32_t)a.E ? b[i] : a.E;
+    }
 }
 
 __global__ __launch_bounds__(kSortThreads) void k_expert_count(PlanArgs a) {
     __shared__ uint32_t s_n[kMaxE + 1];
+    const int run = a.seg / kSortWaves, p0 = blockIdx.x * a.seg + ex_wave() * run, p1 = min(a.n, p0 + run);
+    int b[kChunks];
+    bool odd = false;
+    ex_bins(a, p0, p1, b, odd);
     for (int e = threadIdx.x; e <= a.E; e += kSortThreads) s_n[e] = 0u;
     __syncthreads();
-    const int p0 = blockIdx.x * a.seg, p1 = min(a.n, p0 + a.seg);
-    bool odd = false;
-    for (int p = p0 + threadIdx.x; p < p1; p += kSortThreads) atomicAdd(&s_n[ex_bin(a, p, odd)], 1u);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+        if (b[i] >= 0) atomicAdd(&s_n[b[i]], 1u);
     __syncthreads();
     for (int e = threadIdx.x; e <= a.E; e += kSortThreads) a.count[(size_t)blockIdx.x * (a.E + 1) + e] = s_n[e];
 }
@@ -57,30 +69,40 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_count(PlanArgs a) {
 // LDS (whole numbers, so that the order of the atomics does not matter), prefix sums over
 // waves, segments and bins, then every wave places its run 64 routes at a time: a
 // route's row is its bin's next one plus the lower lanes with the same bin, found by one
-// ballot per bit of the bin.  Bound by latency: 40 routes 5 us, 81,920 ten.
+// ballot per bit of the bin.  Bound by latency.
 __global__ __launch_bounds__(kSortThreads) void k_expert_place(PlanArgs a) {
     __shared__ uint32_t s_at[kSortWaves * (kMaxE + 1)];   // [waves][E + 1]
     __shared__ uint32_t s_sum[kSortWaves];
     const int lane = threadIdx.x & 63, w = ex_wave(), B = a.E + 1, run = a.seg / kSortWaves;
+    const int p0 = blockIdx.x * a.seg + w * run, p1 = min(a.n, p0 + run);
+    int bin[kChunks];
+    bool odd = false;
+    ex_bins(a, p0, p1, bin, odd);
     for (int i = threadIdx.x; i < kSortWaves * B; i += kSortThreads) s_at[i] = 0u;
     __syncthreads();
-    const int p0 = blockIdx.x * a.seg + w * run, p1 = min(a.n, p0 + run);
-    bool odd = false;
-    for (int p = p0 + lane; p < p1; p += 64) atomicAdd(&s_at[w * B + ex_bin(a, p, odd)], 1u);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+        if (bin[i] >= 0) atomicAdd(&s_at[w * B + bin[i]], 1u);
     if (a.status && __any(odd) && lane == 0) atomicOr(a.status, VMI_STATUS_BAD_SLOT);
     __syncthreads();
-    // thread e: bin e's routes in all segments, and in those before this one
-    const int e = threadIdx.x;              // kMaxE + 1 bins: the last one's are thread 0's second turn
+    // thread b: bin b's routes in all segments, and in those before this one (1025 bins: two turns)
     uint32_t carry = 0;
-    for (int e0 = 0; e0 < B; e0 += kSortThreads) {
-        const int b = e0 + e;
+    for (int b0 = 0; b0 < B; b0 += kSortThreads) {
+        const int b = b0 + threadIdx.x;
         uint32_t all = 0, before = 0;
         if (b < B) {
             if (gridDim.x > 1) {
-                for (unsigned i = 0; i < gridDim.x; ++i) {
-                    const uint32_t c = a.count[(size_t)i * B + b];
-                    before += i < blockIdx.x ? c : 0u;
-                    all += c;
+                constexpr int kAhead = 8;
+                for (int i0 = 0; i0 < (int)gridDim.x; i0 += kAhead) {
+                    uint32_t c[kAhead];
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) c[i] = a.count[(size_t)min(i0 + i, (int)gridDim.x - 1) * B + b];
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) {
+                        c[i] = i0 + i < (int)gridDim.x ? c[i] : 0u;
+                        before += i0 + i < (int)blockIdx.x ? c[i] : 0u;
+                        all += c[i];
+                    }
                 }
             } else {
                 for (int i = 0; i < kSortWaves; ++i) all += s_at[i * B + b];
@@ -113,23 +135,23 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_place(PlanArgs a) {
         __syncthreads();
     }
     uint32_t* mine = s_at + w * B;
-    for (int c = p0; c < p1; c += 64) {
-        const int p = c + lane;
-        const bool in = p < p1;
-        const int b = in ? ex_bin(a, p, odd) : 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+        if (p0 + 64 * i >= p1) break;
+        const int p = p0 + 64 * i + lane, b = max(bin[i], 0);
+        const bool in = bin[i] >= 0;
         uint64_t same = __ballot(in);
         for (int bit = 0; (B - 1) >> bit; ++bit) {   // wave-uniform
             const uint64_t m = __ballot((b >> bit) & 1);
             same &= (b >> bit) & 1 ? m : ~m;
         }
         if (in) {
-            const uint32_t low = __builtin_popcountll(same & ((1ull << lane) - 1));
-            const uint32_t at = mine[b];
-            const int32_t row = (int32_t)(at + low);
+            const uint32_t at = mine[b] + __builtin_popcountll(same & ((1ull << lane) - 1));
+            const int32_t row = (int32_t)at;
             a.source[row] = p;
             a.place[p] = b < a.E ? row : ~row;
-            // every lane of the bin has read its start before the last of them moves it on (one wave, in order)
-            if ((same >> lane) == 1ull) mine[b] = at + low + 1;
+            // (every lane of the bin has read its start before the last of them moves it on: one wave, in order)
+            if ((same >> lane) == 1ull) mine[b] = at + 1;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -144,8 +166,17 @@ struct RowArgs {
     const float* scores;
     vmi_u4* out;
     float* dscores;
-    int T, k, U;              // tokens, routes of one, 16-byte units of a row
+    int T, k, U, pieces;      // tokens, routes of one, 16-byte units of a row, its pieces of 64
 };
+
+// The wave's token and unit: the pieces of a row go to waves side by side, so that a row is
+// asked for at once (token by token of one piece, 8192 x 10 rows took 88 us to combine).
+__device__ __forceinline__ bool ex_unit(const RowArgs& a, int& t, int& u) {
+    const uint32_t w = blockIdx.x * 4 + ex_wave();
+    t = (int)(w / (uint32_t)a.pieces);
+    u = (int)(w % (uint32_t)a.pieces) * 64 + (threadIdx.x & 63);
+    return t < a.T;
+}
 
 template <bool F32>
 __device__ __forceinline__ void ex_widen(const vmi_u4& u, float (&v)[F32 ? 4 : 8]) {
@@ -175,9 +206,8 @@ __device__ __forceinline__ vmi_u4 ex_narrow(const float (&v)[F32 ? 4 : 8]) {
 // A wave per token and 64 units of its row: read once, written to its routes' rows; a
 // route without an expert gets zeros.
 __global__ __launch_bounds__(256) void k_expert_rows(RowArgs a) {
-    const int t = blockIdx.x * 4 + ex_wave();
-    if (t >= a.T) return;
-    const int u = blockIdx.y * 64 + (threadIdx.x & 63);
+    int t, u;
+    if (!ex_unit(a, t, u)) return;
     const bool in = u < a.U;
     vmi_u4 v = {0, 0, 0, 0};
     if (in) v = a.x[(size_t)t * a.U + u];
@@ -192,10 +222,8 @@ __global__ __launch_bounds__(256) void k_expert_rows(RowArgs a) {
 template <bool F32>
 __global__ __launch_bounds__(256) void k_expert_combine(RowArgs a) {
     constexpr int N = F32 ? 4 : 8, kAhead = 8;
-    const int t = blockIdx.x * 4 + ex_wave();
-    if (t >= a.T) return;
-    const int u = blockIdx.y * 64 + (threadIdx.x & 63);
-    if (u >= a.U) return;
+    int t, u;
+    if (!ex_unit(a, t, u) || u >= a.U) return;
     float sum[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) sum[i] = 0.0f;
@@ -263,11 +291,10 @@ __global__ __launch_bounds__(256) void k_expert_grad(RowArgs a) {
     }
 }
 
-int plan_segment(int64_t n) {
-    const int64_t seg = std::max<int64_t>(2 * kSortThreads, (n + kMaxSegments - 1) / kMaxSegments);
-    return (int)((seg + kSortThreads - 1) / kSortThreads * kSortThreads);
-}
-int plan_segments(int64_t n) { return n <= 8192 ? 1 : (int)((n + plan_segment(n) - 1) / plan_segment(n)); }
+// Up to kWhole routes one workgroup; above, segments of a quarter of that (40 of them for 8192 x 10) up to 64 segments,
+// then whole ones.
+int plan_segment(int64_t n) { return n <= kWhole || n > 16 * kWhole ? kWhole : kWhole / 4; }
+int plan_segments(int64_t n) { return (int)std::max<int64_t>(1, (n + plan_segment(n) - 1) / plan_segment(n)); }
 
 bool shape_ok(int T, int k) { return T >= 0 && k > 0 && k <= kMaxK && (int64_t)T * k <= (1 << 24); }
 
@@ -280,6 +307,10 @@ int rows_check(const char* what, int dtype, int T, int k, int H, int& U) {
         return vmi::fail(VMI_ERR_UNSUPPORTED, "%s: hidden=%d must be a multiple of %d up to 2^20", what, H, per);
     U = H / per;
     return VMI_OK;
+}
+unsigned row_groups(RowArgs& a) {   // of four waves, one a token and piece
+    a.pieces = (a.U + 63) / 64;
+    return (unsigned)(((int64_t)a.T * a.pieces + 3) / 4);
 }
 bool aligned(std::initializer_list<const void*> ps) {
     uintptr_t m = 0;
@@ -295,7 +326,8 @@ int launched(const char* what) {
 
 extern "C" size_t vmi_expert_plan_workspace_bytes(int T, int k, int num_experts) {
     if (!shape_ok(T, k) || num_experts <= 0 || num_experts > kMaxE) return 0;
-    return vmi::align256((size_t)kMaxSegments * (num_experts + 1) * 4);
+    const int nb = plan_segments((int64_t)T * k);
+    return vmi::align256(nb == 1 ? 1 : (size_t)nb * (num_experts + 1) * 4);
 }
 
 extern "C" int vmi_expert_plan(const int32_t* ids, int T, int k, int num_experts, int32_t* offsets, int32_t* source,
@@ -305,10 +337,10 @@ extern "C" int vmi_expert_plan(const int32_t* ids, int T, int k, int num_experts
     if (num_experts <= 0 || num_experts > kMaxE)
         return vmi::fail(VMI_ERR_UNSUPPORTED, "num_experts=%d must be in [1, %d]", num_experts, kMaxE);
     if (!offsets || (T && (!ids || !source || !place))) return vmi::fail(VMI_ERR_INVALID, "null ids/offsets/source/place");
-    const size_t need = vmi_expert_plan_workspace_bytes(T, k, num_experts);
-    if (!workspace || workspace_bytes < need)
-        return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes (got %zu)", need, workspace_bytes);
     const int n = T * k, nb = plan_segments(n);
+    const size_t need = vmi_expert_plan_workspace_bytes(T, k, num_experts);
+    if (nb > 1 && (!workspace || workspace_bytes < need))
+        return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes (got %zu)", need, workspace_bytes);
     PlanArgs a{ids, n, num_experts, nb == 1 ? (std::max(n, 1) + kSortThreads - 1) / kSortThreads * kSortThreads : plan_segment(n),
                static_cast<uint32_t*>(workspace), offsets, source, place, status};
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -330,7 +362,7 @@ extern "C" int vmi_expert_rows(const void* x, int dtype, int T, int k, int hidde
     a.out = static_cast<vmi_u4*>(rows);
     a.T = T;
     a.k = k;
-    hipLaunchKernelGGL(k_expert_rows, dim3((T + 3) / 4, (a.U + 63) / 64), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(k_expert_rows, dim3(row_groups(a)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
     return launched("k_expert_rows launch");
 }
 
@@ -349,7 +381,7 @@ extern "C" int vmi_expert_combine(const void* y, int dtype, int T, int k, int hi
     a.out = static_cast<vmi_u4*>(out);
     a.T = T;
     a.k = k;
-    const dim3 grid((T + 3) / 4, (a.U + 63) / 64);
+    const dim3 grid(row_groups(a));
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == VMI_F32)
         hipLaunchKernelGGL((k_expert_combine<true>), grid, dim3(256), 0, s, a);

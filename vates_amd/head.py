@@ -119,13 +119,14 @@ class _HeadLoss(torch.autograd.Function):
 
 def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor) -> torch.device:
     dev = _on_current(x)
-    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
-        raise VmiError(f"x must be [T, hidden] and weight [vocab, hidden], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    _matches(x, "x", x.shape, torch.bfloat16, dev)
-    _matches(weight, "weight", weight.shape, torch.bfloat16, dev)
+    xs, ws = x.shape, weight.shape
+    if len(xs) != 2 or len(ws) != 2 or ws[1] != xs[1]:
+        raise VmiError(f"x must be [T, hidden] and weight [vocab, hidden], got {tuple(xs)} and {tuple(ws)}")
+    _matches(x, "x", xs, torch.bfloat16, dev)
+    _matches(weight, "weight", ws, torch.bfloat16, dev)
     if targets.dtype not in (torch.int64, torch.int32):
         raise VmiError(f"targets must be int64 or int32 (got {targets.dtype})")
-    _matches(targets, "targets", (x.shape[0],), targets.dtype, dev)
+    _matches(targets, "targets", xs[:1], targets.dtype, dev)
     return dev
 
 
@@ -161,7 +162,8 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, i
 
 
 def _head_loss_on(x, weight, targets, ignore_index, status):
-    targets = targets.long()
+    if targets.dtype is not torch.int64:
+        targets = targets.long()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _HeadLoss.apply(x, weight, targets, ignore_index, status)
     return _head_loss(x, weight, targets, ignore_index, status)
@@ -191,7 +193,8 @@ def _head_loss_grad(x, weight, targets, lse, d_loss, d_lse, want_dx, dweight_dty
     T, H = x.shape
     V = weight.shape[0]
     lib = load()
-    targets = targets.long()
+    if targets.dtype is not torch.int64:
+        targets = targets.long()
     dx = torch.empty_like(x) if want_dx else None
     dw = None if dweight_dtype is None else weight.new_empty((V, H), dtype=dweight_dtype)
     ws = scratch(lib.vmi_head_loss_grad_workspace_bytes(T, H, V), x.device)

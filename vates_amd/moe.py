@@ -525,7 +525,8 @@ def _rows_dtype(t: torch.Tensor, name: str) -> int:
 
 
 def _matches(t: torch.Tensor, name: str, shape, dtype: torch.dtype, dev: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or (
+            t.shape is not shape and t.shape != shape) or t.device != dev or not t.is_contiguous():
         raise VmiError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {dev}")
 
 
@@ -538,20 +539,29 @@ def expert_plan(ids: torch.Tensor, num_experts: int, *, status: Optional[torch.T
     is any other id outside [0, num_experts), which also ORs
     VMI_STATUS_BAD_SLOT into status (int32 [1] on the device)."""
     dev = _on_current(ids)
-    if ids.dim() != 2 or ids.shape[1] == 0:
-        raise VmiError(f"ids must be [T, k], got {tuple(ids.shape)}")
-    _matches(ids, "ids", ids.shape, torch.int32, dev)
+    shape = ids.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise VmiError(f"ids must be [T, k], got {tuple(shape)}")
+    _matches(ids, "ids", shape, torch.int32, dev)
     if status is not None:
         _matches(status, "status", (1,), torch.int32, dev)
+    if not 0 < num_experts <= 1024:
+        raise VmiError(f"num_experts={num_experts} must be in [1, 1024]")
+    return _on_stream(stream, _plan, ids, num_experts, status)
+
+
+def _plan(ids: torch.Tensor, num_experts: int, status: Optional[torch.Tensor]) -> ExpertPlan:
     T, k = ids.shape
     lib = load()
-    nbytes = lib.vmi_expert_plan_workspace_bytes(T, k, num_experts)
-    buf = _like(ids, (num_experts + 1 + 2 * T * k if nbytes else 0,), torch.int32, stream)
-    offsets, source, place = buf.split([num_experts + 1, T * k, T * k]) if nbytes else (buf, buf, buf)
-    ws = scratch(nbytes, dev, stream)
+    place = torch.empty_like(ids)
+    offsets, source = ids.new_empty(num_experts + 1), ids.new_empty(T * k)
+    ws, nbytes = None, 0
+    if T * k > 8192:      # (up to there the call needs none)
+        nbytes = lib.vmi_expert_plan_workspace_bytes(T, k, num_experts)
+        ws = scratch(nbytes, ids.device)
     check(lib.vmi_expert_plan(ids.data_ptr(), T, k, num_experts, offsets.data_ptr(), source.data_ptr(), place.data_ptr(),
-                              _ptr(status), ws.data_ptr(), ws.numel(), _stream_on(dev, stream)), "vmi_expert_plan")
-    return ExpertPlan(offsets, source, place.view(T, k))
+                              _ptr(status), _ptr(ws), nbytes, _stream_on(ids.device, None)), "vmi_expert_plan")
+    return ExpertPlan(offsets, source, place)
 
 
 def _sorted_rows(x: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
@@ -574,14 +584,13 @@ def _combined(y: torch.Tensor, place: torch.Tensor, scores: Optional[torch.Tenso
 class _SortByExpert(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, place):
-        ctx.save_for_backward(place)
+        ctx.place = place     # (no input of the graph's)
         return _sorted_rows(x, place)
 
     @staticmethod
     @_once
     def backward(ctx, d_rows):
-        place, = ctx.saved_tensors
-        return _combined(d_rows.contiguous(), place, None, None), None
+        return _combined(d_rows.contiguous(), ctx.place, None, None), None
 
 
 class _CombineExperts(torch.autograd.Function):
@@ -607,10 +616,15 @@ class _CombineExperts(torch.autograd.Function):
         return d_y, None, d_scores, d_out if need_residual else None
 
 
-def _check_plan(plan: ExpertPlan, dev: torch.device) -> None:
+def _check_plan(plan: ExpertPlan, dev: torch.device):
+    """(tokens, routes of each) of a plan on `dev`."""
     if not isinstance(plan, ExpertPlan):
         raise VmiError("plan must be an ExpertPlan")
-    _matches(plan.place, "plan.place", plan.place.shape, torch.int32, dev)
+    shape = plan.place.shape
+    if len(shape) != 2:
+        raise VmiError(f"plan.place must be [T, k], got {tuple(shape)}")
+    _matches(plan.place, "plan.place", shape, torch.int32, dev)
+    return shape
 
 
 def sort_by_expert(x: torch.Tensor, plan: ExpertPlan, *, stream=None) -> torch.Tensor:
@@ -621,11 +635,12 @@ def sort_by_expert(x: torch.Tensor, plan: ExpertPlan, *, stream=None) -> torch.T
     [T * k, hidden], rows behind the last expert's are zeros.  Differentiable: a
     token's gradient is the sum of its rows', in rank order in fp32, rounded once."""
     dev = _on_current(x)
-    _check_plan(plan, dev)
-    if x.dim() != 2 or x.shape[0] != plan.tokens:
-        raise VmiError(f"x must be [{plan.tokens}, hidden], got {tuple(x.shape)}")
+    T, _ = _check_plan(plan, dev)
+    shape = x.shape
+    if len(shape) != 2 or shape[0] != T:
+        raise VmiError(f"x must be [{T}, hidden], got {tuple(shape)}")
     _rows_dtype(x, "x")
-    _matches(x, "x", x.shape, x.dtype, dev)
+    _matches(x, "x", shape, x.dtype, dev)
     if torch.is_grad_enabled() and x.requires_grad:
         return _on_stream(stream, _SortByExpert.apply, x, plan.place)
     return _on_stream(stream, _sorted_rows, x, plan.place)
@@ -641,16 +656,16 @@ def combine_experts(y: torch.Tensor, plan: ExpertPlan, scores: Optional[torch.Te
     ones), residual [T, hidden] of y's type or None.  Differentiable in y,
     scores and residual (rows without an expert get zeros)."""
     dev = _on_current(y)
-    _check_plan(plan, dev)
-    T, k = plan.place.shape
-    if y.dim() != 2 or y.shape[0] != T * k:
-        raise VmiError(f"y must be [{T * k}, hidden], got {tuple(y.shape)}")
+    T, k = _check_plan(plan, dev)
+    shape = y.shape
+    if len(shape) != 2 or shape[0] != T * k:
+        raise VmiError(f"y must be [{T * k}, hidden], got {tuple(shape)}")
     _rows_dtype(y, "y")
-    _matches(y, "y", y.shape, y.dtype, dev)
+    _matches(y, "y", shape, y.dtype, dev)
     if scores is not None:
         _matches(scores, "scores", (T, k), torch.float32, dev)
     if residual is not None:
-        _matches(residual, "residual", (T, y.shape[1]), y.dtype, dev)
+        _matches(residual, "residual", (T, shape[1]), y.dtype, dev)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, scores, residual)):
         return _on_stream(stream, _CombineExperts.apply, y, plan.place, scores, residual)
     return _on_stream(stream, _combined, y, plan.place, scores, residual)
