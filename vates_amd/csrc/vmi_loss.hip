@@ -223,7 +223,49 @@ __device__ __forceinline__ Meta ls_meta(const Meta* m) {
     return {vmi_sload_i32(p), vmi_sload_i32(p + 1), vmi_sload_i32(p + 2), vmi_sload_i32(p + 3), vmi_sload_i32(p + 4)};
 }
 
+// Up to 64 tokens every workgroup finds those in the loss by itself: lane t takes token t.
+struct Few {
+    const int64_t* target;
+    int64_t ignore;
+    int T, V;
+    const float *lse, *dloss, *dlse;   // null for the loss
+};
+// Their number; the lane's place among them or -1; y: its target.
+__device__ __forceinline__ int ls_few(const Few& f, int& place, int64_t& y) {
+    const int lane = threadIdx.x & 63;
+    y = f.target[min(lane, f.T - 1)];
+    const bool in = lane < f.T && y >= 0 && y < f.V && y != f.ignore;
+    const uint64_t all = __ballot(in);
+    place = in ? __builtin_popcountll(all & ((1ull << lane) - 1)) : -1;
+    return __builtin_popcountll(all);
+}
+// The same, their rows of x and coefficients into LDS (coefficients of `width` places: zeros behind the last).
+__device__ __forceinline__ int ls_few(const Few& f, int width, int32_t* idx, Coef* coef) {
+    const int lane = threadIdx.x & 63;
+    int place;
+    int64_t y;
+    const int nv = ls_few(f, place, y);
+    if (ls_wave() == 0) {
+        if (coef && lane >= nv && lane < width) coef[lane] = Coef{0.0f, 0.0f, __builtin_inff(), -1};
+        if (place >= 0) {
+            idx[place] = lane;
+            if (coef) {
+                Coef c{0.0f, 0.0f, 0.0f, (int32_t)y};
+                if (f.dloss) {
+                    c.b = f.dloss[lane];
+                    c.a = c.b + (f.dlse ? f.dlse[lane] : 0.0f);
+                    c.lse = f.lse[lane];
+                }
+                coef[place] = c;
+            }
+        }
+    }
+    __syncthreads();
+    return nv;
+}
+
 struct LogitArgs {
+    Few few;                     // up to 64 tokens; else meta, idx and coef
     const uint16_t *x, *w;
     const int32_t* idx;
     const Meta* meta;
@@ -252,7 +294,9 @@ struct LogitJob {
     float m[S::NB], l[S::NB];
     int m0, n0;
 
-    __device__ __forceinline__ LogitJob(const LogitArgs& a_, Coef* coef_, int nv_, int rb_, int v0_, int v1_)
+    // idx: rows of x of the tokens in the loss; coef_: filled here from `from`, unless that is null
+    __device__ __forceinline__ LogitJob(const LogitArgs& a_, const int32_t* idx, Coef* coef_, const Coef* from, int nv_, int rb_,
+                                        int v0_, int v1_)
         : a(a_), coef(coef_), nv(nv_), rb(rb_), v1(v1_) {
         nk = a.H / kBK;
         // Rows of a few KB put the pieces that all workgroups ask for at one time on few memory channels; begun at
@@ -270,12 +314,12 @@ struct LogitJob {
             int row, piece;
             ls_slot<false>(i, row, piece);
             const int c = min(rb * S::BN + row, nv - 1);
-            offb[i] = (uint32_t)(a.idx ? a.idx[c] : c) * (uint32_t)(2 * a.H) + 16 * piece;
+            offb[i] = (uint32_t)idx[c] * (uint32_t)(2 * a.H) + 16 * piece;
         }
         rows();
-        if (threadIdx.x < S::BN) {
+        if (from && threadIdx.x < S::BN) {
             const int t = rb * S::BN + threadIdx.x;
-            coef_[threadIdx.x] = t < nv ? a.coef[t] : Coef{0.0f, 0.0f, __builtin_inff(), -1};
+            coef_[threadIdx.x] = t < nv ? from[t] : Coef{0.0f, 0.0f, __builtin_inff(), -1};
         }
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
@@ -409,7 +453,8 @@ __device__ __forceinline__ void ls_join(float& m, float& l, float m2, float l2) 
 // A workgroup takes a block of tokens and a strip of the vocabulary, whose tiles follow
 // each other without a pause of the DMA.
 template <class S>
-__device__ __forceinline__ void ls_score(const LogitArgs& a, const Meta& me, uint8_t* lds, Coef* coef) {
+__device__ __forceinline__ void ls_score(const LogitArgs& a, const Meta& me, const int32_t* idx, uint8_t* lds, Coef* coef,
+                                         const Coef* from) {
     const int nrb = (me.nv + S::BN - 1) / S::BN, per = ((a.V + me.strips - 1) / me.strips + 15) & ~15;
     for (int turn = 0; turn * (int)gridDim.x < nrb * me.strips; ++turn) {
         const int item = ls_item(turn, nrb * me.strips);
@@ -422,7 +467,7 @@ __device__ __forceinline__ void ls_score(const LogitArgs& a, const Meta& me, uin
             if (threadIdx.x < S::BN) part[threadIdx.x] = make_float2(kLowest, 0.0f);
             continue;
         }
-        LogitJob<S, 0> job(a, coef, me.nv, rb, v0, v1);
+        LogitJob<S, 0> job(a, idx, coef, from, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
         float2* s_ml = reinterpret_cast<float2*>(lds);   // [WM][BN]
 #pragma unroll
@@ -444,7 +489,8 @@ __device__ __forceinline__ void ls_score(const LogitArgs& a, const Meta& me, uin
 
 // The same tiles of one piece of the vocabulary as rows of g.
 template <class S, int GRAD>
-__device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, uint8_t* lds, Coef* coef) {
+__device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, const int32_t* idx, uint8_t* lds, Coef* coef,
+                                     const Coef* from) {
     const int nrb = (me.nv + S::BN - 1) / S::BN, strips = a.last ? me.last : me.strips;
     const int per = ((a.v1 - a.v0 + strips - 1) / strips + 15) & ~15;
     for (int turn = 0; turn * (int)gridDim.x < nrb * strips; ++turn) {
@@ -454,7 +500,7 @@ __device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, uint8_t
         ls_pair(item, nrb, strips, rb, strip);
         const int v0 = a.v0 + strip * per, v1 = min(a.v1, v0 + per);
         if (v0 >= v1) continue;
-        LogitJob<S, GRAD> job(a, coef, me.nv, rb, v0, v1);
+        LogitJob<S, GRAD> job(a, idx, coef, from, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
     }
 }
@@ -475,15 +521,22 @@ __global__ __launch_bounds__(kThreads) void k_loss_logits(LogitArgs a) {
     constexpr int kBytes = WHICH == 32 ? kLds<Score32> : WHICH == 64 ? kLds<Score64> : kLds<ScoreN<160>>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
     __shared__ Coef coef[WHICH ? WHICH : 256];
-    const Meta me = ls_meta(a.meta);
+    __shared__ int32_t s_idx[WHICH ? WHICH : 1];
+    Meta me{0, WHICH, (int)gridDim.x, (int)gridDim.x, 1};   // few: one strip a workgroup, bytes bound it
+    if constexpr (WHICH)
+        me.nv = ls_few(a.few, WHICH, s_idx, coef);
+    else
+        me = ls_meta(a.meta);
     if (me.nv == 0) return;
+    const int32_t* idx = WHICH ? s_idx : a.idx;
+    const Coef* from = WHICH ? nullptr : a.coef;
     auto go = [&](auto s) {
         using S = decltype(s);
         static_assert(kLds<S> <= kBytes, "LDS");
         if constexpr (GRAD)
-            ls_g<S, GRAD>(a, me, lds, coef);
+            ls_g<S, GRAD>(a, me, idx, lds, coef, from);
         else
-            ls_score<S>(a, me, lds, coef);
+            ls_score<S>(a, me, idx, lds, coef, from);
     };
     if constexpr (WHICH == 32) {
         go(Score32{});
@@ -501,6 +554,12 @@ __global__ __launch_bounds__(kThreads) void k_loss_logits(LogitArgs a) {
 }
 
 // ------------------------------------------------------------------------ dx
+// Splits of dx's sums over the columns: as many workgroups as the grid has, of four steps at least.
+__host__ __device__ __forceinline__ int ls_splits(int grid, int blocks, int nht, int steps) {
+    const int fill = grid / (blocks * nht), deep = steps / 4, n = fill < deep ? fill : deep;
+    return n > 1 ? n : 1;
+}
+
 struct DxArgs {
     const uint16_t *w, *g;
     const Meta* meta;
@@ -508,6 +567,7 @@ struct DxArgs {
     int64_t ldg;
     float* sum;              // [split][token block rows][H]
     int add;                 // a later piece than the first: added to the sums
+    int splits;              // up to 64 tokens (else meta's)
 };
 
 template <class S>
@@ -588,13 +648,13 @@ template <int WHICH>
 __global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
     constexpr int kBytes = WHICH == 32 ? kLds<Dx32> : WHICH == 64 ? kLds<Dx64> : kLds<DxN<160>>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
-    const Meta me = ls_meta(a.meta);
-    if (me.nv == 0) return;
     if constexpr (WHICH == 32) {
-        ls_dx<Dx32>(a, 1, me.splits, lds);
+        ls_dx<Dx32>(a, 1, a.splits, lds);
     } else if constexpr (WHICH == 64) {
-        ls_dx<Dx64>(a, 1, me.splits, lds);
+        ls_dx<Dx64>(a, 1, a.splits, lds);
     } else {
+        const Meta me = ls_meta(a.meta);
+        if (me.nv == 0) return;
         auto go = [&](auto s) {
             using S = decltype(s);
             static_assert(kLds<S> <= kBytes, "LDS");
@@ -618,20 +678,21 @@ struct DwArgs {
     int H, V, v0, cols;
     int64_t ldg, ldx;
     void* dw;
-    int few;                 // tokens of g's two parts, or 0
-    const int32_t* idx;
+    Few tokens;              // where there are few: and g in two parts of `few` tokens each
+    int few;
 };
 
 template <class S, bool F32>
 struct DwJob {
     const DwArgs& a;
+    const int32_t* idx;
     int nv, nk, nht, items;
     int turn, item, step;                // asked for
     int kd, done_turn;                   // being multiplied
     uint32_t offa[S::DA], offb[S::DB];
 
-    __device__ __forceinline__ DwJob(const DwArgs& a_, int nv_, int nk_, int nht_, int items_)
-        : a(a_), nv(nv_), nk(nk_), nht(nht_), items(items_), turn(0), item(ls_item(0, items_)), step(0), kd(0), done_turn(0) {
+    __device__ __forceinline__ DwJob(const DwArgs& a_, const int32_t* idx_, int nv_, int nk_, int nht_, int items_)
+        : a(a_), idx(idx_), nv(nv_), nk(nk_), nht(nht_), items(items_), turn(0), item(ls_item(0, items_)), step(0), kd(0), done_turn(0) {
         rows();
     }
     __device__ __forceinline__ void rows() {
@@ -641,7 +702,7 @@ struct DwJob {
             int row, piece;
             ls_slot<S::ASLOW>(i, row, piece);
             if constexpr (S::ASLOW)   // few tokens, by idx (g is zero behind the last)
-                offa[i] = (uint32_t)a.idx[min(row & (a.few - 1), nv - 1)] * (uint32_t)(2 * a.H) +
+                offa[i] = (uint32_t)idx[min(row & (a.few - 1), nv - 1)] * (uint32_t)(2 * a.H) +
                           2 * min(ht * S::BM + 8 * piece, a.H - 8);
             else
                 offa[i] = (uint32_t)min(ht * S::BM + row, a.H - 1) * (uint32_t)(2 * a.ldx) + 16 * piece;
@@ -703,10 +764,19 @@ template <bool FEW, bool F32>
 __global__ __launch_bounds__(kThreads) void k_loss_dw(DwArgs a) {
     using S = Tile<256, 256, 2, 4, 2, FEW, true>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds<S>];
-    const int nv = vmi_sload_i32(&a.meta->nv), nk = nv ? ((FEW ? 2 * a.few : nv) + kBK - 1) / kBK : 0;
+    __shared__ int32_t s_idx[FEW ? kFew : 1];
+    int nv = 0;
+    if constexpr (FEW) {
+        s_idx[threadIdx.x & (kFew - 1)] = 0;
+        __syncthreads();
+        if (a.tokens.T) nv = ls_few(a.tokens, 0, s_idx, nullptr);
+    } else {
+        nv = vmi_sload_i32(&a.meta->nv);
+    }
+    const int nk = nv ? ((FEW ? 2 * a.few : nv) + kBK - 1) / kBK : 0;
     const int nht = (a.H + S::BM - 1) / S::BM, items = nht * ((a.cols + S::BN - 1) / S::BN);
     if (ls_item(0, items) < 0) return;
-    DwJob<S, F32> job(a, max(nv, 1), max(nk, 1), nht, items);
+    DwJob<S, F32> job(a, s_idx, max(nv, 1), max(nk, 1), nht, items);
     const int whole = items / (int)gridDim.x;    // turns in which every workgroup has an item; the last may leave some out
     const int mine = whole + (whole * (int)gridDim.x < items && ls_item(whole, items) >= 0 ? 1 : 0);
     if (nk == 0) {   // no token in the loss: zeros
@@ -729,7 +799,7 @@ struct RowsArgs {
     float *loss, *lse_out;         // score: written for tokens left out
     uint32_t* status;
     const float *lse, *dloss, *dlse;
-    int grid, few;                 // workgroups of the products; their block of tokens where there are few, else 0
+    int grid;                      // workgroups of the products
     int tiles, last, nht, steps;   // vocabulary tiles of a piece and of the last one, hidden tiles, dx's steps of the last piece
 };
 
@@ -751,7 +821,7 @@ __device__ __forceinline__ uint64_t ls_plan(int nrb, int bn, int tiles, int grid
     return ~vmi_wave_max_u64(~best);
 }
 
-// One workgroup: a wave takes a run of tokens, 64 at a time, eight such groups' loads together.
+// More than 64 tokens.  One workgroup: a wave takes a run of tokens, 64 at a time, eight such groups' loads together.
 __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
     __shared__ int s_sum[16];
     __shared__ uint64_t s_work[5];
@@ -809,8 +879,8 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
         }
     }
     // waves 0 to 4 weigh a width each
-    const int bn = a.few ? a.few : 256 - 32 * w, nrb = max((nv + bn - 1) / bn, 1);
-    if (!a.few && nv && bn >= 128) {
+    const int bn = 256 - 32 * w, nrb = max((nv + bn - 1) / bn, 1);
+    if (nv && bn >= 128) {
         const uint64_t p = ls_plan(nrb, bn, a.tiles, a.grid), q = ls_plan(nrb, bn, a.last, a.grid);
         if (lane == 0) {
             s_work[w] = p >> 16;
@@ -819,8 +889,8 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
     }
     __syncthreads();
     if (threadIdx.x != 0) return;
-    Meta me{nv, bn, a.grid, a.grid, 1};   // few: one strip a workgroup, bytes bound it
-    if (!a.few && nv) {
+    Meta me{nv, 256, 1, 1, 1};
+    if (nv) {
         int best = 0;
         for (int i = 1; i < 5; ++i) best = s_work[i] < s_work[best] ? i : best;
         me.bn = 256 - 32 * best;
@@ -828,17 +898,13 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
         me.last = (int)(s_cut[best] >> 16);
     }
     const int blocks = max((nv + me.bn - 1) / me.bn, 1);
-    me.splits = min(max(a.grid / (blocks * a.nht), 1), max(a.steps / 4, 1));
+    me.splits = ls_splits(a.grid, blocks, a.nht, a.steps);
     *a.meta = me;
 }
 
-// A wave per token: its strips' maxima and sums, in a fixed order.
-__global__ __launch_bounds__(256) void k_loss_merge(const Meta* meta, const int32_t* idx, const float2* part,
-                                                    const float* hit, float* loss, float* lse) {
-    const Meta me = ls_meta(meta);
-    const int c = blockIdx.x * 4 + ls_wave(), lane = threadIdx.x & 63;
-    if (c >= me.nv) return;
-    const int nrb = (me.nv + me.bn - 1) / me.bn, rb = c / me.bn;
+// The strips' maxima and sums of a token in the loss, joined by a wave in a fixed order.
+__device__ __forceinline__ void ls_merge(const Meta& me, int c, int t, const float2* part, const float* hit, float* loss, float* lse) {
+    const int lane = threadIdx.x & 63, nrb = (me.nv + me.bn - 1) / me.bn, rb = c / me.bn;
     float m = kLowest, l = 0.0f;
     for (int s = lane; s < me.strips; s += 64) {
         const float2 p = part[((size_t)s * nrb + rb) * me.bn + c % me.bn];
@@ -848,8 +914,32 @@ __global__ __launch_bounds__(256) void k_loss_merge(const Meta* meta, const int3
     for (int d = 1; d < 64; d <<= 1) ls_join(m, l, __shfl_xor(m, d), __shfl_xor(l, d));
     if (lane == 0) {
         const float v = m + logf(l);
-        lse[idx[c]] = v;
-        loss[idx[c]] = v - hit[c];
+        lse[t] = v;
+        loss[t] = v - hit[c];
+    }
+}
+// A wave per token in the loss.
+__global__ __launch_bounds__(256) void k_loss_merge(const Meta* meta, const int32_t* idx, const float2* part,
+                                                    const float* hit, float* loss, float* lse) {
+    const Meta me = ls_meta(meta);
+    const int c = blockIdx.x * 4 + ls_wave();
+    if (c < me.nv) ls_merge(me, c, idx[c], part, hit, loss, lse);
+}
+// A wave per token of few, those left out among them.
+__global__ __launch_bounds__(256) void k_loss_merge_few(Few f, int few, int strips, const float2* part, const float* hit,
+                                                        float* loss, float* lse, uint32_t* status) {
+    const int t = blockIdx.x * 4 + ls_wave();
+    int place;
+    int64_t y;
+    const int nv = ls_few(f, place, y);
+    if (t >= f.T) return;
+    const int c = __builtin_amdgcn_readlane(place, t);
+    if (c >= 0) {
+        ls_merge(Meta{nv, few, strips, strips, 1}, c, t, part, hit, loss, lse);
+    } else if ((int)(threadIdx.x & 63) == t) {
+        const bool bad = y != f.ignore;
+        loss[t] = lse[t] = bad ? __builtin_nanf("") : 0.0f;
+        if (bad && status) atomicOr(status, VMI_STATUS_BAD_TARGET);
     }
 }
 
@@ -877,20 +967,17 @@ __global__ __launch_bounds__(256) void k_loss_turn(const Meta* meta, const int32
     }
 }
 
-// dx of a token: its splits' sums in a fixed order (few: those of g's two parts, few rows
-// apart), zeros for a token left out.  A wave takes 256 hidden values; SPREAD: the
-// workgroup's four waves share one such piece's sums (few tokens, many splits: 22 -> 7 us).
+// dx of a token: the n sums of its row of `rows` in a fixed order (few: those of g's two
+// parts, few rows apart), zeros for a token left out.  A wave takes 256 hidden values;
+// SPREAD: the workgroup's four waves share one such piece's sums (few tokens, many splits: 22 -> 7 us).
 template <bool SPREAD>
-__global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int32_t* pos, const float* sum, int H, int few,
-                                                     uint16_t* dx) {
-    __shared__ vmi_f4 s_part[3][64];
-    const Meta me = ls_meta(meta);
-    const int t = blockIdx.x, c = pos[t], rows = few ? 2 * few : (me.nv + me.bn - 1) / me.bn * me.bn, w = ls_wave();
-    const int lane = threadIdx.x & 63, h = 256 * (SPREAD ? blockIdx.y : 4 * blockIdx.y + w) + 4 * lane;
+__device__ __forceinline__ void ls_dx_out(int t, int c, int n, int rows, int few, const float* sum, int H, uint16_t* dx) {
+    __shared__ vmi_f4 s_part[SPREAD ? 3 : 1][64];
+    const int lane = threadIdx.x & 63, w = ls_wave(), h = 256 * (SPREAD ? blockIdx.y : 4 * blockIdx.y + w) + 4 * lane;
     vmi_f4 v = {0.f, 0.f, 0.f, 0.f};
     if (c >= 0 && h < H) {
         constexpr int kAhead = 8;
-        const int n = few ? 2 * me.splits : me.splits, i0 = SPREAD ? n * w / 4 : 0, i1 = SPREAD ? n * (w + 1) / 4 : n;
+        const int i0 = SPREAD ? n * w / 4 : 0, i1 = SPREAD ? n * (w + 1) / 4 : n;
         for (int i = i0; i < i1; i += kAhead) {
             vmi_f4 u[kAhead];
 #pragma unroll
@@ -911,6 +998,19 @@ __global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int
     }
     if (h < H)
         *reinterpret_cast<uint2*>(dx + (size_t)t * H + h) = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
+}
+template <bool SPREAD>
+__global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int32_t* pos, const float* sum, int H, uint16_t* dx) {
+    const Meta me = ls_meta(meta);
+    const int t = blockIdx.x;
+    ls_dx_out<SPREAD>(t, pos[t], me.splits, (me.nv + me.bn - 1) / me.bn * me.bn, 0, sum, H, dx);
+}
+__global__ __launch_bounds__(256) void k_loss_dx_out_few(Few f, int few, int splits, const float* sum, int H, uint16_t* dx) {
+    int place;
+    int64_t y;
+    ls_few(f, place, y);
+    const int t = blockIdx.x;
+    ls_dx_out<true>(t, __builtin_amdgcn_readlane(place, t), 2 * splits, 2 * few, few, sum, H, dx);
 }
 
 // ---------------------------------------------------------------------- host
@@ -979,6 +1079,19 @@ bool aligned(std::initializer_list<const void*> ps, uintptr_t to) {
     return !(m & (to - 1));
 }
 
+RowsArgs rows_args(const int64_t* target, int64_t ignore, int T, int V, const Layout& l, uint8_t* ws, int grid) {
+    RowsArgs r{};
+    r.target = target;
+    r.ignore = ignore;
+    r.T = T;
+    r.V = V;
+    r.idx = reinterpret_cast<int32_t*>(ws + l.idx);
+    r.pos = reinterpret_cast<int32_t*>(ws + l.pos);
+    r.meta = reinterpret_cast<Meta*>(ws + l.meta);
+    r.coef = reinterpret_cast<Coef*>(ws + l.coef);
+    r.grid = grid;
+    return r;
+}
 template <int GRAD>
 void launch_logits(const LogitArgs& a, int few, int grid, hipStream_t s) {
     constexpr int kSmall = GRAD ? 2 : 0;   // few tokens: g in two parts
@@ -1019,34 +1132,30 @@ extern "C" int vmi_head_loss(const uint16_t* x, int T, int hidden, const uint16_
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int grid = vmi::device_cus();
-    RowsArgs r{};
-    r.target = targets;
-    r.ignore = ignore_index;
-    r.T = T;
-    r.V = vocab;
-    r.grid = grid;
-    r.few = l.few;
-    r.idx = reinterpret_cast<int32_t*>(ws + l.idx);
-    r.pos = reinterpret_cast<int32_t*>(ws + l.pos);
-    r.meta = reinterpret_cast<Meta*>(ws + l.meta);
-    r.coef = reinterpret_cast<Coef*>(ws + l.coef);
+    LogitArgs a{};
+    a.x = x;
+    a.w = weight;
+    a.H = hidden;
+    a.V = vocab;
+    a.part = reinterpret_cast<float2*>(ws + l.part);
+    a.hit = reinterpret_cast<float*>(ws + l.hit);
+    if (l.few) {
+        a.few = Few{targets, ignore_index, T, vocab, nullptr, nullptr, nullptr};
+        launch_logits<0>(a, l.few, grid, s);
+        hipLaunchKernelGGL(k_loss_merge_few, dim3((T + 3) / 4), dim3(256), 0, s, a.few, l.few, grid, a.part, a.hit, loss, lse, status);
+        return launched("k_loss_merge_few launch");
+    }
+    RowsArgs r = rows_args(targets, ignore_index, T, vocab, l, ws, grid);
     r.loss = loss;
     r.lse_out = lse;
     r.status = status;
     r.tiles = r.last = (vocab + 255) / 256;
     r.nht = r.steps = 1;
     hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
-    LogitArgs a{};
-    a.x = x;
-    a.w = weight;
     a.idx = r.idx;
     a.meta = r.meta;
     a.coef = r.coef;
-    a.H = hidden;
-    a.V = vocab;
-    a.part = reinterpret_cast<float2*>(ws + l.part);
-    a.hit = reinterpret_cast<float*>(ws + l.hit);
-    launch_logits<0>(a, l.few, grid, s);
+    launch_logits<0>(a, 0, grid, s);
     hipLaunchKernelGGL(k_loss_merge, dim3((T + 3) / 4), dim3(256), 0, s, r.meta, r.idx, a.part, a.hit, loss, lse);
     return launched("k_loss_merge launch");
 }
@@ -1074,17 +1183,7 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int grid = vmi::device_cus();
-    RowsArgs r{};
-    r.target = targets;
-    r.ignore = ignore_index;
-    r.T = T;
-    r.V = vocab;
-    r.grid = grid;
-    r.few = l.few;
-    r.idx = reinterpret_cast<int32_t*>(ws + l.idx);
-    r.pos = reinterpret_cast<int32_t*>(ws + l.pos);
-    r.meta = reinterpret_cast<Meta*>(ws + l.meta);
-    r.coef = reinterpret_cast<Coef*>(ws + l.coef);
+    RowsArgs r = rows_args(targets, ignore_index, T, vocab, l, ws, grid);
     r.lse = lse;
     r.dloss = d_loss;
     r.dlse = d_lse;
@@ -1092,11 +1191,14 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     r.last = ((vocab - 1) % l.piece + 256) / 256;
     r.nht = (hidden + 255) / 256;
     r.steps = r.last * 256 / kBK;
-    hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
+    if (!l.few) hipLaunchKernelGGL(k_loss_rows, dim3(1), dim3(1024), 0, s, r);
+    const Few few{targets, ignore_index, T, vocab, lse, d_loss, d_lse};
+    const int splits = ls_splits(grid, 1, r.nht, r.steps);
     uint16_t* xt = reinterpret_cast<uint16_t*>(ws + l.x);
     if (dweight && !l.few)
         hipLaunchKernelGGL(k_loss_turn, dim3(l.rows / 64, hidden / 64), dim3(256), 0, s, r.meta, r.idx, x, hidden, l.ldx, xt);
     LogitArgs a{};
+    a.few = few;
     a.x = x;
     a.w = weight;
     a.idx = r.idx;
@@ -1107,6 +1209,7 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     a.g = reinterpret_cast<uint16_t*>(ws + l.g);
     a.ldg = l.ldg;
     DxArgs d{};
+    d.splits = splits;
     d.w = weight;
     d.g = a.g;
     d.meta = r.meta;
@@ -1117,7 +1220,7 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     DwArgs u{};
     u.x = l.few ? x : xt;
     u.ldx = l.ldx;
-    u.idx = r.idx;
+    u.tokens = few;
     u.few = l.few;
     u.g = a.g;
     u.meta = r.meta;
@@ -1150,12 +1253,14 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
         }
     }
     if (dx && T) {
-        if (T <= 1024)
-            hipLaunchKernelGGL(k_loss_dx_out<true>, dim3(T, (hidden + 255) / 256), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden,
-                               l.few, dx);
+        if (l.few)
+            hipLaunchKernelGGL(k_loss_dx_out_few, dim3(T, (hidden + 255) / 256), dim3(256), 0, s, few, l.few, splits, d.sum,
+                               hidden, dx);
+        else if (T <= 1024)
+            hipLaunchKernelGGL(k_loss_dx_out<true>, dim3(T, (hidden + 255) / 256), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden, dx);
         else
             hipLaunchKernelGGL(k_loss_dx_out<false>, dim3(T, (hidden + 1023) / 1024), dim3(256), 0, s, r.meta, r.pos, d.sum,
-                               hidden, l.few, dx);
+                               hidden, dx);
     }
     return launched("vmi_head_loss_grad launch");
 }
