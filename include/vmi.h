@@ -603,8 +603,9 @@ int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x,
  * d_loss, d_lse f32 [T] (d_lse may be NULL: zeros).  Tokens left out of the loss
  * (ignore_index, or outside the vocabulary) have no gradient and add none.  z is
  * formed again, a piece of the vocabulary at a time; g is rounded to bf16 as
- * the operand of the two products, whose sums are fp32, rounded once.  Sums
- * run in a fixed order: the same call gives the same bits.
+ * the operand of the two products (up to 64 tokens in two parts, 16 bits), whose sums are
+ * fp32, rounded once.  Sums run in a fixed order, which depends on T and on how many
+ * tokens are in the loss: the same call gives the same bits.
  * T <= 65536 (0: nothing but a dweight of zeros), hidden a multiple of 64 up to
  * 8192, vocab <= 2^21, pointers 16-byte aligned (targets 8).  workspace: the query's bytes
  * (0: a form that is not built), 256-byte aligned, nothing kept between calls.
@@ -642,7 +643,7 @@ int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const uint16_t* wei
  * without an expert), d_scores[t][j] = d_out[t] . y[place[t][j]] (0 there) in fp32, in a fixed
  * order; d_y or d_scores may be NULL (y is read for d_scores only).
  * x, out, residual, d_out [T, hidden] and rows, y, d_y [T k, hidden] of dtype (VMI_BF16,
- * hidden a multiple of 8, or VMI_F32, of 4), 16-byte aligned; k <= 32, T k <= 2^24; T may be 0.
+ * hidden a multiple of 8, or VMI_F32, of 4), 16-byte aligned; T <= 65536 (0 among them), k <= 32.
  * Outputs must not overlap inputs.  A place past T k reads and writes nothing.
  * ------------------------------------------------------------------------ */
 size_t vmi_expert_plan_workspace_bytes(int T, int k, int num_experts);

@@ -58,7 +58,7 @@ def test_loss_workspaces(lib):
 
 def test_expert_refusals(lib):
     plan = lambda T=4, k=2, E=8, ids=P, o=P, s=P, p=P, ws=P, n=1 << 20: lib.vmi_expert_plan(ids, T, k, E, o, s, p, None, ws, n, None)
-    for kw in ({"T": -1}, {"k": 0}, {"k": 33}, {"T": 1 << 23, "k": 3}, {"ids": None}, {"o": None}, {"s": None}, {"p": None}):
+    for kw in ({"T": -1}, {"k": 0}, {"k": 33}, {"T": 65537}, {"ids": None}, {"o": None}, {"s": None}, {"p": None}):
         assert plan(**kw) == L.VMI_ERR_INVALID, kw
     for E in (0, -1, 1025):
         assert plan(E=E) == L.VMI_ERR_UNSUPPORTED and lib.vmi_expert_plan_workspace_bytes(4, 2, E) == 0
@@ -75,7 +75,7 @@ def test_expert_refusals(lib):
         return lib.vmi_expert_combine_grad(x, None, dt, T, k, H, p, None, r, ds, None)
 
     for call in (rows, combine, grad):
-        for kw in ({"T": -1}, {"k": 0}, {"k": 33}, {"T": 1 << 24}, {"x": None}, {"p": None}, {"x": P + 8}, {"r": P + 4}, {"r": None}):
+        for kw in ({"T": -1}, {"k": 0}, {"k": 33}, {"T": 65537}, {"x": None}, {"p": None}, {"x": P + 8}, {"r": P + 4}, {"r": None}):
             assert call(**kw) == L.VMI_ERR_INVALID, (call, kw)
         for kw in ({"H": 0}, {"H": 12}, {"H": 6, "dt": L.VMI_F32}, {"dt": 2}, {"H": (1 << 20) + 8}):
             assert call(**kw) == L.VMI_ERR_UNSUPPORTED, (call, kw)

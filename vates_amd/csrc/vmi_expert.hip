@@ -21,7 +21,7 @@
 
 namespace {
 
-constexpr int kMaxE = 1024, kMaxK = 32;
+constexpr int kMaxE = 1024, kMaxK = 32, kMaxT = 65536;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kChunks = 8;                               // groups of 64 routes of a wave
 constexpr int kWhole = kSortThreads * kChunks;           // routes of a workgroup at most
@@ -296,12 +296,12 @@ __global__ __launch_bounds__(256) void k_expert_grad(RowArgs a) {
 int plan_segment(int64_t n) { return n <= kWhole || n > 16 * kWhole ? kWhole : kWhole / 4; }
 int plan_segments(int64_t n) { return (int)std::max<int64_t>(1, (n + plan_segment(n) - 1) / plan_segment(n)); }
 
-bool shape_ok(int T, int k) { return T >= 0 && k > 0 && k <= kMaxK && (int64_t)T * k <= (1 << 24); }
+bool shape_ok(int T, int k) { return T >= 0 && T <= kMaxT && k > 0 && k <= kMaxK; }
 
 // Checks what the row entries share; U: 16-byte units of a row.
 int rows_check(const char* what, int dtype, int T, int k, int H, int& U) {
     if (dtype != VMI_F32 && dtype != VMI_BF16) return vmi::fail(VMI_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
-    if (!shape_ok(T, k)) return vmi::fail(VMI_ERR_INVALID, "%s: T=%d k=%d (k <= %d, T k <= 2^24)", what, T, k, kMaxK);
+    if (!shape_ok(T, k)) return vmi::fail(VMI_ERR_INVALID, "%s: T=%d k=%d (T <= %d, k <= %d)", what, T, k, kMaxT, kMaxK);
     const int per = dtype == VMI_F32 ? 4 : 8;
     if (H <= 0 || H % per || H > (1 << 20))
         return vmi::fail(VMI_ERR_UNSUPPORTED, "%s: hidden=%d must be a multiple of %d up to 2^20", what, H, per);
@@ -333,7 +333,7 @@ extern "C" size_t vmi_expert_plan_workspace_bytes(int T, int k, int num_experts)
 extern "C" int vmi_expert_plan(const int32_t* ids, int T, int k, int num_experts, int32_t* offsets, int32_t* source,
                                int32_t* place, uint32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
     vmi::clear_error();
-    if (!shape_ok(T, k)) return vmi::fail(VMI_ERR_INVALID, "T=%d k=%d (k <= %d, T k <= 2^24)", T, k, kMaxK);
+    if (!shape_ok(T, k)) return vmi::fail(VMI_ERR_INVALID, "T=%d k=%d (T <= %d, k <= %d)", T, k, kMaxT, kMaxK);
     if (num_experts <= 0 || num_experts > kMaxE)
         return vmi::fail(VMI_ERR_UNSUPPORTED, "num_experts=%d must be in [1, %d]", num_experts, kMaxE);
     if (!offsets || (T && (!ids || !source || !place))) return vmi::fail(VMI_ERR_INVALID, "null ids/offsets/source/place");

@@ -12,14 +12,26 @@
 // 256 x 256 (less where there are few tokens) on 16 x 16 x 32 bf16 matrix
 // instructions, 64 of k a step, both operands by DMA into LDS while the step before is
 // multiplied:
-//   k_loss_score, k_loss_g   m a vocabulary row, n a token, k a hidden value
-//   k_loss_dx                m a hidden value,   n a token, k a vocabulary row
-//   k_loss_dw                m a hidden value,   n a vocabulary row, k a token
+//   k_loss_logits   m a vocabulary row, n a token, k a hidden value: maxima and sums, or g
+//   k_loss_dx       m a hidden value,   n a token, k a vocabulary row
+//   k_loss_dw       m a hidden value,   n a vocabulary row, k a token
 // An operand whose rows run along k lies in LDS as rows of 64 values, 16-byte pieces
-// at piece ^ (row & 7); one whose rows run along m or n (W for dx; x and g for dW) as
+// at piece ^ (row & 7); one whose rows run along m or n (W for dx, g for dW) as
 // it is in memory, 32-byte pieces at piece ^ (k & 7), and ds_read_b64_tr_b16 turns 4 x 16
 // values as they are read.  Both placements read without bank conflicts (4.7 and 4.3 cycles an
 // instruction, as consecutive addresses do; rows unturned 12.6 and 16).
+//
+// g is rounded to bf16, the type of the matrix instruction's other operand (W, x): half a step is
+// 2^-9 of its value, as much as the outputs' own rounding.  Up to 64 tokens, where the head's
+// bytes are the bound, what that leaves is multiplied too, in a second bf16.
+//
+// What bounds it (MI355X, 151,936 x 2048): one token 99 us, 6.7 TB/s of the head's bytes in the kernel
+// (a read reaches 7.2); 8192 tokens 4.0 ms, 1.28 PFLOP/s; a step of 4096 with both gradients 8.9 ms,
+// 1.15 PFLOP/s with z formed twice (a library product of these shapes 1.35 to 1.57): the matrix cores are busy 56 % of
+// the cycles at 1.9 GHz, the library's 74 % at 1.6 (power).  Tried and slower: 32 of k a step in four or
+// five stages (8192 tokens +7 %), 32 x 32 x 16 instructions (+6 %), a SIMD's two waves by turns in four phases a step
+// (+10 %), operands read half a step ahead (spills at 256 registers), four waves of 128 x 128 (spills), tiles of 128 or 192
+// vocabulary rows with three stages for some hundred tokens (+8 to 15 %).
 //
 // Kernels beside them:
 //   k_loss_rows     the tokens in the loss, and their coefficients
@@ -1027,6 +1039,8 @@ struct Layout {
     size_t idx, pos, meta, coef, part, hit, x, g, sum, bytes;
 };
 
+int workgroups() { return std::max(8, vmi::device_cus() & ~7); }   // one a CU, alike on the eight XCDs
+
 bool form_ok(int T, int H, int V) {
     return T >= 0 && T <= kMaxT && H > 0 && H % kBK == 0 && H <= kMaxH && V > 0 && V <= kMaxV;
 }
@@ -1035,7 +1049,7 @@ Layout carve(int T, int H, int V, bool grad) {
     Layout l{};
     l.few = T <= kFewest ? kFewest : T <= kFew ? kFew : 0;
     l.rows = l.few ? 2 * l.few : (T + 255 + 63) / 64 * 64;   // whole blocks of any width end below T + 256
-    const int cus = vmi::device_cus();
+    const int cus = workgroups();
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t p = at;
@@ -1136,7 +1150,7 @@ extern "C" int vmi_head_loss(const uint16_t* x, int T, int hidden, const uint16_
         return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes, 256-byte aligned (got %zu)", l.bytes, workspace_bytes);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int grid = vmi::device_cus();
+    const int grid = workgroups();
     LogitArgs a{};
     a.x = x;
     a.w = weight;
@@ -1187,7 +1201,7 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
         return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes, 256-byte aligned (got %zu)", l.bytes, workspace_bytes);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int grid = vmi::device_cus();
+    const int grid = workgroups();
     RowsArgs r = rows_args(targets, ignore_index, T, vocab, l, ws, grid);
     r.lse = lse;
     r.dloss = d_loss;

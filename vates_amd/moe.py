@@ -499,10 +499,14 @@ class ExpertPlan:
 
 
 def _on_stream(stream, fn, *args):
-    """fn(*args) on `stream`: what autograd records then runs backward there too."""
+    """fn(*args) on `stream`: what autograd records then runs backward there too.  The
+    tensors among args are not handed out again before that stream is done with them."""
     if stream is None:
         return fn(*args)
     with torch.cuda.stream(stream):
+        for t in args:
+            if isinstance(t, torch.Tensor):
+                t.record_stream(stream)
         return fn(*args)
 
 
