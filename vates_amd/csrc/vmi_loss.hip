@@ -164,14 +164,22 @@ __device__ __forceinline__ void ls_multiply(const uint8_t* lds, vmi_f4 (&acc)[S:
 #pragma unroll
     for (int kk = 0; kk < kBK / 32; ++kk) {
         vmi_u4 a[S::MB], b[S::NB];
+        // by pairs, each product once both its operands are there
+        constexpr int kMost = S::MB > S::NB ? S::MB : S::NB;
 #pragma unroll
-        for (int n = 0; n < S::NB; ++n) b[n] = ls_operand<S::BSLOW>(lds + S::kA, n0 + 16 * n, kk);
+        for (int i = 0; i < kMost; ++i) {
+            if (i < S::MB) a[i] = ls_operand<S::ASLOW>(lds, m0 + 16 * i, kk);
+            if (i < S::NB) b[i] = ls_operand<S::BSLOW>(lds + S::kA, n0 + 16 * i, kk);
+        }
 #pragma unroll
-        for (int m = 0; m < S::MB; ++m) a[m] = ls_operand<S::ASLOW>(lds, m0 + 16 * m, kk);
+        for (int i = 0; i < kMost; ++i) {
 #pragma unroll
-        for (int m = 0; m < S::MB; ++m)
-#pragma unroll
-            for (int n = 0; n < S::NB; ++n) acc[m][n] = vmi_mfma_bf16(a[m], b[n], acc[m][n]);
+            for (int j = 0; j < i; ++j) {
+                if (i < S::MB && j < S::NB) acc[i][j] = vmi_mfma_bf16(a[i], b[j], acc[i][j]);
+                if (i < S::NB && j < S::MB) acc[j][i] = vmi_mfma_bf16(a[j], b[i], acc[j][i]);
+            }
+            if (i < S::MB && i < S::NB) acc[i][i] = vmi_mfma_bf16(a[i], b[i], acc[i][i]);
+        }
     }
 }
 template <class S>
