@@ -854,17 +854,28 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
     const int lane = threadIdx.x & 63, w = ls_wave(), run = (a.T + 1023) / 1024 * 64;
     const int t0 = min(a.T, w * run), t1 = min(a.T, t0 + run);
     constexpr int kAhead = 8;
-    int n = 0;
-    bool bad = false;
-    for (int t = t0; t < t1; t += 64 * kAhead) {
-        int64_t y[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) y[i] = a.target[min(t + 64 * i + lane, a.T - 1)];
+    int64_t y[kAhead];
+    Coef k[kAhead];
+    auto load = [&](int t, bool coef) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const bool here = t + 64 * i + lane < t1, in = here && y[i] >= 0 && y[i] < a.V && y[i] != a.ignore;
-            n += __builtin_popcountll(__ballot(in));
-            bad |= here && !in && y[i] != a.ignore;
+            const int at = min(t + 64 * i + lane, a.T - 1);
+            y[i] = a.target[at];
+            k[i] = Coef{0.0f, 0.0f, 0.0f, 0};
+            if (coef && a.dloss) k[i] = Coef{a.dlse ? a.dlse[at] : 0.0f, a.dloss[at], a.lse[at], 0};
+        }
+    };
+    auto in = [&](int i) { return y[i] >= 0 && y[i] < a.V && y[i] != a.ignore; };
+    int n = 0;
+    bool bad = false;
+    // (backward, so that the first groups, all there are up to 8192 tokens, are still held when they are placed)
+    for (int t = t0 + (t1 - t0 - 1) / (64 * kAhead) * (64 * kAhead); t >= t0 && t < t1; t -= 64 * kAhead) {
+        load(t, t == t0);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const bool here = t + 64 * i + lane < t1;
+            n += __builtin_popcountll(__ballot(here && in(i)));
+            bad |= here && !in(i) && y[i] != a.ignore;
         }
     }
     if (a.status && __any(bad) && lane == 0) atomicOr(a.status, VMI_STATUS_BAD_TARGET);
@@ -876,24 +887,16 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
         nv += s_sum[i];
     }
     for (int t = t0; t < t1; t += 64 * kAhead) {
-        int64_t y[kAhead];
-        Coef k[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int at = min(t + 64 * i + lane, a.T - 1);
-            y[i] = a.target[at];
-            k[i] = Coef{0.0f, 0.0f, 0.0f, 0};
-            if (a.dloss) k[i] = Coef{a.dlse ? a.dlse[at] : 0.0f, a.dloss[at], a.lse[at], 0};
-        }
+        if (t != t0) load(t, true);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int at = t + 64 * i + lane;
-            const bool here = at < t1, in = here && y[i] >= 0 && y[i] < a.V && y[i] != a.ignore;
-            const uint64_t all = __ballot(in);
+            const bool here = at < t1;
+            const uint64_t all = __ballot(here && in(i));
             const int mine = c + __builtin_popcountll(all & ((1ull << lane) - 1));
             c += __builtin_popcountll(all);
-            if (here) a.pos[at] = in ? mine : -1;
-            if (in) {
+            if (here) a.pos[at] = in(i) ? mine : -1;
+            if (here && in(i)) {
                 a.idx[mine] = at;
                 k[i].a += k[i].b;
                 k[i].target = (int32_t)y[i];
@@ -906,7 +909,7 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
     // waves 0 to 4 weigh a width each
     const int bn = 256 - 32 * w, nrb = max((nv + bn - 1) / bn, 1);
     if (nv && bn >= 128) {
-        const uint64_t p = ls_plan(nrb, bn, a.tiles, a.grid), q = ls_plan(nrb, bn, a.last, a.grid);
+        const uint64_t p = ls_plan(nrb, bn, a.tiles, a.grid), q = a.last == a.tiles ? p : ls_plan(nrb, bn, a.last, a.grid);
         if (lane == 0) {
             s_work[w] = p >> 16;
             s_cut[w] = (uint32_t)(p & 0xffffu) | (uint32_t)(q & 0xffffu) << 16;
@@ -994,7 +997,7 @@ __global__ __launch_bounds__(256) void k_loss_turn(const Meta* meta, const int32
 
 // dx of a token: the n sums of its row of `rows` in a fixed order (few: those of g's two
 // parts, few rows apart), zeros for a token left out.  A wave takes 256 hidden values;
-// SPREAD: the workgroup's four waves share one such piece's sums (few tokens, many splits: 22 -> 7 us).
+// SPREAD: the workgroup's four waves share one such piece's sums (few tokens of many splits: 22 -> 7 us; with 200 tokens both take 19).
 template <bool SPREAD>
 __device__ __forceinline__ void ls_dx_out(int t, int c, int n, int rows, int few, const float* sum, int H, uint16_t* dx) {
     __shared__ vmi_f4 s_part[SPREAD ? 3 : 1][64];
@@ -1024,11 +1027,10 @@ __device__ __forceinline__ void ls_dx_out(int t, int c, int n, int rows, int few
     if (h < H)
         *reinterpret_cast<uint2*>(dx + (size_t)t * H + h) = make_uint2(vmi_pack_bf16x2(v[0], v[1]), vmi_pack_bf16x2(v[2], v[3]));
 }
-template <bool SPREAD>
 __global__ __launch_bounds__(256) void k_loss_dx_out(const Meta* meta, const int32_t* pos, const float* sum, int H, uint16_t* dx) {
     const Meta me = ls_meta(meta);
     const int t = blockIdx.x;
-    ls_dx_out<SPREAD>(t, pos[t], me.splits, (me.nv + me.bn - 1) / me.bn * me.bn, 0, sum, H, dx);
+    ls_dx_out<false>(t, pos[t], me.splits, (me.nv + me.bn - 1) / me.bn * me.bn, 0, sum, H, dx);
 }
 __global__ __launch_bounds__(256) void k_loss_dx_out_few(Few f, int few, int splits, const float* sum, int H, uint16_t* dx) {
     int place;
@@ -1283,11 +1285,8 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
         if (l.few)
             hipLaunchKernelGGL(k_loss_dx_out_few, dim3(T, (hidden + 255) / 256), dim3(256), 0, s, few, l.few, splits, d.sum,
                                hidden, dx);
-        else if (T <= 1024)
-            hipLaunchKernelGGL(k_loss_dx_out<true>, dim3(T, (hidden + 255) / 256), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden, dx);
         else
-            hipLaunchKernelGGL(k_loss_dx_out<false>, dim3(T, (hidden + 1023) / 1024), dim3(256), 0, s, r.meta, r.pos, d.sum,
-                               hidden, dx);
+            hipLaunchKernelGGL(k_loss_dx_out, dim3(T, (hidden + 1023) / 1024), dim3(256), 0, s, r.meta, r.pos, d.sum, hidden, dx);
     }
     return launched("vmi_head_loss_grad launch");
 }
