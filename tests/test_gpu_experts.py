@@ -85,7 +85,8 @@ def test_plan_of_one_expert_and_of_none(gpu):
 
 SHAPES = [(1, 1, 1, 8, "bf16", 0), (1, 10, 512, 2048, "bf16", 0), (4, 10, 512, 2048, "bf16", 4), (3, 3, 5, 4, "f32", 2),
           (33, 4, 16, 1000, "bf16", 50), (130, 2, 8, 1000, "f32", 0), (257, 8, 64, 512, "f32", 100), (777, 10, 512, 2048, "bf16", 640),
-          (65, 17, 32, 264, "bf16", 9), (20, 32, 40, 8200, "bf16", 1), (2000, 8, 64, 64, "bf16", 16000)]
+          (65, 17, 32, 264, "bf16", 9), (20, 32, 40, 8200, "bf16", 1), (2000, 8, 64, 64, "bf16", 16000),
+          (9000, 16, 64, 1024, "bf16", 5), (9000, 16, 64, 512, "f32", 5)]   # (rows of more than 256 MB)
 
 
 @pytest.mark.parametrize("T,k,E,H,dt,dropped", SHAPES)
