@@ -99,6 +99,25 @@ def test_loss_and_gradients(gpu, T, H, V):
     assert none is None and torch.equal(dx2, dx)
 
 
+@pytest.mark.parametrize("T,V", [(20, 1003), (64, 1003), (150, 5000), (150, 60000), (185, 60000), (215, 60000), (470, 60000),
+                                 (777, 60000), (1000, 60000)])
+def test_workspaces_that_held_anything(gpu, monkeypatch, T, V):
+    """A workspace of NaNs: nothing of it is read before it is written, at every width of a
+    block (128 tokens with 5,000 rows, 160 to 256 with 60,000), whole steps of 64 tokens or not."""
+    import torch
+    import vates_amd.head as head
+    log(f"case: workspaces of NaNs T={T} V={V}")
+    monkeypatch.setattr(head, "scratch", lambda n, dev: torch.full((n,), 255, dtype=torch.uint8, device=dev))
+    x, w, y, a, b = _inputs(gpu, T, 128, V, ignored=0)
+    loss, lse = head.head_loss(x, w, y)
+    dx, dw = head.head_loss_grad(x, w, y, lse, a, b)
+    ref = _reference(x, w, y, a, b, V)
+    _within(loss, ref["loss"], "loss")
+    _within(lse, ref["lse"], "lse")
+    _within(dx, ref["dx"], "dx")
+    _within(dw, ref["dw"], "dweight", 2.0 ** -8)
+
+
 def test_several_pieces(gpu, monkeypatch):
     """A vocabulary of several pieces, the last one short: tokens enough that g of all
     of it passes 256 MB."""

@@ -527,6 +527,11 @@ __device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, const i
         if (v0 >= v1) continue;
         LogitJob<S, GRAD> job(a, idx, coef, from, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
+        // blocks of 160 or 224 tokens may end inside dW's last step of 64: its rows behind them are zeros
+        if (S::BN % kBK && rb == nrb - 1)
+            for (int r = nrb * S::BN; r < (me.nv + kBK - 1) / kBK * kBK; ++r)
+                for (int c = v0 - a.v0 + 8 * (int)threadIdx.x; c < v1 - a.v0; c += 8 * kThreads)
+                    *reinterpret_cast<vmi_u4*>(a.g + r * a.ldg + c) = vmi_u4{0, 0, 0, 0};
     }
 }
 
