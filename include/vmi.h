@@ -643,7 +643,7 @@ int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const uint16_t* wei
  * without an expert), d_scores[t][j] = d_out[t] . y[place[t][j]] (0 there) in fp32, in a fixed
  * order; d_y or d_scores may be NULL (y is read for d_scores only).
  * x, out, residual, d_out [T, hidden] and rows, y, d_y [T k, hidden] of dtype (VMI_BF16,
- * hidden a multiple of 8, or VMI_F32, of 4), 16-byte aligned; T <= 65536 (0 among them), k <= 32.
+ * hidden a multiple of 8, or VMI_F32, of 4, up to 65536), 16-byte aligned; T <= 65536 (0: nothing), k <= 32.
  * Outputs must not overlap inputs.  A place past T k reads and writes nothing.
  * ------------------------------------------------------------------------ */
 size_t vmi_expert_plan_workspace_bytes(int T, int k, int num_experts);

@@ -169,6 +169,51 @@ def test_gradients_with_strides(gpu):
     out.sum().backward()
 
 
+def test_gradients_off_16_bytes(gpu):
+    """Gradients that begin anywhere in their storage, as behind a concatenation."""
+    import torch
+    from vates_amd.moe import combine_experts, expert_plan, sort_by_expert
+    T, k, H = 5, 3, 64
+    log("case: gradients off 16 bytes")
+    ids = _ids(gpu, T, k, 4, 2)
+    plan = expert_plan(ids, 4)
+    g = torch.Generator(device=gpu).manual_seed(3)
+    for dt in (torch.bfloat16, torch.float32):
+        make = lambda *s: torch.randn(s, generator=g, device=gpu).to(dt).requires_grad_()
+        x, y, s = make(T, H), make(T * k, H), torch.rand((T, k), generator=g, device=gpu).requires_grad_()
+        one = torch.ones(1, dtype=dt, device=gpu)
+        for out, leaves in ((sort_by_expert(x, plan), (x,)), (combine_experts(y, plan, s), (y, s))):
+            d = torch.randn(out.numel() + 1, generator=g, device=gpu).to(dt)
+            got = torch.autograd.grad(torch.cat([one, out.reshape(-1)]), leaves, d, retain_graph=True)
+            want = torch.autograd.grad(out, leaves, d[1:].clone().view(out.shape))
+            assert all(torch.equal(i, j) for i, j in zip(got, want))
+
+
+def test_no_tokens(gpu):
+    import torch
+    from vates_amd.moe import combine_experts, expert_plan, sort_by_expert
+    log("case: no tokens")
+    plan = expert_plan(torch.empty((0, 3), dtype=torch.int32, device=gpu), 4)
+    x = torch.empty((0, 64), dtype=torch.bfloat16, device=gpu, requires_grad=True)
+    s = torch.empty((0, 3), device=gpu, requires_grad=True)
+    out = combine_experts(sort_by_expert(x, plan), plan, s, residual=x)
+    dx, ds = torch.autograd.grad(out.sum(), (x, s))
+    assert out.shape == dx.shape == (0, 64) and ds.shape == (0, 3)
+
+
+def test_a_plan_changed_before_backward_is_refused(gpu):
+    import torch
+    from vates_amd.moe import combine_experts, expert_plan, sort_by_expert
+    log("case: plan changed")
+    for call, n in ((sort_by_expert, 4), (combine_experts, 8)):
+        plan = expert_plan(_ids(gpu, 4, 2, 3), 3)
+        x = torch.ones((n, 64), dtype=torch.bfloat16, device=gpu, requires_grad=True)
+        out = call(x, plan)
+        plan.place.copy_(plan.place.flip(0))
+        with pytest.raises(RuntimeError):
+            out.sum().backward()
+
+
 def test_past_32_bits(gpu):
     """Rows whose elements' numbers pass 2^32."""
     import torch

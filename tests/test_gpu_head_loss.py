@@ -118,6 +118,20 @@ def test_workspaces_that_held_anything(gpu, monkeypatch, T, V):
     _within(dw, ref["dw"], "dweight", 2.0 ** -8)
 
 
+def test_no_tokens(gpu):
+    """Without a token: empty outputs and gradients, a head's gradient of zeros; a frozen head too."""
+    import torch
+    from vates_amd.head import head_loss
+    log("case: no tokens")
+    for frozen in (False, True):
+        x = torch.empty((0, 64), dtype=torch.bfloat16, device=gpu, requires_grad=True)
+        w = torch.ones((9, 64), dtype=torch.bfloat16, device=gpu, requires_grad=not frozen)
+        loss, lse = head_loss(x, w, torch.empty(0, dtype=torch.int64, device=gpu))
+        assert loss.shape == lse.shape == (0,)
+        got = torch.autograd.grad(loss.sum() + lse.sum(), (x,) if frozen else (x, w))
+        assert got[0].shape == (0, 64) and (frozen or not got[1].any())
+
+
 def test_several_pieces(gpu, monkeypatch):
     """A vocabulary of several pieces, the last one short: tokens enough that g of all
     of it passes 256 MB."""

@@ -126,3 +126,24 @@ def test_python_refusals_on_the_device(gpu):
         with pytest.raises(L.VmiError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_calls_without_tokens(lib):
+    """Empty tensors have null pointers: no token is no error, whichever gradient is wanted."""
+    assert _grad(lib, T=0, x=None, y=None, lse=None, d=None, dx=None, dw=None, ws=None, n=0) == L.VMI_OK
+    assert lib.vmi_expert_combine_grad(None, None, L.VMI_BF16, 0, 2, 64, None, None, None, None, None) == L.VMI_OK
+
+
+def test_hidden_sizes_past_a_launch(lib):
+    """65,536 rows of these would pass the threads of one launch."""
+    for H in ((1 << 16) + 8, 1 << 20):
+        assert lib.vmi_expert_rows(P, L.VMI_BF16, 4, 2, H, P, P, None) == L.VMI_ERR_UNSUPPORTED
+        assert lib.vmi_expert_combine(P, L.VMI_BF16, 4, 2, H, P, None, None, P, None) == L.VMI_ERR_UNSUPPORTED
+
+
+def test_a_tiled_head_is_refused():
+    from vates_amd.head import TiledHead, head_loss, head_loss_grad
+    head = object.__new__(TiledHead)
+    for call in (lambda: head_loss(None, head, None), lambda: head_loss_grad(None, head, None, None, None)):
+        with pytest.raises(L.VmiError, match="row-major"):
+            call()

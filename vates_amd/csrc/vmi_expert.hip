@@ -21,7 +21,7 @@
 
 namespace {
 
-constexpr int kMaxE = 1024, kMaxK = 32, kMaxT = 65536;
+constexpr int kMaxE = 1024, kMaxK = 32, kMaxT = 65536, kMaxH = 65536;   // (kMaxT rows of kMaxH: 2^30 threads)
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kChunks = 8;                               // groups of 64 routes of a wave
 constexpr int kWhole = kSortThreads * kChunks;           // routes of a workgroup at most
@@ -315,8 +315,8 @@ int rows_check(const char* what, int dtype, int T, int k, int H, int& U) {
     if (dtype != VMI_F32 && dtype != VMI_BF16) return vmi::fail(VMI_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
     if (!shape_ok(T, k)) return vmi::fail(VMI_ERR_INVALID, "%s: T=%d k=%d (T <= %d, k <= %d)", what, T, k, kMaxT, kMaxK);
     const int per = dtype == VMI_F32 ? 4 : 8;
-    if (H <= 0 || H % per || H > (1 << 20))
-        return vmi::fail(VMI_ERR_UNSUPPORTED, "%s: hidden=%d must be a multiple of %d up to 2^20", what, H, per);
+    if (H <= 0 || H % per || H > kMaxH)
+        return vmi::fail(VMI_ERR_UNSUPPORTED, "%s: hidden=%d must be a multiple of %d up to %d", what, H, per, kMaxH);
     U = H / per;
     return VMI_OK;
 }
@@ -413,8 +413,8 @@ extern "C" int vmi_expert_combine_grad(const void* d_out, const void* y, int dty
     vmi::clear_error();
     RowArgs a{};
     if (const int rc = rows_check("vmi_expert_combine_grad", dtype, T, k, hidden, a.U)) return rc;
+    if (T == 0) return VMI_OK;   // (empty outputs are null)
     if (!d_y && !d_scores) return vmi::fail(VMI_ERR_INVALID, "nothing to compute (d_y and d_scores both null)");
-    if (T == 0) return VMI_OK;
     if (!d_out || !place || (d_scores && !y)) return vmi::fail(VMI_ERR_INVALID, "null d_out/place/y");
     if (!aligned({d_out, y, d_y})) return vmi::fail(VMI_ERR_INVALID, "d_out, y and d_y must be 16-byte aligned");
     a.x = static_cast<const vmi_u4*>(d_out);

@@ -1204,6 +1204,7 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
                                   size_t workspace_bytes, void* stream) {
     vmi::clear_error();
     if (const int rc = check_form(T, hidden, vocab)) return rc;
+    if (T == 0 && !dweight) return VMI_OK;   // (an empty dx is null)
     if (!dx && !dweight) return vmi::fail(VMI_ERR_INVALID, "nothing to compute (dx and dweight both null)");
     if (dweight && dweight_dtype != VMI_BF16 && dweight_dtype != VMI_F32)
         return vmi::fail(VMI_ERR_UNSUPPORTED, "dweight_dtype %d", dweight_dtype);

@@ -118,6 +118,8 @@ class _HeadLoss(torch.autograd.Function):
 
 
 def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor) -> torch.device:
+    if isinstance(weight, TiledHead):
+        raise VmiError("weight must be the row-major head, not a TiledHead")
     dev = _on_current(x)
     xs, ws = x.shape, weight.shape
     if len(xs) != 2 or len(ws) != 2 or ws[1] != xs[1]:

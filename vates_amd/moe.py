@@ -568,6 +568,12 @@ def _plan(ids: torch.Tensor, num_experts: int, status: Optional[torch.Tensor]) -
     return ExpertPlan(offsets, source, place)
 
 
+def _rows_of(grad: torch.Tensor) -> torch.Tensor:
+    """A gradient as the kernels read it: contiguous, from an address of 16 bytes on."""
+    grad = grad.contiguous()
+    return grad.clone() if grad.data_ptr() & 15 else grad
+
+
 def _sorted_rows(x: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
     T, k = place.shape
     rows = x.new_empty((T * k, x.shape[1]))
@@ -588,13 +594,13 @@ def _combined(y: torch.Tensor, place: torch.Tensor, scores: Optional[torch.Tenso
 class _SortByExpert(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, place):
-        ctx.place = place     # (no input of the graph's)
+        ctx.save_for_backward(place)
         return _sorted_rows(x, place)
 
     @staticmethod
     @_once
     def backward(ctx, d_rows):
-        return _combined(d_rows.contiguous(), ctx.place, None, None), None
+        return _combined(_rows_of(d_rows), *ctx.saved_tensors, None, None), None
 
 
 class _CombineExperts(torch.autograd.Function):
@@ -608,7 +614,7 @@ class _CombineExperts(torch.autograd.Function):
     def backward(ctx, d_out):
         y, place, scores = ctx.saved_tensors
         need_y, _, need_scores, need_residual = ctx.needs_input_grad
-        d_out = d_out.contiguous()
+        d_out = _rows_of(d_out)
         T, k = place.shape
         d_y = d_out.new_empty((T * k, d_out.shape[1])) if need_y else None
         d_scores = torch.empty_like(scores) if need_scores else None
