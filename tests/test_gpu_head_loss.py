@@ -72,7 +72,7 @@ def _within(got, want, name, rounding=0.0):
     assert (err <= bound).all(), f"{name}: {worst:.3g} of the bound"
 
 
-# (one token to few, few in the two sizes of their block, every width of a block of many, several turns of the grid)
+# (one token to few, few in the two sizes of their block, blocks of 128 tokens; the wider ones are below, with more rows of the head)
 CASES = [(1, 64, 1), (300, 64, 1), (33, 64, 5000), (150, 128, 5000), (185, 64, 9000), (215, 128, 30000), (1000, 64, 1200), (8192, 64, 300), (1, 512, 16), (3, 64, 257), (5, 512, 4099), (16, 2048, 1601), (63, 192, 1000), (64, 1024, 1003),
          (65, 320, 2048), (130, 512, 777), (256, 64, 70), (257, 2048, 3001), (777, 512, 8200), (300, 8192, 129)]
 

@@ -527,11 +527,6 @@ __device__ __forceinline__ void ls_g(const LogitArgs& a, const Meta& me, const i
         if (v0 >= v1) continue;
         LogitJob<S, GRAD> job(a, idx, coef, from, me.nv, rb, v0, v1);
         ls_run<S>(lds, job, (v1 - v0 + S::BM - 1) / S::BM * job.nk);
-        // blocks of 160 or 224 tokens may end inside dW's last step of 64: its rows behind them are zeros
-        if (S::BN % kBK && rb == nrb - 1)
-            for (int r = nrb * S::BN; r < (me.nv + kBK - 1) / kBK * kBK; ++r)
-                for (int c = v0 - a.v0 + 8 * (int)threadIdx.x; c < v1 - a.v0; c += 8 * kThreads)
-                    *reinterpret_cast<vmi_u4*>(a.g + r * a.ldg + c) = vmi_u4{0, 0, 0, 0};
     }
 }
 
@@ -978,11 +973,16 @@ __global__ __launch_bounds__(256) void k_loss_merge_few(Few f, int few, int stri
 
 // x of the tokens in the loss turned, out[h][c], zeros from nv on: the head's gradient then
 // reads one operand of its two along memory (both turned as they were read, LDS took longer than the
-// products: 4096 tokens 2.5 -> 2.1 ms).  64 tokens by 64 hidden values a workgroup.
+// products: 4096 tokens 2.5 -> 2.1 ms).  64 tokens by 64 hidden values a workgroup.  Blocks of 160 or 224 tokens may end
+// inside the last 64: g's rows behind them, which no piece writes, are zeros too.
 __global__ __launch_bounds__(256) void k_loss_turn(const Meta* meta, const int32_t* idx, const uint16_t* x, int H, int64_t ldx,
-                                                   uint16_t* out) {
+                                                   uint16_t* out, uint16_t* g, int64_t ldg) {
     __shared__ uint32_t s_x[64][33];
-    const int nv = vmi_sload_i32(&meta->nv), c0 = blockIdx.x * 64, h0 = blockIdx.y * 64, t = threadIdx.x;
+    const Meta me = ls_meta(meta);
+    const int nv = me.nv, c0 = blockIdx.x * 64, h0 = blockIdx.y * 64, t = threadIdx.x;
+    for (int r = (nv + me.bn - 1) / me.bn * me.bn; r < (nv + kBK - 1) / kBK * kBK; ++r)
+        for (int c = 8 * ((blockIdx.y * gridDim.x + blockIdx.x) * 256 + t); c < ldg; c += 8 * 256 * gridDim.x * gridDim.y)
+            *reinterpret_cast<vmi_u4*>(g + r * ldg + c) = vmi_u4{0, 0, 0, 0};
     if (c0 >= (nv + kBK - 1) / kBK * kBK) return;
     for (int i = t; i < 64 * 8; i += 256) {
         const int c = i >> 3, u = i & 7;
@@ -1231,7 +1231,8 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     const int splits = ls_splits(grid, 1, r.nht, r.steps);
     uint16_t* xt = reinterpret_cast<uint16_t*>(ws + l.x);
     if (dweight && !l.few)
-        hipLaunchKernelGGL(k_loss_turn, dim3(l.rows / 64, hidden / 64), dim3(256), 0, s, r.meta, r.idx, x, hidden, l.ldx, xt);
+        hipLaunchKernelGGL(k_loss_turn, dim3(l.rows / 64, hidden / 64), dim3(256), 0, s, r.meta, r.idx, x, hidden, l.ldx, xt,
+                           reinterpret_cast<uint16_t*>(ws + l.g), l.ldg);
     LogitArgs a{};
     a.few = few;
     a.x = x;
