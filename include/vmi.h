@@ -633,7 +633,7 @@ int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const uint16_t* wei
  * comes behind all others and its place is ~row; so has one with another
  * id outside [0, num_experts), which also ORs VMI_STATUS_BAD_SLOT into *status (may be
  * NULL).  num_experts <= 1024; workspace: the query's bytes (0: sizes not taken),
- * not used up to 8192 routes (then it may be NULL).
+ * 16-byte aligned, not used up to 8192 routes (then it may be NULL).
  * vmi_expert_rows -- rows[place[t][j]] = x[t]; rows of routes without an expert
  * are zeros.
  * vmi_expert_combine -- out[t] = sum_j scores[t][j] y[place[t][j]] (+ residual[t]), over

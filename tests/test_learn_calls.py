@@ -147,3 +147,7 @@ def test_a_tiled_head_is_refused():
     for call in (lambda: head_loss(None, head, None), lambda: head_loss_grad(None, head, None, None, None)):
         with pytest.raises(L.VmiError, match="row-major"):
             call()
+
+
+def test_a_plan_workspace_off_16_bytes(lib):
+    assert lib.vmi_expert_plan(P, 4097, 2, 8, P, P, P, None, P + 2, 1 << 20, None) == L.VMI_ERR_WORKSPACE

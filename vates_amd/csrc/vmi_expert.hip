@@ -204,7 +204,7 @@ __device__ __forceinline__ vmi_u4 ex_narrow(const float (&v)[F32 ? 4 : 8]) {
 }
 
 // PAST: all routes' rows together are more than the last cache holds (256 MB), and go past it (8192 x 10 rows of 4 KB
-// sorted with gradient 147.6 -> 142.6 us, combined with gradients 220 -> 214).
+// sorted with gradient 147.6 -> 142.6 us, combined with gradients 220 -> 209).
 template <bool PAST>
 __device__ __forceinline__ void ex_store(const vmi_u4& v, vmi_u4* at) {
     if constexpr (PAST)
@@ -351,8 +351,8 @@ extern "C" int vmi_expert_plan(const int32_t* ids, int T, int k, int num_experts
     if (!offsets || (T && (!ids || !source || !place))) return vmi::fail(VMI_ERR_INVALID, "null ids/offsets/source/place");
     const int n = T * k, nb = plan_segments(n);
     const size_t need = vmi_expert_plan_workspace_bytes(T, k, num_experts);
-    if (nb > 1 && (!workspace || workspace_bytes < need))
-        return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes (got %zu)", need, workspace_bytes);
+    if (nb > 1 && (!workspace || workspace_bytes < need || !aligned({workspace})))
+        return vmi::fail(VMI_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned (got %zu)", need, workspace_bytes);
     PlanArgs a{ids, n, num_experts, nb == 1 ? (std::max(n, 1) + kSortThreads - 1) / kSortThreads * kSortThreads : plan_segment(n),
                static_cast<uint32_t*>(workspace), offsets, source, place, status};
     hipStream_t s = static_cast<hipStream_t>(stream);

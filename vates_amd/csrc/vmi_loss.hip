@@ -31,7 +31,9 @@
 // the cycles at 1.9 GHz, the library's 74 % at 1.6 (power).  Tried and slower: 32 of k a step in four or
 // five stages (8192 tokens +7 %), 32 x 32 x 16 instructions (+6 %), a SIMD's two waves by turns in four phases a step
 // (+10 %), operands read half a step ahead (spills at 256 registers), four waves of 128 x 128 (spills), tiles of 128 or 192
-// vocabulary rows with three stages for some hundred tokens (+8 to 15 %).
+// vocabulary rows with three stages for some hundred tokens (+8 to 15 %), the head's lines of the step after next asked for
+// into L2 (8192 tokens +5 %).  Where the rest goes at 8192 tokens, 4.06 ms: 3.77 if every line were in L2, 3.13 without the DMA,
+// 3.83 with half the LDS reads; two stages of 64 KB are what LDS holds.
 //
 // Kernels beside them:
 //   k_loss_rows     the tokens in the loss, and their coefficients
