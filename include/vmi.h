@@ -591,7 +591,8 @@ int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x,
  * texts nor trains): for x bf16 [T, hidden] (behind the final norm), weight bf16
  * [vocab, hidden] and targets int64 [T]
  *   z = x . weight (fp32 sums of bf16 products), lse[t] = log sum_v exp z[t][v],
- *   loss[t] = lse[t] - z[t][target],  both f32 [T].
+ *   loss[t] = lse[t] - z[t][target],  both f32 [T]; the loss is not formed from the rounded
+ * lse: a small one is as exact as the sum 1 + (the others' exp(z - z[target])), whatever the logits' size.
  * A token whose target is ignore_index has loss and lse 0 and is not read
  * beyond that; a target outside [0, vocab) gives NaN in both and ORs
  * VMI_STATUS_BAD_TARGET into *status (uint32 on the device, or NULL).  A token with
@@ -601,7 +602,8 @@ int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x,
  *   dx = g . weight  (bf16 [T, hidden], or NULL),
  *   dweight = g^T . x  (dweight_dtype VMI_BF16 or VMI_F32 [vocab, hidden], or NULL).
  * d_loss, d_lse f32 [T] (d_lse may be NULL: zeros).  Tokens left out of the loss
- * (ignore_index, or outside the vocabulary) have no gradient and add none.  z is
+ * (ignore_index, or outside the vocabulary) have no gradient and add none.  Probabilities come from
+ * the lse given: 1 - p of a foreseen target is known to half a step of the lse (2^-24 of it), no closer.  z is
  * formed again, a piece of the vocabulary at a time; g is rounded to bf16 as
  * the operand of the two products (up to 64 tokens in two parts, 16 bits), whose sums are
  * fp32, rounded once.  Sums run in a fixed order, which depends on T and on how many

@@ -943,9 +943,10 @@ __device__ __forceinline__ void ls_merge(const Meta& me, int c, int t, const flo
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) ls_join(m, l, __shfl_xor(m, d), __shfl_xor(l, d));
     if (lane == 0) {
-        const float v = m + logf(l);
-        lse[t] = v;
-        loss[t] = v - hit[c];
+        // (m - z is exact near m, and 0 for a token foreseen: lse - z would round log l to a step of the logits' size first)
+        const float v = logf(l);
+        lse[t] = m + v;
+        loss[t] = m - hit[c] + v;
     }
 }
 // A wave per token in the loss.
