@@ -596,7 +596,8 @@ int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x,
  * A token whose target is ignore_index has loss and lse 0 and is not read
  * beyond that; a target outside [0, vocab) gives NaN in both and ORs
  * VMI_STATUS_BAD_TARGET into *status (uint32 on the device, or NULL).  A token with
- * a logit that is NaN or plus infinity has NaN.
+ * a logit that is NaN or plus infinity has NaN; one whose logits are all minus infinity has lse
+ * minus infinity and loss NaN.
  * vmi_head_loss_grad -- its gradients, from the lse that it wrote:
  *   g[t][v] = (d_loss[t] + d_lse[t]) exp(z[t][v] - lse[t]) - d_loss[t] [v == target],
  *   dx = g . weight  (bf16 [T, hidden], or NULL),

@@ -46,3 +46,24 @@ def test_foreseen_tokens(gpu, T):
         log(f"  A={A}: loss {want.min().item():.3g} .. {want.max().item():.3g}, error over bar {(err / bar).max().item():.3f}")
         assert (err <= bar).all() and (loss >= 0).all()
         assert ((lse.double() - (A + want)).abs() <= bar + U * (A + want).abs()).all()
+
+
+@pytest.mark.parametrize("T", [3, 40, 100])
+@pytest.mark.parametrize("V", [1, 5, 300, 1024])
+def test_every_logit_minus_infinity(gpu, T, V):
+    """A token all of whose logits are minus infinity: lse minus infinity, and NaN for the loss, as
+    the formula gives, whether or not the vocabulary ends inside a tile; one word with a
+    finite logit among them is certain."""
+    import torch
+    from vates_amd.head import head_loss
+    H = 64
+    log(f"case: every logit minus infinity T={T} V={V}")
+    x = torch.ones((T, H), dtype=torch.bfloat16, device=gpu)
+    w = torch.full((V, H), -float("inf"), dtype=torch.bfloat16, device=gpu)
+    y = torch.arange(T, device=gpu) % V
+    loss, lse = head_loss(x, w, y)
+    assert (lse == -float("inf")).all() and loss.isnan().all()
+    w[V - 1] = -0.25
+    loss, lse = head_loss(x, w, y)
+    assert (lse == -16.0).all()
+    assert (loss == torch.where(y == V - 1, 0.0, float("inf"))).all()

@@ -392,14 +392,14 @@ struct LogitJob {
     // Running maximum and sum of a lane's own rows of the tiles, joined over lanes at the end only.
     __device__ __forceinline__ void sum(vmi_f4 (&acc)[S::MB][S::NB]) {
         const int last = v1 - 1 - tile - m0;   // rows of the lane up to this one
-        if (tile + S::BM > v1) {
+        if (tile + S::BM > v1) {   // (below the maxima's start, so that they add nothing even where every logit is minus infinity)
 #pragma unroll
             for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
                 for (int n = 0; n < S::NB; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (16 * mb + r > last) acc[mb][n][r] = kLowest;
+                        if (16 * mb + r > last) acc[mb][n][r] = -__builtin_inff();
         }
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
