@@ -67,3 +67,32 @@ def test_every_logit_minus_infinity(gpu, T, V):
     loss, lse = head_loss(x, w, y)
     assert (lse == -16.0).all()
     assert (loss == torch.where(y == V - 1, 0.0, float("inf"))).all()
+
+
+@pytest.mark.parametrize("T", [1, 32, 33, 64])
+def test_a_few_tokens_none_in_the_loss(gpu, monkeypatch, T):
+    """Up to 64 tokens of which none is in the loss: gradients of zeros, and no product of the head with what the
+    workspace held, so that it holds the same afterwards."""
+    import torch
+    import vates_amd.head as head
+    H, V = 512, 5003
+    log(f"case: none in the loss T={T}")
+    held = []
+
+    def scratch(n, dev):
+        held.append(torch.full((n,), 17, dtype=torch.uint8, device=dev))
+        return held[-1]
+
+    monkeypatch.setattr(head, "scratch", scratch)
+    g = torch.Generator(device=gpu).manual_seed(T)
+    x = torch.randn((T, H), generator=g, device=gpu).to(torch.bfloat16)
+    w = torch.randn((V, H), generator=g, device=gpu).to(torch.bfloat16)
+    y = torch.full((T,), -100, device=gpu)
+    y[T // 2:] = V                       # outside the vocabulary
+    f = torch.ones(T, device=gpu)
+    for wants in ({}, {"want_dweight": False}, {"want_dx": False}):
+        dx, dw = head.head_loss_grad(x, w, y, f, f, f, **wants)
+        assert (dx is None or not dx.any()) and (dw is None or not dw.any())
+    loss, lse = head.head_loss(x, w, y)
+    assert not loss[:T // 2].any() and loss[T // 2:].isnan().all() and lse[T // 2:].isnan().all()
+    assert len(held) == 4 and all((ws == 17).all() for ws in held)

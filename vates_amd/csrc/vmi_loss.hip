@@ -42,6 +42,7 @@
 //   k_loss_dx_out   the split sums of dx joined
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vmi_device.h"
 #include "vmi_internal.h"
@@ -595,6 +596,7 @@ struct DxArgs {
     float* sum;              // [split][token block rows][H]
     int add;                 // a later piece than the first: added to the sums
     int splits;              // up to 64 tokens (else meta's)
+    Few tokens;              // the same: without one in the loss g isn't there
 };
 
 template <class S>
@@ -675,10 +677,11 @@ template <int WHICH>
 __global__ __launch_bounds__(kThreads) void k_loss_dx(DxArgs a) {
     constexpr int kBytes = WHICH == 32 ? kLds<Dx32> : WHICH == 64 ? kLds<Dx64> : kLds<DxN<160>>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kBytes];
-    if constexpr (WHICH == 32) {
-        ls_dx<Dx32>(a, 1, a.splits, lds);
-    } else if constexpr (WHICH == 64) {
-        ls_dx<Dx64>(a, 1, a.splits, lds);
+    if constexpr (WHICH) {
+        int place;
+        int64_t y;
+        if (ls_few(a.tokens, place, y) == 0) return;
+        ls_dx<std::conditional_t<WHICH == 32, Dx32, Dx64>>(a, 1, a.splits, lds);
     } else {
         const Meta me = ls_meta(a.meta);
         if (me.nv == 0) return;
@@ -1249,6 +1252,7 @@ extern "C" int vmi_head_loss_grad(const uint16_t* x, int T, int hidden, const ui
     a.ldg = l.ldg;
     DxArgs d{};
     d.splits = splits;
+    d.tokens = few;
     d.w = weight;
     d.g = a.g;
     d.meta = r.meta;
