@@ -151,3 +151,36 @@ def test_a_tiled_head_is_refused():
 
 def test_a_plan_workspace_off_16_bytes(lib):
     assert lib.vmi_expert_plan(P, 4097, 2, 8, P, P, P, None, P + 2, 1 << 20, None) == L.VMI_ERR_WORKSPACE
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(gpu):
+    """Tensors with a tangent, in whichever argument, and gradients with one: refused, where a result
+    without its tangent would be a wrong derivative. Plain calls inside a dual level go on."""
+    import torch
+    import torch.autograd.forward_ad as ad
+    from vates_amd.head import head_loss, head_loss_grad
+    from vates_amd.moe import combine_experts, expert_plan, sort_by_expert
+    r = lambda *s, dt=torch.bfloat16: torch.ones(s, dtype=dt, device=gpu)
+    x, w, t, f = r(4, 64), r(9, 64), torch.zeros(4, dtype=torch.int64, device=gpu), r(4, dt=torch.float32)
+    plan = expert_plan(torch.zeros((4, 2), dtype=torch.int32, device=gpu), 3)
+    y, s = r(8, 64), r(4, 2, dt=torch.float32)
+    lse = head_loss(x, w, t)[1]
+    with ad.dual_level():
+        dual = lambda v: ad.make_dual(v, torch.ones_like(v))
+        calls = [lambda: head_loss(dual(x), w, t), lambda: head_loss(x, dual(w), t),
+                 lambda: head_loss_grad(dual(x), w, t, lse, f), lambda: head_loss_grad(x, dual(w), t, lse, f),
+                 lambda: head_loss_grad(x, w, t, dual(lse), f), lambda: head_loss_grad(x, w, t, lse, dual(f)),
+                 lambda: head_loss_grad(x, w, t, lse, f, dual(f)), lambda: sort_by_expert(dual(x), plan),
+                 lambda: combine_experts(dual(y), plan), lambda: combine_experts(y, plan, dual(s)),
+                 lambda: combine_experts(y, plan, s, residual=dual(x))]
+        for i, call in enumerate(calls):
+            with pytest.raises(L.VmiError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was taken")
+        leaf = x.clone().requires_grad_()
+        for out in (head_loss(leaf, w, t)[0], sort_by_expert(leaf, plan), combine_experts(y, plan, s, residual=leaf)):
+            with pytest.raises(L.VmiError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, dual(torch.ones_like(out)), retain_graph=True)
+            torch.autograd.grad(out, leaf, torch.ones_like(out))
+        assert torch.equal(head_loss(x, w, t)[1], lse) and combine_experts(y, plan, s).shape == (4, 64)

@@ -13,7 +13,8 @@ from typing import Optional
 import torch
 
 from ._lib import VMI_BF16, VMI_F32, VmiError, check, load
-from .moe import _matches, _on_current, _on_stream, _once, _ptr, _require, _stream_handle, _stream_on, scratch, workspace
+from .moe import (_matches, _no_tangent, _on_current, _on_stream, _once, _ptr, _require, _stream_handle, _stream_on, scratch,
+                  workspace)
 
 
 class TiledHead:
@@ -129,6 +130,7 @@ def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor) ->
     if targets.dtype not in (torch.int64, torch.int32):
         raise VmiError(f"targets must be int64 or int32 (got {targets.dtype})")
     _matches(targets, "targets", xs[:1], targets.dtype, dev)
+    _no_tangent(x, weight)
     return dev
 
 
@@ -155,8 +157,8 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, i
     int32 [T].  A token with target ignore_index has loss and lse 0 and is not read;
     a target outside the vocabulary gives NaN and ORs VMI_STATUS_BAD_TARGET into
     status (int32 [1] on the device).  Differentiable in x and weight through
-    both outputs (``head_loss_grad``; a weight that needs no gradient costs none);
-    tokens left out of the loss have zeros and add nothing."""
+    both outputs (``head_loss_grad``; a weight that needs no gradient costs none), once and
+    in reverse mode; tokens left out of the loss have zeros and add nothing."""
     dev = _check_loss(x, weight, targets)
     if status is not None:
         _matches(status, "status", (1,), torch.int32, dev)
@@ -183,6 +185,7 @@ def head_loss_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
     for t, name in ((lse, "lse"), (d_loss, "d_loss"), (d_lse, "d_lse")):
         if t is not None or name != "d_lse":
             _matches(t, name, (T,), torch.float32, dev)
+    _no_tangent(lse, d_loss, d_lse)
     if dweight_dtype not in (torch.bfloat16, torch.float32):
         raise VmiError(f"dweight_dtype must be bf16 or f32 (got {dweight_dtype})")
     if not (want_dx or want_dweight):

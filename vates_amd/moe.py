@@ -20,6 +20,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import QMat, MoeLayerDesc, VmiError, check, load
@@ -510,12 +511,20 @@ def _on_stream(stream, fn, *args):
         return fn(*args)
 
 
+def _no_tangent(*tensors) -> None:
+    """Refuses tensors of forward-mode differentiation, whose tangents a kernel's result would not have."""
+    if forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise VmiError("forward-mode differentiation is not supported (a tensor has a tangent)")
+
+
 def _once(backward):
     """torch's once_differentiable, whose own cost (5 us) is paid only where a graph of
     the gradients is asked for."""
     twice = torch.autograd.function.once_differentiable(backward)
 
     def either(ctx, *grads):
+        _no_tangent(*grads)
         return (twice if torch.is_grad_enabled() else backward)(ctx, *grads)
     return either
 
@@ -642,8 +651,8 @@ def sort_by_expert(x: torch.Tensor, plan: ExpertPlan, *, stream=None) -> torch.T
     experts of the caller's own (expert e's rows are plan.offsets[e] ..).
 
     x bf16 or f32 [T, hidden] (hidden a multiple of 8, f32 of 4); returns
-    [T * k, hidden], rows behind the last expert's are zeros.  Differentiable: a
-    token's gradient is the sum of its rows', in rank order in fp32, rounded once."""
+    [T * k, hidden], rows behind the last expert's are zeros.  Differentiable
+    (once, in reverse mode, as ``combine_experts``): a token's gradient is the sum of its rows', in rank order in fp32, rounded once."""
     dev = _on_current(x)
     T, _ = _check_plan(plan, dev)
     shape = x.shape
@@ -651,6 +660,7 @@ def sort_by_expert(x: torch.Tensor, plan: ExpertPlan, *, stream=None) -> torch.T
         raise VmiError(f"x must be [{T}, hidden], got {tuple(shape)}")
     _rows_dtype(x, "x")
     _matches(x, "x", shape, x.dtype, dev)
+    _no_tangent(x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _on_stream(stream, _SortByExpert.apply, x, plan.place)
     return _on_stream(stream, _sorted_rows, x, plan.place)
@@ -676,6 +686,7 @@ def combine_experts(y: torch.Tensor, plan: ExpertPlan, scores: Optional[torch.Te
         _matches(scores, "scores", (T, k), torch.float32, dev)
     if residual is not None:
         _matches(residual, "residual", (T, shape[1]), y.dtype, dev)
+    _no_tangent(y, scores, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, scores, residual)):
         return _on_stream(stream, _CombineExperts.apply, y, plan.place, scores, residual)
     return _on_stream(stream, _combined, y, plan.place, scores, residual)
