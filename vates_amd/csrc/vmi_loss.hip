@@ -912,8 +912,8 @@ __global__ __launch_bounds__(1024) void k_loss_rows(RowsArgs a) {
         }
     }
     // waves 0 to 4 weigh a width each
-    const int bn = 256 - 32 * w, nrb = max((nv + bn - 1) / bn, 1);
-    if (nv && bn >= 128) {
+    if (nv && w < 5) {
+        const int bn = 256 - 32 * w, nrb = (nv + bn - 1) / bn;
         const uint64_t p = ls_plan(nrb, bn, a.tiles, a.grid), q = a.last == a.tiles ? p : ls_plan(nrb, bn, a.last, a.grid);
         if (lane == 0) {
             s_work[w] = p >> 16;

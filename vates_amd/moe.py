@@ -652,7 +652,8 @@ def sort_by_expert(x: torch.Tensor, plan: ExpertPlan, *, stream=None) -> torch.T
 
     x bf16 or f32 [T, hidden] (hidden a multiple of 8, f32 of 4); returns
     [T * k, hidden], rows behind the last expert's are zeros.  Differentiable
-    (once, in reverse mode, as ``combine_experts``): a token's gradient is the sum of its rows', in rank order in fp32, rounded once."""
+    (once, in reverse mode, as ``combine_experts``): a token's gradient is the
+    sum of its rows', in rank order in fp32, rounded once."""
     dev = _on_current(x)
     T, _ = _check_plan(plan, dev)
     shape = x.shape
