@@ -184,3 +184,21 @@ def test_forward_mode_is_refused(gpu):
                 torch.autograd.grad(out, leaf, dual(torch.ones_like(out)), retain_graph=True)
             torch.autograd.grad(out, leaf, torch.ones_like(out))
         assert torch.equal(head_loss(x, w, t)[1], lse) and combine_experts(y, plan, s).shape == (4, 64)
+
+
+def test_streams_of_another_device_are_refused(monkeypatch):
+    """A stream that is not on the tensors' device, which is the current one: the call would
+    go to that device's own stream, not to the one asked for."""
+    import torch
+    from vates_amd.moe import _on_stream
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+
+    class Stream:
+        device_index = 1
+
+    ran = []
+    with pytest.raises(L.VmiError, match="stream"):
+        _on_stream(Stream(), ran.append, 1)
+    assert not ran
+    _on_stream(None, ran.append, 1)
+    assert ran == [1]

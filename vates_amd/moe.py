@@ -504,6 +504,8 @@ def _on_stream(stream, fn, *args):
     tensors among args are not handed out again before that stream is done with them."""
     if stream is None:
         return fn(*args)
+    if stream.device_index != torch._C._cuda_getDevice():
+        raise VmiError(f"the stream is on device {stream.device_index}, not the current HIP device")
     with torch.cuda.stream(stream):
         for t in args:
             if isinstance(t, torch.Tensor):
