@@ -324,8 +324,10 @@ struct LogitJob {
         nk = a.H / kBK;
         // Rows of a few KB put the pieces that all workgroups ask for at one time on few memory channels; begun at
         // steps of their own, strips spread over them all (one token 129 -> 109 us, 100 tokens 156 -> 129).
-        // Where blocks of tokens share a strip in an XCD's L2, groups of them do (8192 tokens 4014 -> 3965 us).
-        turn = nv <= 4 * S::BN ? v0_ / 16 % nk : (rb >> 3) * 11 % nk;
+        // Where blocks of tokens share a strip in an XCD's L2, groups of eight do.  Strips against groups, 151,936 x 2048:
+        // 100 tokens 116 and 143 us, 300 (two blocks) 221 and 226, 640 (three) 397 and 400, 850 (four) 523 and 505,
+        // 1000 591 and 567, 1280 730 and 692, 2048 1143 and 1076, 8192 alike.
+        turn = nv <= 2 * S::BN ? v0_ / 16 % nk : (rb >> 3) * 11 % nk;
         tile = v0_;
         next = min(v0_, a.V - 1);   // (a piece's last tile may lie behind the vocabulary: its columns are zeros)
         k = kd = 0;
@@ -837,7 +839,8 @@ constexpr int kMaxItems = 4;       // workgroups' turns at most that the strips 
 
 // The least work, in tokens' widths of a tile, of `tiles` cut into s strips by nrb blocks
 // of bn tokens: turns of the grid times a turn's tiles in quarters, which the waves behind a strip's end leave out (a tile's own
-// cost beside its products about 16 tokens, a turn's 24); lane l tries s = l + 1, l + 65, ..  Returns work * 2^16 + s.
+// cost beside its products about 16 tokens: counted as none, 1200 tokens over 151,936 x 2048 took 746 us for 688, 4096 2390 for
+// 2100; as 32 the same as 16.  A turn's, 24: none or 48 changed no size tried by more than 1 %); lane l tries s = l + 1, l + 65, ..  Returns work * 2^16 + s.
 __device__ __forceinline__ uint64_t ls_plan(int nrb, int bn, int tiles, int grid) {
     const int most = min(tiles, max(1, kMaxItems * grid / nrb));
     const float per_grid = (float)nrb / (float)grid;
