@@ -606,8 +606,8 @@ int vmi_attention_prompt_kv8(const vmi_attn_layer_desc* desc, const uint16_t* x,
  * (ignore_index, or outside the vocabulary) have no gradient and add none.  Probabilities come from
  * the lse given: 1 - p of a foreseen target is known to half a step of the lse (2^-24 of it), no closer.  z is
  * formed again, a piece of the vocabulary at a time; g is rounded to bf16 as
- * the operand of the two products (up to 64 tokens in two parts, 16 bits), whose sums are
- * fp32, rounded once.  Sums run in a fixed order, which depends on T and on how many
+ * the operand of the two products (T up to 64: in two parts, 16 bits; above, 2^-8 of each token's share in dx and
+ * dweight, a VMI_F32 one too), whose sums are fp32, rounded once.  Sums run in a fixed order, which depends on T and on how many
  * tokens are in the loss: the same call gives the same bits.
  * T <= 65536 (0: nothing but a dweight of zeros), hidden a multiple of 64 up to
  * 8192, vocab <= 2^21, pointers 16-byte aligned (targets 8).  workspace: the query's bytes

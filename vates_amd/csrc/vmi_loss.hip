@@ -21,13 +21,14 @@
 // values as they are read.  Both placements read without bank conflicts (4.7 and 4.3 cycles an
 // instruction, as consecutive addresses do; rows unturned 12.6 and 16).
 //
-// g is rounded to bf16, the type of the matrix instruction's other operand (W, x): half a step is
-// 2^-9 of its value, as much as the outputs' own rounding.  Up to 64 tokens, where the head's
+// g is rounded to bf16, the type of the matrix instruction's other operand (W, x): off by 2^-8 of its
+// value at most, as much as a bf16 output's own rounding (647 tokens: dx 2.4e-3 from the 64-bit one, 1.7e-3 if only the output
+// were rounded; dW in f32 1.7e-3, all of it g's).  Up to 64 tokens, where the head's
 // bytes are the bound, what that leaves is multiplied too, in a second bf16.
 //
-// What bounds it (MI355X, 151,936 x 2048): one token 99 us, 6.7 TB/s of the head's bytes in the kernel
-// (a read reaches 7.2); 8192 tokens 4.0 ms, 1.28 PFLOP/s; a step of 4096 with both gradients 8.9 ms,
-// 1.15 PFLOP/s with z formed twice (a library product of these shapes 1.35 to 1.57): the matrix cores are busy 56 % of
+// What bounds it (MI355X, 151,936 x 2048): one token 100 us, 6.7 TB/s of the head's bytes in the kernel
+// (a read reaches 7.2); 8192 tokens 3.97 to 4.25 ms over the cards, 1.20 to 1.28 PFLOP/s; a step of 4096 with both gradients 8.8 ms,
+// 1.16 PFLOP/s with z formed twice (a library product of these shapes 1.38 to 1.57): the matrix cores are busy 56 % of
 // the cycles at 1.9 GHz, the library's 74 % at 1.6 (power).  Tried and slower: 32 of k a step in four or
 // five stages (8192 tokens +7 %), 32 x 32 x 16 instructions (+6 %), a SIMD's two waves by turns in four phases a step
 // (+10 %), operands read half a step ahead (spills at 256 registers), four waves of 128 x 128 (spills), tiles of 128 or 192
@@ -982,7 +983,7 @@ __global__ __launch_bounds__(256) void k_loss_merge_few(Few f, int few, int stri
 
 // x of the tokens in the loss turned, out[h][c], zeros from nv on: the head's gradient then
 // reads one operand of its two along memory (both turned as they were read, LDS took longer than the
-// products: 4096 tokens 2.5 -> 2.1 ms).  64 tokens by 64 hidden values a workgroup.  Blocks of 160 or 224 tokens may end
+// products: 4096 tokens 2.5 -> 2.3 ms).  64 tokens by 64 hidden values a workgroup.  Blocks of 160 or 224 tokens may end
 // inside the last 64: g's rows behind them, which no piece writes, are zeros too.
 __global__ __launch_bounds__(256) void k_loss_turn(const Meta* meta, const int32_t* idx, const uint16_t* x, int H, int64_t ldx,
                                                    uint16_t* out, uint16_t* g, int64_t ldg) {

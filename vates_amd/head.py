@@ -178,8 +178,9 @@ def head_loss_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
                    dweight_dtype: torch.dtype = torch.bfloat16, ignore_index: int = -100, stream=None):
     """(dx bf16 [T, hidden] or None, dweight [vocab, hidden] or None): the gradients
     of ``head_loss`` from the lse that it returned and those of its outputs, f32
-    [T] (``vmi_head_loss_grad``).  dweight_dtype: bf16, or f32 for gradients that a
-    caller adds up itself.  The same call gives the same bits."""
+    [T] (``vmi_head_loss_grad``).  dweight_dtype: bf16, or f32, which spares gradients that a
+    caller adds up itself the output's rounding; that of g to bf16 stays above 64 tokens (half a step,
+    2^-8, of every token's share).  Not differentiable itself.  The same call gives the same bits."""
     dev = _check_loss(x, weight, targets)
     T = x.shape[0]
     for t, name in ((lse, "lse"), (d_loss, "d_loss"), (d_lse, "d_lse")):
